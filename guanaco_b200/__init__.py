@@ -116,6 +116,14 @@ SIGNATURES = {
     "gb_attention_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp]),
     "gb_attention_decode_static": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
     "gb_attention_static_error": (_i, [_i]),
+    "gb_kv_page_bytes": (_sz, [_i, _i, _i, _i]),
+    "gb_kv_append": (_i, [_vp, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp]),
+    "gb_kv_read": (_i, [_vp, _vp, _i, _vp, _i, _vp, _i, _vp]),
+    "gb_paged_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "gb_paged_attention_decode": (_i, [_vp, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _vp]),
+    "gb_paged_attention_prefill": (_i, [_vp, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _vp]),
+    "gb_paged_error": (_i, [_i]),
+    "gb_sample": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "gb_rmsnorm": (_i, [_vp, _vp, _vp, _i, _f, _vp]),
     "gb_silu_mul": (_i, [_vp, _vp, _i, _vp]),
     "gb_argmax": (_i, [_vp, _i, _vp, _vp]),
@@ -257,6 +265,133 @@ def attention_decode_static(q, k, v, k_cache, v_cache, rope_cs, d_pos, n_heads, 
     check("gb_attention_decode_static", lib().gb_attention_decode_static(
         _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(rope_cs), _ptr(d_pos),
         n_heads, n_kv, head_dim, max_seq, _ptr(out), _stream(stream)))
+
+
+# ------------------------------------------------- batched serving (paged KV cache)
+class KVCache(C.Structure):
+    """gb_kv_cache: K and V pools of n_pages pages (F16 or Q8_0 rows), held as
+    torch tensors or raw device pointers.  :func:`kv_page_bytes` sizes them."""
+    _fields_ = [("dtype", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("page_size", C.c_int),
+                ("n_pages", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+    def __init__(self, dtype, n_kv_heads, head_dim, page_size, n_pages, k_pool, v_pool):
+        need = n_pages * kv_page_bytes(dtype, n_kv_heads, head_dim, page_size)
+        for t in (k_pool, v_pool):
+            if need <= 0 or (not isinstance(t, int) and t.numel() * t.element_size() < need):
+                raise GBError("KVCache", GB_ESIZE)
+        super().__init__(dtype, n_kv_heads, head_dim, page_size, n_pages, _ptr(k_pool), _ptr(v_pool))
+        self._keep = (k_pool, v_pool)
+        self.ref = C.addressof(self)
+
+
+class KVBatch(C.Structure):
+    """gb_kv_batch: int32 device tensors cu_seqlens [n_seq + 1] (None: one
+    token per sequence), kv_len [n_seq] and page_table [n_seq][stride]."""
+    _fields_ = [("n_seq", C.c_int), ("n_tokens", C.c_int), ("cu_seqlens", C.c_void_p), ("kv_len", C.c_void_p),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int)]
+
+    def __init__(self, n_seq, n_tokens, kv_len, page_table, cu_seqlens=None):
+        import torch
+        for t, n in ((kv_len, n_seq), (cu_seqlens, n_seq + 1)):
+            if t is not None and (t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous()):
+                raise GBError("KVBatch", GB_EINVAL)
+        if (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] < n_seq
+                or page_table.stride(1) != 1):
+            raise GBError("KVBatch", GB_EINVAL)
+        super().__init__(n_seq, n_tokens, _ptr(cu_seqlens), _ptr(kv_len), _ptr(page_table), page_table.stride(0))
+        self._keep = (kv_len, page_table, cu_seqlens)
+        self.ref = C.addressof(self)
+
+
+_ACT = {}
+
+
+def _rows(fn, n_tokens, *ts):
+    """dtype code of activation rows [n_tokens][width] (F32 or F16, unit inner stride)."""
+    if not _ACT:
+        import torch
+        _ACT.update({torch.float32: DT_F32, torch.float16: DT_F16})
+    dt = _ACT.get(ts[0].dtype)
+    for t in ts:
+        if (dt is None or t.dim() != 2 or t.shape[0] < n_tokens or t.stride(1) != 1 or t.dtype != ts[0].dtype
+                or t.shape[1] != ts[0].shape[1]):
+            raise GBError(fn, GB_EINVAL)
+    return dt
+
+
+def kv_page_bytes(dtype, n_kv_heads, head_dim, page_size) -> int:
+    return int(lib().gb_kv_page_bytes(dtype, n_kv_heads, head_dim, page_size))
+
+
+def kv_append(cache, batch, k, v, q=None, q_out=None, rope_cs=None, stream=None) -> None:
+    """Write the batch's k / v rows into the cache, rotated and quantised; with
+    q, also its rotated rows into q_out."""
+    dt = _rows("gb_kv_append", batch.n_tokens, k, v)
+    if k.shape[1] != cache.n_kv_heads * cache.head_dim:
+        raise GBError("gb_kv_append", GB_EINVAL)
+    ldq = ldqo = nh = 0
+    if q is not None:
+        if q_out is None or _rows("gb_kv_append", batch.n_tokens, q, q_out) != dt or q.shape[1] % cache.head_dim:
+            raise GBError("gb_kv_append", GB_EINVAL)
+        ldq, ldqo, nh = q.stride(0), q_out.stride(0), q.shape[1] // cache.head_dim
+    rope_len = 0 if rope_cs is None else rope_cs.numel() // cache.head_dim
+    check("gb_kv_append", lib().gb_kv_append(cache.ref, batch.ref, dt, _ptr(q), ldq, nh, _ptr(q_out), ldqo, _ptr(k),
+                                             k.stride(0), _ptr(v), v.stride(0), _ptr(rope_cs), rope_len,
+                                             _stream(stream)))
+
+
+def kv_read(cache, batch, k, v, stream=None) -> None:
+    """The cache's values at the batch's tokens, into k and v rows."""
+    dt = _rows("gb_kv_read", batch.n_tokens, k, v)
+    if k.shape[1] != cache.n_kv_heads * cache.head_dim:
+        raise GBError("gb_kv_read", GB_EINVAL)
+    check("gb_kv_read", lib().gb_kv_read(cache.ref, batch.ref, dt, _ptr(k), k.stride(0), _ptr(v), v.stride(0),
+                                         _stream(stream)))
+
+
+def paged_workspace_bytes(n_heads, n_kv_heads, head_dim, n_seq) -> int:
+    return int(lib().gb_paged_workspace_bytes(n_heads, n_kv_heads, head_dim, n_seq))
+
+
+def _paged_attention(name, cache, batch, q, out, ws, stream):
+    dt = _rows(name, batch.n_tokens, q, out)
+    hd = cache.head_dim
+    nh = q.shape[1] // hd
+    need = paged_workspace_bytes(nh, cache.n_kv_heads, hd, batch.n_seq)
+    if q.shape[1] % hd or ws.numel() * ws.element_size() < need:
+        raise GBError(name, GB_ESIZE if q.shape[1] % hd == 0 else GB_EINVAL)
+    check(name, getattr(lib(), name)(cache.ref, batch.ref, dt, _ptr(q), q.stride(0), nh, _ptr(out), out.stride(0),
+                                     _ptr(ws), _stream(stream)))
+
+
+def paged_attention_decode(cache, batch, q, out, ws, stream=None) -> None:
+    """Attention of one new token per sequence over its cached rows."""
+    _paged_attention("gb_paged_attention_decode", cache, batch, q, out, ws, stream)
+
+
+def paged_attention_prefill(cache, batch, q, out, ws, stream=None) -> None:
+    """Causal attention of packed prompts (cu_seqlens) over their cached rows."""
+    _paged_attention("gb_paged_attention_prefill", cache, batch, q, out, ws, stream)
+
+
+def paged_error(clear=False) -> int:
+    return lib().gb_paged_error(int(clear))
+
+
+def sample(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=None) -> None:
+    """Draw out[r] (int32) from logits[r] (fp32 rows) with u[r] in [0, 1);
+    temperature / top_k / top_p / min_p: per-row device tensors or None."""
+    import torch
+    n = logits.shape[0]
+    if (logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1 or out.dtype != torch.int32
+            or (top_k is not None and top_k.dtype != torch.int32)):
+        raise GBError("gb_sample", GB_EINVAL)
+    for t in (out, u, temperature, top_k, top_p, min_p):
+        if t is not None and (t.numel() < n or not t.is_contiguous()
+                              or (t is not out and t is not top_k and t.dtype != torch.float32)):
+            raise GBError("gb_sample", GB_EINVAL)
+    check("gb_sample", lib().gb_sample(_ptr(logits), logits.stride(0), n, logits.shape[1], _ptr(temperature),
+                                       _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(u), _ptr(out), _stream(stream)))
 
 
 def rmsnorm(x, w, out, n, eps, stream=None) -> None:

@@ -242,6 +242,96 @@ int gb_silu_mul(float* gate, const float* up, int n, void* stream);
 /* first index of the maximum (strict >, src/tokenizer/tokenizer.c:175-185). */
 int gb_argmax(const float* x, int n, int* d_out, void* stream);
 
+/* ---- Serving a batch: a paged, quantised KV cache, attention over it, and
+ * the sampler.  No reference counterpart but the samplers (the reference
+ * keeps one fp32 cache per sequence, src/memory/kv_cache.c, and samples on
+ * the host, src/tokenizer/tokenizer.c:187-335). ---- */
+
+/* K and V pools of n_pages pages each, shared by any number of sequences.
+ * A page holds page_size rows of every KV head: per head a slab of
+ *   dtype 1 (F16)   [page_size][head_dim] halves
+ *   dtype 2 (Q8_0)  [page_size][head_dim] int8 codes, then
+ *                   [page_size][head_dim / 32] half scales
+ * (GGUF's Q8_0 block as two planes).  head_dim 64 or 128; page_size a power
+ * of two from 16 to 256; pools 16-byte aligned, n_pages * gb_kv_page_bytes()
+ * bytes each (0 for an unsupported layout). */
+typedef struct {
+    int dtype, n_kv_heads, head_dim, page_size, n_pages;
+    void *k, *v;
+} gb_kv_cache;
+size_t gb_kv_page_bytes(int dtype, int n_kv_heads, int head_dim, int page_size);
+
+/* A batch of n_seq sequences with n_tokens packed tokens; the arrays are in
+ * device memory, so one captured call serves changing lengths.  Sequence s
+ * has tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1 and kv_len[s] cached rows,
+ * the batch's own tokens included: its token t is at position
+ * kv_len[s] - (cu_seqlens[s + 1] - t), row position % page_size of page
+ * page_table[s * table_stride + position / page_size].  cu_seqlens NULL: one
+ * token per sequence (n_tokens == n_seq).  Tokens past cu_seqlens[n_seq] are
+ * padding and left alone.  A length or page outside the table or the pool, or
+ * a negative position when writing or reading, records GB_EPOS
+ * (gb_paged_error); memory outside the pools is never touched.  Such a token
+ * is not written and reads as zeros; a sequence with such a length counts as
+ * empty; attention over such a page gives its sequence unspecified values.
+ * page_table entries past a sequence's length are not read. */
+typedef struct {
+    int n_seq, n_tokens;
+    const int *cu_seqlens, *kv_len, *page_table;
+    int table_stride;
+} gb_kv_batch;
+
+/* Writes the batch's k and v rows (n_tokens rows of n_kv_heads * head_dim,
+ * ldk / ldv elements apart; dtype 0 F32 or 1 F16) into the cache, quantised
+ * to its type.  rope_cs (gb_rope_table, rope_len rows; may be NULL): k is
+ * rotated at its position first, and when q is not NULL the rotated q
+ * (n_heads heads) goes to q_out (which may be q).  Q8_0: per 32 columns
+ * d = half(max |x| / 127) (at most 65504), code = x / d rounded to nearest
+ * even; NaN and d = 0 give code 0.  Rows 16-byte aligned.  Asynchronous. */
+int gb_kv_append(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q, int ldq, int n_heads,
+                 void* q_out, int ldqo, const void* k, int ldk, const void* v, int ldv, const float* rope_cs,
+                 int rope_len, void* stream);
+/* Reads the rows of the batch's tokens back as dtype F32 or F16 (k or v may
+ * be NULL).  With cu_seqlens = running sums of kv_len: the whole cache. */
+int gb_kv_read(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, void* k, int ldk, void* v, int ldv,
+               void* stream);
+
+/* Attention of the batch's query rows q [n_tokens][n_heads * head_dim] over
+ * the cache: a token at position p sees rows 0 .. p of its sequence (append
+ * first); scores scaled by 1 / sqrt(head_dim); a token that sees nothing gets
+ * zeros.  n_heads a multiple of n_kv_heads.  fp32 softmax and sums.
+ * _decode: one token per sequence (cu_seqlens NULL), split over the cache's
+ * length and joined.  _prefill: packed prompts of any lengths, on the tensor
+ * cores.  ws: gb_paged_workspace_bytes(...) bytes for the largest n_seq it
+ * will serve, 16-byte aligned, zeroed once; calls that share it must not
+ * overlap in time.  Asynchronous. */
+size_t gb_paged_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int n_seq);
+int gb_paged_attention_decode(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q, int ldq,
+                              int n_heads, void* out, int ldo, void* ws, void* stream);
+int gb_paged_attention_prefill(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q, int ldq,
+                               int n_heads, void* out, int ldo, void* ws, void* stream);
+/* The paged entry points' device error word (GB_EPOS, GB_ETIMEOUT; 0 none);
+ * clear != 0 resets it.  Synchronous. */
+int gb_paged_error(int clear);
+
+/* One token per row of logits [rows][vocab] (fp32, rows ldl apart; vocab up
+ * to GB_SAMPLE_MAX_VOCAB), drawn with the row's u in [0, 1).  The per-row
+ * parameter arrays may be NULL (off).  Tokens are ordered by logit, ties by
+ * index (lowest first); NaN counts as -inf, and -inf is never drawn.
+ *   temperature <= 0: the first token (argmax); NULL: 1
+ *   w_i = rint(2^40 exp((l_i - max) / temperature)), an integer
+ *   top_k > 0: the first top_k tokens; W = the sum of their w
+ *   top_p < 1: of those, the tokens before which the running sum is below
+ *              floor(W rint(2^24 top_p) / 2^24), and always the first
+ *   min_p > 0: of those, the tokens with exp(...) >= min(min_p, 1)
+ *   drawn: the first kept index whose running sum (in index order) exceeds
+ *          floor(W' floor(2^24 u) / 2^24), W' the kept sum
+ * Sums of integers do not depend on their order: the same row gives the same
+ * token in every batch.  A row without a token to draw gives -1.
+ * Asynchronous. */
+#define GB_SAMPLE_MAX_VOCAB 262144
+int gb_sample(const float* logits, int ldl, int rows, int vocab, const float* temperature, const int* top_k,
+              const float* top_p, const float* min_p, const float* u, int* out, void* stream);
+
 /* ---- Device-resident decode model (the fast path behind forward()) ---- */
 typedef struct gb_model gb_model;
 
