@@ -44,40 +44,6 @@ int paged_views(const gb_kv_cache* c, const gb_kv_batch* b, PagedView* pv, Batch
     return GB_OK;
 }
 
-// ---------------------------------------------------------------- activations
-// 8 consecutive activations as fp32, and back.
-__device__ __forceinline__ void act_load8(const float* p, float (&x)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-__device__ __forceinline__ void act_load8(const __half* p, float (&x)[8]) {
-    const uint4 r = ldg4(p);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
-    }
-}
-__device__ __forceinline__ uint4 pack_half8(const float (&x)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ void act_store8(float* p, const float (&x)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-}
-__device__ __forceinline__ void act_store8(__half* p, const float (&x)[8]) {
-    *reinterpret_cast<uint4*>(p) = pack_half8(x);
-}
-
 // ---------------------------------------------------------------- append
 // A thread takes 8 columns of one head of one token: 4 RoPE pairs, and a
 // quarter of a Q8_0 block (its maximum by two shuffles).  Heads of a token in
