@@ -177,7 +177,7 @@ def _ptr(t) -> int | None:
 def _stream(stream) -> int | None:
     if stream is None:
         import torch
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())   # current_stream() without its object
     return stream
 
 
@@ -300,23 +300,25 @@ class KVBatch(C.Structure):
             raise GBError("KVBatch", GB_EINVAL)
         super().__init__(n_seq, n_tokens, _ptr(cu_seqlens), _ptr(kv_len), _ptr(page_table), page_table.stride(0))
         self._keep = (kv_len, page_table, cu_seqlens)
+        self._ws_need = {}
         self.ref = C.addressof(self)
 
 
-_ACT = {}
+_ACT: dict = {}   # torch dtype -> dtype code of activation rows
 
 
-def _rows(fn, n_tokens, *ts):
-    """dtype code of activation rows [n_tokens][width] (F32 or F16, unit inner stride)."""
+def _rows(fn, n_tokens, a, b):
+    """(dtype code, width) of two tensors of activation rows [n_tokens][width]
+    (F32 or F16, unit inner stride)."""
     if not _ACT:
         import torch
         _ACT.update({torch.float32: DT_F32, torch.float16: DT_F16})
-    dt = _ACT.get(ts[0].dtype)
-    for t in ts:
-        if (dt is None or t.dim() != 2 or t.shape[0] < n_tokens or t.stride(1) != 1 or t.dtype != ts[0].dtype
-                or t.shape[1] != ts[0].shape[1]):
-            raise GBError(fn, GB_EINVAL)
-    return dt
+    t = a.dtype
+    sa, sb = a.shape, b.shape
+    if (t not in _ACT or b.dtype is not t or len(sa) != 2 or len(sb) != 2 or sa[1] != sb[1] or sa[0] < n_tokens
+            or sb[0] < n_tokens or a.stride(1) != 1 or b.stride(1) != 1):
+        raise GBError(fn, GB_EINVAL)
+    return _ACT[t], sa[1]
 
 
 def kv_page_bytes(dtype, n_kv_heads, head_dim, page_size) -> int:
@@ -326,52 +328,67 @@ def kv_page_bytes(dtype, n_kv_heads, head_dim, page_size) -> int:
 def kv_append(cache, batch, k, v, q=None, q_out=None, rope_cs=None, stream=None) -> None:
     """Write the batch's k / v rows into the cache, rotated and quantised; with
     q, also its rotated rows into q_out."""
-    dt = _rows("gb_kv_append", batch.n_tokens, k, v)
-    if k.shape[1] != cache.n_kv_heads * cache.head_dim:
+    n, hd = batch.n_tokens, cache.head_dim
+    dt, width = _rows("gb_kv_append", n, k, v)
+    if width != cache.n_kv_heads * hd:
         raise GBError("gb_kv_append", GB_EINVAL)
+    pq = pqo = None
     ldq = ldqo = nh = 0
     if q is not None:
-        if q_out is None or _rows("gb_kv_append", batch.n_tokens, q, q_out) != dt or q.shape[1] % cache.head_dim:
+        if q_out is None:
             raise GBError("gb_kv_append", GB_EINVAL)
-        ldq, ldqo, nh = q.stride(0), q_out.stride(0), q.shape[1] // cache.head_dim
-    rope_len = 0 if rope_cs is None else rope_cs.numel() // cache.head_dim
-    check("gb_kv_append", lib().gb_kv_append(cache.ref, batch.ref, dt, _ptr(q), ldq, nh, _ptr(q_out), ldqo, _ptr(k),
-                                             k.stride(0), _ptr(v), v.stride(0), _ptr(rope_cs), rope_len,
-                                             _stream(stream)))
+        dq, wq = _rows("gb_kv_append", n, q, q_out)
+        if dq != dt or wq % hd:
+            raise GBError("gb_kv_append", GB_EINVAL)
+        pq, pqo, ldq, ldqo, nh = q.data_ptr(), q_out.data_ptr(), q.stride(0), q_out.stride(0), wq // hd
+    pcs, rope_len = (None, 0) if rope_cs is None else (rope_cs.data_ptr(), rope_cs.numel() // hd)
+    rc = lib().gb_kv_append(cache.ref, batch.ref, dt, pq, ldq, nh, pqo, ldqo, k.data_ptr(), k.stride(0), v.data_ptr(),
+                            v.stride(0), pcs, rope_len, _stream(stream))
+    if rc:
+        raise GBError("gb_kv_append", rc)
 
 
 def kv_read(cache, batch, k, v, stream=None) -> None:
     """The cache's values at the batch's tokens, into k and v rows."""
-    dt = _rows("gb_kv_read", batch.n_tokens, k, v)
-    if k.shape[1] != cache.n_kv_heads * cache.head_dim:
+    dt, width = _rows("gb_kv_read", batch.n_tokens, k, v)
+    if width != cache.n_kv_heads * cache.head_dim:
         raise GBError("gb_kv_read", GB_EINVAL)
-    check("gb_kv_read", lib().gb_kv_read(cache.ref, batch.ref, dt, _ptr(k), k.stride(0), _ptr(v), v.stride(0),
-                                         _stream(stream)))
+    rc = lib().gb_kv_read(cache.ref, batch.ref, dt, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                          _stream(stream))
+    if rc:
+        raise GBError("gb_kv_read", rc)
 
 
 def paged_workspace_bytes(n_heads, n_kv_heads, head_dim, n_seq) -> int:
     return int(lib().gb_paged_workspace_bytes(n_heads, n_kv_heads, head_dim, n_seq))
 
 
-def _paged_attention(name, cache, batch, q, out, ws, stream):
-    dt = _rows(name, batch.n_tokens, q, out)
+def _paged_attention(name, fn, cache, batch, q, out, ws, stream):
     hd = cache.head_dim
-    nh = q.shape[1] // hd
-    need = paged_workspace_bytes(nh, cache.n_kv_heads, hd, batch.n_seq)
-    if q.shape[1] % hd or ws.numel() * ws.element_size() < need:
-        raise GBError(name, GB_ESIZE if q.shape[1] % hd == 0 else GB_EINVAL)
-    check(name, getattr(lib(), name)(cache.ref, batch.ref, dt, _ptr(q), q.stride(0), nh, _ptr(out), out.stride(0),
-                                     _ptr(ws), _stream(stream)))
+    dt, width = _rows(name, batch.n_tokens, q, out)
+    nh = width // hd
+    key = (nh, cache.n_kv_heads, hd)
+    need = batch._ws_need.get(key)
+    if need is None:   # (0 for a head layout that the call itself refuses)
+        need = batch._ws_need[key] = paged_workspace_bytes(nh, cache.n_kv_heads, hd, batch.n_seq)
+    if width % hd:
+        raise GBError(name, GB_EINVAL)
+    if ws.nbytes < need:
+        raise GBError(name, GB_ESIZE)
+    rc = fn(cache.ref, batch.ref, dt, q.data_ptr(), q.stride(0), nh, out.data_ptr(), out.stride(0), ws.data_ptr(),
+            _stream(stream))
+    if rc:
+        raise GBError(name, rc)
 
 
 def paged_attention_decode(cache, batch, q, out, ws, stream=None) -> None:
     """Attention of one new token per sequence over its cached rows."""
-    _paged_attention("gb_paged_attention_decode", cache, batch, q, out, ws, stream)
+    _paged_attention("gb_paged_attention_decode", lib().gb_paged_attention_decode, cache, batch, q, out, ws, stream)
 
 
 def paged_attention_prefill(cache, batch, q, out, ws, stream=None) -> None:
     """Causal attention of packed prompts (cu_seqlens) over their cached rows."""
-    _paged_attention("gb_paged_attention_prefill", cache, batch, q, out, ws, stream)
+    _paged_attention("gb_paged_attention_prefill", lib().gb_paged_attention_prefill, cache, batch, q, out, ws, stream)
 
 
 def paged_error(clear=False) -> int:
@@ -382,16 +399,21 @@ def sample(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=None,
     """Draw out[r] (int32) from logits[r] (fp32 rows) with u[r] in [0, 1);
     temperature / top_k / top_p / min_p: per-row device tensors or None."""
     import torch
-    n = logits.shape[0]
-    if (logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1 or out.dtype != torch.int32
-            or (top_k is not None and top_k.dtype != torch.int32)):
+    f32, i32 = torch.float32, torch.int32
+    shape = logits.shape
+    if len(shape) != 2 or logits.dtype is not f32 or logits.stride(1) != 1:
         raise GBError("gb_sample", GB_EINVAL)
-    for t in (out, u, temperature, top_k, top_p, min_p):
-        if t is not None and (t.numel() < n or not t.is_contiguous()
-                              or (t is not out and t is not top_k and t.dtype != torch.float32)):
+    n, ptr = shape[0], []
+    for t, dt in ((temperature, f32), (top_k, i32), (top_p, f32), (min_p, f32), (u, f32), (out, i32)):
+        if t is None and len(ptr) < 4:   # u and out are needed
+            ptr.append(None)
+            continue
+        if t is None or t.dtype is not dt or t.numel() < n or not t.is_contiguous():
             raise GBError("gb_sample", GB_EINVAL)
-    check("gb_sample", lib().gb_sample(_ptr(logits), logits.stride(0), n, logits.shape[1], _ptr(temperature),
-                                       _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(u), _ptr(out), _stream(stream)))
+        ptr.append(t.data_ptr())
+    rc = lib().gb_sample(logits.data_ptr(), logits.stride(0), n, shape[1], *ptr, _stream(stream))
+    if rc:
+        raise GBError("gb_sample", rc)
 
 
 def rmsnorm(x, w, out, n, eps, stream=None) -> None:

@@ -8,13 +8,24 @@
 // a s + b c, no contraction).
 #include "gb_paged.cuh"
 
+#include <atomic>
+
 namespace gb {
 
 __device__ unsigned g_paged_err;
 
 unsigned* paged_err() {
-    void* p = nullptr;
-    return cudaGetSymbolAddress(&p, g_paged_err) == cudaSuccess ? static_cast<unsigned*>(p) : nullptr;
+    static std::atomic<unsigned*> at[64];   // per device, looked up once
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    unsigned* e = at[dev].load(std::memory_order_acquire);
+    if (!e) {
+        void* p = nullptr;
+        if (cudaGetSymbolAddress(&p, g_paged_err) != cudaSuccess) return nullptr;
+        e = static_cast<unsigned*>(p);
+        at[dev].store(e, std::memory_order_release);
+    }
+    return e;
 }
 
 int paged_views(const gb_kv_cache* c, const gb_kv_batch* b, PagedView* pv, BatchView* bv) {

@@ -10,6 +10,8 @@
 #include "gb_paged.cuh"
 #include "gb_tc.cuh"
 
+#include <type_traits>
+
 namespace gb {
 
 constexpr int PR_WARPS = 4;
@@ -69,14 +71,15 @@ k_paged_attn_rows(const PagedView c, const BatchView b, const A* __restrict__ q,
 }
 
 // ---------------------------------------------------------------- single tokens
-// S = Q K^T and O = P V on mma.sync m16n8k16 (fp16 operands, fp32 sums): the
-// 16 rows of the A operand are 8 query heads of one KV head twice, the high
-// halves (11 bits) of their values in rows 0-7 and the remainders in rows
-// 8-15, so that the padding a group of 8 leaves carries fp32 precision for
-// free: the two halves of a C fragment are in one thread and are added.  K
-// and V enter exactly: halves as they are, Q8_0 codes as whole numbers in
-// fp16, their scales applied to the sums of 32 columns (K) or to the
-// probabilities of that column block (V).
+// S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16 (fp16 operands, fp32
+// sums): keys, then output columns, are the 16 rows, the 8 query heads of one
+// KV head the 8 columns.  fp32 precision: q and the probabilities are split
+// into an fp16 value and an fp16 remainder, a product each.  K and V enter
+// exactly: halves as they are, Q8_0 codes as whole numbers in fp16, their
+// scales applied to the sums of 32 columns (K) or to the probabilities of that
+// column block (V).  The probabilities leave the first product as (key, 2
+// heads) pairs and enter the second as (2 keys, head) pairs: an 8 x 8
+// transposition in registers (movmatrix).
 //
 // Work: a step is 16 keys of one (sequence, KV head, 8 query heads); all
 // steps of the batch, in that order, are cut into one equal run per CTA
@@ -87,12 +90,14 @@ k_paged_attn_rows(const PagedView c, const BatchView b, const A* __restrict__ q,
 // partial per CTA; the last of them to arrive joins them in CTA order.
 //
 // The running maximum m moves only when a score exceeds it by more than
-// PD_TAU (log2 units); p = 2^(x - m + PD_LIFT) keeps the fp16 parts of small
-// probabilities normal.  Q8_0: p times a scale is brought below 2^14 by a
-// power of two, 2^-E, shared by the warp; O is in units of 2^E.
+// PD_TAU (log2 units), so a step needs no reduction but one vote; p = 2^(x - m
+// + PD_LIFT) keeps the fp16 parts of small probabilities normal.  Q8_0: p
+// times a scale is brought below 2^14 by a power of two, 2^-E, shared by the
+// warp; O is in units of 2^E.
 constexpr int PD_W = 4;              // warps
 constexpr int PD_MAX_CTAS = 4;       // CTAs per SM the workspace has room for
 constexpr int PD_MIN_STEPS = 4;      // fewest steps of a CTA
+constexpr int PD_MC = 16;            // partials of a join in flight
 constexpr int PD_HEADS = 8;          // query heads of a segment
 constexpr float PD_TAU = 8.f, PD_LIFT = 6.f;
 
@@ -102,21 +107,29 @@ struct PdCfg {
     static constexpr int KB = 16 * HD * (Q8 ? 1 : 2);   // bytes of a step's K (or V) rows
     static constexpr int SB = Q8 ? HD : 0;              // and of their scales
     static constexpr int STAGE = 2 * (KB + SB);
-    static constexpr int NST = Q8 ? 5 : (HD == 128 ? 3 : 5);
+    static constexpr int NST = 3;
     static constexpr int OP = HD + 4;                   // row pitch of the meeting area (bank spread)
     static constexpr int MEET = PD_W * PD_HEADS * OP * 4 + PD_W * PD_HEADS * 8;
     static constexpr int SMEM = PD_W * NST * STAGE + MEET;
 };
 
+// CTAs per SM: what the shared memory holds, at most PD_MAX_CTAS (registers follow).
+template <int HD, int DT>
+constexpr int pd_ctas() {
+    return (227 * 1024) / (PdCfg<HD, DT>::SMEM + 2048) < PD_MAX_CTAS ? (227 * 1024) / (PdCfg<HD, DT>::SMEM + 2048)
+                                                                     : PD_MAX_CTAS;
+}
+
 __device__ __forceinline__ void pd_cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void pd_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void pd_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // x, y as fp16 pairs: the rounded values and what the rounding left.
 __device__ __forceinline__ void pd_split(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -125,6 +138,25 @@ __device__ __forceinline__ void pd_split(float x, float y, uint32_t& hi, uint32_
     const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&r);
+}
+// A pair of values as operands: split for fp32 activations; for fp16 ones
+// rounded to fp16 without a remainder (q is fp16 already; for a probability
+// the error is of the size of the output's own rounding, 2.9e-4 against
+// 2.1e-4 of the 64-bit result together).
+template <typename A>
+__device__ __forceinline__ void pd_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+    if (sizeof(A) == 4) {
+        pd_split(x, y, hi, lo);
+    } else {
+        const __half2 h = __floats2half2_rn(x, y);
+        hi = *reinterpret_cast<const uint32_t*>(&h);
+        lo = 0u;
+    }
+}
+__device__ __forceinline__ uint32_t pd_transpose(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 // Bytes {lo, hi} of w (each 128 more than a code) as a pair of halves: placed
 // in the mantissa of 1024, 1152 taken off (exact).
@@ -163,7 +195,7 @@ __device__ __forceinline__ int pd_col(int p) {
 }
 
 template <typename A, int HD, int DT>
-__global__ void __launch_bounds__(PD_W * 32)
+__global__ void __launch_bounds__(PD_W * 32, (pd_ctas<HD, DT>()))
 k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, int ldq, int group, int n_hg,
                A* __restrict__ out, int ldo, unsigned* __restrict__ tickets, float* __restrict__ part, int min_steps,
                unsigned* err) {
@@ -201,9 +233,9 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
     for (int s = blockIdx.x; s < b.n_seq; s += gridDim.x)
         if (seq_len(b, s, err) == 0)
             for (int i = tid; i < c.n_kv * group * HD; i += PD_W * 32) out[(size_t)s * ldo + i] = (A)0.f;
-    const unsigned long long G = min((unsigned long long)gridDim.x, max(1ull, T / min_steps));
-    if (blockIdx.x >= G || T == 0) return;
-    const unsigned long long a0 = blockIdx.x * T / G, a1 = (blockIdx.x + 1) * T / G;
+    const unsigned long long run = max((T + gridDim.x - 1) / gridDim.x, (unsigned long long)min_steps);
+    const unsigned long long a0 = blockIdx.x * run, a1 = min(a0 + run, T);
+    if (a0 >= T) return;
     {
         unsigned long long at = (base + incl - mine) * H;   // first step of sequence s_lo
         for (int s = s_lo; s < s_hi; s++) {
@@ -259,13 +291,14 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
                                 vs + ((kk >> 1) * 8 + (kk & 1)) * HD * 2 + j * 128);
             } else {   // rows as they lie, 32-byte units exchanged so that the reads below spread over the banks
                 constexpr int CPR = HD / 16;   // 16-byte runs per row
+                const uint8_t* ks = c.k + off + row * HD + lane * 16;
+                const uint8_t* vs = c.v + off + row * HD + lane * 16;
 #pragma unroll
                 for (int i = 0; i < 16 * CPR / 32; i++) {
-                    const int r = (i * 32 + lane) / CPR, ch = (i * 32 + lane) % CPR;
+                    const int r = i * (32 / CPR) + lane / CPR, ch = lane % CPR;
                     const int fk = HD == 128 ? (r & 3) : ((r >> 1) & 1), fv = HD == 128 ? ((r >> 1) & 3) : ((r >> 1) & 1);
-                    const size_t src = off + (size_t)(row + r) * HD + ch * 16;
-                    pd_cp16(dst + r * HD + ((ch ^ (2 * fk)) * 16), c.k + src);
-                    pd_cp16(dst + C::KB + r * HD + ((ch ^ (2 * fv)) * 16), c.v + src);
+                    pd_cp16(dst + r * HD + ((ch ^ (2 * fk)) * 16), ks + i * 512);
+                    pd_cp16(dst + C::KB + r * HD + ((ch ^ (2 * fv)) * 16), vs + i * 512);
                 }
                 if (lane < 2 * (HD / 16)) {   // scales: 16 rows of HD / 32 halves
                     const int ch = lane % (HD / 16);
@@ -292,16 +325,18 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
         const int kvh = seg.h / n_hg, hg = seg.h % n_hg;
         const int n_heads = min(PD_HEADS, group - hg * PD_HEADS);
         const int len = seq_len(b, seg.s, err);
-        float m = -INFINITY, l = 0.f, O[NT][4];
+        // state of heads 2 t, 2 t + 1; O: tile pair u's columns 16 u + g, 16 u + 8 + g (fragment order)
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, thr[2] = {-INFINITY, -INFINITY}, O[NT / 2][4];
         int E = -40;
+        __half top = __float2half_rn(0.f);   // 2^E, the scales' bound (0 before the first step)
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT / 2; n++)
 #pragma unroll
             for (int i = 0; i < 4; i++) O[n][i] = 0.f;
         if (next < done + seg_n) {
             // ---- q of head g: columns 32 j + 8 t .. + 7, scaled by a power of two and split
-            uint32_t qa[2 * NB][4];
-            float sc;
+            uint32_t qh[2 * NB][2], ql[2 * NB][2];
+            float sc[2], isc[2];   // raw score -> log2 units of heads 2 t, 2 t + 1, and back
             {
                 float x[NB][8], mx = 0.f;
                 const A* src = q + (size_t)seg.s * ldq + (size_t)(kvh * group + hg * PD_HEADS + g) * HD + 8 * t;
@@ -317,121 +352,149 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const int e = tc::f16_scale_exp(__float_as_uint(mx));
                 const float up = tc::pow2f(e);
-                sc = scale2 * tc::pow2f(-e);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int eh = __shfl_sync(0xffffffffu, e, 4 * (2 * t + i));
+                    sc[i] = scale2 * tc::pow2f(-eh);
+                    isc[i] = (1.0f / scale2) * tc::pow2f(eh);
+                }
 #pragma unroll
                 for (int j = 0; j < NB; j++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        pd_split(x[j][2 * i] * up, x[j][2 * i + 1] * up, qa[2 * j + (i >> 1)][2 * (i & 1)],
-                                 qa[2 * j + (i >> 1)][2 * (i & 1) + 1]);
+                        pd_pair<A>(x[j][2 * i] * up, x[j][2 * i + 1] * up, qh[2 * j + (i >> 1)][i & 1],
+                                   ql[2 * j + (i >> 1)][i & 1]);
             }
-            for (; next < done + seg_n; next += PD_W) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(C::NST - 2) : "memory");
-                __syncwarp();
-                issue(slot == 0 ? C::NST - 1 : slot - 1);
-                const uint8_t* st = ring_p + slot * C::STAGE;
-                slot = slot + 1 == C::NST ? 0 : slot + 1;
-                const int k0 = (seg.st + next - done) << 4;
-                // ---- scores of keys k0 + 8 i + 2 t, + 1
-                float x[4];
+            // One step; TAIL: only `left` of its keys belong to the sequence.
+            auto step = [&](const uint8_t* st, auto tail, int left) {
+                constexpr bool TAIL = decltype(tail)::value;
+                // ---- raw scores x[i][h] of keys g + 8 i, heads 2 t + h
+                float x[2][2];
+                if (!C::Q8) {
+                    float sa[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    if (!C::Q8) {
-                        float sa[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int j = 0; j < NB; j++) {
-                            const uint4 kk = *reinterpret_cast<const uint4*>(st + (i * NB + j) * 512 + lane * 16);
-                            pd_mma(sa, qa[2 * j], kk.x, kk.y);
-                            pd_mma(sa, qa[2 * j + 1], kk.z, kk.w);
-                        }
-                        x[2 * i] = sa[0] + sa[2];
-                        x[2 * i + 1] = sa[1] + sa[3];
-                    } else {
-                        const int r = 8 * i + g;
-                        const int f = HD == 128 ? (r & 3) : ((r >> 1) & 1);
-                        x[2 * i] = x[2 * i + 1] = 0.f;
-                        __half sk[2][NB];   // scales of keys 8 i + 2 t, + 1
-                        const uint8_t* sp = st + 2 * C::KB + (8 * i + 2 * t) * (HD / 16);
-                        if (HD == 128) *reinterpret_cast<uint4*>(&sk[0][0]) = *reinterpret_cast<const uint4*>(sp);
-                        else *reinterpret_cast<uint2*>(&sk[0][0]) = *reinterpret_cast<const uint2*>(sp);
-#pragma unroll
-                        for (int j = 0; j < NB; j++) {
-                            uint2 w = *reinterpret_cast<const uint2*>(st + r * HD + ((j ^ f) * 32) + 8 * t);
-                            w.x ^= 0x80808080u;
-                            w.y ^= 0x80808080u;
-                            float sa[4] = {0.f, 0.f, 0.f, 0.f};
-                            pd_mma(sa, qa[2 * j], pd_codes(w.x, 0x4140), pd_codes(w.x, 0x4342));
-                            pd_mma(sa, qa[2 * j + 1], pd_codes(w.y, 0x4140), pd_codes(w.y, 0x4342));
-                            x[2 * i] = fmaf(sa[0] + sa[2], __half2float(sk[0][j]), x[2 * i]);
-                            x[2 * i + 1] = fmaf(sa[1] + sa[3], __half2float(sk[1][j]), x[2 * i + 1]);
+                    for (int j = 0; j < NB; j++) {
+                        const uint4 k0 = *reinterpret_cast<const uint4*>(st + j * 512 + lane * 16);
+                        const uint4 k1 = *reinterpret_cast<const uint4*>(st + (NB + j) * 512 + lane * 16);
+                        pd_mma(sa, k0.x, k1.x, k0.y, k1.y, qh[2 * j][0], qh[2 * j][1]);
+                        pd_mma(sa, k0.z, k1.z, k0.w, k1.w, qh[2 * j + 1][0], qh[2 * j + 1][1]);
+                        if (sizeof(A) == 4) {
+                            pd_mma(sa, k0.x, k1.x, k0.y, k1.y, ql[2 * j][0], ql[2 * j][1]);
+                            pd_mma(sa, k0.z, k1.z, k0.w, k1.w, ql[2 * j + 1][0], ql[2 * j + 1][1]);
                         }
                     }
-                }
-                // ---- running softmax (base 2); keys past the sequence weigh nothing
-                const int left = len - k0;   // valid keys of the step, at least 1
-                float mx = -INFINITY;
+                    x[0][0] = sa[0]; x[0][1] = sa[1]; x[1][0] = sa[2]; x[1][1] = sa[3];
+                } else {
+                    const int f = HD == 128 ? (g & 3) : ((g >> 1) & 1);   // the same for row g + 8
+                    __half sk[2][NB];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int key = (i >> 1) * 8 + 2 * t + (i & 1);
-                    x[i] = key < left ? x[i] * sc : -INFINITY;
-                    mx = fmaxf(mx, x[i]);
-                }
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                float alpha = 1.f;
-                if (mx > m + PD_TAU || m == -INFINITY) {
-                    alpha = pd_ex2(m - mx);
-                    if (m == -INFINITY) alpha = 0.f;
-                    m = mx;
-                }
-                float p[4];
-                const float ml = m - PD_LIFT;
-                l *= alpha;
+                    for (int i = 0; i < 2; i++) {
+                        x[i][0] = x[i][1] = 0.f;
+                        const uint8_t* sp = st + 2 * C::KB + (8 * i + g) * (HD / 16);
+                        if (HD == 128) *reinterpret_cast<uint2*>(&sk[i][0]) = *reinterpret_cast<const uint2*>(sp);
+                        else *reinterpret_cast<uint32_t*>(&sk[i][0]) = *reinterpret_cast<const uint32_t*>(sp);
+                    }
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    p[i] = pd_ex2(x[i] - ml);
-                    l += p[i];
+                    for (int j = 0; j < NB; j++) {
+                        uint2 w0 = *reinterpret_cast<const uint2*>(st + g * HD + ((j ^ f) * 32) + 8 * t);
+                        uint2 w1 = *reinterpret_cast<const uint2*>(st + (g + 8) * HD + ((j ^ f) * 32) + 8 * t);
+                        w0.x ^= 0x80808080u; w0.y ^= 0x80808080u; w1.x ^= 0x80808080u; w1.y ^= 0x80808080u;
+                        const uint32_t a0 = pd_codes(w0.x, 0x4140), a1 = pd_codes(w1.x, 0x4140);
+                        const uint32_t a2 = pd_codes(w0.x, 0x4342), a3 = pd_codes(w1.x, 0x4342);
+                        const uint32_t c0 = pd_codes(w0.y, 0x4140), c1 = pd_codes(w1.y, 0x4140);
+                        const uint32_t c2 = pd_codes(w0.y, 0x4342), c3 = pd_codes(w1.y, 0x4342);
+                        float sa[4] = {0.f, 0.f, 0.f, 0.f};
+                        pd_mma(sa, a0, a1, a2, a3, qh[2 * j][0], qh[2 * j][1]);
+                        pd_mma(sa, c0, c1, c2, c3, qh[2 * j + 1][0], qh[2 * j + 1][1]);
+                        if (sizeof(A) == 4) {
+                            pd_mma(sa, a0, a1, a2, a3, ql[2 * j][0], ql[2 * j][1]);
+                            pd_mma(sa, c0, c1, c2, c3, ql[2 * j + 1][0], ql[2 * j + 1][1]);
+                        }
+                        const float d0 = __half2float(sk[0][j]), d1 = __half2float(sk[1][j]);
+                        x[0][0] = fmaf(sa[0], d0, x[0][0]);
+                        x[0][1] = fmaf(sa[1], d0, x[0][1]);
+                        x[1][0] = fmaf(sa[2], d1, x[1][0]);
+                        x[1][1] = fmaf(sa[3], d1, x[1][1]);
+                    }
                 }
-                // ---- Q8_0: the V scales of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-                __half sv[4][NB];
+                // ---- the V scales of keys g, g + 8; keys past the sequence weigh nothing
+                __half sv[2][NB];
                 if (C::Q8) {
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        const uint8_t* sp = st + 2 * C::KB + C::SB + (8 * i + 2 * t) * (HD / 16);
-                        if (HD == 128) *reinterpret_cast<uint4*>(&sv[2 * i][0]) = *reinterpret_cast<const uint4*>(sp);
-                        else *reinterpret_cast<uint2*>(&sv[2 * i][0]) = *reinterpret_cast<const uint2*>(sp);
-                    }
-                    if (left < 16) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int j = 0; j < NB; j++)
-                                if ((i >> 1) * 8 + 2 * t + (i & 1) >= left) sv[i][j] = __float2half_rn(0.f);
-                    }
-                    float top = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int j = 0; j < NB; j++) top = fmaxf(top, __half2float(sv[i][j]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const int e = (int)(__float_as_uint(top) >> 23) - 126;   // top < 2^e
-                    if (e > E) {
-                        alpha *= tc::pow2f(max(E - e, -126));
-                        E = e;
+                        const uint8_t* sp = st + 2 * C::KB + C::SB + (8 * i + g) * (HD / 16);
+                        if (HD == 128) *reinterpret_cast<uint2*>(&sv[i][0]) = *reinterpret_cast<const uint2*>(sp);
+                        else *reinterpret_cast<uint32_t*>(&sv[i][0]) = *reinterpret_cast<const uint32_t*>(sp);
                     }
                 }
-                if (__any_sync(0xffffffffu, alpha != 1.f)) {
+                if (TAIL) {
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+                    for (int i = 0; i < 2; i++)
+                        if (8 * i + g >= left) {
+                            x[i][0] = x[i][1] = -INFINITY;
+                            if (C::Q8)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) O[n][i] *= alpha;
+                                for (int j = 0; j < NB; j++) sv[i][j] = __float2half_rn(0.f);
+                        }
                 }
-                // ---- O += P V
+                // ---- does a score pass the maximum by PD_TAU, or a scale its bound?
+                bool moved = fmaxf(x[0][0], x[1][0]) > thr[0] || fmaxf(x[0][1], x[1][1]) > thr[1];
+                __half dm = __float2half_rn(0.f);
+                if (C::Q8) {
+                    const __half2* d2 = reinterpret_cast<const __half2*>(&sv[0][0]);
+                    __half2 y = d2[0];
+#pragma unroll
+                    for (int j = 1; j < NB; j++) y = __hmax2(y, d2[j]);
+                    dm = __hmax(__low2half(y), __high2half(y));
+                    moved |= __hgt(dm, top);
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+                    float up = 1.f;
+                    if (C::Q8) {
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) dm = __hmax(dm, __shfl_xor_sync(0xffffffffu, dm, o));
+                        const int e = (int)(__float_as_uint(__half2float(dm)) >> 23) - 126;   // dm < 2^e
+                        if (e > E) {
+                            up = tc::pow2f(max(E - e, -126));
+                            E = e;
+                            top = e > 15 ? __float2half_rn(65504.f) : __float2half_rn(tc::pow2f(e));
+                        }
+                    }
+                    float al[2];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float mx = fmaxf(x[0][h], x[1][h]);
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        const float mn = fmaxf(m[h], mx * sc[h]);
+                        al[h] = m[h] == -INFINITY ? 0.f : pd_ex2(m[h] - mn);
+                        l[h] *= al[h];
+                        m[h] = mn;
+                        thr[h] = (mn + PD_TAU) * isc[h];
+                        al[h] *= up;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT / 2; n++) {
+                        O[n][0] *= al[0]; O[n][1] *= al[1]; O[n][2] *= al[0]; O[n][3] *= al[1];
+                    }
+                }
+                float p[2][2];
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        p[i][h] = pd_ex2(fmaf(x[i][h], sc[h], PD_LIFT - m[h]));
+                        l[h] += p[i][h];
+                    }
+                // ---- O^T += V^T P^T
                 if (!C::Q8) {
-                    uint32_t pa[4];
-                    pd_split(p[0], p[1], pa[0], pa[1]);
-                    pd_split(p[2], p[3], pa[2], pa[3]);
+                    uint32_t bh[2], bl[2];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        pd_pair<A>(p[i][0], p[i][1], bh[i], bl[i]);
+                        bh[i] = pd_transpose(bh[i]);
+                        if (sizeof(A) == 4) bl[i] = pd_transpose(bl[i]);
+                    }
 #pragma unroll
                     for (int j = 0; j < HD / 64; j++) {
                         uint32_t v[4][4];
@@ -439,57 +502,83 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
                         for (int kk = 0; kk < 4; kk++) {
                             const uint4 w =
                                 *reinterpret_cast<const uint4*>(st + C::KB + (kk * (HD / 64) + j) * 512 + lane * 16);
-                            const bool in = (kk >> 1) * 8 + 2 * t + (kk & 1) < left;   // stale rows may hold anything
-                            v[kk][0] = in ? w.x : 0u;
-                            v[kk][1] = in ? w.y : 0u;
-                            v[kk][2] = in ? w.z : 0u;
-                            v[kk][3] = in ? w.w : 0u;
+                            v[kk][0] = w.x;
+                            v[kk][1] = w.y;
+                            v[kk][2] = w.z;
+                            v[kk][3] = w.w;
+                            if (TAIL && (kk >> 1) * 8 + 2 * t + (kk & 1) >= left)   // stale rows may hold anything
+                                v[kk][0] = v[kk][1] = v[kk][2] = v[kk][3] = 0u;
                         }
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const uint32_t sel = (e & 1) ? 0x7632 : 0x5410;
-                            pd_mma(O[j * 8 + e], pa, __byte_perm(v[0][e >> 1], v[1][e >> 1], sel),
-                                   __byte_perm(v[2][e >> 1], v[3][e >> 1], sel));
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t a0 = __byte_perm(v[0][e], v[1][e], 0x5410), a1 = __byte_perm(v[0][e], v[1][e], 0x7632);
+                            const uint32_t a2 = __byte_perm(v[2][e], v[3][e], 0x5410), a3 = __byte_perm(v[2][e], v[3][e], 0x7632);
+                            pd_mma(O[j * 4 + e], a0, a1, a2, a3, bh[0], bh[1]);
+                            if (sizeof(A) == 4) pd_mma(O[j * 4 + e], a0, a1, a2, a3, bl[0], bl[1]);
                         }
                     }
                 } else {
                     const float down = tc::pow2f(-E);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) p[i] *= down;
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) p[i][h] *= down;
 #pragma unroll
                     for (int j = 0; j < NB; j++) {
-                        uint32_t pa[4], w[4];
-                        pd_split(p[0] * __half2float(sv[0][j]), p[1] * __half2float(sv[1][j]), pa[0], pa[1]);
-                        pd_split(p[2] * __half2float(sv[2][j]), p[3] * __half2float(sv[3][j]), pa[2], pa[3]);
+                        uint32_t bh[2], bl[2], w[4];
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const float d = __half2float(sv[i][j]);
+                            pd_pair<A>(p[i][0] * d, p[i][1] * d, bh[i], bl[i]);
+                            bh[i] = pd_transpose(bh[i]);
+                            if (sizeof(A) == 4) bl[i] = pd_transpose(bl[i]);
+                        }
 #pragma unroll
                         for (int kk = 0; kk < 4; kk++) {
                             const int r = (kk >> 1) * 8 + 2 * t + (kk & 1);
-                            const int f = HD == 128 ? ((r >> 1) & 3) : ((r >> 1) & 1);
+                            const int f = HD == 128 ? t : (t & 1);   // (r >> 1) & 3, & 1
                             w[kk] = *reinterpret_cast<const uint32_t*>(st + C::KB + r * HD + ((j ^ f) * 32) + 4 * g) ^
                                     0x80808080u;
                         }
 #pragma unroll
-                        for (int e2 = 0; e2 < 2; e2++) {   // bytes 2 e2, 2 e2 + 1 of the keys' words
-                            const uint32_t lo = __byte_perm(w[0], w[1], e2 ? 0x7362 : 0x5140);
-                            const uint32_t hi = __byte_perm(w[2], w[3], e2 ? 0x7362 : 0x5140);
-                            pd_mma(O[j * 4 + 2 * e2], pa, pd_codes(lo, 0x4140), pd_codes(hi, 0x4140));
-                            pd_mma(O[j * 4 + 2 * e2 + 1], pa, pd_codes(lo, 0x4342), pd_codes(hi, 0x4342));
+                        for (int e = 0; e < 2; e++) {   // bytes 2 e, 2 e + 1 of the keys' words
+                            const uint32_t lo = __byte_perm(w[0], w[1], e ? 0x7362 : 0x5140);
+                            const uint32_t hi = __byte_perm(w[2], w[3], e ? 0x7362 : 0x5140);
+                            const uint32_t a0 = pd_codes(lo, 0x4140), a1 = pd_codes(lo, 0x4342);
+                            const uint32_t a2 = pd_codes(hi, 0x4140), a3 = pd_codes(hi, 0x4342);
+                            pd_mma(O[j * 2 + e], a0, a1, a2, a3, bh[0], bh[1]);
+                            if (sizeof(A) == 4) pd_mma(O[j * 2 + e], a0, a1, a2, a3, bl[0], bl[1]);
                         }
                     }
                 }
+            };
+            for (; next < done + seg_n; next += PD_W) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(C::NST - 2) : "memory");
+                __syncwarp();
+                issue(slot == 0 ? C::NST - 1 : slot - 1);
+                const uint8_t* st = ring_p + slot * C::STAGE;
+                slot = slot + 1 == C::NST ? 0 : slot + 1;
+                const int left = len - ((seg.st + next - done) << 4);   // at least 1
+                if (left >= 16) step(st, std::false_type{}, 16);
+                else step(st, std::true_type{}, left);
             }
         }
         // ---- the warps meet
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
         {
-            const float u = C::Q8 ? tc::pow2f(max(E, -126)) : 1.f;
-            if (t == 0) meet_ml[warp * PD_HEADS + g] = make_float2(m, l);
-            float* row = meet + (warp * PD_HEADS + g) * C::OP + 2 * t;
-            if (g < n_heads)
+            const float u = C::Q8 ? tc::pow2f(E) : 1.f;
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-                    *reinterpret_cast<float2*>(row + 8 * n) = make_float2((O[n][0] + O[n][2]) * u, (O[n][1] + O[n][3]) * u);
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
+                if (g == 0) meet_ml[warp * PD_HEADS + 2 * t + h] = make_float2(m[h], l[h]);
+                float* row = meet + (warp * PD_HEADS + 2 * t + h) * C::OP + g;
+                if (2 * t + h < n_heads)
+#pragma unroll
+                    for (int n = 0; n < NT / 2; n++) {
+                        row[16 * n] = O[n][h] * u;
+                        row[16 * n + 8] = O[n][2 + h] * u;
+                    }
+            }
         }
         __syncthreads();
         const unsigned long long gs = a0 + done - seg.st, ge = gs + seg.nst;   // the whole segment's steps
@@ -524,7 +613,7 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
         }
         if (!whole) {
             // the CTAs of the segment: those that hold its first and last step
-            const int c0 = (int)(((gs + 1) * G - 1) / T), c1 = (int)((ge * G - 1) / T);
+            const int c0 = (int)(gs / run), c1 = (int)((ge - 1) / run);
             __syncthreads();
             if (tid == 0) {
                 unsigned prev;
@@ -536,21 +625,42 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
             }
             __syncthreads();
             if (s_last) {
+                // thread: four neighbouring positions of a head, PD_MC partials in flight
                 constexpr size_t PS = 2 * PD_HEADS * (HD + 2);   // floats of a CTA's two partials
-                for (int i = tid; i < n_heads * seg_cols; i += PD_W * 32) {
+                for (int i = 4 * tid; i < n_heads * HD; i += 4 * PD_W * 32) {
                     const int h = i / HD, p = i % HD;
-                    float M = -INFINITY, L = 0.f, V = 0.f;
-                    for (int cc = c0; cc <= c1; cc++) {
-                        const float* pp = part + cc * PS + (cc == c0 ? PD_HEADS * (HD + 2) : 0);
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(pp) + h);
-                        const float v = __ldcg(pp + 2 * PD_HEADS + i);
-                        const float mn = fmaxf(M, ml.x);
-                        const float fa = M == -INFINITY ? 0.f : pd_ex2(M - mn), fb = pd_ex2(ml.x - mn);
-                        L = fmaf(L, fa, ml.y * fb);
-                        V = fmaf(V, fa, v * fb);
+                    float M = -INFINITY, L = 0.f;
+                    float4 V = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int cc = c0; cc <= c1; cc += PD_MC) {
+                        float2 ml[PD_MC];
+                        float4 v[PD_MC];
+                        float mn = M;
+#pragma unroll
+                        for (int u = 0; u < PD_MC; u++) {
+                            const float* pp = part + min(cc + u, c1) * PS + (cc + u == c0 ? PD_HEADS * (HD + 2) : 0);
+                            ml[u] = __ldcg(reinterpret_cast<const float2*>(pp) + h);
+                            v[u] = __ldcg(reinterpret_cast<const float4*>(pp + 2 * PD_HEADS + i));
+                        }
+#pragma unroll
+                        for (int u = 0; u < PD_MC; u++) {
+                            if (cc + u > c1) ml[u] = make_float2(-INFINITY, 0.f);
+                            mn = fmaxf(mn, ml[u].x);
+                        }
+                        const float fa = pd_ex2(M - mn);   // 0 before the first partial
                         M = mn;
+                        L *= fa;
+                        V = make_float4(V.x * fa, V.y * fa, V.z * fa, V.w * fa);
+#pragma unroll
+                        for (int u = 0; u < PD_MC; u++) {
+                            const float f = pd_ex2(ml[u].x - M);
+                            L = fmaf(ml[u].y, f, L);
+                            V = make_float4(fmaf(v[u].x, f, V.x), fmaf(v[u].y, f, V.y), fmaf(v[u].z, f, V.z),
+                                            fmaf(v[u].w, f, V.w));
+                        }
                     }
-                    out[o0 + (size_t)h * HD + pd_col<HD, DT>(p)] = (A)(V / L);
+                    const float inv = 1.0f / L, r[4] = {V.x * inv, V.y * inv, V.z * inv, V.w * inv};
+#pragma unroll
+                    for (int u = 0; u < 4; u++) out[o0 + (size_t)h * HD + pd_col<HD, DT>(p + u)] = (A)r[u];
                 }
                 if (tid == 0) tickets[(size_t)seg.s * H + seg.h] = 0u;   // every CTA has arrived
             }
