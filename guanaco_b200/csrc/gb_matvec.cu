@@ -34,6 +34,7 @@
 #include "gb_common.cuh"
 #include "gb_internal.h"
 #include "gb_mt.cuh"
+#include "gb_paged.cuh"
 #include "gb_tc.cuh"
 
 #include <cuda.h>
@@ -1183,6 +1184,18 @@ bool mt_encode_rows(void* map128, const void* W, int rows, int nb, int box_u64) 
     cuuint32_t es[3] = {1, 1, 1};
     return enc(reinterpret_cast<CUtensorMap*>(map128), CU_TENSOR_MAP_DATA_TYPE_UINT64, 3, const_cast<void*>(W), dims,
                strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool paged_encode(void* map128, const void* pool, int hd, int page_size, size_t slabs, int rows) {
+    auto enc = tensor_map_encoder();
+    if (!enc || slabs > 0xffffffffull) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)page_size, (cuuint64_t)slabs};
+    cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)page_size * hd * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)rows, 1};
+    cuuint32_t es[3] = {1, 1, 1};
+    return enc(reinterpret_cast<CUtensorMap*>(map128), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(pool), dims,
+               strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

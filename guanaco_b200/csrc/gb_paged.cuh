@@ -37,6 +37,19 @@ int paged_views(const gb_kv_cache* c, const gb_kv_batch* b, PagedView* pv, Batch
 inline bool paged_rows_ok(int dtype, const void* p, int ld, int width) {
     return p && !(reinterpret_cast<uintptr_t>(p) & 15) && ld >= width && ld % (dtype == GB_DT_F16 ? 8 : 4) == 0;
 }
+// Workspace of the attention entry points: partials (of the prompts' CTAs that
+// share a row block, only launched when all of them fit the SMs; or of the
+// single tokens' CTAs), then a ticket per row block, then one per (sequence,
+// KV head, 8 query heads).  Tickets are zero between calls, and never where a
+// call of another shape leaves partials.
+constexpr size_t PAGED_PART_BYTES = (size_t)GB_MAX_SMS * 2 * (128 + 2) * 128 * sizeof(float);
+constexpr size_t PAGED_TICKETS_AT = PAGED_PART_BYTES + GB_MAX_SMS * sizeof(unsigned);
+// Packed prompts (gb_paged_prefill.cu).
+int paged_prefill(const gb_kv_cache* cache, const PagedView& c, const BatchView& b, int dtype, const void* q, int ldq,
+                  int n_heads, void* out, int ldo, void* ws, unsigned* err, cudaStream_t st);
+// Tensor map of an F16 pool as {hd halves, page_size rows, slabs} with boxes
+// {64, rows, 1}, 128-byte swizzle (gb_matvec.cu, beside the other encoders).
+bool paged_encode(void* map128, const void* pool, int hd, int page_size, size_t slabs, int rows);
 unsigned* paged_err();   // the module's device error word (nullptr: CUDA error)
 
 // Sequence of token t: the largest s with cu[s] <= t (empty sequences share a

@@ -3,72 +3,14 @@
 //
 //   out[t][h] = sum_p softmax_p(q[t][h] . k[p] / sqrt(hd)) v[p],  p <= position of t
 //
-// A CTA takes one token and one KV head; its warps take the query heads of
-// the group.  A warp walks the keys, the lanes share a row's columns, and the
-// running maximum m and sum l of the softmax rescale the output by
-// exp(m_old - m).  A token without keys gets zeros.
+// This file: the single-token kernel and both entry points; the prompts' kernel
+// is gb_paged_prefill.cu.
 #include "gb_paged.cuh"
 #include "gb_tc.cuh"
 
 #include <type_traits>
 
 namespace gb {
-
-constexpr int PR_WARPS = 4;
-
-template <typename A, int HD, int DT>
-__global__ void __launch_bounds__(PR_WARPS * 32)
-k_paged_attn_rows(const PagedView c, const BatchView b, const A* __restrict__ q, int ldq, int group,
-                  A* __restrict__ out, int ldo, unsigned* err) {
-    constexpr int E = HD / 32;   // columns per lane
-    const int t = blockIdx.x, g = blockIdx.y, lane = threadIdx.x & 31;
-    const int s = seq_of(b, t);
-    if (s < 0) return;
-    const int end = b.cu ? __ldg(b.cu + s + 1) : t + 1;
-    const int n = seq_len(b, s, err) - (end - t) + 1;   // keys 0 .. n - 1
-    const float scale = 1.0f / sqrtf((float)HD);
-    for (int j = threadIdx.x >> 5; j < group; j += PR_WARPS) {
-        const int h = g * group + j;
-        float qv[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            qv[i] = (float)q[(size_t)t * ldq + (size_t)h * HD + i * 32 + lane];
-            o[i] = 0.f;
-        }
-        for (int p = 0; p < n; p++) {
-            const int page = page_of(c, b, s, p, err);
-            if (page < 0) continue;
-            const int row = p & ((1 << c.shift) - 1);
-            const size_t off = (size_t)page * c.page_bytes + (size_t)g * c.slab;
-            float d = 0.f, vv[E];
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                const size_t e = (size_t)row * HD + i * 32 + lane;
-                float kk;
-                if (DT == GB_DT_F16) {
-                    kk = __half2float(reinterpret_cast<const __half*>(c.k + off)[e]);
-                    vv[i] = __half2float(reinterpret_cast<const __half*>(c.v + off)[e]);
-                } else {
-                    const size_t so = off + ((size_t)HD << c.shift) + ((size_t)row * E + i) * 2;
-                    kk = __half2float(*reinterpret_cast<const __half*>(c.k + so)) * (float)(int8_t)c.k[off + e];
-                    vv[i] = __half2float(*reinterpret_cast<const __half*>(c.v + so)) * (float)(int8_t)c.v[off + e];
-                }
-                d = fmaf(qv[i], kk, d);
-            }
-            d = warp_sum(d) * scale;
-            const float mn = fmaxf(m, d);
-            const float a = expf(m - mn), pr = expf(d - mn);
-            l = fmaf(l, a, pr);
-            m = mn;
-#pragma unroll
-            for (int i = 0; i < E; i++) o[i] = fmaf(o[i], a, pr * vv[i]);
-        }
-        const float inv = l > 0.f ? 1.0f / l : 0.f;
-#pragma unroll
-        for (int i = 0; i < E; i++)
-            out[(size_t)t * ldo + (size_t)h * HD + i * 32 + lane] = (A)(o[i] * inv);
-    }
-}
 
 // ---------------------------------------------------------------- single tokens
 // S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16 (fp16 operands, fp32
@@ -672,9 +614,7 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Workspace: the decode CTAs' partials, then one ticket per (sequence, KV
-// head, 8 query heads), zero between calls.
-constexpr size_t PD_PART_BYTES = (size_t)GB_MAX_SMS * PD_MAX_CTAS * 2 * PD_HEADS * (128 + 2) * 4;
+static_assert((size_t)GB_MAX_SMS * PD_MAX_CTAS * 2 * PD_HEADS * (128 + 2) * 4 <= PAGED_PART_BYTES, "workspace");
 
 template <typename A, int HD, int DT>
 static cudaError_t launch_decode(const PagedView& c, const BatchView& b, const void* q, int ldq, int group, void* out,
@@ -689,7 +629,7 @@ static cudaError_t launch_decode(const PagedView& c, const BatchView& b, const v
         return n < 1 ? 1 : n > PD_MAX_CTAS ? PD_MAX_CTAS : n;
     }();
     const int n_hg = (group + PD_HEADS - 1) / PD_HEADS;
-    unsigned* tickets = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(ws) + PD_PART_BYTES);
+    unsigned* tickets = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(ws) + PAGED_TICKETS_AT);
     k_paged_decode<A, HD, DT><<<sm_count() * per_sm, PD_W * 32, C::SMEM, st>>>(
         c, b, static_cast<const A*>(q), ldq, group, n_hg, static_cast<A*>(out), ldo, tickets, static_cast<float*>(ws),
         PD_MIN_STEPS, err);
@@ -723,20 +663,7 @@ static int paged_attention(const gb_kv_cache* cache, const gb_kv_batch* batch, i
 #undef GB_DECODE
         return e == cudaSuccess ? GB_OK : GB_ECUDA;
     }
-    const dim3 grid(b.n_tokens, c.n_kv);
-#define GB_ROWS(A, HD, DT)                                                                                       \
-    k_paged_attn_rows<A, HD, DT><<<grid, PR_WARPS * 32, 0, st>>>(c, b, static_cast<const A*>(q), ldq, group,     \
-                                                                  static_cast<A*>(out), ldo, err)
-#define GB_ROWS_DT(A, HD) \
-    if (cache->dtype == GB_DT_F16) GB_ROWS(A, HD, GB_DT_F16); else GB_ROWS(A, HD, GB_DT_Q8_0)
-    if (dtype == GB_DT_F32) {
-        if (hd == 128) { GB_ROWS_DT(float, 128); } else { GB_ROWS_DT(float, 64); }
-    } else {
-        if (hd == 128) { GB_ROWS_DT(__half, 128); } else { GB_ROWS_DT(__half, 64); }
-    }
-#undef GB_ROWS_DT
-#undef GB_ROWS
-    return cudaGetLastError() == cudaSuccess ? GB_OK : GB_ECUDA;
+    return paged_prefill(cache, c, b, dtype, q, ldq, n_heads, out, ldo, ws, err, st);
 }
 
 }  // namespace gb
@@ -747,7 +674,7 @@ extern "C" size_t gb_paged_workspace_bytes(int n_heads, int n_kv_heads, int head
     if (n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) || n_seq < 0)
         return 0;
     const int group = n_heads / n_kv_heads, n_hg = (group + PD_HEADS - 1) / PD_HEADS;
-    return PD_PART_BYTES + ((size_t)n_seq * n_kv_heads * n_hg * sizeof(unsigned) + 15) / 16 * 16;
+    return PAGED_TICKETS_AT + ((size_t)n_seq * n_kv_heads * n_hg * sizeof(unsigned) + 15) / 16 * 16;
 }
 
 extern "C" int gb_paged_attention_decode(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q,

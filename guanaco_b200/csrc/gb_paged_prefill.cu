@@ -1,0 +1,606 @@
+// gb_paged_prefill.cu -- causal attention of packed prompts over the paged
+// KV cache, on the tcgen05 tensor cores.
+//
+// A CTA takes one KV head and 2 x 128 rows of one sequence: row = (query,
+// query head of the group), 128 / group queries a tile, so that a K / V tile
+// read from the cache serves every head that shares it.  Keys come in tiles of
+// NK.  For each of the two row tiles, alternately:
+//   S = Q K^T    A = Q, B = K, both K-major in shared memory (128-byte swizzle)
+//   softmax      one warpgroup per row tile, thread = row = tensor-memory lane:
+//                scale, causal mask, running maximum and sum; P = 2^(x - m)
+//                back into tensor memory over S
+//   O += P V     A = P from tensor memory, B = V as it lies in the cache (rows
+//                = keys, MN-major): V is never transposed
+// While one warpgroup computes its softmax the tensor cores work for the other.
+// The maximum moves only when a score exceeds it by more than PP_TAU (log2
+// units), so O in tensor memory is rarely rescaled.
+//
+// Precision.  fp16 activations: Q exact, P rounded to fp16, Q8_0 values rounded
+// to fp16 (each an error of the size of the fp16 output's own rounding).
+// fp32 activations: Q (scaled by a power of two per row) and P are split into
+// an fp16 value and an fp16 remainder, and so are Q8_0 values (code x scale
+// has 18 bits): hi.hi + lo.hi (+ hi.lo), fp32 sums.
+//
+// An F16 cache's tiles are TMA copies, one box per page and 64 columns; Q8_0
+// tiles are dequantised by four warps, a row per thread.  Rows past the last
+// key are zeroed in V (stale cache rows may hold anything).
+//
+// Few rows over a long axis: the host cuts the keys over gridDim.y CTAs, which
+// leave (m, l, O) partials; the last to arrive joins them in order.
+#include "gb_mt.cuh"
+#include "gb_paged.cuh"
+#include "gb_tc.cuh"
+
+#include <cuda.h>
+
+namespace gb {
+
+constexpr float PP_TAU = 8.f, PP_LIFT = 6.f;   // p <= 2^14; small p stay normal fp16 numbers
+constexpr int PP_SOFT = 256;                    // softmax threads: two warpgroups
+constexpr int PP_SMEM_MAX = 227 * 1024 - 1280;  // less alignment slack and static shared memory
+
+template <typename A, int HD, int DT>
+struct PpCfg {
+    static constexpr bool F32 = sizeof(A) == 4, Q8 = DT == GB_DT_Q8_0;
+    static constexpr int NK = F32 ? 64 : 128;          // keys per tile
+    static constexpr int QS = F32 ? 2 : 1;             // fp16 parts of Q and P
+    static constexpr int KS = F32 && Q8 ? 2 : 1;       // fp16 parts of K and V
+    static constexpr int G = HD / 64;                  // 64-column groups (128 bytes)
+    static constexpr int QB = 128 * HD * 2;            // bytes of a row tile's part
+    static constexpr int KB = NK * HD * 2;             // bytes of a K (or V) tile's part
+    static constexpr int ST0 = (PP_SMEM_MAX - 2 * QS * QB) / (2 * KS * KB);
+    static constexpr int ST = ST0 > 4 ? 4 : ST0;       // K / V stages
+    static constexpr int SMEM = 2 * QS * QB + ST * 2 * KS * KB + 1024;
+    static constexpr int PROD = Q8 ? 4 : 1;            // producer warps
+    static constexpr int THREADS = PP_SOFT + 32 + PROD * 32;
+    // tensor memory columns: S (and P over it) of tile i at 128 i, O at 256 + 128 i
+    static constexpr uint32_t PLO = NK;                // P's remainders, from S's base
+    static_assert(ST >= 1, "shared memory");
+};
+
+struct PpArgs {
+    PagedView c;
+    BatchView b;
+    const void* q;
+    void* out;
+    int ldq, ldo, group, bq;      // bq: queries per row tile
+    float* part;
+    unsigned* tickets;
+    unsigned* err;
+};
+
+__device__ __forceinline__ float pp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pp_pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Byte offset of the 16-byte unit u (8 halves) of row r in a swizzled tile of R rows.
+__device__ __forceinline__ uint32_t pp_off(int r, int u, int R) {
+    return (uint32_t)((u >> 3) * R * 128 + r * 128 + (((u ^ r) & 7) << 4));
+}
+
+template <typename A, int HD, int DT>
+__global__ void __launch_bounds__((PpCfg<A, HD, DT>::THREADS), 1)
+k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PpArgs a) {
+    using C = PpCfg<A, HD, DT>;
+    constexpr int NK = C::NK, ST = C::ST;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* qs = sm;                                   // [2 tiles][QS]
+    uint8_t* ks = sm + 2 * C::QS * C::QB;               // [ST][KS]
+    uint8_t* vs = ks + ST * C::KS * C::KB;              // [ST][KS]
+    __shared__ __align__(8) uint64_t bars[4 * ST + 7];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int s_seq, s_blk;
+    __shared__ unsigned s_last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const PagedView& c = a.c;
+    const BatchView& b = a.b;
+    const int kvh = blockIdx.x % c.n_kv, y = blockIdx.x / c.n_kv;
+
+    // ---- which sequence and query block: the blocks of the sequences in order, the longest of each first
+    if (warp == 0) {
+        if (lane == 0) s_seq = -1;
+        __syncwarp();
+        int base = 0;
+        for (int s0 = 0; s0 < b.n_seq; s0 += 32) {
+            const int s = s0 + lane;
+            int n = 0;
+            if (s < b.n_seq) n = b.cu ? max(__ldg(b.cu + s + 1) - __ldg(b.cu + s), 0) : 1;
+            const int nb = (n + 2 * a.bq - 1) / (2 * a.bq);
+            int incl = nb;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, y < base + incl);
+            if (hit) {
+                if (lane == __ffs(hit) - 1) {
+                    s_seq = s;
+                    s_blk = nb - 1 - (y - (base + incl - nb));
+                }
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    __syncthreads();
+    const int seq = s_seq;
+    if (seq < 0) return;
+    const int t_begin = b.cu ? __ldg(b.cu + seq) : seq, t_end = min(b.cu ? __ldg(b.cu + seq + 1) : seq + 1, b.n_tokens);
+    const int n_q = t_end - t_begin;
+    const int q0 = s_blk * 2 * a.bq;
+    if (q0 >= n_q || t_begin < 0) return;
+    const int len = seq_len(b, seq, a.err);
+    const int pos0 = len - n_q;                          // position of the first query (may be negative)
+    const bool two = q0 + a.bq < n_q;                    // the second row tile has queries
+    const int kend = len == 0 ? 0 : pos0 + min(q0 + 2 * a.bq, n_q);   // keys 0 .. kend - 1
+    const int nt_all = kend > 0 ? (kend + NK - 1) / NK : 0;
+    const int per = (nt_all + gridDim.y - 1) / gridDim.y;
+    const int n_split = nt_all > 0 ? (nt_all + per - 1) / per : 1;
+    if ((int)blockIdx.y >= n_split) return;
+    const int j0 = blockIdx.y * per, nt = min(per, nt_all - j0);   // this CTA's key tiles j0 ..
+
+    // ---- rows
+    const int wg = warp >> 2, r = tid & 127;             // softmax threads: tile, row
+    const int qi = q0 + wg * a.bq + r / a.group, h = kvh * a.group + r % a.group;
+    const bool live = warp < 8 && r < a.bq * a.group && qi < n_q;
+    if (nt_all == 0) {   // nothing to see
+        if (live) {
+            A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
+            const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            for (int d = 0; d < HD; d += 8) act_store8(dst + d, z);
+        }
+        return;
+    }
+
+    const uint32_t b0 = tc::smem_u32(&bars[0]);
+    const uint32_t kfull = b0, kfree = b0 + 8 * ST, vfull = b0 + 16 * ST, vfree = b0 + 24 * ST;   // [ST] each
+    const uint32_t sfull = b0 + 32 * ST, pfull = sfull + 16, ofull = sfull + 32, tail = sfull + 48;   // [2], [2], [2], 1
+    if (tid == 0) {
+        for (int i = 0; i < ST; i++) {
+            mbs_init(kfull + 8 * i, C::PROD);
+            mbs_init(kfree + 8 * i, 1);
+            mbs_init(vfull + 8 * i, C::PROD);
+            mbs_init(vfree + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbs_init(sfull + 8 * i, 1);
+            mbs_init(pfull + 8 * i, 4);
+            mbs_init(ofull + 8 * i, 1);
+        }
+        mbs_init(tail, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) tc::tmem_alloc(&tmem_slot, 512);
+
+    // ---- Q rows into shared memory, split for fp32 activations
+    float up_inv = 1.f;   // 2^-e of this thread's row
+    if (warp < 8) {
+        const A* src = static_cast<const A*>(a.q) + (size_t)(t_begin + qi) * a.ldq + (size_t)h * HD;
+        uint8_t* dst = qs + wg * C::QS * C::QB;
+        if (!C::F32) {
+#pragma unroll 4
+            for (int u = 0; u < HD / 8; u++) {
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (live) w = ldg4(src + 8 * u);
+                *reinterpret_cast<uint4*>(dst + pp_off(r, u, 128)) = w;
+            }
+        } else {
+            float mx = 0.f;
+#pragma unroll 4
+            for (int u = 0; u < HD / 8; u++) {
+                float x[8];
+                if (live) {
+                    act_load8(src + 8 * u, x);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]));
+                }
+            }
+            const int e = tc::f16_scale_exp(__float_as_uint(mx));
+            const float up = tc::pow2f(e);
+            up_inv = tc::pow2f(-e);
+#pragma unroll 2
+            for (int u = 0; u < HD / 8; u++) {
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (live) act_load8(src + 8 * u, x);
+                float hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[i] *= up;
+                    hi[i] = __half2float(__float2half_rn(x[i]));
+                    lo[i] = x[i] - hi[i];
+                }
+                *reinterpret_cast<uint4*>(dst + pp_off(r, u, 128)) = pack_half8(hi);
+                *reinterpret_cast<uint4*>(dst + C::QB + pp_off(r, u, 128)) = pack_half8(lo);
+            }
+        }
+        tc::fence_async_smem();
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    bool ok = true;
+
+    if (warp == 8) {   // ---- MMA issue (one lane)
+        if (lane == 0) {
+            constexpr uint32_t idS = tc::idesc_f16(128, NK), idO = tc::idesc_f16_bmn(128, HD);
+            const uint32_t qb = tc::smem_u32(qs), kb = tc::smem_u32(ks), vb = tc::smem_u32(vs);
+            auto scores = [&](int i, int st) {   // S_i = Q_i K^T
+                const uint32_t S = tmem + 128u * i;
+#pragma unroll
+                for (int p = 0; p < (C::KS == 2 ? 3 : C::QS); p++) {   // hi.hi, lo.hi, hi.lo
+                    const uint32_t qa = qb + (i * C::QS + (p == 1)) * C::QB, ka = kb + (st * C::KS + (p == 2)) * C::KB;
+#pragma unroll
+                    for (int k = 0; k < HD / 16; k++)
+                        tc::mma_f16(S, tc::smem_desc_sw128(qa + (k >> 2) * 128 * 128 + (k & 3) * 32, 16, 1024),
+                                    tc::smem_desc_sw128(ka + (k >> 2) * NK * 128 + (k & 3) * 32, 16, 1024), idS,
+                                    p > 0 || k > 0);
+                }
+                tc::mma_commit(sfull + 8 * i);
+            };
+            auto output = [&](int i, int st, bool first) {   // O_i (+)= P_i V
+                const uint32_t O = tmem + 256u + 128u * i, P = tmem + 128u * i;
+#pragma unroll
+                for (int p = 0; p < (C::KS == 2 ? 3 : C::QS); p++) {
+                    const uint32_t pa = P + (p == 1 ? C::PLO : 0u), va = vb + (st * C::KS + (p == 2)) * C::KB;
+#pragma unroll
+                    for (int k = 0; k < NK / 16; k++)
+                        tc::mma_f16_ta(O, pa + 8u * k, tc::smem_desc_sw128(va + k * 2048, NK * 128, 1024), idO,
+                                       !first || p > 0 || k > 0);
+                }
+            };
+            const int n_tiles = two ? 2 : 1;
+            ok = mbs_wait(kfull, 0, a.err);
+            tc::fence_after_sync();
+            for (int i = 0; i < n_tiles; i++) scores(i, 0);
+            tc::mma_commit(kfree);
+            for (int j = 0; j < nt; j++) {
+                const int st = j % ST, sn = (j + 1) % ST;
+                if (ok) ok = mbs_wait(vfull + 8 * st, (j / ST) & 1, a.err);
+                for (int i = 0; i < n_tiles; i++) {
+                    if (ok) ok = mbs_wait(pfull + 8 * i, j & 1, a.err);
+                    tc::fence_after_sync();
+                    output(i, st, j == 0);
+                    if (j + 1 < nt) {
+                        if (i == 0) {
+                            if (ok) ok = mbs_wait(kfull + 8 * sn, ((j + 1) / ST) & 1, a.err);
+                            tc::fence_after_sync();
+                        }
+                        scores(i, sn);
+                    } else {
+                        tc::mma_commit(ofull + 8 * i);
+                    }
+                }
+                tc::mma_commit(vfree + 8 * st);
+                if (j + 1 < nt) tc::mma_commit(kfree + 8 * sn);
+            }
+        }
+        __syncwarp();
+    } else if (warp > 8) {   // ---- K and V tiles
+        const int pw = warp - 9;
+        if (!C::Q8) {
+            const int R = min(1 << c.shift, NK);         // rows of a box
+            for (int j = 0; j < nt; j++) {
+                const int st = j % ST, key0 = (j0 + j) * NK;
+                const int valid = min(kend - key0, NK);  // keys of the tile
+                const int nb = (valid + R - 1) / R;      // boxes that hold some
+                const bool part = valid < NK;
+                // a lane's boxes: page of box i (lanes share the work over boxes)
+                const uint32_t bytes = (uint32_t)(nb * R * HD * 2);
+                if (j >= ST) {
+                    if (ok) ok = mbs_wait(kfree + 8 * st, ((j / ST) - 1) & 1, a.err);
+                }
+                if (lane == 0) mbs_expect(kfull + 8 * st, bytes);
+                __syncwarp();
+                for (int i = lane; i < nb; i += 32) {
+                    const int key = key0 + i * R;
+                    int page = page_of(c, b, seq, key, a.err);
+                    if (page < 0) page = 0;
+                    const int row = key & ((1 << c.shift) - 1);
+#pragma unroll
+                    for (int g = 0; g < C::G; g++)
+                        tma_load_3d(tc::smem_u32(ks + st * C::KB) + g * NK * 128 + i * R * 128, &kmap, g * 64, row,
+                                    page * c.n_kv + kvh, kfull + 8 * st);
+                }
+                if (j >= ST) {
+                    if (ok) ok = mbs_wait(vfree + 8 * st, ((j / ST) - 1) & 1, a.err);
+                }
+                const uint32_t vbar = part ? tail : vfull + 8 * st;
+                if (lane == 0) mbs_expect(vbar, bytes);
+                __syncwarp();
+                for (int i = lane; i < nb; i += 32) {
+                    const int key = key0 + i * R;
+                    int page = page_of(c, b, seq, key, a.err);
+                    if (page < 0) page = 0;
+                    const int row = key & ((1 << c.shift) - 1);
+#pragma unroll
+                    for (int g = 0; g < C::G; g++)
+                        tma_load_3d(tc::smem_u32(vs + st * C::KB) + g * NK * 128 + i * R * 128, &vmap, g * 64, row,
+                                    page * c.n_kv + kvh, vbar);
+                }
+                if (part) {   // the last tile: zero the rows past the last key once the copies are in
+                    if (ok) ok = mbs_wait(tail, 0, a.err);
+                    for (int i = lane; i < (NK - valid) * 8 * C::G; i += 32) {
+                        const int g = i / ((NK - valid) * 8), e = i % ((NK - valid) * 8);
+                        *reinterpret_cast<uint4*>(vs + st * C::KB + g * NK * 128 + valid * 128 + e * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    tc::fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbs_arrive(vfull + 8 * st);
+                }
+            }
+        } else {
+            // a thread: row (key) rr of the tile, 16-column runs u0 .. u0 + NU - 1
+            constexpr int TPR = 128 / NK;                // threads per row
+            constexpr int NU = HD / 16 / TPR;
+            const int pt = pw * 32 + lane, rr = pt % NK, u0 = (pt / NK) * NU;
+            for (int j = 0; j < nt; j++) {
+                const int st = j % ST, key = (j0 + j) * NK + rr;
+                const bool in = key < kend;
+                int page = in ? page_of(c, b, seq, key, a.err) : 0;
+                if (page < 0) page = 0;
+                const int row = key & ((1 << c.shift) - 1);
+                const size_t off = (size_t)page * c.page_bytes + (size_t)kvh * c.slab;
+                const size_t co = off + (size_t)row * HD + u0 * 16, so = off + ((size_t)HD << c.shift) + row * (HD / 16);
+#pragma unroll
+                for (int kv = 0; kv < 2; kv++) {
+                    const uint8_t* pool = kv ? c.v : c.k;
+                    uint4 w[NU];
+                    __half d[NU];
+#pragma unroll
+                    for (int i = 0; i < NU; i++) {
+                        w[i] = make_uint4(0u, 0u, 0u, 0u);
+                        d[i] = __float2half_rn(0.f);
+                        if (in) {
+                            w[i] = ldg4(pool + co + i * 16);
+                            d[i] = __ldg(reinterpret_cast<const __half*>(pool + so) + (u0 + i) / 2);
+                        }
+                    }
+                    if (j >= ST) {
+                        if (ok) ok = mbs_wait((kv ? vfree : kfree) + 8 * st, ((j / ST) - 1) & 1, a.err);
+                    }
+                    uint8_t* dst = (kv ? vs : ks) + st * C::KS * C::KB;
+#pragma unroll
+                    for (int i = 0; i < NU; i++) {
+                        const uint32_t ww[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u,
+                                                w[i].w ^ 0x80808080u};
+                        uint32_t hi[8], lo[8];
+                        const __half2 d2 = __half2half2(d[i]);
+#pragma unroll
+                        for (int x = 0; x < 8; x++) {   // codes as halves (1024 + 128 + code, less 1152), times the scale
+                            uint32_t by = __byte_perm(ww[x >> 1], 0x64646464u, x & 1 ? 0x4342 : 0x4140);
+                            const __half2 cd = __hsub2(*reinterpret_cast<__half2*>(&by), __floats2half2_rn(1152.f, 1152.f));
+                            const __half2 v = __hmul2(cd, d2);
+                            hi[x] = *reinterpret_cast<const uint32_t*>(&v);
+                            if (C::KS == 2) {
+                                const __half2 rest = __hfma2(cd, d2, __hneg2(v));
+                                lo[x] = *reinterpret_cast<const uint32_t*>(&rest);
+                            }
+                        }
+                        const int u = 2 * (u0 + i);
+                        *reinterpret_cast<uint4*>(dst + pp_off(rr, u, NK)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(dst + pp_off(rr, u + 1, NK)) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                        if (C::KS == 2) {
+                            *reinterpret_cast<uint4*>(dst + C::KB + pp_off(rr, u, NK)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            *reinterpret_cast<uint4*>(dst + C::KB + pp_off(rr, u + 1, NK)) =
+                                make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                        }
+                    }
+                    tc::fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbs_arrive((kv ? vfull : kfull) + 8 * st);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (wg == 0 || two) {   // ---- softmax: thread = row
+        const uint32_t lb = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t S = lb + 128u * wg, O = lb + 256u + 128u * wg;
+        const float sc = up_inv * (1.4426950408889634f / sqrtf((float)HD));
+        const int lim = pos0 + qi;                       // the last key this row sees
+        const int lim_min = pos0 + q0 + wg * a.bq;       // and the tile's first query
+        float m = -INFINITY, l = 0.f;
+        for (int j = 0; j < nt; j++) {
+            const int key0 = (j0 + j) * NK;
+            const bool masked = key0 + NK - 1 > lim_min;
+            const int left = live ? lim - key0 : -1;     // keys 0 .. left of the tile are seen
+            if (ok) ok = mbs_wait(sfull + 8 * wg, j & 1, a.err);
+            tc::fence_after_sync();
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c0 = 0; c0 < NK; c0 += 32) {
+                float x[32];
+                tc::tmem_ld32(S + c0, x);
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    if (masked) x[i] = c0 + i <= left ? x[i] : -INFINITY;
+                    mx = fmaxf(mx, x[i]);
+                }
+            }
+            mx *= sc;
+            const bool move = mx > m + PP_TAU || (m == -INFINITY && mx > -INFINITY);
+            if (__any_sync(0xffffffffu, move)) {
+                const float mn = move ? mx : m;
+                const float al = move ? (m == -INFINITY ? 0.f : pp_ex2(m - mn)) : 1.f;
+                l *= al;
+                m = mn;
+                if (j > 0) {   // P V of the tile before is in O: its commit came before this S
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HD; c0 += 32) {
+                        float o[32];
+                        tc::tmem_ld32(O + c0, o);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] *= al;
+                        tc::tmem_st32_nowait(O + c0, o);
+                    }
+                    tc::tmem_wait_st();
+                }
+            }
+            const float off = PP_LIFT - (m == -INFINITY ? 0.f : m);
+            float sum = 0.f;
+#pragma unroll
+            for (int c0 = 0; c0 < NK; c0 += 32) {
+                float x[32];
+                uint32_t ph[16], pl[16];
+                tc::tmem_ld32(S + c0, x);
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    x[i] = pp_ex2(fmaf(x[i], sc, off));
+                    if (masked) x[i] = c0 + i <= left ? x[i] : 0.f;
+                    sum += x[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    ph[i] = pp_pack(x[2 * i], x[2 * i + 1]);
+                    if (C::F32) {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&ph[i]));
+                        pl[i] = pp_pack(x[2 * i] - f.x, x[2 * i + 1] - f.y);
+                    }
+                }
+                tc::tmem_st16_nowait(S + c0 / 2, ph);
+                if (C::F32) tc::tmem_st16_nowait(S + C::PLO + c0 / 2, pl);
+            }
+            l += sum;
+            tc::tmem_wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbs_arrive(pfull + 8 * wg);
+        }
+        if (ok) ok = mbs_wait(ofull + 8 * wg, 0, a.err);
+        tc::fence_after_sync();
+        if (n_split == 1) {
+            const float inv = l > 0.f ? 1.0f / l : 0.f;   // no keys: zeros
+            A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 32) {
+                float o[32];
+                tc::tmem_ld32(O + c0, o);
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int x = 0; x < 8; x++) v[x] = l > 0.f ? o[i + x] * inv : 0.f;
+                        act_store8(dst + c0 + i, v);
+                    }
+                }
+            }
+        } else {   // [HD + 2][128 rows] of this CTA's tile
+            float* pp = a.part + (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + wg) * (HD + 2) * 128 + r;
+            pp[0] = m;
+            pp[128] = l;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 32) {
+                float o[32];
+                tc::tmem_ld32(O + c0, o);
+#pragma unroll
+                for (int i = 0; i < 32; i++) pp[(2 + c0 + i) * 128] = o[i];
+            }
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 8) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, 512);
+    }
+    if (n_split == 1) return;
+    // ---- the last split of this row block joins them
+    if (tid == 0) {
+        unsigned prev;
+        asm volatile("fence.acq_rel.gpu;\n\tatom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
+                     : "=r"(prev)
+                     : "l"(a.tickets + blockIdx.x)
+                     : "memory");
+        s_last = prev == (unsigned)(n_split - 1);
+    }
+    __syncthreads();
+    if (!s_last) return;
+    if (tid == 0) a.tickets[blockIdx.x] = 0u;   // every split has arrived
+    if (live) {
+        const size_t step = (size_t)gridDim.x * 2 * (HD + 2) * 128;   // from one split to the next
+        const float* pp = a.part + ((size_t)blockIdx.x * 2 + wg) * (HD + 2) * 128 + r;
+        float M = -INFINITY, L = 0.f;
+        for (int z = 0; z < n_split; z++) M = fmaxf(M, __ldcg(pp + z * step));
+        for (int z = 0; z < n_split; z++) {
+            const float mz = __ldcg(pp + z * step);
+            if (mz > -INFINITY) L = fmaf(__ldcg(pp + z * step + 128), pp_ex2(mz - M), L);
+        }
+        const float inv = L > 0.f ? 1.0f / L : 0.f;
+        A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
+#pragma unroll 1
+        for (int c0 = 0; c0 < HD; c0 += 8) {
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            for (int z = 0; z < n_split; z++) {
+                const float mz = __ldcg(pp + z * step);
+                const float f = mz > -INFINITY ? pp_ex2(mz - M) * inv : 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = fmaf(f, __ldcg(pp + z * step + (2 + c0 + i) * 128), v[i]);
+            }
+            act_store8(dst + c0, v);
+        }
+    }
+}
+
+template <typename A, int HD, int DT>
+static int launch_prefill(const gb_kv_cache* cache, PpArgs& a, void* ws, cudaStream_t st) {
+    using C = PpCfg<A, HD, DT>;
+    CUtensorMap km = {}, vm = {};
+    if (!C::Q8) {
+        const int R = cache->page_size < C::NK ? cache->page_size : C::NK;
+        if (!paged_encode(&km, cache->k, HD, cache->page_size, (size_t)cache->n_pages * a.c.n_kv, R) ||
+            !paged_encode(&vm, cache->v, HD, cache->page_size, (size_t)cache->n_pages * a.c.n_kv, R))
+            return GB_ECUDA;
+    }
+    const void* f = reinterpret_cast<const void*>(k_paged_prefill<A, HD, DT>);
+    if (set_smem_once(f, C::SMEM) != cudaSuccess) return GB_ECUDA;
+    // query blocks at most: the lengths are on the device
+    long long blocks = a.b.cu ? (long long)a.b.n_tokens / (2 * a.bq) + a.b.n_seq : a.b.n_seq;
+    if (blocks > a.b.n_tokens) blocks = a.b.n_tokens;
+    const long long grid = blocks * a.c.n_kv;
+    if (grid > 0x7fffffffLL) return GB_ELIMIT;
+    // fewer CTAs than half the SMs: cut the keys too, at least 4 tiles a CTA
+    const int sms = sm_count();
+    long long split = sms / grid;
+    const long long most = ((long long)a.b.cap + 4 * C::NK - 1) / (4 * C::NK);
+    if (split > most) split = most;
+    if (split < 1) split = 1;
+    a.part = static_cast<float*>(ws);
+    a.tickets = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(ws) + PAGED_PART_BYTES);
+    k_paged_prefill<A, HD, DT><<<dim3((unsigned)grid, (unsigned)split), C::THREADS, C::SMEM, st>>>(km, vm, a);
+    return cudaGetLastError() == cudaSuccess ? GB_OK : GB_ECUDA;
+}
+
+int paged_prefill(const gb_kv_cache* cache, const PagedView& c, const BatchView& b, int dtype, const void* q, int ldq,
+                  int n_heads, void* out, int ldo, void* ws, unsigned* err, cudaStream_t st) {
+    PpArgs a;
+    a.c = c;
+    a.b = b;
+    a.q = q;
+    a.out = out;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.group = n_heads / c.n_kv;
+    if (a.group > 128) return GB_ELIMIT;
+    a.bq = 128 / a.group;
+    a.err = err;
+    const int hd = cache->head_dim;
+#define GB_PREFILL(T, A, HD, DT) \
+    if (dtype == T && hd == HD && cache->dtype == DT) return launch_prefill<A, HD, DT>(cache, a, ws, st);
+    GB_PREFILL(GB_DT_F32, float, 128, GB_DT_F16) GB_PREFILL(GB_DT_F32, float, 128, GB_DT_Q8_0)
+    GB_PREFILL(GB_DT_F32, float, 64, GB_DT_F16) GB_PREFILL(GB_DT_F32, float, 64, GB_DT_Q8_0)
+    GB_PREFILL(GB_DT_F16, __half, 128, GB_DT_F16) GB_PREFILL(GB_DT_F16, __half, 128, GB_DT_Q8_0)
+    GB_PREFILL(GB_DT_F16, __half, 64, GB_DT_F16) GB_PREFILL(GB_DT_F16, __half, 64, GB_DT_Q8_0)
+#undef GB_PREFILL
+    return GB_EINVAL;
+}
+
+}  // namespace gb
