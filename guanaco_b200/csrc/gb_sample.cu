@@ -4,17 +4,37 @@
 // The weights are integers, w = rint(2^40 e), e = exp((l - max) / T) in fp32,
 // so every sum is exact and the token does not depend on how the row is split.
 // Every filter keeps a prefix of the order (logit descending, index
-// ascending), so a cut is a logit key and a number of equal logits that are
-// kept, lowest index first: found by radix selection over the keys, with the
-// digits' counts (top-k) or weights (top-p).
+// ascending).  With the 64-bit rank (key of the logit, complement of the
+// index), unique and ordered the same way, a filter is one cut: kept = rank >=
+// cut.
 //
-// One CTA per row; the row is read again for each pass.
+// A cluster of SMP_CL CTAs takes a row, each a slice of it in shared memory,
+// read from HBM once:
+//   maximum      registers, exchanged over the cluster
+//   histogram    of (max - l), SMP_BINS linear bins over the distances whose
+//                weights are not zero, the rest in the last bin; counts for
+//                top-k, weights for top-p
+//   cut          each CTA adds up a part of the bins over the cluster; the bin
+//                in which the running sum reaches the goal; its tokens go to
+//                one CTA, which cuts them by their ranks.  A bin of more than
+//                SMP_CAND tokens (many equal logits) is first cut again by the
+//                whole cluster.
+//   draw         sums by index, the CTA, the warp, the token of the target
 #include "gb_common.cuh"
 #include "gb_internal.h"
 
+#include <cooperative_groups.h>
+
 namespace gb {
 
-constexpr int SMP_THREADS = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int SMP_THREADS = 512;
+constexpr int SMP_CL = 8;               // CTAs of a row
+constexpr int SMP_BINS = 2048;
+constexpr int SMP_CAND = 512;           // tokens of a bin that are ranked directly
+constexpr int SMP_W = SMP_THREADS / 32;
+static_assert(SMP_CAND <= SMP_THREADS && SMP_BINS % (SMP_CL * 32) == 0, "thread map");
 typedef unsigned long long u64;
 
 // Order-preserving key of a logit: larger logits have larger keys, NaN is
@@ -30,164 +50,428 @@ __device__ __forceinline__ float smp_logit(uint32_t key) {
 __device__ __forceinline__ float smp_exp(float l, float mx, float t) {
     return l == mx ? 1.f : expf(__fdiv_rn(l - mx, t));   // mx may be +inf: the others weigh nothing
 }
-__device__ __forceinline__ u64 smp_weight(float e) { return __float2ull_rn(e * 1099511627776.f); }
+// rint(2^40 e), e <= 1: below 2^23 by adding 2^23 (rounds to nearest even),
+// above it the mantissa is a whole number already.
+__device__ __forceinline__ u64 smp_weight(float e) {
+    const float y = e * 1099511627776.f;
+    if (y < 8388608.f) return __float_as_uint(y + 8388608.f) - 0x4B000000u;
+    const uint32_t b = __float_as_uint(y);
+    return (u64)((b & 0x7fffffu) | 0x800000u) << ((b >> 23) - 150u);
+}
 // floor(total * part / 2^24), part <= 2^24
 __device__ __forceinline__ u64 smp_share(u64 total, uint32_t part) {
     return (total >> 24) * part + (((total & 0xFFFFFFull) * part) >> 24);
 }
 
-template <typename T, typename F>
-__device__ T block_reduce(T v, F f, T* sh) {
+struct SmpShared {
+    uint32_t count[SMP_BINS], wlo[SMP_BINS], whi[SMP_BINS];   // whi:wlo a 64-bit weight
+    u64 cand[SMP_CAND], cand_w[SMP_CAND];                     // ranks and weights of a bin's tokens (CTA 0)
+    // written by the cluster's CTAs
+    u64 peer_max[SMP_CL], peer_a[SMP_CL], peer_b[SMP_CL], peer_sum[SMP_CL];
+    u64 cut_a, cut_b, cut_rank, cut_sum;                      // results of a search
+    uint32_t cut_bin, n_cand;
+    u64 warp64[SMP_W], warp64b[SMP_W];
+    u64 tot_a, tot_b;
+    uint32_t n_list;
+};
+
+// Inclusive sums over the block's threads of two values.
+__device__ __forceinline__ void smp_scan2(u64& a, u64& b, u64* sa, u64* sb) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+        if (lane >= o) {
+            a += x;
+            b += y;
+        }
+    }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    if (lane == 31) {
+        sa[warp] = a;
+        sb[warp] = b;
+    }
     __syncthreads();
-    v = sh[threadIdx.x & 31];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    for (int w = 0; w < warp; w++) {
+        a += sa[w];
+        b += sb[w];
+    }
 }
 
-__global__ void __launch_bounds__(SMP_THREADS)
-k_sample(const float* __restrict__ logits, int ldl, int vocab, const float* __restrict__ temperature,
+__global__ void __cluster_dims__(SMP_CL, 1, 1) __launch_bounds__(SMP_THREADS, 2)
+k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const float* __restrict__ temperature,
          const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p,
          const float* __restrict__ uu, int* __restrict__ out) {
-    __shared__ u64 hist[256], sh64[32];
-    __shared__ uint32_t sh32[32];
-    __shared__ u64 s_gt, s_bin;
-    __shared__ uint32_t s_digit;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const float* x = logits + (size_t)r * ldl;
-    auto vmax = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
-    auto vmin = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
-    auto add = [](u64 a, u64 b) { return a + b; };
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    SmpShared& sh = *reinterpret_cast<SmpShared*>(smem_raw);
+    float* x = reinterpret_cast<float*>(smem_raw + (sizeof(SmpShared) + 15) / 16 * 16);   // [slice]
+    cg::cluster_group cl = cg::this_cluster();
+    const int rank = cl.block_rank(), row = blockIdx.x / SMP_CL;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int i0 = min(rank * slice, vocab), n = min(slice, vocab - i0);   // this CTA's indices i0 .. i0 + n - 1
+    const float* src = logits + (size_t)row * ldl + i0;
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");   // every CTA of the cluster runs before remote stores
 
-    uint32_t kmax = 0;
-    for (int i = tid; i < vocab; i += SMP_THREADS) kmax = vmax(kmax, smp_key(x[i]));
-    kmax = block_reduce(kmax, vmax, sh32);
-    const float mx = smp_logit(kmax);
-    if (mx == -INFINITY) {
-        if (tid == 0) out[r] = -1;
-        return;
-    }
-    const float t = temperature ? temperature[r] : 1.f;
-    if (!(t > 0.f)) {
-        uint32_t first = 0xffffffffu;
-        for (int i = tid; i < vocab; i += SMP_THREADS)
-            if (smp_key(x[i]) == kmax) first = vmin(first, (uint32_t)i);
-        first = block_reduce(first, vmin, sh32);
-        if (tid == 0) out[r] = (int)first;
-        return;
-    }
-    const int k = top_k ? top_k[r] : 0;
-    const float p = top_p ? top_p[r] : 1.f;
-    const float mp = min_p && min_p[r] > 0.f ? fminf(min_p[r], 1.f) : 0.f;
-
-    // kept so far: key > cut, and the first `ties` indices of key == cut
-    uint32_t cut = 0, ties = 0xffffffffu;
-    // Finds the digit string of the first key, from the top, at which the
-    // running sum of `what` (1 or the weight) reaches `goal` >= 1; `gt` = the
-    // sum above it.
-    auto select = [&](u64 goal, bool count, u64& gt, u64& at) {
-        uint32_t prefix = 0;
-        gt = 0;
-        for (int sft = 24; sft >= 0; sft -= 8) {
-            __syncthreads();
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < vocab; i += SMP_THREADS) {
-                const uint32_t key = smp_key(x[i]);
-                if (sft < 24 && (key >> (sft + 8)) != prefix) continue;
-                if (!count && key < cut) continue;
-                const u64 w = count ? 1ull : smp_weight(smp_exp(smp_logit(key), mx, t));
-                if (w) atomicAdd(&hist[(key >> sft) & 255], w);
+    // ---- the slice, and the rank of its first maximum
+    u64 best = 0;
+    {
+        uint32_t bk = 0, bi = 0;
+        auto see = [&](float v, int i) {
+            const uint32_t key = smp_key(v);
+            if (key > bk) {   // indices ascend: the first of equals stays
+                bk = key;
+                bi = (uint32_t)i;
             }
-            __syncthreads();
-            if (tid == 0) {
-                u64 g = gt;
-                int dgt = 255;
-                for (; dgt > 0; dgt--) {
-                    if (g + hist[dgt] >= goal) break;
-                    g += hist[dgt];
-                }
-                s_gt = g;
-                s_digit = dgt;
-                s_bin = hist[dgt];
+        };
+        if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+            const int n4 = n >> 2;
+#pragma unroll 8
+            for (int i = tid; i < n4; i += SMP_THREADS) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(src) + i);
+                *reinterpret_cast<float4*>(x + 4 * i) = v;
+                see(v.x, 4 * i);
+                see(v.y, 4 * i + 1);
+                see(v.z, 4 * i + 2);
+                see(v.w, 4 * i + 3);
             }
-            __syncthreads();
-            gt = s_gt;
-            prefix = (prefix << 8) | s_digit;
-        }
-        at = s_bin;   // sum at the key itself
-        return prefix;
-    };
-    if (k > 0 && k < vocab) {
-        u64 gt, at;
-        cut = select((u64)k, true, gt, at);
-        ties = (uint32_t)((u64)k - gt);
-    }
-    if (p < 1.f) {
-        u64 gt, at, total = 0;
-        for (int i = tid; i < vocab; i += SMP_THREADS) {
-            const uint32_t key = smp_key(x[i]);
-            if (key > cut || (key == cut && ties == 0xffffffffu)) total += smp_weight(smp_exp(smp_logit(key), mx, t));
-        }
-        total = block_reduce(total, add, sh64);
-        const u64 wcut = smp_weight(smp_exp(smp_logit(cut), mx, t));
-        if (ties != 0xffffffffu) total += ties * wcut;
-        const u64 goal = smp_share(total, (uint32_t)rintf(fmaxf(p, 0.f) * 16777216.f));
-        if (goal == 0) {
-            cut = kmax;
-            ties = 1;
+            for (int i = 4 * n4 + tid; i < n; i += SMP_THREADS) see(x[i] = __ldg(src + i), i);
         } else {
-            cut = select(goal, false, gt, at);
-            const u64 w = smp_weight(smp_exp(smp_logit(cut), mx, t));
-            const u64 need = goal - gt;   // the j-th tie is kept while j w < need
-            ties = (uint32_t)((need + w - 1) / w);
+#pragma unroll 8
+            for (int i = tid; i < n; i += SMP_THREADS) see(x[i] = __ldg(src + i), i);
+        }
+        if (bk) best = (u64)bk << 32 | ~(uint32_t)(i0 + bi);
+    }
+    for (int i = tid; i < SMP_BINS; i += SMP_THREADS) sh.count[i] = sh.wlo[i] = sh.whi[i] = 0;
+    if (tid == 0) sh.n_cand = 0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const u64 y = __shfl_xor_sync(0xffffffffu, best, o);
+        best = y > best ? y : best;
+    }
+    if (lane == 0) sh.warp64[warp] = best;
+    __syncthreads();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (tid < SMP_CL) {
+        u64 b = 0;
+#pragma unroll
+        for (int w = 0; w < SMP_W; w++) b = sh.warp64[w] > b ? sh.warp64[w] : b;
+        cl.map_shared_rank(&sh, tid)->peer_max[rank] = b;
+    }
+    cl.sync();
+#pragma unroll
+    for (int c = 0; c < SMP_CL; c++) best = c == 0 ? sh.peer_max[0] : (sh.peer_max[c] > best ? sh.peer_max[c] : best);
+    const float mx = smp_logit((uint32_t)(best >> 32));
+    const float t = temperature ? temperature[row] : 1.f;
+    if (mx == -INFINITY || !(t > 0.f)) {   // nothing to draw; greedy
+        if (rank == 0 && tid == 0) out[row] = mx == -INFINITY ? -1 : (int)~(uint32_t)best;
+        return;   // no CTA touches another's memory any more
+    }
+    const int k = top_k ? top_k[row] : 0;
+    const float p = top_p ? top_p[row] : 1.f;
+    const float mp = min_p && min_p[row] > 0.f ? fminf(min_p[row], 1.f) : 0.f;
+    const bool by_k = k > 0 && k < vocab, by_p = p < 1.f;
+    u64 cut = 0;   // kept: rank >= cut
+
+    if (by_k || by_p) {
+        // e < 2^-41 rounds to 0 and ln 2^41 = 28.42: the last bin (from 28.486) holds no weight
+        const float inv_bin = SMP_BINS / (28.5f * t);
+        auto bin_of = [&](float l) {   // monotone in the rank; +inf's distance to itself is 0, NaN is -inf
+            const float d = l == mx ? 0.f : (mx - l) * inv_bin;
+            return d < (float)(SMP_BINS - 1) ? (int)d : SMP_BINS - 1;
+        };
+        auto rank_of = [&](int i) { return (u64)smp_key(x[i]) << 32 | ~(uint32_t)(i0 + i); };
+        auto weight_of = [&](float l) { return l == l ? smp_weight(smp_exp(l, mx, t)) : 0ull; };
+        auto clear = [&] {
+            for (int i = tid; i < SMP_BINS; i += SMP_THREADS) sh.count[i] = sh.wlo[i] = sh.whi[i] = 0;
+            __syncthreads();
+        };
+        auto put = [&](int b, u64 w) {   // a 64-bit sum in two words; the high one rarely moves
+            const uint32_t lo = (uint32_t)w, old = atomicAdd(&sh.wlo[b], lo);
+            const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old);
+            if (hi) atomicAdd(&sh.whi[b], hi);
+        };
+        constexpr int PER = SMP_BINS / SMP_CL;
+        // The cluster's sums of this thread's bin (a: tokens, b: weights), their
+        // running sums over the bins up to it, and the sums of all bins.
+        auto merge = [&](u64& own_a, u64& own_b, u64& run_a, u64& run_b, u64& all_a, u64& all_b) {
+            cl.sync();   // every histogram is done
+            u64 a = 0, b = 0;
+            if (tid < PER) {
+                const int i = rank * PER + tid;
+#pragma unroll
+                for (int c = 0; c < SMP_CL; c++) {
+                    const SmpShared* o = cl.map_shared_rank(&sh, c);
+                    if (by_k) a += o->count[i];
+                    if (by_p) b += (u64)o->whi[i] << 32 | o->wlo[i];
+                }
+            }
+            own_a = a;
+            own_b = b;
+            smp_scan2(a, b, sh.warp64, sh.warp64b);
+            if (tid == SMP_THREADS - 1) {
+                sh.tot_a = a;
+                sh.tot_b = b;
+            }
+            __syncthreads();
+            if (tid < SMP_CL) {
+                SmpShared* o = cl.map_shared_rank(&sh, tid);
+                o->peer_a[rank] = sh.tot_a;
+                o->peer_b[rank] = sh.tot_b;
+            }
+            cl.sync();
+            all_a = all_b = 0;
+#pragma unroll
+            for (int c = 0; c < SMP_CL; c++) {
+                if (c == rank) {
+                    a += all_a;
+                    b += all_b;
+                }
+                all_a += sh.peer_a[c];
+                all_b += sh.peer_b[c];
+            }
+            run_a = a;
+            run_b = b;
+        };
+        // The bin at which the running sum reaches goal, and the sums before it: to every CTA.
+        auto cross = [&](u64 goal, bool counts, u64 own_a, u64 own_b, u64 run_a, u64 run_b, u64 off_a, u64 off_b) {
+            const u64 upto = counts ? off_a + run_a : off_b + run_b, own = counts ? own_a : own_b;
+            if (tid < PER && upto - own < goal && goal <= upto)   // one thread of the cluster
+                for (int c = 0; c < SMP_CL; c++) {
+                    SmpShared* o = cl.map_shared_rank(&sh, c);
+                    o->cut_bin = (uint32_t)(rank * PER + tid);
+                    o->cut_a = off_a + run_a - own_a;
+                    o->cut_b = off_b + run_b - own_b;
+                }
+            cl.sync();
+        };
+        // In CTA 0: the candidate at which the sum, from (ga, gb), reaches goal; to every CTA.
+        auto resolve = [&](u64 goal, bool counts, u64 ga, u64 gb) {
+            const int m = (int)sh.n_cand;
+            bool in = tid < m;
+            const u64 me = in ? sh.cand[tid] : 0, w = in ? sh.cand_w[tid] : 0;
+            int left = m;
+            while (left > 32) {   // cut them by their ranks' leading bits, SMP_THREADS bins
+                u64 lo = in ? me : ~0ull, hi = me;
+                if (!in) hi = 0;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) {
+                    const u64 y = __shfl_xor_sync(0xffffffffu, lo, o), z = __shfl_xor_sync(0xffffffffu, hi, o);
+                    lo = y < lo ? y : lo;
+                    hi = z > hi ? z : hi;
+                }
+                __syncthreads();
+                if (lane == 0) {
+                    sh.warp64[warp] = lo;
+                    sh.warp64b[warp] = hi;
+                }
+                sh.count[tid] = sh.wlo[tid] = sh.whi[tid] = 0;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < SMP_W; i++) {
+                    lo = sh.warp64[i] < lo ? sh.warp64[i] : lo;
+                    hi = sh.warp64b[i] > hi ? sh.warp64b[i] : hi;
+                }
+                const int shift = max(0, 64 - __clzll(hi - lo) - 9);   // (hi - lo) >> shift < 512
+                const int bin = in ? (int)((hi - me) >> shift) : 0;
+                if (in) {
+                    atomicAdd(&sh.count[bin], 1u);
+                    put(bin, w);
+                }
+                __syncthreads();
+                const u64 own_a = sh.count[tid], own_b = (u64)sh.whi[tid] << 32 | sh.wlo[tid];
+                u64 a = own_a, b = own_b;
+                smp_scan2(a, b, sh.warp64, sh.warp64b);
+                const u64 upto = counts ? ga + a : gb + b, own = counts ? own_a : own_b;
+                if (upto - own < goal && goal <= upto) {
+                    sh.n_list = (uint32_t)own_a;
+                    sh.cut_bin = (uint32_t)tid;
+                    sh.tot_a = ga + a - own_a;
+                    sh.tot_b = gb + b - own_b;
+                }
+                __syncthreads();
+                ga = sh.tot_a;
+                gb = sh.tot_b;
+                left = (int)sh.n_list;
+                in = in && bin == (int)sh.cut_bin;
+            }
+            __syncthreads();
+            if (tid == 0) sh.n_list = 0;
+            __syncthreads();
+            if (in) {
+                const uint32_t at = atomicAdd(&sh.n_list, 1u);
+                sh.cand[at] = me;
+                sh.cand_w[at] = w;
+            }
+            __syncthreads();
+            if (warp == 0 && lane < left) {
+                const u64 mine = sh.cand[lane], mine_w = sh.cand_w[lane];
+                u64 above = ga, above_w = gb;
+                for (int j = 0; j < left; j++)
+                    if (sh.cand[j] > mine) {
+                        above++;
+                        above_w += sh.cand_w[j];
+                    }
+                const u64 before = counts ? above : above_w, own = counts ? 1ull : mine_w;
+                if (before < goal && goal <= before + own)
+                    for (int c = 0; c < SMP_CL; c++) {
+                        SmpShared* o = cl.map_shared_rank(&sh, c);
+                        o->cut_rank = mine;
+                        o->cut_sum = above_w + mine_w;
+                    }
+            }
+            __syncthreads();
+            if (tid == 0) sh.n_cand = 0;
+        };
+
+        if (by_p) {
+            for (int i = tid; i < n; i += SMP_THREADS) {
+                const float l = x[i];
+                const int bin = bin_of(l);
+                if (by_k) atomicAdd(&sh.count[bin], 1u);
+                const u64 w = weight_of(l);
+                if (w) put(bin, w);
+            }
+        } else {
+            for (int i = tid; i < n; i += SMP_THREADS) atomicAdd(&sh.count[bin_of(x[i])], 1u);
+        }
+        u64 own_a, own_b, run_a, run_b, all_a, all_b;
+        merge(own_a, own_b, run_a, run_b, all_a, all_b);
+
+        // Cut at which the running sum (of tokens or weights) reaches goal, at
+        // most the sum of all: its rank, and the weights kept.
+        auto search = [&](u64 goal, bool counts, u64& rank_cut, u64& kept) {
+            cross(goal, counts, own_a, own_b, run_a, run_b, 0, 0);
+            uint32_t bin = sh.cut_bin;
+            u64 ga = sh.cut_a, gb = sh.cut_b;
+            if (bin == SMP_BINS - 1) return;   // only tokens without weight are cut
+            u64 lo = 0, hi = ~0ull;
+            int shift = 0;
+            for (bool first = true;; first = false) {
+                auto in_bin = [&](int i) {
+                    if (first) return bin_of(x[i]) == (int)bin;
+                    const u64 rk = rank_of(i);
+                    return rk >= lo && rk <= hi && (hi - rk) >> shift == bin;
+                };
+                SmpShared* o = cl.map_shared_rank(&sh, 0);
+                u64 mn = ~0ull, mxr = 0;
+                for (int i = tid; i < n; i += SMP_THREADS)
+                    if (in_bin(i)) {
+                        const u64 rk = rank_of(i);
+                        mn = rk < mn ? rk : mn;
+                        mxr = rk > mxr ? rk : mxr;
+                        const uint32_t at = atomicAdd(&o->n_cand, 1u);
+                        if (at < SMP_CAND) {
+                            o->cand[at] = rk;
+                            o->cand_w[at] = weight_of(x[i]);
+                        }
+                    }
+                cl.sync();
+                const uint32_t m = o->n_cand;
+                if (m <= SMP_CAND) break;
+                // too many: bins over the ranks between the first and the last of them
+#pragma unroll
+                for (int z = 16; z; z >>= 1) {
+                    const u64 y = __shfl_xor_sync(0xffffffffu, mn, z), v = __shfl_xor_sync(0xffffffffu, mxr, z);
+                    mn = y < mn ? y : mn;
+                    mxr = v > mxr ? v : mxr;
+                }
+                __syncthreads();
+                if (lane == 0) {
+                    sh.warp64[warp] = mn;
+                    sh.warp64b[warp] = mxr;
+                }
+                __syncthreads();
+                if (tid < SMP_CL) {
+#pragma unroll
+                    for (int i = 0; i < SMP_W; i++) {
+                        mn = sh.warp64[i] < mn ? sh.warp64[i] : mn;
+                        mxr = sh.warp64b[i] > mxr ? sh.warp64b[i] : mxr;
+                    }
+                    SmpShared* q = cl.map_shared_rank(&sh, tid);
+                    q->peer_a[rank] = mn;
+                    q->peer_b[rank] = mxr;
+                }
+                cl.sync();
+                if (rank == 0 && tid == 0) sh.n_cand = 0;
+                lo = ~0ull;
+                hi = 0;
+#pragma unroll
+                for (int i = 0; i < SMP_CL; i++) {
+                    lo = sh.peer_a[i] < lo ? sh.peer_a[i] : lo;
+                    hi = sh.peer_b[i] > hi ? sh.peer_b[i] : hi;
+                }
+                shift = max(0, 64 - __clzll(hi - lo) - 11);   // (hi - lo) >> shift < 2048
+                clear();
+                for (int i = tid; i < n; i += SMP_THREADS) {
+                    const u64 rk = rank_of(i);
+                    if (rk < lo || rk > hi) continue;
+                    const int at = (int)((hi - rk) >> shift);
+                    if (by_k) atomicAdd(&sh.count[at], 1u);
+                    if (by_p) {
+                        const u64 w = weight_of(x[i]);
+                        if (w) put(at, w);
+                    }
+                }
+                u64 oa, ob, ra, rb, ta, tb;
+                merge(oa, ob, ra, rb, ta, tb);
+                cross(goal, counts, oa, ob, ra, rb, ga, gb);
+                bin = sh.cut_bin;
+                ga = sh.cut_a;
+                gb = sh.cut_b;
+            }
+            if (rank == 0) resolve(goal, counts, ga, gb);
+            cl.sync();
+            rank_cut = sh.cut_rank;
+            kept = sh.cut_sum;
+        };
+        u64 kept = all_b;
+        if (by_k) search((u64)k, true, cut, kept);
+        if (by_p) {
+            const u64 goal = smp_share(kept, (uint32_t)rintf(fmaxf(p, 0.f) * 16777216.f));
+            u64 c2 = best, unused;   // goal 0: the first token alone
+            if (goal) search(goal, false, c2, unused);
+            cut = c2 > cut ? c2 : cut;
         }
     }
-    // ---- the draw, in index order: warps take consecutive runs of indices
-    const int run = (vocab + SMP_THREADS / 32 - 1) / (SMP_THREADS / 32);
-    const int i0 = min(warp * run, vocab), i1 = min(i0 + run, vocab);
-    // ties before this warp's run
-    uint32_t eq = 0;
-    for (int i = i0 + lane; i < i1; i += 32) eq += smp_key(x[i]) == cut;
-    eq = __reduce_add_sync(0xffffffffu, eq);
-    __syncthreads();
-    if (lane == 0) sh32[warp] = eq;
-    __syncthreads();
-    uint32_t before = 0;
-    for (int w = 0; w < warp; w++) before += sh32[w];
-    auto weight_at = [&](int i, uint32_t& seen) {   // weight of index i after the filters; seen: ties before the warp's step
-        const uint32_t key = i < i1 ? smp_key(x[i]) : 0u;
-        const bool tie = i < i1 && key == cut;
-        const uint32_t m = __ballot_sync(0xffffffffu, tie);
-        const uint32_t at = seen + __popc(m & ((1u << lane) - 1));
-        seen += __popc(m);
-        if (i >= i1 || key < cut || (tie && at >= ties)) return 0ull;
-        const float e = smp_exp(smp_logit(key), mx, t);
+
+    // ---- the draw, in index order: warps take consecutive runs of the slice
+    const int run = (slice + SMP_W - 1) / SMP_W;
+    const int r0 = min(warp * run, n), r1 = min(r0 + run, n);
+    const uint32_t cut_key = (uint32_t)(cut >> 32);
+    auto kept_weight = [&](int i) {
+        if (i >= r1) return 0ull;
+        const float l = x[i];
+        const uint32_t key = smp_key(l);
+        if (key < cut_key || (key == cut_key && ~(uint32_t)(i0 + i) < (uint32_t)cut) || l != l) return 0ull;
+        const float e = smp_exp(l, mx, t);
         return e >= mp ? smp_weight(e) : 0ull;
     };
     u64 sum = 0;
-    uint32_t seen = before;
-    for (int i = i0; i < i1; i += 32) sum += weight_at(i + lane, seen);
+    for (int i = r0 + lane; i < r1; i += 32) sum += kept_weight(i);
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sh64[warp] = sum;
     __syncthreads();
-    u64 upto = 0, total = 0;
-    for (int w = 0; w < SMP_THREADS / 32; w++) {
-        if (w < warp) upto += sh64[w];
-        total += sh64[w];
+    if (lane == 0) sh.warp64[warp] = sum;
+    __syncthreads();
+    if (tid < SMP_CL) {
+        u64 s = 0;
+#pragma unroll
+        for (int w = 0; w < SMP_W; w++) s += sh.warp64[w];
+        cl.map_shared_rank(&sh, tid)->peer_sum[rank] = s;
     }
-    const float uf = fminf(fmaxf(uu[r], 0.f), 1.f) * 16777216.f;
+    cl.sync();   // after this no CTA touches another's memory
+    u64 upto = 0, total = 0;
+#pragma unroll
+    for (int c = 0; c < SMP_CL; c++) {
+        if (c < rank) upto += sh.peer_sum[c];
+        total += sh.peer_sum[c];
+    }
+    for (int w = 0; w < warp; w++) upto += sh.warp64[w];
+    const float uf = fminf(fmaxf(uu[row], 0.f), 1.f) * 16777216.f;
     const u64 target = smp_share(total, min((uint32_t)uf, 0xFFFFFFu));
-    if (target < upto || target >= upto + sh64[warp]) return;
-    seen = before;
-    for (int i = i0; i < i1; i += 32) {   // the run that holds the target: find the index
-        const u64 w = weight_at(i + lane, seen);
-        u64 c = w;
+    if (target < upto || target >= upto + sum) return;
+    for (int i = r0; i < r1; i += 32) {   // the run that holds the target: find the index
+        u64 c = kept_weight(i + lane);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const u64 y = __shfl_up_sync(0xffffffffu, c, o);
@@ -195,7 +479,7 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, const float* __re
         }
         const uint32_t m = __ballot_sync(0xffffffffu, upto + c > target);
         if (m) {
-            if (lane == 0) out[r] = i + __ffs(m) - 1;
+            if (lane == 0) out[row] = i0 + i + __ffs(m) - 1;
             return;
         }
         upto += __shfl_sync(0xffffffffu, c, 31);
@@ -209,7 +493,13 @@ extern "C" int gb_sample(const float* logits, int ldl, int rows, int vocab, cons
     if (!logits || !u || !out || rows < 0 || vocab <= 0 || ldl < vocab) return GB_EINVAL;
     if (vocab > GB_SAMPLE_MAX_VOCAB) return GB_ELIMIT;
     if (rows == 0) return GB_OK;
-    gb::k_sample<<<rows, gb::SMP_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(logits, ldl, vocab, temperature, top_k,
-                                                                               top_p, min_p, u, out);
+    if (rows > 0x7fffffff / gb::SMP_CL) return GB_ELIMIT;
+    const int slice = ((vocab + gb::SMP_CL - 1) / gb::SMP_CL + 3) / 4 * 4;
+    const size_t smem = (sizeof(gb::SmpShared) + 15) / 16 * 16 + (size_t)slice * sizeof(float);
+    constexpr size_t most = (sizeof(gb::SmpShared) + 15) / 16 * 16 + (size_t)GB_SAMPLE_MAX_VOCAB / gb::SMP_CL * sizeof(float);
+    static_assert(most <= 227 * 1024, "shared memory");
+    if (gb::set_smem_once(reinterpret_cast<const void*>(gb::k_sample), (int)most) != cudaSuccess) return GB_ECUDA;
+    gb::k_sample<<<rows * gb::SMP_CL, gb::SMP_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(
+        logits, ldl, vocab, slice, temperature, top_k, top_p, min_p, u, out);
     return cudaGetLastError() == cudaSuccess ? GB_OK : GB_ECUDA;
 }
