@@ -37,26 +37,31 @@ constexpr int SMP_W = SMP_THREADS / 32;
 static_assert(SMP_CAND <= SMP_THREADS && SMP_BINS % (SMP_CL * 32) == 0, "thread map");
 typedef unsigned long long u64;
 
-// Order-preserving key of a logit: larger logits have larger keys, NaN is
-// -inf and -0 is +0.
+// Order-preserving key of a logit (NaN and -0 replaced): larger logits have larger keys.
 __device__ __forceinline__ uint32_t smp_key(float l) {
-    if (l != l) l = -INFINITY;
-    const uint32_t b = __float_as_uint(l + 0.f);
+    const uint32_t b = __float_as_uint(l);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float smp_logit(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
-__device__ __forceinline__ float smp_exp(float l, float mx, float t) {
-    return l == mx ? 1.f : expf(__fdiv_rn(l - mx, t));   // mx may be +inf: the others weigh nothing
+// NaN is -inf (fmaxf passes over it), -0 is +0.
+__device__ __forceinline__ float smp_clean(float l) { return fmaxf(l, -INFINITY) + 0.f; }
+// rint(2^40 e), 0 <= e <= 1, as hi 2^23 + lo: hi = rint(2^17 e), lo the rounded
+// rest (at most 2^22 in size; e has 24 bits, so the rest is exact).  Rounding
+// by adding 2^23 and 1.5 2^23.  Sums of a few thousand parts fit 32 bits.
+__device__ __forceinline__ void smp_parts(float e, uint32_t& hi, int& lo) {
+    const float y = e * 131072.f, r = y + 8388608.f;
+    hi = __float_as_uint(r) - 0x4B000000u;
+    const float rest = y - (r - 8388608.f);
+    lo = (int)(__float_as_uint(fmaf(rest, 8388608.f, 12582912.f)) - 0x4B400000u);
 }
-// rint(2^40 e), e <= 1: below 2^23 by adding 2^23 (rounds to nearest even),
-// above it the mantissa is a whole number already.
+__device__ __forceinline__ u64 smp_join(uint32_t hi, int lo) { return ((u64)hi << 23) + (u64)(long long)lo; }
 __device__ __forceinline__ u64 smp_weight(float e) {
-    const float y = e * 1099511627776.f;
-    if (y < 8388608.f) return __float_as_uint(y + 8388608.f) - 0x4B000000u;
-    const uint32_t b = __float_as_uint(y);
-    return (u64)((b & 0x7fffffu) | 0x800000u) << ((b >> 23) - 150u);
+    uint32_t hi;
+    int lo;
+    smp_parts(e, hi, lo);
+    return smp_join(hi, lo);
 }
 // floor(total * part / 2^24), part <= 2^24
 __device__ __forceinline__ u64 smp_share(u64 total, uint32_t part) {
@@ -112,43 +117,28 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
     const float* src = logits + (size_t)row * ldl + i0;
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");   // every CTA of the cluster runs before remote stores
 
-    // ---- the slice, and the rank of its first maximum
-    u64 best = 0;
-    {
-        uint32_t bk = 0, bi = 0;
-        auto see = [&](float v, int i) {
-            const uint32_t key = smp_key(v);
-            if (key > bk) {   // indices ascend: the first of equals stays
-                bk = key;
-                bi = (uint32_t)i;
-            }
-        };
-        if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-            const int n4 = n >> 2;
+    // ---- the slice and its maximum; -inf up to whole float4s
+    const int n4 = (n + 3) >> 2;
+    float mx = -INFINITY;
+    if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
 #pragma unroll 8
-            for (int i = tid; i < n4; i += SMP_THREADS) {
-                const float4 v = __ldg(reinterpret_cast<const float4*>(src) + i);
-                *reinterpret_cast<float4*>(x + 4 * i) = v;
-                see(v.x, 4 * i);
-                see(v.y, 4 * i + 1);
-                see(v.z, 4 * i + 2);
-                see(v.w, 4 * i + 3);
-            }
-            for (int i = 4 * n4 + tid; i < n; i += SMP_THREADS) see(x[i] = __ldg(src + i), i);
-        } else {
-#pragma unroll 8
-            for (int i = tid; i < n; i += SMP_THREADS) see(x[i] = __ldg(src + i), i);
+        for (int i = tid; i < n >> 2; i += SMP_THREADS) {
+            float4 v = __ldg(reinterpret_cast<const float4*>(src) + i);
+            v = make_float4(smp_clean(v.x), smp_clean(v.y), smp_clean(v.z), smp_clean(v.w));
+            *reinterpret_cast<float4*>(x + 4 * i) = v;
+            mx = fmaxf(mx, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
         }
-        if (bk) best = (u64)bk << 32 | ~(uint32_t)(i0 + bi);
+        const int i = (n & ~3) + tid;
+        if (i < 4 * n4) mx = fmaxf(mx, x[i] = i < n ? smp_clean(__ldg(src + i)) : -INFINITY);
+    } else {
+#pragma unroll 8
+        for (int i = tid; i < 4 * n4; i += SMP_THREADS)
+            mx = fmaxf(mx, x[i] = i < n ? smp_clean(__ldg(src + i)) : -INFINITY);
     }
     for (int i = tid; i < SMP_BINS; i += SMP_THREADS) sh.count[i] = sh.wlo[i] = sh.whi[i] = 0;
     if (tid == 0) sh.n_cand = 0;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const u64 y = __shfl_xor_sync(0xffffffffu, best, o);
-        best = y > best ? y : best;
-    }
-    if (lane == 0) sh.warp64[warp] = best;
+    mx = warp_max(mx);
+    if (lane == 0) sh.warp64[warp] = smp_key(mx);
     __syncthreads();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (tid < SMP_CL) {
@@ -158,14 +148,68 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
         cl.map_shared_rank(&sh, tid)->peer_max[rank] = b;
     }
     cl.sync();
+    {
+        u64 b = 0;
 #pragma unroll
-    for (int c = 0; c < SMP_CL; c++) best = c == 0 ? sh.peer_max[0] : (sh.peer_max[c] > best ? sh.peer_max[c] : best);
-    const float mx = smp_logit((uint32_t)(best >> 32));
+        for (int c = 0; c < SMP_CL; c++) b = sh.peer_max[c] > b ? sh.peer_max[c] : b;
+        mx = smp_logit((uint32_t)b);
+    }
     const float t = temperature ? temperature[row] : 1.f;
-    if (mx == -INFINITY || !(t > 0.f)) {   // nothing to draw; greedy
-        if (rank == 0 && tid == 0) out[row] = mx == -INFINITY ? -1 : (int)~(uint32_t)best;
+    // The first index of the maximum (all CTAs call it).
+    auto first_max = [&] {
+        uint32_t at = 0xffffffffu;
+        for (int i = tid; i < n; i += SMP_THREADS)
+            if (x[i] == mx) at = min(at, (uint32_t)(i0 + i));
+        at = __reduce_min_sync(0xffffffffu, at);
+        __syncthreads();
+        if (lane == 0) sh.warp64[warp] = at;
+        __syncthreads();
+        if (tid < SMP_CL) {
+            u64 b = ~0ull;
+#pragma unroll
+            for (int w = 0; w < SMP_W; w++) b = sh.warp64[w] < b ? sh.warp64[w] : b;
+            cl.map_shared_rank(&sh, tid)->peer_max[rank] = b;
+        }
+        cl.sync();
+        u64 b = ~0ull;
+#pragma unroll
+        for (int c = 0; c < SMP_CL; c++) b = sh.peer_max[c] < b ? sh.peer_max[c] : b;
+        return (uint32_t)b;
+    };
+    if (mx == -INFINITY) {   // nothing to draw
+        if (rank == 0 && tid == 0) out[row] = -1;
         return;   // no CTA touches another's memory any more
     }
+    if (!(t > 0.f)) {        // greedy
+        cl.sync();           // peer_max has been read
+        const uint32_t at = first_max();
+        if (rank == 0 && tid == 0) out[row] = (int)at;
+        return;
+    }
+    if (mx == INFINITY) {    // certain: the others weigh nothing
+        for (int i = tid; i < 4 * n4; i += SMP_THREADS) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+        mx = 0.f;
+        __syncthreads();
+    }
+    // (l - max) / t correctly rounded: quotient from the rounded reciprocal and
+    // one step on its remainder (Markstein, IBM J. Res. Dev. 34, 1990, theorem
+    // on division: exact unless t's fraction is all ones), away from over- and
+    // underflow; any other t takes the division.  Distances past 30 t weigh
+    // nothing: 2^40 e^-30 rounds to 0.
+    const float far = -30.f * t, rt = __frcp_rn(t);
+    const bool quick = t > 8.6736174e-19f && t < 1.1529215e18f && (__float_as_uint(t) & 0x7fffffu) != 0x7fffffu;
+    auto exp_of = [&](float l) {
+        const float d = fmaxf(l - mx, far);
+        float q;
+        if (quick) {
+            q = d * rt;
+            q = fmaf(fmaf(-t, q, d), rt, q);
+        } else {
+            q = __fdiv_rn(d, t);
+        }
+        return expf(q);
+    };
+    auto weight_of = [&](float l) { return smp_weight(exp_of(l)); };
     const int k = top_k ? top_k[row] : 0;
     const float p = top_p ? top_p[row] : 1.f;
     const float mp = min_p && min_p[row] > 0.f ? fminf(min_p[row], 1.f) : 0.f;
@@ -173,14 +217,13 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
     u64 cut = 0;   // kept: rank >= cut
 
     if (by_k || by_p) {
-        // e < 2^-41 rounds to 0 and ln 2^41 = 28.42: the last bin (from 28.486) holds no weight
+        // e < 2^-41 rounds to 0 and ln 2^41 = 28.42: the last bin (from 28.47) holds no weight
         const float inv_bin = SMP_BINS / (28.5f * t);
-        auto bin_of = [&](float l) {   // monotone in the rank; +inf's distance to itself is 0, NaN is -inf
-            const float d = l == mx ? 0.f : (mx - l) * inv_bin;
-            return d < (float)(SMP_BINS - 1) ? (int)d : SMP_BINS - 1;
+        auto bin_of = [&](float l) {   // monotone in l; 0 where NaN (inf - inf, 0 inf)
+            const float d = fminf(fmaxf((mx - l) * inv_bin, 0.f), (float)(SMP_BINS - 1));
+            return (int)(__float_as_uint(d + 8388608.f) - 0x4B000000u);   // rounded
         };
         auto rank_of = [&](int i) { return (u64)smp_key(x[i]) << 32 | ~(uint32_t)(i0 + i); };
-        auto weight_of = [&](float l) { return l == l ? smp_weight(smp_exp(l, mx, t)) : 0ull; };
         auto clear = [&] {
             for (int i = tid; i < SMP_BINS; i += SMP_THREADS) sh.count[i] = sh.wlo[i] = sh.whi[i] = 0;
             __syncthreads();
@@ -323,16 +366,18 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
             if (tid == 0) sh.n_cand = 0;
         };
 
-        if (by_p) {
-            for (int i = tid; i < n; i += SMP_THREADS) {
-                const float l = x[i];
-                const int bin = bin_of(l);
+        for (int i = tid; i < n4; i += SMP_THREADS) {
+            const float4 v = *reinterpret_cast<const float4*>(x + 4 * i);
+            const float l[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int bin = bin_of(l[j]);
                 if (by_k) atomicAdd(&sh.count[bin], 1u);
-                const u64 w = weight_of(l);
-                if (w) put(bin, w);
+                if (by_p) {
+                    const u64 w = weight_of(l[j]);
+                    if (w) put(bin, w);
+                }
             }
-        } else {
-            for (int i = tid; i < n; i += SMP_THREADS) atomicAdd(&sh.count[bin_of(x[i])], 1u);
         }
         u64 own_a, own_b, run_a, run_b, all_a, all_b;
         merge(own_a, own_b, run_a, run_b, all_a, all_b);
@@ -347,24 +392,31 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
             u64 lo = 0, hi = ~0ull;
             int shift = 0;
             for (bool first = true;; first = false) {
-                auto in_bin = [&](int i) {
-                    if (first) return bin_of(x[i]) == (int)bin;
-                    const u64 rk = rank_of(i);
-                    return rk >= lo && rk <= hi && (hi - rk) >> shift == bin;
-                };
                 SmpShared* o = cl.map_shared_rank(&sh, 0);
                 u64 mn = ~0ull, mxr = 0;
-                for (int i = tid; i < n; i += SMP_THREADS)
-                    if (in_bin(i)) {
-                        const u64 rk = rank_of(i);
-                        mn = rk < mn ? rk : mn;
-                        mxr = rk > mxr ? rk : mxr;
-                        const uint32_t at = atomicAdd(&o->n_cand, 1u);
-                        if (at < SMP_CAND) {
-                            o->cand[at] = rk;
-                            o->cand_w[at] = weight_of(x[i]);
-                        }
+                auto take = [&](int i, float l) {
+                    const u64 rk = rank_of(i);
+                    mn = rk < mn ? rk : mn;
+                    mxr = rk > mxr ? rk : mxr;
+                    const uint32_t at = atomicAdd(&o->n_cand, 1u);
+                    if (at < SMP_CAND) {
+                        o->cand[at] = rk;
+                        o->cand_w[at] = weight_of(l);
                     }
+                };
+                for (int i = tid; i < n4; i += SMP_THREADS) {
+                    const float4 v = *reinterpret_cast<const float4*>(x + 4 * i);
+                    const float l[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        bool in = bin_of(l[j]) == (int)bin;
+                        if (!first) {
+                            const u64 rk = rank_of(4 * i + j);
+                            in = rk >= lo && rk <= hi && (hi - rk) >> shift == bin;
+                        }
+                        if (in) take(4 * i + j, l[j]);
+                    }
+                }
                 cl.sync();
                 const uint32_t m = o->n_cand;
                 if (m <= SMP_CAND) break;
@@ -407,10 +459,7 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
                     if (rk < lo || rk > hi) continue;
                     const int at = (int)((hi - rk) >> shift);
                     if (by_k) atomicAdd(&sh.count[at], 1u);
-                    if (by_p) {
-                        const u64 w = weight_of(x[i]);
-                        if (w) put(at, w);
-                    }
+                    if (by_p) put(at, weight_of(x[i]));
                 }
                 u64 oa, ob, ra, rb, ta, tb;
                 merge(oa, ob, ra, rb, ta, tb);
@@ -428,26 +477,51 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
         if (by_k) search((u64)k, true, cut, kept);
         if (by_p) {
             const u64 goal = smp_share(kept, (uint32_t)rintf(fmaxf(p, 0.f) * 16777216.f));
-            u64 c2 = best, unused;   // goal 0: the first token alone
+            u64 c2, unused;
             if (goal) search(goal, false, c2, unused);
+            else c2 = (u64)smp_key(mx) << 32 | ~first_max();   // the first token alone
             cut = c2 > cut ? c2 : cut;
         }
     }
 
-    // ---- the draw, in index order: warps take consecutive runs of the slice
-    const int run = (slice + SMP_W - 1) / SMP_W;
-    const int r0 = min(warp * run, n), r1 = min(r0 + run, n);
-    const uint32_t cut_key = (uint32_t)(cut >> 32);
-    auto kept_weight = [&](int i) {
-        if (i >= r1) return 0ull;
-        const float l = x[i];
-        const uint32_t key = smp_key(l);
-        if (key < cut_key || (key == cut_key && ~(uint32_t)(i0 + i) < (uint32_t)cut) || l != l) return 0ull;
-        const float e = smp_exp(l, mx, t);
-        return e >= mp ? smp_weight(e) : 0ull;
+    // ---- the draw, in index order: warps take consecutive runs of the slice, lanes four neighbours
+    const int run = (slice / 4 + SMP_W - 1) / SMP_W;
+    const int r0 = min(warp * run, n4), r1 = min(r0 + run, n4);
+    const float cut_l = cut ? smp_logit((uint32_t)(cut >> 32)) : -INFINITY;
+    const uint32_t cut_i = cut ? ~(uint32_t)cut : 0xffffffffu;   // the last kept index of logit cut_l
+    // the weights of float4 i after the filters, as parts
+    auto weights = [&](int i, uint32_t (&hi)[4], int (&lo)[4]) {
+        const float4 v = i < r1 ? *reinterpret_cast<const float4*>(x + 4 * i)
+                                : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        const float l[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            hi[j] = 0;
+            lo[j] = 0;
+        }
+        if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) < cut_l) return;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const bool in = l[j] > cut_l || (l[j] == cut_l && (uint32_t)(i0 + 4 * i + j) <= cut_i);
+            const float e = exp_of(l[j]);
+            uint32_t h;
+            int w;
+            smp_parts(e, h, w);
+            hi[j] = in && e >= mp ? h : 0u;
+            lo[j] = in && e >= mp ? w : 0;
+        }
     };
     u64 sum = 0;
-    for (int i = r0 + lane; i < r1; i += 32) sum += kept_weight(i);
+    {
+        uint32_t h4[4], h = 0;   // a lane's part of a slice: at most 2^15 / 512 float4s, 2^17 x 2^8
+        int l4[4], l = 0;
+        for (int i = r0 + lane; i < r1; i += 32) {
+            weights(i, h4, l4);
+            h += h4[0] + h4[1] + h4[2] + h4[3];
+            l += l4[0] + l4[1] + l4[2] + l4[3];
+        }
+        sum = smp_join(h, l);
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     __syncthreads();
@@ -471,7 +545,11 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
     const u64 target = smp_share(total, min((uint32_t)uf, 0xFFFFFFu));
     if (target < upto || target >= upto + sum) return;
     for (int i = r0; i < r1; i += 32) {   // the run that holds the target: find the index
-        u64 c = kept_weight(i + lane);
+        uint32_t h4[4];
+        int l4[4];
+        weights(i + lane, h4, l4);
+        const u64 own = smp_join(h4[0] + h4[1] + h4[2] + h4[3], l4[0] + l4[1] + l4[2] + l4[3]);
+        u64 c = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const u64 y = __shfl_up_sync(0xffffffffu, c, o);
@@ -479,7 +557,15 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
         }
         const uint32_t m = __ballot_sync(0xffffffffu, upto + c > target);
         if (m) {
-            if (lane == 0) out[row] = i0 + i + __ffs(m) - 1;
+            if (lane == __ffs(m) - 1) {
+                u64 at = upto + c - own;
+                int j = 0;
+                while (j < 3 && at + smp_join(h4[j], l4[j]) <= target) {
+                    at += smp_join(h4[j], l4[j]);
+                    j++;
+                }
+                out[row] = i0 + 4 * (i + lane) + j;
+            }
             return;
         }
         upto += __shfl_sync(0xffffffffu, c, 31);
