@@ -35,6 +35,7 @@
 
 namespace gb {
 
+constexpr int PP_POLY = 8;                      // of this many pairs of exponentials one is a polynomial
 constexpr float PP_TAU = 8.f, PP_LIFT = 6.f;   // p <= 2^14; small p stay normal fp16 numbers
 constexpr int PP_SOFT = 256;                    // softmax threads: two warpgroups
 constexpr int PP_SMEM_MAX = 227 * 1024 - 1280;  // less alignment slack and static shared memory
@@ -43,19 +44,21 @@ template <typename A, int HD, int DT>
 struct PpCfg {
     static constexpr bool F32 = sizeof(A) == 4, Q8 = DT == GB_DT_Q8_0;
     static constexpr int NK = F32 ? 64 : 128;          // keys per tile
-    static constexpr int QS = F32 ? 2 : 1;             // fp16 parts of Q and P
-    static constexpr int KS = F32 && Q8 ? 2 : 1;       // fp16 parts of K and V
+    static constexpr int KS = F32 && Q8 ? 2 : 1;       // fp16 parts of K and V (of Q and P: 2 for fp32)
     static constexpr int G = HD / 64;                  // 64-column groups (128 bytes)
     static constexpr int QB = 128 * HD * 2;            // bytes of a row tile's part
     static constexpr int KB = NK * HD * 2;             // bytes of a K (or V) tile's part
-    static constexpr int ST0 = (PP_SMEM_MAX - 2 * QS * QB) / (2 * KS * KB);
+    static constexpr int ST0 = (PP_SMEM_MAX - 2 * QB) / (2 * KS * KB);
     static constexpr int ST = ST0 > 4 ? 4 : ST0;       // K / V stages
-    static constexpr int SMEM = 2 * QS * QB + ST * 2 * KS * KB + 1024;
+    static constexpr int SMEM = 2 * QB + ST * 2 * KS * KB + 1024;
     static constexpr int PROD = Q8 ? 4 : 1;            // producer warps
     static constexpr int THREADS = PP_SOFT + 32 + PROD * 32;
-    // tensor memory columns: S (and P over it) of tile i at 128 i, O at 256 + 128 i
-    static constexpr uint32_t PLO = NK;                // P's remainders, from S's base
-    static_assert(ST >= 1, "shared memory");
+    // tensor memory columns: S (and P over it) of tile i at NK i; fp32: Q's
+    // high parts of tile i at 128 + 64 i; O of tile i at 256 + 128 i
+    static constexpr uint32_t PLO = NK / 2;            // P's remainders, from S's base
+    static constexpr bool HOLD = !Q8 || NK == 64;      // a row's scores stay in registers (else read twice)
+    static constexpr int PARTS = NK / 64;              // P is handed over in runs of 64 keys
+    static_assert(ST >= 2, "shared memory");
 };
 
 struct PpArgs {
@@ -74,6 +77,24 @@ __device__ __forceinline__ float pp_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 2^x of a pair without the special function unit, whose 16 results a cycle
+// bound the kernel: x = j + r, j the nearest integer, 2^r by the degree-4
+// polynomial of least relative error on [-1/2, 1/2] (2.6e-6, a hundredth of
+// P's rounding), j added to the exponent.  x is kept above -126.
+__device__ __forceinline__ float2 pp_ex2_poly(float2 x) {
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const float2 big = make_float2(12582912.f, 12582912.f);   // 1.5 2^23: adding it rounds to an integer
+    const float2 t = __fadd2_rn(x, big);
+    const float2 j = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+    const float2 r = __fadd2_rn(x, make_float2(-j.x, -j.y));
+    float2 y = __ffma2_rn(make_float2(0.009570086f, 0.009570086f), r, make_float2(0.05591785f, 0.05591785f));
+    y = __ffma2_rn(y, r, make_float2(0.24024744f, 0.24024744f));
+    y = __ffma2_rn(y, r, make_float2(0.6931218f, 0.6931218f));
+    y = __ffma2_rn(y, r, make_float2(0.9999993f, 0.9999993f));
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+}
 __device__ __forceinline__ uint32_t pp_pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -90,10 +111,10 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     constexpr int NK = C::NK, ST = C::ST;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* qs = sm;                                   // [2 tiles][QS]
-    uint8_t* ks = sm + 2 * C::QS * C::QB;               // [ST][KS]
+    uint8_t* qs = sm;                                   // [2 tiles]: Q, for fp32 its remainders
+    uint8_t* ks = sm + 2 * C::QB;                       // [ST][KS]
     uint8_t* vs = ks + ST * C::KS * C::KB;              // [ST][KS]
-    __shared__ __align__(8) uint64_t bars[4 * ST + 7];
+    __shared__ __align__(8) uint64_t bars[4 * ST + 2 * C::PARTS + 5];
     __shared__ uint32_t tmem_slot;
     __shared__ int s_seq, s_blk;
     __shared__ unsigned s_last;
@@ -145,6 +166,9 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const int n_split = nt_all > 0 ? (nt_all + per - 1) / per : 1;
     if ((int)blockIdx.y >= n_split) return;
     const int j0 = blockIdx.y * per, nt = min(per, nt_all - j0);   // this CTA's key tiles j0 ..
+    // the first row tile's queries may end before the last key tiles
+    const int kend0 = max(pos0 + min(q0 + a.bq, n_q), 0);
+    const int nt0 = min(nt, max((kend0 + NK - 1) / NK - j0, 0));
 
     // ---- rows
     const int wg = warp >> 2, r = tid & 127;             // softmax threads: tile, row
@@ -161,7 +185,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 
     const uint32_t b0 = tc::smem_u32(&bars[0]);
     const uint32_t kfull = b0, kfree = b0 + 8 * ST, vfull = b0 + 16 * ST, vfree = b0 + 24 * ST;   // [ST] each
-    const uint32_t sfull = b0 + 32 * ST, pfull = sfull + 16, ofull = sfull + 32, tail = sfull + 48;   // [2], [2], [2], 1
+    const uint32_t sfull = b0 + 32 * ST, ofull = sfull + 16, tail = sfull + 32, pfull = sfull + 40;   // [2], [2], 1, [2][PARTS]
     if (tid == 0) {
         for (int i = 0; i < ST; i++) {
             mbs_init(kfull + 8 * i, C::PROD);
@@ -171,19 +195,24 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         }
         for (int i = 0; i < 2; i++) {
             mbs_init(sfull + 8 * i, 1);
-            mbs_init(pfull + 8 * i, 4);
+            for (int h = 0; h < C::PARTS; h++) mbs_init(pfull + 8 * (i * C::PARTS + h), 4);
             mbs_init(ofull + 8 * i, 1);
         }
         mbs_init(tail, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 8) tc::tmem_alloc(&tmem_slot, 512);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
 
-    // ---- Q rows into shared memory, split for fp32 activations
+    // ---- Q rows: fp16 into shared memory; fp32 split, the high parts into
+    // tensor memory (the A operand of two products of three), the rest into shared memory
     float up_inv = 1.f;   // 2^-e of this thread's row
     if (warp < 8) {
         const A* src = static_cast<const A*>(a.q) + (size_t)(t_begin + qi) * a.ldq + (size_t)h * HD;
-        uint8_t* dst = qs + wg * C::QS * C::QB;
+        uint8_t* dst = qs + wg * C::QB;
         if (!C::F32) {
 #pragma unroll 4
             for (int u = 0; u < HD / 8; u++) {
@@ -205,27 +234,33 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const int e = tc::f16_scale_exp(__float_as_uint(mx));
             const float up = tc::pow2f(e);
             up_inv = tc::pow2f(-e);
-#pragma unroll 2
-            for (int u = 0; u < HD / 8; u++) {
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (live) act_load8(src + 8 * u, x);
-                float hi[8], lo[8];
+            const uint32_t qh = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 64u * wg;
+#pragma unroll 1
+            for (int u = 0; u < HD / 8; u += 4) {
+                uint32_t hi[16];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    x[i] *= up;
-                    hi[i] = __half2float(__float2half_rn(x[i]));
-                    lo[i] = x[i] - hi[i];
+                for (int v = 0; v < 4; v++) {
+                    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    if (live) act_load8(src + 8 * (u + v), x);
+                    float lo[8];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        hi[4 * v + i] = pp_pack(x[2 * i] * up, x[2 * i + 1] * up);
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[4 * v + i]));
+                        lo[2 * i] = x[2 * i] * up - f.x;
+                        lo[2 * i + 1] = x[2 * i + 1] * up - f.y;
+                    }
+                    *reinterpret_cast<uint4*>(dst + pp_off(r, u + v, 128)) = pack_half8(lo);
                 }
-                *reinterpret_cast<uint4*>(dst + pp_off(r, u, 128)) = pack_half8(hi);
-                *reinterpret_cast<uint4*>(dst + C::QB + pp_off(r, u, 128)) = pack_half8(lo);
+                tc::tmem_st16_nowait(qh + 4 * u, hi);
             }
+            tc::tmem_wait_st();
         }
         tc::fence_async_smem();
     }
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    const uint32_t tmem = tmem_slot;
     bool ok = true;
 
     if (warp == 8) {   // ---- MMA issue (one lane)
@@ -233,50 +268,55 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             constexpr uint32_t idS = tc::idesc_f16(128, NK), idO = tc::idesc_f16_bmn(128, HD);
             const uint32_t qb = tc::smem_u32(qs), kb = tc::smem_u32(ks), vb = tc::smem_u32(vs);
             auto scores = [&](int i, int st) {   // S_i = Q_i K^T
-                const uint32_t S = tmem + 128u * i;
+                const uint32_t S = tmem + (uint32_t)(NK * i), qa = qb + i * C::QB, ka = kb + st * C::KS * C::KB;
+                if (C::F32) {
+                    const uint32_t qh = tmem + 128u + 64u * i;
 #pragma unroll
-                for (int p = 0; p < (C::KS == 2 ? 3 : C::QS); p++) {   // hi.hi, lo.hi, hi.lo
-                    const uint32_t qa = qb + (i * C::QS + (p == 1)) * C::QB, ka = kb + (st * C::KS + (p == 2)) * C::KB;
+                    for (int p = 0; p < C::KS; p++)
 #pragma unroll
-                    for (int k = 0; k < HD / 16; k++)
-                        tc::mma_f16(S, tc::smem_desc_sw128(qa + (k >> 2) * 128 * 128 + (k & 3) * 32, 16, 1024),
-                                    tc::smem_desc_sw128(ka + (k >> 2) * NK * 128 + (k & 3) * 32, 16, 1024), idS,
-                                    p > 0 || k > 0);
+                        for (int k = 0; k < HD / 16; k++)
+                            tc::mma_f16_ta(S, qh + 8u * k,
+                                           tc::smem_desc_sw128(ka + p * C::KB + (k >> 2) * NK * 128 + (k & 3) * 32, 16, 1024),
+                                           idS, p > 0 || k > 0);
                 }
+#pragma unroll
+                for (int k = 0; k < HD / 16; k++)
+                    tc::mma_f16(S, tc::smem_desc_sw128(qa + (k >> 2) * 128 * 128 + (k & 3) * 32, 16, 1024),
+                                tc::smem_desc_sw128(ka + (k >> 2) * NK * 128 + (k & 3) * 32, 16, 1024), idS,
+                                C::F32 || k > 0);
                 tc::mma_commit(sfull + 8 * i);
             };
-            auto output = [&](int i, int st, bool first) {   // O_i (+)= P_i V
-                const uint32_t O = tmem + 256u + 128u * i, P = tmem + 128u * i;
+            auto output = [&](int i, int st, int j) {   // O_i (+)= P_i V, as the parts of P arrive
+                const uint32_t O = tmem + 256u + 128u * i, P = tmem + (uint32_t)(NK * i);
 #pragma unroll
-                for (int p = 0; p < (C::KS == 2 ? 3 : C::QS); p++) {
-                    const uint32_t pa = P + (p == 1 ? C::PLO : 0u), va = vb + (st * C::KS + (p == 2)) * C::KB;
+                for (int h = 0; h < C::PARTS; h++) {
+                    if (ok) ok = mbs_wait(pfull + 8 * (i * C::PARTS + h), j & 1, a.err);
+                    tc::fence_after_sync();
 #pragma unroll
-                    for (int k = 0; k < NK / 16; k++)
-                        tc::mma_f16_ta(O, pa + 8u * k, tc::smem_desc_sw128(va + k * 2048, NK * 128, 1024), idO,
-                                       !first || p > 0 || k > 0);
+                    for (int p = 0; p < (C::F32 ? C::KS + 1 : 1); p++) {   // hi.hi, lo.hi, hi.lo
+                        const uint32_t pa = P + (p == 1 ? C::PLO : 0u), va = vb + (st * C::KS + (p == 2)) * C::KB;
+#pragma unroll
+                        for (int k = 4 * h; k < 4 * h + 4; k++)
+                            tc::mma_f16_ta(O, pa + 8u * k, tc::smem_desc_sw128(va + k * 2048, NK * 128, 1024), idO,
+                                           j > 0 || p > 0 || k > 0);
+                    }
                 }
             };
-            const int n_tiles = two ? 2 : 1;
+            const int tiles[2] = {nt0, two ? nt : 0};   // key tiles of each row tile
             ok = mbs_wait(kfull, 0, a.err);
             tc::fence_after_sync();
-            for (int i = 0; i < n_tiles; i++) scores(i, 0);
+            for (int i = 0; i < 2; i++)
+                if (tiles[i] > 0) scores(i, 0);
             tc::mma_commit(kfree);
             for (int j = 0; j < nt; j++) {
                 const int st = j % ST, sn = (j + 1) % ST;
                 if (ok) ok = mbs_wait(vfull + 8 * st, (j / ST) & 1, a.err);
-                for (int i = 0; i < n_tiles; i++) {
-                    if (ok) ok = mbs_wait(pfull + 8 * i, j & 1, a.err);
-                    tc::fence_after_sync();
-                    output(i, st, j == 0);
-                    if (j + 1 < nt) {
-                        if (i == 0) {
-                            if (ok) ok = mbs_wait(kfull + 8 * sn, ((j + 1) / ST) & 1, a.err);
-                            tc::fence_after_sync();
-                        }
-                        scores(i, sn);
-                    } else {
-                        tc::mma_commit(ofull + 8 * i);
-                    }
+                if (j + 1 < nt && ok) ok = mbs_wait(kfull + 8 * sn, ((j + 1) / ST) & 1, a.err);
+                for (int i = 0; i < 2; i++) {
+                    if (j >= tiles[i]) continue;
+                    output(i, st, j);
+                    if (j + 1 < tiles[i]) scores(i, sn);
+                    else tc::mma_commit(ofull + 8 * i);
                 }
                 tc::mma_commit(vfree + 8 * st);
                 if (j + 1 < nt) tc::mma_commit(kfree + 8 * sn);
@@ -403,26 +443,41 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         __syncwarp();
     } else if (wg == 0 || two) {   // ---- softmax: thread = row
         const uint32_t lb = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t S = lb + 128u * wg, O = lb + 256u + 128u * wg;
+        const uint32_t S = lb + (uint32_t)(NK * wg), O = lb + 256u + 128u * wg;
         const float sc = up_inv * (1.4426950408889634f / sqrtf((float)HD));
         const int lim = pos0 + qi;                       // the last key this row sees
         const int lim_min = pos0 + q0 + wg * a.bq;       // and the tile's first query
+        const int n_tiles = wg == 0 ? nt0 : nt;          // without any O is not read
         float m = -INFINITY, l = 0.f;
-        for (int j = 0; j < nt; j++) {
+        for (int j = 0; j < n_tiles; j++) {
             const int key0 = (j0 + j) * NK;
             const bool masked = key0 + NK - 1 > lim_min;
             const int left = live ? lim - key0 : -1;     // keys 0 .. left of the tile are seen
             if (ok) ok = mbs_wait(sfull + 8 * wg, j & 1, a.err);
             tc::fence_after_sync();
+            float x[C::HOLD ? NK : 32];
             float mx = -INFINITY;
+            if (C::HOLD) {
 #pragma unroll
-            for (int c0 = 0; c0 < NK; c0 += 32) {
-                float x[32];
-                tc::tmem_ld32(S + c0, x);
+                for (int c0 = 0; c0 < NK; c0 += 64)
+                    tc::tmem_ld32x2(S + c0, S + c0 + 32, *reinterpret_cast<float (*)[32]>(x + c0),
+                                    *reinterpret_cast<float (*)[32]>(x + c0 + 32));
+                if (masked) {
 #pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    if (masked) x[i] = c0 + i <= left ? x[i] : -INFINITY;
-                    mx = fmaxf(mx, x[i]);
+                    for (int i = 0; i < NK; i++) x[i] = i <= left ? x[i] : -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < NK; i += 2) mx = fmaxf(mx, fmaxf(x[i], x[i + 1]));
+            } else {
+#pragma unroll
+                for (int c0 = 0; c0 < NK; c0 += 32) {
+                    tc::tmem_ld32(S + c0, *reinterpret_cast<float (*)[32]>(x));
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[i] = c0 + i <= left ? x[i] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) mx = fmaxf(mx, fmaxf(x[i], x[i + 1]));
                 }
             }
             mx *= sc;
@@ -434,48 +489,59 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 m = mn;
                 if (j > 0) {   // P V of the tile before is in O: its commit came before this S
 #pragma unroll 1
-                    for (int c0 = 0; c0 < HD; c0 += 32) {
-                        float o[32];
-                        tc::tmem_ld32(O + c0, o);
+                    for (int c0 = 0; c0 < HD; c0 += 16) {
+                        float o[16];
+                        tc::tmem_ld16(O + c0, o);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] *= al;
-                        tc::tmem_st32_nowait(O + c0, o);
+                        for (int i = 0; i < 16; i++) o[i] *= al;
+                        tc::tmem_st16(O + c0, o);
                     }
-                    tc::tmem_wait_st();
                 }
             }
             const float off = PP_LIFT - (m == -INFINITY ? 0.f : m);
-            float sum = 0.f;
-#pragma unroll
-            for (int c0 = 0; c0 < NK; c0 += 32) {
-                float x[32];
+            const float2 sc2 = make_float2(sc, sc), off2 = make_float2(off, off);
+            float2 sum = make_float2(0.f, 0.f);
+            // probabilities of 32 keys from the scores y, the last of a run of 64 hands it over
+            auto probs = [&](float* y, int c0) {
                 uint32_t ph[16], pl[16];
-                tc::tmem_ld32(S + c0, x);
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    x[i] = pp_ex2(fmaf(x[i], sc, off));
-                    if (masked) x[i] = c0 + i <= left ? x[i] : 0.f;
-                    sum += x[i];
-                }
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    ph[i] = pp_pack(x[2 * i], x[2 * i + 1]);
+                    float2 v = __ffma2_rn(make_float2(y[2 * i], y[2 * i + 1]), sc2, off2);
+                    if (!C::F32 && i % PP_POLY == PP_POLY - 1) v = pp_ex2_poly(v);
+                    else v = make_float2(pp_ex2(v.x), pp_ex2(v.y));
+                    sum = __fadd2_rn(sum, v);
+                    ph[i] = pp_pack(v.x, v.y);
                     if (C::F32) {
                         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&ph[i]));
-                        pl[i] = pp_pack(x[2 * i] - f.x, x[2 * i + 1] - f.y);
+                        pl[i] = pp_pack(v.x - f.x, v.y - f.y);
                     }
                 }
                 tc::tmem_st16_nowait(S + c0 / 2, ph);
                 if (C::F32) tc::tmem_st16_nowait(S + C::PLO + c0 / 2, pl);
+                if (c0 % 64 == 32) {
+                    tc::tmem_wait_st();
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbs_arrive(pfull + 8 * (wg * C::PARTS + c0 / 64));
+                }
+            };
+#pragma unroll
+            for (int c0 = 0; c0 < NK; c0 += 32) {
+                if (!C::HOLD) {
+                    tc::tmem_ld32(S + c0, *reinterpret_cast<float (*)[32]>(x));
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[i] = c0 + i <= left ? x[i] : -INFINITY;
+                    }
+                }
+                probs(C::HOLD ? x + c0 : x, c0);
             }
-            l += sum;
-            tc::tmem_wait_st();
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbs_arrive(pfull + 8 * wg);
+            l += sum.x + sum.y;
         }
-        if (ok) ok = mbs_wait(ofull + 8 * wg, 0, a.err);
-        tc::fence_after_sync();
+        if (n_tiles > 0) {
+            if (ok) ok = mbs_wait(ofull + 8 * wg, 0, a.err);
+            tc::fence_after_sync();
+        }
         if (n_split == 1) {
             const float inv = l > 0.f ? 1.0f / l : 0.f;   // no keys: zeros
             A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
@@ -502,7 +568,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 float o[32];
                 tc::tmem_ld32(O + c0, o);
 #pragma unroll
-                for (int i = 0; i < 32; i++) pp[(2 + c0 + i) * 128] = o[i];
+                for (int i = 0; i < 32; i++) pp[(2 + c0 + i) * 128] = l > 0.f ? o[i] : 0.f;
             }
         }
     }
