@@ -6,14 +6,16 @@
 // read from the cache serves every head that shares it.  Keys come in tiles of
 // NK.  For each of the two row tiles, alternately:
 //   S = Q K^T    A = Q, B = K, both K-major in shared memory (128-byte swizzle)
-//   softmax      one warpgroup per row tile, thread = row = tensor-memory lane:
-//                scale, causal mask, running maximum and sum; P = 2^(x - m)
-//                back into tensor memory over S
+//   softmax      two warpgroups per row tile, a thread takes half the tile's
+//                keys of one row (= tensor-memory lane): scale, causal mask,
+//                running maximum and sum; P = 2^(x - m) back into tensor
+//                memory over S, each half handed over by itself
 //   O += P V     A = P from tensor memory, B = V as it lies in the cache (rows
 //                = keys, MN-major): V is never transposed
-// While one warpgroup computes its softmax the tensor cores work for the other.
+// While one row tile's softmax runs the tensor cores work for the other.
 // The maximum moves only when a score exceeds it by more than PP_TAU (log2
-// units), so O in tensor memory is rarely rescaled.
+// units), so O in tensor memory is rarely rescaled, and the two threads of a
+// row only exchange a vote per key tile.
 //
 // Precision.  fp16 activations: Q exact, P rounded to fp16, Q8_0 values rounded
 // to fp16 (each an error of the size of the fp16 output's own rounding).
@@ -37,8 +39,8 @@ namespace gb {
 
 constexpr int PP_POLY = 8;                      // of this many pairs of exponentials one is a polynomial
 constexpr float PP_TAU = 8.f, PP_LIFT = 6.f;   // p <= 2^14; small p stay normal fp16 numbers
-constexpr int PP_SOFT = 256;                    // softmax threads: two warpgroups
-constexpr int PP_SMEM_MAX = 227 * 1024 - 1280;  // less alignment slack and static shared memory
+constexpr int PP_SOFT = 512;                    // softmax threads: two warpgroups per row tile
+constexpr int PP_SMEM_MAX = 227 * 1024 - 4096;  // less alignment slack and static shared memory
 
 template <typename A, int HD, int DT>
 struct PpCfg {
@@ -55,9 +57,9 @@ struct PpCfg {
     static constexpr int THREADS = PP_SOFT + 32 + PROD * 32;
     // tensor memory columns: S (and P over it) of tile i at NK i; fp32: Q's
     // high parts of tile i at 128 + 64 i; O of tile i at 256 + 128 i
-    static constexpr uint32_t PLO = NK / 2;            // P's remainders, from S's base
-    static constexpr bool HOLD = !Q8 || NK == 64;      // a row's scores stay in registers (else read twice)
-    static constexpr int PARTS = NK / 64;              // P is handed over in runs of 64 keys
+    static constexpr uint32_t PLO = NK / 4;            // a half's P over its scores: the remainders' columns
+    static constexpr int NH = NK / 2;                  // keys of a thread's half
+    static constexpr bool HOLD = !(Q8 && NH == 64);    // its scores stay in registers (else read twice)
     static_assert(ST >= 2, "shared memory");
 };
 
@@ -99,6 +101,20 @@ __device__ __forceinline__ uint32_t pp_pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// Among the PP_SOFT / 2 threads of a row tile (barrier id): a vote, a barrier.
+__device__ __forceinline__ bool pp_vote(int id, bool v) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)v), "r"(id), "n"(PP_SOFT / 2)
+        : "memory");
+    return any != 0;
+}
+__device__ __forceinline__ void pp_sync(int id) {
+    asm volatile("barrier.cta.sync.aligned %0, %1;" ::"r"(id), "n"(PP_SOFT / 2) : "memory");
+}
 // Byte offset of the 16-byte unit u (8 halves) of row r in a swizzled tile of R rows.
 __device__ __forceinline__ uint32_t pp_off(int r, int u, int R) {
     return (uint32_t)((u >> 3) * R * 128 + r * 128 + (((u ^ r) & 7) << 4));
@@ -114,7 +130,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     uint8_t* qs = sm;                                   // [2 tiles]: Q, for fp32 its remainders
     uint8_t* ks = sm + 2 * C::QB;                       // [ST][KS]
     uint8_t* vs = ks + ST * C::KS * C::KB;              // [ST][KS]
-    __shared__ __align__(8) uint64_t bars[4 * ST + 2 * C::PARTS + 5];
+    __shared__ __align__(8) uint64_t bars[4 * ST + 9];
+    __shared__ float s_row[2][2][128];                  // what the two threads of a row exchange
     __shared__ uint32_t tmem_slot;
     __shared__ int s_seq, s_blk;
     __shared__ unsigned s_last;
@@ -171,21 +188,21 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const int nt0 = min(nt, max((kend0 + NK - 1) / NK - j0, 0));
 
     // ---- rows
-    const int wg = warp >> 2, r = tid & 127;             // softmax threads: tile, row
-    const int qi = q0 + wg * a.bq + r / a.group, h = kvh * a.group + r % a.group;
-    const bool live = warp < 8 && r < a.bq * a.group && qi < n_q;
+    const int rt = warp >> 3, hf = (warp >> 2) & 1, r = tid & 127;   // softmax threads: row tile, half, row
+    const int qi = q0 + rt * a.bq + r / a.group, h = kvh * a.group + r % a.group;
+    const bool live = warp < 16 && r < a.bq * a.group && qi < n_q;
     if (nt_all == 0) {   // nothing to see
         if (live) {
             A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
             const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            for (int d = 0; d < HD; d += 8) act_store8(dst + d, z);
+            for (int d = hf * (HD / 2); d < (hf + 1) * (HD / 2); d += 8) act_store8(dst + d, z);
         }
         return;
     }
 
     const uint32_t b0 = tc::smem_u32(&bars[0]);
     const uint32_t kfull = b0, kfree = b0 + 8 * ST, vfull = b0 + 16 * ST, vfree = b0 + 24 * ST;   // [ST] each
-    const uint32_t sfull = b0 + 32 * ST, ofull = sfull + 16, tail = sfull + 32, pfull = sfull + 40;   // [2], [2], 1, [2][PARTS]
+    const uint32_t sfull = b0 + 32 * ST, ofull = sfull + 16, tail = sfull + 32, pfull = sfull + 40;   // [2], [2], 1, [2][2]
     if (tid == 0) {
         for (int i = 0; i < ST; i++) {
             mbs_init(kfull + 8 * i, C::PROD);
@@ -195,13 +212,13 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         }
         for (int i = 0; i < 2; i++) {
             mbs_init(sfull + 8 * i, 1);
-            for (int h = 0; h < C::PARTS; h++) mbs_init(pfull + 8 * (i * C::PARTS + h), 4);
+            for (int h2 = 0; h2 < 2; h2++) mbs_init(pfull + 8 * (2 * i + h2), 4);
             mbs_init(ofull + 8 * i, 1);
         }
         mbs_init(tail, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) tc::tmem_alloc(&tmem_slot, 512);
+    if (warp == 16) tc::tmem_alloc(&tmem_slot, 512);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -210,121 +227,133 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     // ---- Q rows: fp16 into shared memory; fp32 split, the high parts into
     // tensor memory (the A operand of two products of three), the rest into shared memory
     float up_inv = 1.f;   // 2^-e of this thread's row
-    if (warp < 8) {
-        const A* src = static_cast<const A*>(a.q) + (size_t)(t_begin + qi) * a.ldq + (size_t)h * HD;
-        uint8_t* dst = qs + wg * C::QB;
-        if (!C::F32) {
+    constexpr int UH = HD / 16;   // 8-column units of a thread's half of the row
+    const A* qsrc = static_cast<const A*>(a.q) + (size_t)(t_begin + qi) * a.ldq + (size_t)h * HD + hf * (HD / 2);
+    uint8_t* qdst = qs + rt * C::QB;
+    if (!C::F32) {
+        if (warp < 16) {
 #pragma unroll 4
-            for (int u = 0; u < HD / 8; u++) {
+            for (int u = 0; u < UH; u++) {
                 uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (live) w = ldg4(src + 8 * u);
-                *reinterpret_cast<uint4*>(dst + pp_off(r, u, 128)) = w;
+                if (live) w = ldg4(qsrc + 8 * u);
+                *reinterpret_cast<uint4*>(qdst + pp_off(r, hf * UH + u, 128)) = w;
             }
-        } else {
-            float mx = 0.f;
-#pragma unroll 4
-            for (int u = 0; u < HD / 8; u++) {
-                float x[8];
-                if (live) {
-                    act_load8(src + 8 * u, x);
+        }
+    } else {
+        float x[UH][8], mx = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]));
-                }
-            }
-            const int e = tc::f16_scale_exp(__float_as_uint(mx));
+        for (int u = 0; u < UH; u++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[u][i] = 0.f;
+            if (live) act_load8(qsrc + 8 * u, x[u]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[u][i]));
+        }
+        if (warp < 16) s_row[rt][hf][r] = mx;
+        __syncthreads();
+        if (warp < 16) {
+            const int e = tc::f16_scale_exp(__float_as_uint(fmaxf(mx, s_row[rt][hf ^ 1][r])));
             const float up = tc::pow2f(e);
             up_inv = tc::pow2f(-e);
-            const uint32_t qh = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 64u * wg;
-#pragma unroll 1
-            for (int u = 0; u < HD / 8; u += 4) {
+            const uint32_t qh = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 64u * rt + (uint32_t)(hf * (HD / 4));
+#pragma unroll
+            for (int u = 0; u < UH; u += 4) {
                 uint32_t hi[16];
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
-                    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (live) act_load8(src + 8 * (u + v), x);
                     float lo[8];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        hi[4 * v + i] = pp_pack(x[2 * i] * up, x[2 * i + 1] * up);
+                        const float y = x[u + v][2 * i] * up, z = x[u + v][2 * i + 1] * up;
+                        hi[4 * v + i] = pp_pack(y, z);
                         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[4 * v + i]));
-                        lo[2 * i] = x[2 * i] * up - f.x;
-                        lo[2 * i + 1] = x[2 * i + 1] * up - f.y;
+                        lo[2 * i] = y - f.x;
+                        lo[2 * i + 1] = z - f.y;
                     }
-                    *reinterpret_cast<uint4*>(dst + pp_off(r, u + v, 128)) = pack_half8(lo);
+                    *reinterpret_cast<uint4*>(qdst + pp_off(r, hf * UH + u + v, 128)) = pack_half8(lo);
                 }
                 tc::tmem_st16_nowait(qh + 4 * u, hi);
             }
             tc::tmem_wait_st();
         }
-        tc::fence_async_smem();
     }
+    tc::fence_async_smem();
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
     bool ok = true;
 
-    if (warp == 8) {   // ---- MMA issue (one lane)
-        if (lane == 0) {
+    if (warp == 16) {   // ---- MMA issue: the whole warp, uniform; one lane's instructions
+        {
+            // 512 columns are all of tensor memory: its base is 0
+            const uint32_t lead = tc::elect();
+            auto wait = [&](uint32_t bar, uint32_t parity) {
+                if (ok) ok = __all_sync(0xffffffffu, mbs_wait(bar, parity, a.err));
+            };
             constexpr uint32_t idS = tc::idesc_f16(128, NK), idO = tc::idesc_f16_bmn(128, HD);
-            const uint32_t qb = tc::smem_u32(qs), kb = tc::smem_u32(ks), vb = tc::smem_u32(vs);
+            // descriptors are built once and moved by adding to their address field (16-byte units)
+            const uint64_t qd = tc::smem_desc_sw128(tc::smem_u32(qs), 16, 1024);
+            const uint64_t kd = tc::smem_desc_sw128(tc::smem_u32(ks), 16, 1024);
+            const uint64_t vd = tc::smem_desc_sw128(tc::smem_u32(vs), NK * 128, 1024);
             auto scores = [&](int i, int st) {   // S_i = Q_i K^T
-                const uint32_t S = tmem + (uint32_t)(NK * i), qa = qb + i * C::QB, ka = kb + st * C::KS * C::KB;
+                const uint32_t S = (uint32_t)(NK * i);
+                const uint64_t qa = qd + (uint32_t)(i * (C::QB >> 4)), ka = kd + (uint32_t)(st * (C::KS * C::KB >> 4));
                 if (C::F32) {
-                    const uint32_t qh = tmem + 128u + 64u * i;
+                    const uint32_t qh = 128u + 64u * i;
 #pragma unroll
                     for (int p = 0; p < C::KS; p++)
 #pragma unroll
                         for (int k = 0; k < HD / 16; k++)
-                            tc::mma_f16_ta(S, qh + 8u * k,
-                                           tc::smem_desc_sw128(ka + p * C::KB + (k >> 2) * NK * 128 + (k & 3) * 32, 16, 1024),
+                            tc::mma_f16_ta_w(lead, S, qh + 8u * k, ka + (uint32_t)((p * C::KB + (k >> 2) * NK * 128 + (k & 3) * 32) >> 4),
                                            idS, p > 0 || k > 0);
                 }
 #pragma unroll
                 for (int k = 0; k < HD / 16; k++)
-                    tc::mma_f16(S, tc::smem_desc_sw128(qa + (k >> 2) * 128 * 128 + (k & 3) * 32, 16, 1024),
-                                tc::smem_desc_sw128(ka + (k >> 2) * NK * 128 + (k & 3) * 32, 16, 1024), idS,
-                                C::F32 || k > 0);
-                tc::mma_commit(sfull + 8 * i);
+                    tc::mma_f16_w(lead, S, qa + (uint32_t)(((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4),
+                                ka + (uint32_t)(((k >> 2) * NK * 128 + (k & 3) * 32) >> 4), idS, C::F32 || k > 0);
+                tc::mma_commit_w(lead, sfull + 8 * i);
             };
-            auto output = [&](int i, int st, int j) {   // O_i (+)= P_i V, as the parts of P arrive
-                const uint32_t O = tmem + 256u + 128u * i, P = tmem + (uint32_t)(NK * i);
+            auto output = [&](int i, int st, int j) {   // O_i (+)= P_i V, as the halves of P arrive
+                const uint32_t O = 256u + 128u * i, P = (uint32_t)(NK * i);
+                const uint64_t va = vd + (uint32_t)(st * (C::KS * C::KB >> 4));
 #pragma unroll
-                for (int h = 0; h < C::PARTS; h++) {
-                    if (ok) ok = mbs_wait(pfull + 8 * (i * C::PARTS + h), j & 1, a.err);
+                for (int h2 = 0; h2 < 2; h2++) {
+                    wait(pfull + 8 * (2 * i + h2), j & 1);
                     tc::fence_after_sync();
 #pragma unroll
                     for (int p = 0; p < (C::F32 ? C::KS + 1 : 1); p++) {   // hi.hi, lo.hi, hi.lo
-                        const uint32_t pa = P + (p == 1 ? C::PLO : 0u), va = vb + (st * C::KS + (p == 2)) * C::KB;
+                        const uint32_t pa = P + (uint32_t)(C::NH * h2) + (p == 1 ? C::PLO : 0u);
 #pragma unroll
-                        for (int k = 4 * h; k < 4 * h + 4; k++)
-                            tc::mma_f16_ta(O, pa + 8u * k, tc::smem_desc_sw128(va + k * 2048, NK * 128, 1024), idO,
-                                           j > 0 || p > 0 || k > 0);
+                        for (int k = 0; k < NK / 32; k++)
+                            tc::mma_f16_ta_w(lead, O, pa + 8u * k,
+                                           va + (uint32_t)(((p == 2) * C::KB + (h2 * (NK / 32) + k) * 2048) >> 4), idO,
+                                           j > 0 || h2 > 0 || p > 0 || k > 0);
                     }
                 }
             };
             const int tiles[2] = {nt0, two ? nt : 0};   // key tiles of each row tile
-            ok = mbs_wait(kfull, 0, a.err);
+            wait(kfull, 0);
             tc::fence_after_sync();
             for (int i = 0; i < 2; i++)
                 if (tiles[i] > 0) scores(i, 0);
-            tc::mma_commit(kfree);
+            tc::mma_commit_w(lead, kfree);
             for (int j = 0; j < nt; j++) {
                 const int st = j % ST, sn = (j + 1) % ST;
-                if (ok) ok = mbs_wait(vfull + 8 * st, (j / ST) & 1, a.err);
-                if (j + 1 < nt && ok) ok = mbs_wait(kfull + 8 * sn, ((j + 1) / ST) & 1, a.err);
+                wait(vfull + 8 * st, (j / ST) & 1);
+                if (j + 1 < nt) wait(kfull + 8 * sn, ((j + 1) / ST) & 1);
                 for (int i = 0; i < 2; i++) {
                     if (j >= tiles[i]) continue;
                     output(i, st, j);
                     if (j + 1 < tiles[i]) scores(i, sn);
-                    else tc::mma_commit(ofull + 8 * i);
+                    else tc::mma_commit_w(lead, ofull + 8 * i);
                 }
-                tc::mma_commit(vfree + 8 * st);
-                if (j + 1 < nt) tc::mma_commit(kfree + 8 * sn);
+                tc::mma_commit_w(lead, vfree + 8 * st);
+                if (j + 1 < nt) tc::mma_commit_w(lead, kfree + 8 * sn);
             }
         }
         __syncwarp();
-    } else if (warp > 8) {   // ---- K and V tiles
-        const int pw = warp - 9;
+    } else if (warp > 16) {   // ---- K and V tiles
+        const int pw = warp - 17;
         if (!C::Q8) {
             const int R = min(1 << c.shift, NK);         // rows of a box
             for (int j = 0; j < nt; j++) {
@@ -378,42 +407,58 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
             }
         } else {
-            // a thread: row (key) rr of the tile, 16-column runs u0 .. u0 + NU - 1
+            // a thread: row (key) rr of the tile and 16-column runs u0 .., four at
+            // a time; the next four are loaded before these are converted
             constexpr int TPR = 128 / NK;                // threads per row
-            constexpr int NU = HD / 16 / TPR;
-            const int pt = pw * 32 + lane, rr = pt % NK, u0 = (pt / NK) * NU;
-            for (int j = 0; j < nt; j++) {
-                const int st = j % ST, key = (j0 + j) * NK + rr;
-                const bool in = key < kend;
-                int page = in ? page_of(c, b, seq, key, a.err) : 0;
+            constexpr int SUB = HD / 64 / TPR > 0 ? HD / 64 / TPR : 1;   // groups of four runs per thread and tile
+            constexpr int NU = HD / 16 / TPR / SUB;      // runs of a group (two at hd 64 with two threads per row)
+            const int pt = pw * 32 + lane, rr = pt % NK, u0 = (pt / NK) * SUB * NU;
+            auto place = [&](int j) {                    // the row's place in a pool; none: -1
+                const int key = (j0 + j) * NK + rr;
+                if (j >= nt || key >= kend) return (long long)-1;
+                int page = page_of(c, b, seq, key, a.err);
                 if (page < 0) page = 0;
-                const int row = key & ((1 << c.shift) - 1);
-                const size_t off = (size_t)page * c.page_bytes + (size_t)kvh * c.slab;
-                const size_t co = off + (size_t)row * HD + u0 * 16, so = off + ((size_t)HD << c.shift) + row * (HD / 16);
+                return (long long)((size_t)page * c.page_bytes + (size_t)kvh * c.slab) +
+                       (long long)(key & ((1 << c.shift) - 1)) * HD;
+            };
+            struct Runs {
+                uint4 w[NU];
+                uint32_t d;
+            };
+            auto load = [&](long long at, int j, int kv, int sub, Runs& o) {
 #pragma unroll
-                for (int kv = 0; kv < 2; kv++) {
+                for (int i = 0; i < NU; i++) o.w[i] = make_uint4(0u, 0u, 0u, 0u);
+                o.d = 0u;
+                if (at >= 0) {
                     const uint8_t* pool = kv ? c.v : c.k;
-                    uint4 w[NU];
-                    __half d[NU];
+                    const int u = u0 + sub * NU, row = ((j0 + j) * NK + rr) & ((1 << c.shift) - 1);
 #pragma unroll
-                    for (int i = 0; i < NU; i++) {
-                        w[i] = make_uint4(0u, 0u, 0u, 0u);
-                        d[i] = __float2half_rn(0.f);
-                        if (in) {
-                            w[i] = ldg4(pool + co + i * 16);
-                            d[i] = __ldg(reinterpret_cast<const __half*>(pool + so) + (u0 + i) / 2);
-                        }
-                    }
-                    if (j >= ST) {
+                    for (int i = 0; i < NU; i++) o.w[i] = ldg4(pool + at + (u + i) * 16);
+                    const uint8_t* sp = pool + at - (long long)row * HD + ((size_t)HD << c.shift) + row * (HD / 16) + u;
+                    o.d = NU == 4 ? ldg1(sp) : ldg_u16(sp);
+                }
+            };
+            long long at = place(0), at_next = place(1);
+            Runs cur, nxt;
+            load(at, 0, 0, 0, cur);
+            for (int j = 0; j < nt; j++) {
+                const int st = j % ST;
+#pragma unroll
+                for (int it = 0; it < 2 * SUB; it++) {
+                    const int kv = it / SUB, sub = it % SUB;
+                    if (it + 1 < 2 * SUB) load(at, j, (it + 1) / SUB, (it + 1) % SUB, nxt);
+                    else load(at_next, j + 1, 0, 0, nxt);
+                    if (j >= ST && sub == 0) {
                         if (ok) ok = mbs_wait((kv ? vfree : kfree) + 8 * st, ((j / ST) - 1) & 1, a.err);
                     }
                     uint8_t* dst = (kv ? vs : ks) + st * C::KS * C::KB;
 #pragma unroll
                     for (int i = 0; i < NU; i++) {
-                        const uint32_t ww[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u,
-                                                w[i].w ^ 0x80808080u};
+                        const uint32_t ww[4] = {cur.w[i].x ^ 0x80808080u, cur.w[i].y ^ 0x80808080u,
+                                                cur.w[i].z ^ 0x80808080u, cur.w[i].w ^ 0x80808080u};
                         uint32_t hi[8], lo[8];
-                        const __half2 d2 = __half2half2(d[i]);
+                        const uint32_t dd = __byte_perm(cur.d, 0u, i / 2 ? 0x3232 : 0x1010);
+                        const __half2 d2 = *reinterpret_cast<const __half2*>(&dd);
 #pragma unroll
                         for (int x = 0; x < 8; x++) {   // codes as halves (1024 + 128 + code, less 1152), times the scale
                             uint32_t by = __byte_perm(ww[x >> 1], 0x64646464u, x & 1 ? 0x4342 : 0x4140);
@@ -425,7 +470,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                                 lo[x] = *reinterpret_cast<const uint32_t*>(&rest);
                             }
                         }
-                        const int u = 2 * (u0 + i);
+                        const int u = 2 * (u0 + sub * NU + i);
                         *reinterpret_cast<uint4*>(dst + pp_off(rr, u, NK)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                         *reinterpret_cast<uint4*>(dst + pp_off(rr, u + 1, NK)) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
                         if (C::KS == 2) {
@@ -434,75 +479,87 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                                 make_uint4(lo[4], lo[5], lo[6], lo[7]);
                         }
                     }
-                    tc::fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbs_arrive((kv ? vfull : kfull) + 8 * st);
+                    if (sub == SUB - 1) {
+                        tc::fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbs_arrive((kv ? vfull : kfull) + 8 * st);
+                    }
+                    cur = nxt;
                 }
+                at = at_next;
+                at_next = place(j + 2);
             }
         }
         __syncwarp();
-    } else if (wg == 0 || two) {   // ---- softmax: thread = row
+    } else if (rt == 0 || two) {   // ---- softmax: thread = row, half the keys
+        constexpr int NH = C::NH;
         const uint32_t lb = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t S = lb + (uint32_t)(NK * wg), O = lb + 256u + 128u * wg;
+        const uint32_t S = lb + (uint32_t)(NK * rt + NH * hf), O = lb + 256u + 128u * rt + (uint32_t)(hf * (HD / 2));
+        const uint32_t P = S;   // over the scores that this thread has read
         const float sc = up_inv * (1.4426950408889634f / sqrtf((float)HD));
         const int lim = pos0 + qi;                       // the last key this row sees
-        const int lim_min = pos0 + q0 + wg * a.bq;       // and the tile's first query
-        const int n_tiles = wg == 0 ? nt0 : nt;          // without any O is not read
-        float m = -INFINITY, l = 0.f;
+        const int lim_min = pos0 + q0 + rt * a.bq;       // and the tile's first query
+        const int n_tiles = rt == 0 ? nt0 : nt;          // without any O is not read
+        float m = -INFINITY, l = 0.f;                    // the row's maximum, this half's sum
         for (int j = 0; j < n_tiles; j++) {
             const int key0 = (j0 + j) * NK;
             const bool masked = key0 + NK - 1 > lim_min;
-            const int left = live ? lim - key0 : -1;     // keys 0 .. left of the tile are seen
-            if (ok) ok = mbs_wait(sfull + 8 * wg, j & 1, a.err);
+            const int left = (live ? lim : -1) - key0 - hf * NH;   // keys 0 .. left of the half are seen
+            if (ok) ok = mbs_wait(sfull + 8 * rt, j & 1, a.err);
             tc::fence_after_sync();
-            float x[C::HOLD ? NK : 32];
+            float x[C::HOLD ? NH : 32];
             float mx = -INFINITY;
-            if (C::HOLD) {
-#pragma unroll
-                for (int c0 = 0; c0 < NK; c0 += 64)
-                    tc::tmem_ld32x2(S + c0, S + c0 + 32, *reinterpret_cast<float (*)[32]>(x + c0),
-                                    *reinterpret_cast<float (*)[32]>(x + c0 + 32));
+            auto read = [&](int c0, float* y, int n) {   // n scores from key c0, masked; their maximum
+                if (n == 64) tc::tmem_ld32x2(S + c0, S + c0 + 32, *reinterpret_cast<float (*)[32]>(y), *reinterpret_cast<float (*)[32]>(y + 32 * (n / 64)));
+                else tc::tmem_ld32(S + c0, *reinterpret_cast<float (*)[32]>(y));
                 if (masked) {
 #pragma unroll
-                    for (int i = 0; i < NK; i++) x[i] = i <= left ? x[i] : -INFINITY;
+                    for (int i = 0; i < n; i++) y[i] = c0 + i <= left ? y[i] : -INFINITY;
                 }
 #pragma unroll
-                for (int i = 0; i < NK; i += 2) mx = fmaxf(mx, fmaxf(x[i], x[i + 1]));
+                for (int i = 0; i < n; i += 2) mx = fmaxf(mx, fmaxf(y[i], y[i + 1]));
+            };
+            if (C::HOLD) {
+                read(0, x, NH);
             } else {
 #pragma unroll
-                for (int c0 = 0; c0 < NK; c0 += 32) {
-                    tc::tmem_ld32(S + c0, *reinterpret_cast<float (*)[32]>(x));
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) x[i] = c0 + i <= left ? x[i] : -INFINITY;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) mx = fmaxf(mx, fmaxf(x[i], x[i + 1]));
-                }
+                for (int c0 = 0; c0 < NH; c0 += 32) read(c0, x, 32);
             }
             mx *= sc;
-            const bool move = mx > m + PP_TAU || (m == -INFINITY && mx > -INFINITY);
-            if (__any_sync(0xffffffffu, move)) {
-                const float mn = move ? mx : m;
-                const float al = move ? (m == -INFINITY ? 0.f : pp_ex2(m - mn)) : 1.f;
-                l *= al;
-                m = mn;
+            // both threads of every row of the tile: does any maximum move?
+            if (pp_vote(1 + rt, mx > m + PP_TAU || (m == -INFINITY && mx > -INFINITY))) {
+                s_row[rt][hf][r] = mx;
+                pp_sync(1 + rt);
+                mx = fmaxf(mx, s_row[rt][hf ^ 1][r]);
+                if (mx > m + PP_TAU || (m == -INFINITY && mx > -INFINITY)) {
+                    const float al = m == -INFINITY ? 0.f : pp_ex2(m - mx);
+                    l *= al;
+                    m = mx;
+                    mx = al;
+                } else {
+                    mx = 1.f;
+                }
                 if (j > 0) {   // P V of the tile before is in O: its commit came before this S
 #pragma unroll 1
-                    for (int c0 = 0; c0 < HD; c0 += 16) {
+                    for (int c0 = 0; c0 < HD / 2; c0 += 16) {
                         float o[16];
                         tc::tmem_ld16(O + c0, o);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] *= al;
+                        for (int i = 0; i < 16; i++) o[i] *= mx;
                         tc::tmem_st16(O + c0, o);
                     }
+                    tc::fence_before_sync();
                 }
+                pp_sync(1 + rt);   // O is rescaled before either half of P is handed over; s_row is free again
+                tc::fence_after_sync();
             }
             const float off = PP_LIFT - (m == -INFINITY ? 0.f : m);
             const float2 sc2 = make_float2(sc, sc), off2 = make_float2(off, off);
             float2 sum = make_float2(0.f, 0.f);
-            // probabilities of 32 keys from the scores y, the last of a run of 64 hands it over
-            auto probs = [&](float* y, int c0) {
+#pragma unroll
+            for (int c0 = 0; c0 < NH; c0 += 32) {
+                if (!C::HOLD) read(c0, x, 32);
+                const float* y = C::HOLD ? x + c0 : x;
                 uint32_t ph[16], pl[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
@@ -516,37 +573,27 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         pl[i] = pp_pack(v.x - f.x, v.y - f.y);
                     }
                 }
-                tc::tmem_st16_nowait(S + c0 / 2, ph);
-                if (C::F32) tc::tmem_st16_nowait(S + C::PLO + c0 / 2, pl);
-                if (c0 % 64 == 32) {
-                    tc::tmem_wait_st();
-                    tc::fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbs_arrive(pfull + 8 * (wg * C::PARTS + c0 / 64));
-                }
-            };
-#pragma unroll
-            for (int c0 = 0; c0 < NK; c0 += 32) {
-                if (!C::HOLD) {
-                    tc::tmem_ld32(S + c0, *reinterpret_cast<float (*)[32]>(x));
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) x[i] = c0 + i <= left ? x[i] : -INFINITY;
-                    }
-                }
-                probs(C::HOLD ? x + c0 : x, c0);
+                tc::tmem_st16_nowait(P + c0 / 2, ph);
+                if (C::F32) tc::tmem_st16_nowait(P + C::PLO + c0 / 2, pl);
             }
             l += sum.x + sum.y;
+            tc::tmem_wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbs_arrive(pfull + 8 * (2 * rt + hf));
         }
         if (n_tiles > 0) {
-            if (ok) ok = mbs_wait(ofull + 8 * wg, 0, a.err);
+            if (ok) ok = mbs_wait(ofull + 8 * rt, 0, a.err);
             tc::fence_after_sync();
         }
+        s_row[rt][hf][r] = l;
+        pp_sync(1 + rt);
+        l += s_row[rt][hf ^ 1][r];
         if (n_split == 1) {
             const float inv = l > 0.f ? 1.0f / l : 0.f;   // no keys: zeros
-            A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
+            A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD + hf * (HD / 2);
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD; c0 += 32) {
+            for (int c0 = 0; c0 < HD / 2; c0 += 32) {
                 float o[32];
                 tc::tmem_ld32(O + c0, o);
                 if (live) {
@@ -560,21 +607,23 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
             }
         } else {   // [HD + 2][128 rows] of this CTA's tile
-            float* pp = a.part + (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + wg) * (HD + 2) * 128 + r;
-            pp[0] = m;
-            pp[128] = l;
+            float* pp = a.part + (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + rt) * (HD + 2) * 128 + r;
+            if (hf == 0) {
+                pp[0] = m;
+                pp[128] = l;
+            }
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD; c0 += 32) {
+            for (int c0 = 0; c0 < HD / 2; c0 += 32) {
                 float o[32];
                 tc::tmem_ld32(O + c0, o);
 #pragma unroll
-                for (int i = 0; i < 32; i++) pp[(2 + c0 + i) * 128] = l > 0.f ? o[i] : 0.f;
+                for (int i = 0; i < 32; i++) pp[(2 + hf * (HD / 2) + c0 + i) * 128] = l > 0.f ? o[i] : 0.f;
             }
         }
     }
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, 512);
     }
@@ -593,7 +642,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     if (tid == 0) a.tickets[blockIdx.x] = 0u;   // every split has arrived
     if (live) {
         const size_t step = (size_t)gridDim.x * 2 * (HD + 2) * 128;   // from one split to the next
-        const float* pp = a.part + ((size_t)blockIdx.x * 2 + wg) * (HD + 2) * 128 + r;
+        const float* pp = a.part + ((size_t)blockIdx.x * 2 + rt) * (HD + 2) * 128 + r;
         float M = -INFINITY, L = 0.f;
         for (int z = 0; z < n_split; z++) M = fmaxf(M, __ldcg(pp + z * step));
         for (int z = 0; z < n_split; z++) {
@@ -603,7 +652,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const float inv = L > 0.f ? 1.0f / L : 0.f;
         A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
 #pragma unroll 1
-        for (int c0 = 0; c0 < HD; c0 += 8) {
+        for (int c0 = hf * (HD / 2); c0 < (hf + 1) * (HD / 2); c0 += 8) {
             float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             for (int z = 0; z < n_split; z++) {
                 const float mz = __ldcg(pp + z * step);

@@ -123,20 +123,46 @@ __device__ __forceinline__ void mma_tf32_ta(uint32_t tmem_d, uint32_t a_tmem, ui
         "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
-// The same with fp16 operands: A packed two per 32-bit column (even k in the
-// low half), K = 16 (8 columns) per instruction.
-__device__ __forceinline__ void mma_f16_ta(uint32_t tmem_d, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                           bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
-}
 // Arrive once on an mbarrier when every MMA this thread issued so far has completed.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                  : "memory");
+}
+
+// fp16 MMAs and the commit for a whole converged warp (A of the _ta form in
+// tensor memory: packed two per 32-bit column, even k in the low half, K = 16
+// per instruction), issued by its elected lane `lead`
+// (tc::elect): with control flow and operands uniform over the warp they stay
+// in uniform registers, where the instruction takes them from; inside a
+// one-lane branch every operand is moved there again for every instruction
+// (80 cycles an MMA against 64 of its execution).
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t lead;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(lead));
+    return lead;
+}
+__device__ __forceinline__ void mma_f16_w(uint32_t lead, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void mma_f16_ta_w(uint32_t lead, uint32_t tmem_d, uint32_t a_tmem, uint64_t bdesc,
+                                             uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit_w(uint32_t lead, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(lead)
+        : "memory");
 }
 
 // 16 consecutive fp32 columns of this thread's tensor-memory lane (warp w of
