@@ -1199,6 +1199,28 @@ bool paged_encode(void* map128, const void* pool, int hd, int page_size, size_t 
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool paged_encode_steps(void* map128, const void* pool, int dtype, int hd, int page_size, size_t slabs) {
+    auto enc = tensor_map_encoder();
+    if (!enc || slabs > 0xffffffffull) return false;
+    const cuuint64_t slab = paged_slab(dtype, hd, page_size);
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    if (dtype == GB_DT_F16) {
+        const cuuint64_t dims[4] = {64, (cuuint64_t)page_size, (cuuint64_t)hd / 64, (cuuint64_t)slabs};
+        const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, 128, slab};
+        const cuuint32_t box[4] = {64, 16, (cuuint32_t)hd / 64, 1};
+        return enc(reinterpret_cast<CUtensorMap*>(map128), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(pool),
+                   dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+    const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)page_size, (cuuint64_t)slabs};
+    const cuuint64_t strides[2] = {(cuuint64_t)hd, slab};
+    const cuuint32_t box[3] = {(cuuint32_t)hd, 16, 1};
+    return enc(reinterpret_cast<CUtensorMap*>(map128), CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pool), dims,
+               strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool gemm_encode_x(void* map128, const float* X, int T, int K, int box_k, int box_t) {
     auto enc = tensor_map_encoder();
     if (!enc || (reinterpret_cast<uintptr_t>(X) & 15) || K % 4 || box_k * 4 % 16) return false;

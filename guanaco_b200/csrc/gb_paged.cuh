@@ -50,6 +50,27 @@ int paged_prefill(const gb_kv_cache* cache, const PagedView& c, const BatchView&
 // Tensor map of an F16 pool as {hd halves, page_size rows, slabs} with boxes
 // {64, rows, 1}, 128-byte swizzle (gb_matvec.cu, beside the other encoders).
 bool paged_encode(void* map128, const void* pool, int hd, int page_size, size_t slabs, int rows);
+// Tensor map of a pool for steps of 16 rows of one slab: F16 {64 halves, rows,
+// hd / 64, slabs}, box {64, 16, hd / 64, 1}, 128-byte swizzle; Q8_0 codes {hd
+// bytes, rows, slabs}, box {hd, 16, 1}, hd-byte swizzle.
+bool paged_encode_steps(void* map128, const void* pool, int dtype, int hd, int page_size, size_t slabs);
+// Launch that may start while the kernel before it on the stream ends
+// (programmatic stream serialization): the kernel executes griddepcontrol.wait
+// before it touches global memory.
+template <typename F, typename... Args>
+cudaError_t launch_pdl(F f, dim3 grid, int threads, int smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, f, args...);
+}
 unsigned* paged_err();   // the module's device error word (nullptr: CUDA error)
 
 // Sequence of token t: the largest s with cu[s] <= t (empty sequences share a

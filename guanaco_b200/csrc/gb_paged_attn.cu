@@ -5,8 +5,11 @@
 //
 // This file: the single-token kernel and both entry points; the prompts' kernel
 // is gb_paged_prefill.cu.
+#include "gb_mt.cuh"
 #include "gb_paged.cuh"
 #include "gb_tc.cuh"
+
+#include <cuda.h>
 
 #include <type_traits>
 
@@ -26,9 +29,9 @@ namespace gb {
 // Work: a step is 16 keys of one (sequence, KV head, 8 query heads); all
 // steps of the batch, in that order, are cut into one equal run per CTA
 // whatever the sequences' lengths, and the CTA's warps take its steps in turn.
-// Each warp streams its own steps through a ring of cp.async stages and keeps
-// its own (m, l, O); they meet once per segment (the steps of one such triple
-// in this CTA) in shared memory.  A segment cut by CTA borders leaves a
+// Each warp streams its own steps through a ring of TMA copies (16 rows of K and
+// of V, 128- or 64-byte swizzle) and keeps its own (m, l, O); they meet once per
+// segment (the steps of one such triple in this CTA) in shared memory.  A segment cut by CTA borders leaves a
 // partial per CTA; the last of them to arrive joins them in CTA order.
 //
 // The running maximum m moves only when a score exceeds it by more than
@@ -48,22 +51,48 @@ struct PdCfg {
     static constexpr bool Q8 = DT == GB_DT_Q8_0;
     static constexpr int KB = 16 * HD * (Q8 ? 1 : 2);   // bytes of a step's K (or V) rows
     static constexpr int SB = Q8 ? HD : 0;              // and of their scales
-    static constexpr int STAGE = 2 * (KB + SB);
     static constexpr int NST = 3;
     static constexpr int OP = HD + 4;                   // row pitch of the meeting area (bank spread)
-    static constexpr int MEET = PD_W * PD_HEADS * OP * 4 + PD_W * PD_HEADS * 8;
-    static constexpr int SMEM = PD_W * NST * STAGE + MEET;
+    // shared: rows [PD_W][NST][2 KB], scales [PD_W][NST][2 SB], meeting area
+    // O [PD_W][8][OP] and (m, l) [PD_W][8], barriers [PD_W][NST], scan [PD_W], start [4], last
+    static constexpr int SCALES = PD_W * NST * 2 * KB;
+    static constexpr int MEET = SCALES + PD_W * NST * 2 * SB;
+    static constexpr int BARS = MEET + PD_W * PD_HEADS * (OP * 4 + 8);
+    static constexpr int SCAN = BARS + PD_W * NST * 8;
+    static constexpr int SMEM = SCAN + (PD_W + 5) * 4;
 };
 
 // CTAs per SM: what the shared memory holds, at most PD_MAX_CTAS (registers follow).
 template <int HD, int DT>
 constexpr int pd_ctas() {
-    return (227 * 1024) / (PdCfg<HD, DT>::SMEM + 2048) < PD_MAX_CTAS ? (227 * 1024) / (PdCfg<HD, DT>::SMEM + 2048)
+    return (228 * 1024) / (PdCfg<HD, DT>::SMEM + 1024) < PD_MAX_CTAS ? (228 * 1024) / (PdCfg<HD, DT>::SMEM + 1024)
                                                                      : PD_MAX_CTAS;
 }
 
-__device__ __forceinline__ void pd_cp16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void pd_tma(uint32_t dst, const void* map, int row, int slab, bool f16, uint32_t bar) {
+    if (f16)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4}], [%5];"
+            ::"r"(dst), "l"(map), "r"(0), "r"(row), "r"(slab), "r"(bar)
+            : "memory");
+    else
+        tma_load_3d(dst, map, 0, row, slab, bar);
+}
+__device__ __forceinline__ void pd_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+// Cache row (of 8) that stands at the MMA's row n.  The swizzle spreads a
+// column over the banks by the row's bits; with this order the rows that the
+// lanes of one access phase read, for K (rows n) and for V (even n, odd n), all
+// differ in the bits that matter.
+template <int HD, int DT>
+__device__ __forceinline__ int pd_row(int n) {
+    if (DT == GB_DT_F16) return n ^ ((n & 1) << 2);                       // 0 5 2 7 4 1 6 3
+    if (HD == 128) return n < 4 ? 2 * n : 2 * ((n & 3) ^ 1) + 1;          // 0 2 4 6 3 1 7 5
+    const int h = (n & 3) ^ (n >> 2);                                     // 0 1 4 5 3 2 7 6
+    return (h & 1) | (h >> 1) << 2 | (n >> 2) << 1;
 }
 __device__ __forceinline__ void pd_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
@@ -113,19 +142,22 @@ __device__ __forceinline__ float pd_ex2(float x) {
     return y;
 }
 
-// A walk over steps: sequence s, segment h of it, step st of nst.
+// A walk over steps: sequence s, segment h of it, step st of nst; kvh: the
+// segment's KV head.
 struct PdWalk {
-    int s, h, st, nst;
-    __device__ __forceinline__ void go(int by, const BatchView& b, int H, unsigned* err) {
+    int s, h, st, nst, kvh;
+    __device__ __forceinline__ void go(int by, const BatchView& b, int H, int n_hg, unsigned* err) {
         st += by;
-        while (st >= nst) {
+        if (st < nst) return;
+        do {
             st -= nst;
             if (++h == H) {
                 h = 0;
                 do nst = ++s < b.n_seq ? (seq_len(b, s, err) + 15) >> 4 : 0x7fffffff;   // past the end: no step is taken
                 while (nst == 0);
             }
-        }
+        } while (st >= nst);
+        kvh = h / n_hg;
     }
 };
 
@@ -138,70 +170,91 @@ __device__ __forceinline__ int pd_col(int p) {
 
 template <typename A, int HD, int DT>
 __global__ void __launch_bounds__(PD_W * 32, (pd_ctas<HD, DT>()))
-k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, int ldq, int group, int n_hg,
+k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedView c, const BatchView b, const A* __restrict__ q, int ldq, int group, int n_hg,
                A* __restrict__ out, int ldo, unsigned* __restrict__ tickets, float* __restrict__ part, int min_steps,
                unsigned* err) {
     using C = PdCfg<HD, DT>;
     constexpr int NT = HD / 8;   // output tiles of 8 columns
     constexpr int NB = HD / 32;  // 32-column blocks
-    extern __shared__ __align__(16) uint8_t sm[];
-    __shared__ unsigned long long s_scan[PD_W];
-    __shared__ int s_start[4];
-    __shared__ unsigned s_last;
+    extern __shared__ __align__(1024) uint8_t sm[];   // no static shared memory: the ring starts 1024-byte aligned
+    unsigned* s_scan = reinterpret_cast<unsigned*>(sm + C::SCAN);
+    int* s_start = reinterpret_cast<int*>(s_scan + PD_W);
+    unsigned& s_last = s_scan[PD_W + 4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int H = c.n_kv * n_hg, seg_cols = HD;
+    const int H = c.n_kv * n_hg;
+    const uint32_t bars = (uint32_t)__cvta_generic_to_shared(sm + C::BARS) + warp * C::NST * 8;
+    if (lane == 0) {
+        for (int i = 0; i < C::NST; i++) mbs_init(bars + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    griddep_wait();   // launched ahead of the kernel before it: nothing of it is read above
 
-    // ---- the batch's steps and this CTA's run of them
+    // ---- the batch's steps and this CTA's run of them (steps < 2^31: checked on the host)
     const int per = (b.n_seq + PD_W * 32 - 1) / (PD_W * 32);
     const int s_lo = min(tid * per, b.n_seq), s_hi = min(s_lo + per, b.n_seq);
-    unsigned long long mine = 0;
+    unsigned mine = 0;
     for (int s = s_lo; s < s_hi; s++) mine += (seq_len(b, s, err) + 15) >> 4;
-    unsigned long long incl = mine;
+    unsigned incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o);
+        const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += y;
     }
     if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
-    unsigned long long T = 0, base = 0;
+    unsigned T = 0, base = 0;
 #pragma unroll
     for (int w = 0; w < PD_W; w++) {
         if (w < warp) base += s_scan[w];
         T += s_scan[w];
     }
     T *= H;
+    const unsigned run = max((T + gridDim.x - 1) / gridDim.x, (unsigned)min_steps);
+    const unsigned a0 = blockIdx.x * run, a1 = min(a0 + run, T);
     // sequences without keys: zeros
     for (int s = blockIdx.x; s < b.n_seq; s += gridDim.x)
         if (seq_len(b, s, err) == 0)
             for (int i = tid; i < c.n_kv * group * HD; i += PD_W * 32) out[(size_t)s * ldo + i] = (A)0.f;
-    const unsigned long long run = max((T + gridDim.x - 1) / gridDim.x, (unsigned long long)min_steps);
-    const unsigned long long a0 = blockIdx.x * run, a1 = min(a0 + run, T);
     if (a0 >= T) return;
     {
-        unsigned long long at = (base + incl - mine) * H;   // first step of sequence s_lo
+        unsigned at = (base + incl - mine) * H;   // first step of sequence s_lo
         for (int s = s_lo; s < s_hi; s++) {
-            const int n = (seq_len(b, s, err) + 15) >> 4;
-            const unsigned long long next = at + (unsigned long long)n * H;
+            const unsigned n = (unsigned)(seq_len(b, s, err) + 15) >> 4, next = at + n * H;
             if (a0 >= at && a0 < next) {
                 s_start[0] = s;
                 s_start[1] = (int)((a0 - at) / n);
                 s_start[2] = (int)((a0 - at) % n);
-                s_start[3] = n;
+                s_start[3] = (int)n;
             }
             at = next;
         }
     }
     __syncthreads();
     const int total = (int)(a1 - a0);
-    PdWalk seg = {s_start[0], s_start[1], s_start[2], s_start[3]};
+    PdWalk seg = {s_start[0], s_start[1], s_start[2], s_start[3], s_start[1] / n_hg};
     PdWalk iss = seg;
     int iss_i = warp;   // local index of the next step to issue
-    iss.go(warp, b, H, err);
+    iss.go(warp, b, H, n_hg, err);
 
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * C::NST * C::STAGE;
-    const uint8_t* ring_p = sm + warp * C::NST * C::STAGE;
-    float* meet = reinterpret_cast<float*>(sm + PD_W * C::NST * C::STAGE);
+    // q of head g: columns 32 j + 8 t .. + 7
+    float qx[NB][8];
+    auto load_q = [&](const PdWalk& w) {
+        const int kvh = w.kvh, hg = w.h - w.kvh * n_hg;
+        const A* src = q + (size_t)w.s * ldq + (size_t)(kvh * group + hg * PD_HEADS + g) * HD + 8 * t;
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) qx[j][i] = 0.f;
+            if (g < group - hg * PD_HEADS) act_load8(src + 32 * j, qx[j]);
+        }
+    };
+    load_q(seg);
+
+    uint8_t* ring_p = sm + warp * C::NST * 2 * C::KB;
+    uint8_t* scales_p = sm + C::SCALES + warp * C::NST * 2 * C::SB;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_p), scales = (uint32_t)__cvta_generic_to_shared(scales_p);
+    float* meet = reinterpret_cast<float*>(sm + C::MEET);
     float2* meet_ml = reinterpret_cast<float2*>(meet + PD_W * PD_HEADS * C::OP);
 
     int iss_page = 0;
@@ -212,59 +265,49 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
         }
     };
     fetch_page();
-    auto issue = [&](int slot) {
-        if (iss_i < total) {
-            const int row = (iss.st << 4) & ((1 << c.shift) - 1);
-            const size_t off = (size_t)iss_page * c.page_bytes + (size_t)(iss.h / n_hg) * c.slab;
-            const uint32_t dst = ring + slot * C::STAGE;
-            if (!C::Q8) {   // every lane copies the 16-byte runs that it will use itself
-                const uint8_t* ks = c.k + off + (size_t)(row + g) * HD * 2 + t * 16;
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int j = 0; j < NB; j++)
-                        pd_cp16(dst + (i * NB + j) * 512 + lane * 16, ks + i * 8 * HD * 2 + j * 64);
-                const uint8_t* vs = c.v + off + (size_t)(row + 2 * t) * HD * 2 + g * 16;
-#pragma unroll
-                for (int kk = 0; kk < 4; kk++)
-#pragma unroll
-                    for (int j = 0; j < HD / 64; j++)
-                        pd_cp16(dst + C::KB + (kk * (HD / 64) + j) * 512 + lane * 16,
-                                vs + ((kk >> 1) * 8 + (kk & 1)) * HD * 2 + j * 128);
-            } else {   // rows as they lie, 32-byte units exchanged so that the reads below spread over the banks
-                constexpr int CPR = HD / 16;   // 16-byte runs per row
-                const uint8_t* ks = c.k + off + row * HD + lane * 16;
-                const uint8_t* vs = c.v + off + row * HD + lane * 16;
-#pragma unroll
-                for (int i = 0; i < 16 * CPR / 32; i++) {
-                    const int r = i * (32 / CPR) + lane / CPR, ch = lane % CPR;
-                    const int fk = HD == 128 ? (r & 3) : ((r >> 1) & 1), fv = HD == 128 ? ((r >> 1) & 3) : ((r >> 1) & 1);
-                    pd_cp16(dst + r * HD + ((ch ^ (2 * fk)) * 16), ks + i * 512);
-                    pd_cp16(dst + C::KB + r * HD + ((ch ^ (2 * fv)) * 16), vs + i * 512);
-                }
-                if (lane < 2 * (HD / 16)) {   // scales: 16 rows of HD / 32 halves
-                    const int ch = lane % (HD / 16);
-                    const uint8_t* src = (lane < HD / 16 ? c.k : c.v) + off + ((size_t)HD << c.shift) +
-                                         (size_t)row * (HD / 16) + ch * 16;
-                    pd_cp16(dst + 2 * C::KB + (lane < HD / 16 ? 0 : C::SB) + ch * 16, src);
-                }
+    auto issue = [&](int slot) {   // every lane is done with the slot's rows
+        if (iss_i >= total) return;
+        if (lane == 0) {
+            const int row = (iss.st << 4) & ((1 << c.shift) - 1), kvh = iss.kvh;
+            const uint32_t dst = ring + slot * 2 * C::KB, bar = bars + 8 * slot;
+            mbs_expect(bar, 2 * (C::KB + C::SB));
+            pd_tma(dst, &kmap, row, iss_page * c.n_kv + kvh, !C::Q8, bar);
+            pd_tma(dst + C::KB, &vmap, row, iss_page * c.n_kv + kvh, !C::Q8, bar);
+            if (C::Q8) {
+                const size_t off = (size_t)iss_page * c.page_bytes + (size_t)kvh * c.slab + ((size_t)HD << c.shift) +
+                                   (size_t)row * (HD / 16);
+                pd_bulk(scales + slot * 2 * C::SB, c.k + off, C::SB, bar);
+                pd_bulk(scales + slot * 2 * C::SB + C::SB, c.v + off, C::SB, bar);
             }
-            iss_i += PD_W;
-            iss.go(PD_W, b, H, err);
-            fetch_page();
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        iss_i += PD_W;
+        iss.go(PD_W, b, H, n_hg, err);
+        fetch_page();
     };
 #pragma unroll
     for (int i = 0; i < C::NST - 1; i++) issue(i);
     int slot = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+
+    // This lane's places in a step's rows; the column block j only flips bits of
+    // the swizzled offset, and rows 8 on are a constant further.
+    auto unit = [](int r, int u) {   // 16-byte unit u of row r
+        if (!C::Q8 || HD == 128) return r * 128 + (((u ^ r) & 7) << 4);
+        return r * 64 + (((u ^ (r >> 1)) & 3) << 4);
+    };
+    const int k_off = C::Q8 ? unit(pd_row<HD, DT>(g), t >> 1) + (t & 1) * 8 : unit(pd_row<HD, DT>(g), t);
+    int v_off[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        v_off[i] = C::Q8 ? unit(pd_row<HD, DT>(2 * t + i), g >> 2) + (g & 3) * 4 : unit(pd_row<HD, DT>(2 * t + i), g);
 
     const float scale2 = (1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
     int done = 0;            // local index where the segment starts
     int next = warp;         // local index of this warp's next step
     while (done < total) {
         const int seg_n = min(seg.nst - seg.st, total - done);   // steps of this segment here
-        const int kvh = seg.h / n_hg, hg = seg.h % n_hg;
+        const int kvh = seg.kvh, hg = seg.h - seg.kvh * n_hg;
         const int n_heads = min(PD_HEADS, group - hg * PD_HEADS);
         const int len = seq_len(b, seg.s, err);
         // state of heads 2 t, 2 t + 1; O: tile pair u's columns 16 u + g, 16 u + 8 + g (fragment order)
@@ -276,20 +319,15 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
 #pragma unroll
             for (int i = 0; i < 4; i++) O[n][i] = 0.f;
         if (next < done + seg_n) {
-            // ---- q of head g: columns 32 j + 8 t .. + 7, scaled by a power of two and split
+            // ---- q scaled by a power of two per head, and split
             uint32_t qh[2 * NB][2], ql[2 * NB][2];
             float sc[2], isc[2];   // raw score -> log2 units of heads 2 t, 2 t + 1, and back
             {
-                float x[NB][8], mx = 0.f;
-                const A* src = q + (size_t)seg.s * ldq + (size_t)(kvh * group + hg * PD_HEADS + g) * HD + 8 * t;
+                float mx = 0.f;
 #pragma unroll
-                for (int j = 0; j < NB; j++) {
+                for (int j = 0; j < NB; j++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[j][i] = 0.f;
-                    if (g < n_heads) act_load8(src + 32 * j, x[j]);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[j][i]));
-                }
+                    for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(qx[j][i]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const int e = tc::f16_scale_exp(__float_as_uint(mx));
@@ -304,20 +342,22 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
                 for (int j = 0; j < NB; j++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        pd_pair<A>(x[j][2 * i] * up, x[j][2 * i + 1] * up, qh[2 * j + (i >> 1)][i & 1],
+                        pd_pair<A>(qx[j][2 * i] * up, qx[j][2 * i + 1] * up, qh[2 * j + (i >> 1)][i & 1],
                                    ql[2 * j + (i >> 1)][i & 1]);
             }
             // One step; TAIL: only `left` of its keys belong to the sequence.
-            auto step = [&](const uint8_t* st, auto tail, int left) {
+            auto step = [&](const uint8_t* st, const uint8_t* ss, auto tail, int left) {
                 constexpr bool TAIL = decltype(tail)::value;
-                // ---- raw scores x[i][h] of keys g + 8 i, heads 2 t + h
+                const int rg = pd_row<HD, DT>(g);   // keys rg, rg + 8 stand at rows g, g + 8
+                // ---- raw scores x[i][h] of keys rg + 8 i, heads 2 t + h
                 float x[2][2];
                 if (!C::Q8) {
                     float sa[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int j = 0; j < NB; j++) {
-                        const uint4 k0 = *reinterpret_cast<const uint4*>(st + j * 512 + lane * 16);
-                        const uint4 k1 = *reinterpret_cast<const uint4*>(st + (NB + j) * 512 + lane * 16);
+                        const uint8_t* kp = st + (j >> 1) * 2048 + (k_off ^ ((j & 1) * 64));
+                        const uint4 k0 = *reinterpret_cast<const uint4*>(kp);
+                        const uint4 k1 = *reinterpret_cast<const uint4*>(kp + 8 * 128);
                         pd_mma(sa, k0.x, k1.x, k0.y, k1.y, qh[2 * j][0], qh[2 * j][1]);
                         pd_mma(sa, k0.z, k1.z, k0.w, k1.w, qh[2 * j + 1][0], qh[2 * j + 1][1]);
                         if (sizeof(A) == 4) {
@@ -327,19 +367,18 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
                     }
                     x[0][0] = sa[0]; x[0][1] = sa[1]; x[1][0] = sa[2]; x[1][1] = sa[3];
                 } else {
-                    const int f = HD == 128 ? (g & 3) : ((g >> 1) & 1);   // the same for row g + 8
                     __half sk[2][NB];
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         x[i][0] = x[i][1] = 0.f;
-                        const uint8_t* sp = st + 2 * C::KB + (8 * i + g) * (HD / 16);
+                        const uint8_t* sp = ss + (8 * i + rg) * (HD / 16);
                         if (HD == 128) *reinterpret_cast<uint2*>(&sk[i][0]) = *reinterpret_cast<const uint2*>(sp);
                         else *reinterpret_cast<uint32_t*>(&sk[i][0]) = *reinterpret_cast<const uint32_t*>(sp);
                     }
 #pragma unroll
                     for (int j = 0; j < NB; j++) {
-                        uint2 w0 = *reinterpret_cast<const uint2*>(st + g * HD + ((j ^ f) * 32) + 8 * t);
-                        uint2 w1 = *reinterpret_cast<const uint2*>(st + (g + 8) * HD + ((j ^ f) * 32) + 8 * t);
+                        const uint8_t* kp = st + (k_off ^ (j * 32));
+                        uint2 w0 = *reinterpret_cast<const uint2*>(kp), w1 = *reinterpret_cast<const uint2*>(kp + 8 * HD);
                         w0.x ^= 0x80808080u; w0.y ^= 0x80808080u; w1.x ^= 0x80808080u; w1.y ^= 0x80808080u;
                         const uint32_t a0 = pd_codes(w0.x, 0x4140), a1 = pd_codes(w1.x, 0x4140);
                         const uint32_t a2 = pd_codes(w0.x, 0x4342), a3 = pd_codes(w1.x, 0x4342);
@@ -359,12 +398,12 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
                         x[1][1] = fmaf(sa[3], d1, x[1][1]);
                     }
                 }
-                // ---- the V scales of keys g, g + 8; keys past the sequence weigh nothing
+                // ---- the V scales of keys rg, rg + 8; keys past the sequence weigh nothing
                 __half sv[2][NB];
                 if (C::Q8) {
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        const uint8_t* sp = st + 2 * C::KB + C::SB + (8 * i + g) * (HD / 16);
+                        const uint8_t* sp = ss + C::SB + (8 * i + rg) * (HD / 16);
                         if (HD == 128) *reinterpret_cast<uint2*>(&sv[i][0]) = *reinterpret_cast<const uint2*>(sp);
                         else *reinterpret_cast<uint32_t*>(&sv[i][0]) = *reinterpret_cast<const uint32_t*>(sp);
                     }
@@ -372,7 +411,7 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
                 if (TAIL) {
 #pragma unroll
                     for (int i = 0; i < 2; i++)
-                        if (8 * i + g >= left) {
+                        if (8 * i + rg >= left) {
                             x[i][0] = x[i][1] = -INFINITY;
                             if (C::Q8)
 #pragma unroll
@@ -442,13 +481,13 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
                         uint32_t v[4][4];
 #pragma unroll
                         for (int kk = 0; kk < 4; kk++) {
-                            const uint4 w =
-                                *reinterpret_cast<const uint4*>(st + C::KB + (kk * (HD / 64) + j) * 512 + lane * 16);
+                            const int r = pd_row<HD, DT>(2 * t + (kk & 1)) + (kk >> 1) * 8;
+                            const uint4 w = *reinterpret_cast<const uint4*>(st + C::KB + j * 2048 + (kk >> 1) * 1024 + v_off[kk & 1]);
                             v[kk][0] = w.x;
                             v[kk][1] = w.y;
                             v[kk][2] = w.z;
                             v[kk][3] = w.w;
-                            if (TAIL && (kk >> 1) * 8 + 2 * t + (kk & 1) >= left)   // stale rows may hold anything
+                            if (TAIL && r >= left)   // stale rows may hold anything
                                 v[kk][0] = v[kk][1] = v[kk][2] = v[kk][3] = 0u;
                         }
 #pragma unroll
@@ -477,9 +516,7 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
                         }
 #pragma unroll
                         for (int kk = 0; kk < 4; kk++) {
-                            const int r = (kk >> 1) * 8 + 2 * t + (kk & 1);
-                            const int f = HD == 128 ? t : (t & 1);   // (r >> 1) & 3, & 1
-                            w[kk] = *reinterpret_cast<const uint32_t*>(st + C::KB + r * HD + ((j ^ f) * 32) + 4 * g) ^
+                            w[kk] = *reinterpret_cast<const uint32_t*>(st + C::KB + (kk >> 1) * 8 * HD + (v_off[kk & 1] ^ (j * 32))) ^
                                     0x80808080u;
                         }
 #pragma unroll
@@ -495,15 +532,24 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
                 }
             };
             for (; next < done + seg_n; next += PD_W) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(C::NST - 2) : "memory");
-                __syncwarp();
+                __syncwarp();   // the slot before has been read
                 issue(slot == 0 ? C::NST - 1 : slot - 1);
-                const uint8_t* st = ring_p + slot * C::STAGE;
-                slot = slot + 1 == C::NST ? 0 : slot + 1;
+                if (ok) ok = mbs_wait(bars + 8 * slot, parity, err);
+                const uint8_t *st = ring_p + slot * 2 * C::KB, *ss = scales_p + slot * 2 * C::SB;
+                if (++slot == C::NST) {
+                    slot = 0;
+                    parity ^= 1;
+                }
                 const int left = len - ((seg.st + next - done) << 4);   // at least 1
-                if (left >= 16) step(st, std::false_type{}, 16);
-                else step(st, std::true_type{}, left);
+                if (left >= 16) step(st, ss, std::false_type{}, 16);
+                else step(st, ss, std::true_type{}, left);
             }
+        }
+        // the next segment and its q, ahead of the meeting
+        PdWalk after = seg;
+        if (done + seg_n < total) {
+            after.go(seg_n, b, H, n_hg, err);
+            load_q(after);
         }
         // ---- the warps meet
         {
@@ -523,12 +569,12 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
             }
         }
         __syncthreads();
-        const unsigned long long gs = a0 + done - seg.st, ge = gs + seg.nst;   // the whole segment's steps
+        const unsigned gs = a0 + done - seg.st, ge = gs + seg.nst;   // the whole segment's steps
         const bool whole = gs >= a0 && ge <= a1;
         const int slot_out = gs >= a0 ? 1 : 0;
         float* mp = part + ((size_t)blockIdx.x * 2 + slot_out) * (PD_HEADS * (HD + 2));
         const size_t o0 = (size_t)seg.s * ldo + (size_t)(kvh * group + hg * PD_HEADS) * HD;
-        for (int i = tid; i < n_heads * seg_cols; i += PD_W * 32) {
+        for (int i = tid; i < n_heads * HD; i += PD_W * 32) {
             const int h = i / HD, p = i % HD;
             float2 ml[PD_W];
             float M = -INFINITY, L = 0.f, V = 0.f;
@@ -609,9 +655,8 @@ k_paged_decode(const PagedView c, const BatchView b, const A* __restrict__ q, in
         }
         __syncthreads();   // the meeting area is free again
         done += seg_n;
-        if (done < total) seg.go(seg_n, b, H, err);
+        seg = after;
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 static_assert((size_t)GB_MAX_SMS * PD_MAX_CTAS * 2 * PD_HEADS * (128 + 2) * 4 <= PAGED_PART_BYTES, "workspace");
@@ -623,17 +668,15 @@ static cudaError_t launch_decode(const PagedView& c, const BatchView& b, const v
     const void* f = reinterpret_cast<const void*>(k_paged_decode<A, HD, DT>);
     cudaError_t e = set_smem_once(f, C::SMEM);
     if (e != cudaSuccess) return e;
-    static const int per_sm = [&] {   // CTAs an SM holds: a property of the build
-        int n = 0;
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, f, PD_W * 32, C::SMEM);
-        return n < 1 ? 1 : n > PD_MAX_CTAS ? PD_MAX_CTAS : n;
-    }();
+    CUtensorMap km = {}, vm = {};
+    if (!paged_encode_steps(&km, c.k, DT, HD, 1 << c.shift, (size_t)c.n_pages * c.n_kv) ||
+        !paged_encode_steps(&vm, c.v, DT, HD, 1 << c.shift, (size_t)c.n_pages * c.n_kv))
+        return cudaErrorUnknown;
     const int n_hg = (group + PD_HEADS - 1) / PD_HEADS;
     unsigned* tickets = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(ws) + PAGED_TICKETS_AT);
-    k_paged_decode<A, HD, DT><<<sm_count() * per_sm, PD_W * 32, C::SMEM, st>>>(
-        c, b, static_cast<const A*>(q), ldq, group, n_hg, static_cast<A*>(out), ldo, tickets, static_cast<float*>(ws),
-        PD_MIN_STEPS, err);
-    return cudaGetLastError();
+    return launch_pdl(k_paged_decode<A, HD, DT>, dim3(sm_count() * pd_ctas<HD, DT>()), PD_W * 32, C::SMEM, st, km, vm, c, b,
+                      static_cast<const A*>(q), ldq, group, n_hg, static_cast<A*>(out), ldo, tickets,
+                      static_cast<float*>(ws), PD_MIN_STEPS, err);
 }
 
 static int paged_attention(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q, int ldq,
@@ -652,6 +695,8 @@ static int paged_attention(const gb_kv_cache* cache, const gb_kv_batch* batch, i
     if (!err) return GB_ECUDA;
     const int group = n_heads / c.n_kv;
     if (decode) {
+        const long long heads8 = (long long)c.n_kv * ((group + PD_HEADS - 1) / PD_HEADS);
+        if ((long long)b.n_seq * (b.cap / 16 + 1) * heads8 > 0x7fffffffLL) return GB_ELIMIT;   // steps
         cudaError_t e = cudaErrorInvalidValue;
 #define GB_DECODE(T, A, HD, DT)                                \
     if (dtype == T && hd == HD && cache->dtype == DT)          \
