@@ -26,7 +26,8 @@ namespace gb {
 // heads) pairs and enter the second as (2 keys, head) pairs: an 8 x 8
 // transposition in registers (movmatrix).
 //
-// Work: a step is 16 keys of one (sequence, KV head, 8 query heads); all
+// Work: a step is 16 keys (Q8_0: 32, the same bytes) of one (sequence, KV
+// head, 8 query heads); all
 // steps of the batch, in that order, are cut into one equal run per CTA
 // whatever the sequences' lengths, and the CTA's warps take its steps in turn.
 // Each warp streams its own steps through a ring of TMA copies (16 rows of K and
@@ -38,7 +39,7 @@ namespace gb {
 // PD_TAU (log2 units), so a step needs no reduction but one vote; p = 2^(x - m
 // + PD_LIFT) keeps the fp16 parts of small probabilities normal.  Q8_0: p
 // times a scale is brought below 2^14 by a power of two, 2^-E, shared by the
-// warp; O is in units of 2^E.
+// warp; l and O are in units of 2^E.
 constexpr int PD_W = 4;              // warps
 constexpr int PD_MAX_CTAS = 4;       // CTAs per SM the workspace has room for
 constexpr int PD_MIN_STEPS = 4;      // fewest steps of a CTA
@@ -49,17 +50,22 @@ constexpr float PD_TAU = 8.f, PD_LIFT = 6.f;
 template <int HD, int DT>
 struct PdCfg {
     static constexpr bool Q8 = DT == GB_DT_Q8_0;
-    static constexpr int KB = 16 * HD * (Q8 ? 1 : 2);   // bytes of a step's K (or V) rows
-    static constexpr int SB = Q8 ? HD : 0;              // and of their scales
-    static constexpr int NST = 3;
+    static constexpr int KEYS = Q8 ? 32 : 16;           // keys of a step
+    static constexpr int SUB = KEYS / 16;               // its runs of 16, a TMA box each
+    static constexpr int SHIFT = Q8 ? 5 : 4;
+    static constexpr int KB = KEYS * HD * (Q8 ? 1 : 2); // bytes of a step's K (or V) rows
+    static constexpr int SB = Q8 ? KEYS * HD / 16 : 0;  // and of their scales
+    static constexpr int NST = Q8 && HD == 128 ? 2 : 3; // stages: three CTAs an SM at Q8_0 and hd 128
     static constexpr int OP = HD + 4;                   // row pitch of the meeting area (bank spread)
-    // shared: rows [PD_W][NST][2 KB], scales [PD_W][NST][2 SB], meeting area
-    // O [PD_W][8][OP] and (m, l) [PD_W][8], barriers [PD_W][NST], scan [PD_W], start [4], last
+    // shared: rows [PD_W][NST][2 KB], scales [PD_W][NST][2 SB], barriers
+    // [PD_W][NST], scan [PD_W], start [4], last, free slot [PD_W].  The warps
+    // meet in their rings: a warp's slot before the current one is free then,
+    // and takes its O [8][OP] and (m, l) [8].
     static constexpr int SCALES = PD_W * NST * 2 * KB;
-    static constexpr int MEET = SCALES + PD_W * NST * 2 * SB;
-    static constexpr int BARS = MEET + PD_W * PD_HEADS * (OP * 4 + 8);
+    static constexpr int BARS = SCALES + PD_W * NST * 2 * SB;
     static constexpr int SCAN = BARS + PD_W * NST * 8;
-    static constexpr int SMEM = SCAN + (PD_W + 5) * 4;
+    static_assert(PD_HEADS * (OP * 4 + 8) <= 2 * KB, "a slot holds a warp's results");
+    static constexpr int SMEM = SCAN + (2 * PD_W + 5) * 4;
 };
 
 // CTAs per SM: what the shared memory holds, at most PD_MAX_CTAS (registers follow).
@@ -144,6 +150,7 @@ __device__ __forceinline__ float pd_ex2(float x) {
 
 // A walk over steps: sequence s, segment h of it, step st of nst; kvh: the
 // segment's KV head.
+template <int SHIFT>
 struct PdWalk {
     int s, h, st, nst, kvh;
     __device__ __forceinline__ void go(int by, const BatchView& b, int H, int n_hg, unsigned* err) {
@@ -153,7 +160,7 @@ struct PdWalk {
             st -= nst;
             if (++h == H) {
                 h = 0;
-                do nst = ++s < b.n_seq ? (seq_len(b, s, err) + 15) >> 4 : 0x7fffffff;   // past the end: no step is taken
+                do nst = ++s < b.n_seq ? (seq_len(b, s, err) + (1 << SHIFT) - 1) >> SHIFT : 0x7fffffff;   // past the end: no step is taken
                 while (nst == 0);
             }
         } while (st >= nst);
@@ -180,6 +187,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
     unsigned* s_scan = reinterpret_cast<unsigned*>(sm + C::SCAN);
     int* s_start = reinterpret_cast<int*>(s_scan + PD_W);
     unsigned& s_last = s_scan[PD_W + 4];
+    unsigned* s_free = s_scan + PD_W + 5;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int H = c.n_kv * n_hg;
     const uint32_t bars = (uint32_t)__cvta_generic_to_shared(sm + C::BARS) + warp * C::NST * 8;
@@ -194,7 +202,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
     const int per = (b.n_seq + PD_W * 32 - 1) / (PD_W * 32);
     const int s_lo = min(tid * per, b.n_seq), s_hi = min(s_lo + per, b.n_seq);
     unsigned mine = 0;
-    for (int s = s_lo; s < s_hi; s++) mine += (seq_len(b, s, err) + 15) >> 4;
+    for (int s = s_lo; s < s_hi; s++) mine += (seq_len(b, s, err) + C::KEYS - 1) >> C::SHIFT;
     unsigned incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -220,7 +228,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
     {
         unsigned at = (base + incl - mine) * H;   // first step of sequence s_lo
         for (int s = s_lo; s < s_hi; s++) {
-            const unsigned n = (unsigned)(seq_len(b, s, err) + 15) >> 4, next = at + n * H;
+            const unsigned n = (unsigned)(seq_len(b, s, err) + C::KEYS - 1) >> C::SHIFT, next = at + n * H;
             if (a0 >= at && a0 < next) {
                 s_start[0] = s;
                 s_start[1] = (int)((a0 - at) / n);
@@ -232,14 +240,15 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
     }
     __syncthreads();
     const int total = (int)(a1 - a0);
-    PdWalk seg = {s_start[0], s_start[1], s_start[2], s_start[3], s_start[1] / n_hg};
-    PdWalk iss = seg;
+    using Walk = PdWalk<C::SHIFT>;
+    Walk seg = {s_start[0], s_start[1], s_start[2], s_start[3], s_start[1] / n_hg};
+    Walk iss = seg;
     int iss_i = warp;   // local index of the next step to issue
     iss.go(warp, b, H, n_hg, err);
 
     // q of head g: columns 32 j + 8 t .. + 7
     float qx[NB][8];
-    auto load_q = [&](const PdWalk& w) {
+    auto load_q = [&](const Walk& w) {
         const int kvh = w.kvh, hg = w.h - w.kvh * n_hg;
         const A* src = q + (size_t)w.s * ldq + (size_t)(kvh * group + hg * PD_HEADS + g) * HD + 8 * t;
 #pragma unroll
@@ -254,30 +263,33 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
     uint8_t* ring_p = sm + warp * C::NST * 2 * C::KB;
     uint8_t* scales_p = sm + C::SCALES + warp * C::NST * 2 * C::SB;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_p), scales = (uint32_t)__cvta_generic_to_shared(scales_p);
-    float* meet = reinterpret_cast<float*>(sm + C::MEET);
-    float2* meet_ml = reinterpret_cast<float2*>(meet + PD_W * PD_HEADS * C::OP);
 
-    int iss_page = 0;
+    // lane i < SUB sees to the step's keys 16 i .. + 15: page, box, scales
+    int iss_page = 0, iss_n = 0;   // page of this lane's run; runs with keys of the sequence
     auto fetch_page = [&] {
         if (iss_i < total) {
-            iss_page = page_of(c, b, iss.s, iss.st << 4, err);
+            iss_n = C::SUB == 1 ? 1 : min(C::SUB, (seq_len(b, iss.s, err) - (iss.st << C::SHIFT) + 15) >> 4);
+            iss_page = page_of(c, b, iss.s, (iss.st << C::SHIFT) + (C::SUB == 1 ? 0 : 16 * min(lane, iss_n - 1)), err);
             if (iss_page < 0) iss_page = 0;
         }
     };
     fetch_page();
     auto issue = [&](int slot) {   // every lane is done with the slot's rows
         if (iss_i >= total) return;
-        if (lane == 0) {
-            const int row = (iss.st << 4) & ((1 << c.shift) - 1), kvh = iss.kvh;
-            const uint32_t dst = ring + slot * 2 * C::KB, bar = bars + 8 * slot;
-            mbs_expect(bar, 2 * (C::KB + C::SB));
-            pd_tma(dst, &kmap, row, iss_page * c.n_kv + kvh, !C::Q8, bar);
-            pd_tma(dst + C::KB, &vmap, row, iss_page * c.n_kv + kvh, !C::Q8, bar);
+        const uint32_t bar = bars + 8 * slot;
+        if (lane == 0) mbs_expect(bar, iss_n * (2 * (C::KB + C::SB) / C::SUB));
+        __syncwarp();
+        if (lane < iss_n) {
+            const int row = ((iss.st << C::SHIFT) + 16 * lane) & ((1 << c.shift) - 1);
+            const uint32_t dst = ring + slot * 2 * C::KB + lane * (C::KB / C::SUB);
+            pd_tma(dst, &kmap, row, iss_page * c.n_kv + iss.kvh, !C::Q8, bar);
+            pd_tma(dst + C::KB, &vmap, row, iss_page * c.n_kv + iss.kvh, !C::Q8, bar);
             if (C::Q8) {
-                const size_t off = (size_t)iss_page * c.page_bytes + (size_t)kvh * c.slab + ((size_t)HD << c.shift) +
+                const size_t off = (size_t)iss_page * c.page_bytes + (size_t)iss.kvh * c.slab + ((size_t)HD << c.shift) +
                                    (size_t)row * (HD / 16);
-                pd_bulk(scales + slot * 2 * C::SB, c.k + off, C::SB, bar);
-                pd_bulk(scales + slot * 2 * C::SB + C::SB, c.v + off, C::SB, bar);
+                const uint32_t sdst = scales + slot * 2 * C::SB + lane * HD;
+                pd_bulk(sdst, c.k + off, HD, bar);
+                pd_bulk(sdst + C::SB, c.v + off, HD, bar);
             }
         }
         iss_i += PD_W;
@@ -311,7 +323,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
         const int n_heads = min(PD_HEADS, group - hg * PD_HEADS);
         const int len = seq_len(b, seg.s, err);
         // state of heads 2 t, 2 t + 1; O: tile pair u's columns 16 u + g, 16 u + 8 + g (fragment order)
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, thr[2] = {-INFINITY, -INFINITY}, O[NT / 2][4];
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, thr[2] = {-INFINITY, -INFINITY}, off[2] = {0.f, 0.f}, O[NT / 2][4];
         int E = -40;
         __half top = __float2half_rn(0.f);   // 2^E, the scales' bound (0 before the first step)
 #pragma unroll
@@ -350,7 +362,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                 constexpr bool TAIL = decltype(tail)::value;
                 const int rg = pd_row<HD, DT>(g);   // keys rg, rg + 8 stand at rows g, g + 8
                 // ---- raw scores x[i][h] of keys rg + 8 i, heads 2 t + h
-                float x[2][2];
+                float x[2 * C::SUB][2];
                 if (!C::Q8) {
                     float sa[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -367,42 +379,45 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                     }
                     x[0][0] = sa[0]; x[0][1] = sa[1]; x[1][0] = sa[2]; x[1][1] = sa[3];
                 } else {
-                    __half sk[2][NB];
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        x[i][0] = x[i][1] = 0.f;
-                        const uint8_t* sp = ss + (8 * i + rg) * (HD / 16);
-                        if (HD == 128) *reinterpret_cast<uint2*>(&sk[i][0]) = *reinterpret_cast<const uint2*>(sp);
-                        else *reinterpret_cast<uint32_t*>(&sk[i][0]) = *reinterpret_cast<const uint32_t*>(sp);
-                    }
+                    for (int u = 0; u < C::SUB; u++) {
+                        __half sk[2][NB];
 #pragma unroll
-                    for (int j = 0; j < NB; j++) {
-                        const uint8_t* kp = st + (k_off ^ (j * 32));
-                        uint2 w0 = *reinterpret_cast<const uint2*>(kp), w1 = *reinterpret_cast<const uint2*>(kp + 8 * HD);
-                        w0.x ^= 0x80808080u; w0.y ^= 0x80808080u; w1.x ^= 0x80808080u; w1.y ^= 0x80808080u;
-                        const uint32_t a0 = pd_codes(w0.x, 0x4140), a1 = pd_codes(w1.x, 0x4140);
-                        const uint32_t a2 = pd_codes(w0.x, 0x4342), a3 = pd_codes(w1.x, 0x4342);
-                        const uint32_t c0 = pd_codes(w0.y, 0x4140), c1 = pd_codes(w1.y, 0x4140);
-                        const uint32_t c2 = pd_codes(w0.y, 0x4342), c3 = pd_codes(w1.y, 0x4342);
-                        float sa[4] = {0.f, 0.f, 0.f, 0.f};
-                        pd_mma(sa, a0, a1, a2, a3, qh[2 * j][0], qh[2 * j][1]);
-                        pd_mma(sa, c0, c1, c2, c3, qh[2 * j + 1][0], qh[2 * j + 1][1]);
-                        if (sizeof(A) == 4) {
-                            pd_mma(sa, a0, a1, a2, a3, ql[2 * j][0], ql[2 * j][1]);
-                            pd_mma(sa, c0, c1, c2, c3, ql[2 * j + 1][0], ql[2 * j + 1][1]);
+                        for (int i = 0; i < 2; i++) {
+                            x[2 * u + i][0] = x[2 * u + i][1] = 0.f;
+                            const uint8_t* sp = ss + (16 * u + 8 * i + rg) * (HD / 16);
+                            if (HD == 128) *reinterpret_cast<uint2*>(&sk[i][0]) = *reinterpret_cast<const uint2*>(sp);
+                            else *reinterpret_cast<uint32_t*>(&sk[i][0]) = *reinterpret_cast<const uint32_t*>(sp);
                         }
-                        const float d0 = __half2float(sk[0][j]), d1 = __half2float(sk[1][j]);
-                        x[0][0] = fmaf(sa[0], d0, x[0][0]);
-                        x[0][1] = fmaf(sa[1], d0, x[0][1]);
-                        x[1][0] = fmaf(sa[2], d1, x[1][0]);
-                        x[1][1] = fmaf(sa[3], d1, x[1][1]);
+#pragma unroll
+                        for (int j = 0; j < NB; j++) {
+                            const uint8_t* kp = st + u * 16 * HD + (k_off ^ (j * 32));
+                            uint2 w0 = *reinterpret_cast<const uint2*>(kp), w1 = *reinterpret_cast<const uint2*>(kp + 8 * HD);
+                            w0.x ^= 0x80808080u; w0.y ^= 0x80808080u; w1.x ^= 0x80808080u; w1.y ^= 0x80808080u;
+                            const uint32_t a0 = pd_codes(w0.x, 0x4140), a1 = pd_codes(w1.x, 0x4140);
+                            const uint32_t a2 = pd_codes(w0.x, 0x4342), a3 = pd_codes(w1.x, 0x4342);
+                            const uint32_t c0 = pd_codes(w0.y, 0x4140), c1 = pd_codes(w1.y, 0x4140);
+                            const uint32_t c2 = pd_codes(w0.y, 0x4342), c3 = pd_codes(w1.y, 0x4342);
+                            float sa[4] = {0.f, 0.f, 0.f, 0.f};
+                            pd_mma(sa, a0, a1, a2, a3, qh[2 * j][0], qh[2 * j][1]);
+                            pd_mma(sa, c0, c1, c2, c3, qh[2 * j + 1][0], qh[2 * j + 1][1]);
+                            if (sizeof(A) == 4) {
+                                pd_mma(sa, a0, a1, a2, a3, ql[2 * j][0], ql[2 * j][1]);
+                                pd_mma(sa, c0, c1, c2, c3, ql[2 * j + 1][0], ql[2 * j + 1][1]);
+                            }
+                            const float d0 = __half2float(sk[0][j]), d1 = __half2float(sk[1][j]);
+                            x[2 * u][0] = fmaf(sa[0], d0, x[2 * u][0]);
+                            x[2 * u][1] = fmaf(sa[1], d0, x[2 * u][1]);
+                            x[2 * u + 1][0] = fmaf(sa[2], d1, x[2 * u + 1][0]);
+                            x[2 * u + 1][1] = fmaf(sa[3], d1, x[2 * u + 1][1]);
+                        }
                     }
                 }
-                // ---- the V scales of keys rg, rg + 8; keys past the sequence weigh nothing
-                __half sv[2][NB];
+                // ---- the V scales of keys rg + 8 i; keys past the sequence weigh nothing
+                __half sv[2 * C::SUB][NB];
                 if (C::Q8) {
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
+                    for (int i = 0; i < 2 * C::SUB; i++) {
                         const uint8_t* sp = ss + C::SB + (8 * i + rg) * (HD / 16);
                         if (HD == 128) *reinterpret_cast<uint2*>(&sv[i][0]) = *reinterpret_cast<const uint2*>(sp);
                         else *reinterpret_cast<uint32_t*>(&sv[i][0]) = *reinterpret_cast<const uint32_t*>(sp);
@@ -410,7 +425,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                 }
                 if (TAIL) {
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
+                    for (int i = 0; i < 2 * C::SUB; i++)
                         if (8 * i + rg >= left) {
                             x[i][0] = x[i][1] = -INFINITY;
                             if (C::Q8)
@@ -419,13 +434,19 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                         }
                 }
                 // ---- does a score pass the maximum by PD_TAU, or a scale its bound?
-                bool moved = fmaxf(x[0][0], x[1][0]) > thr[0] || fmaxf(x[0][1], x[1][1]) > thr[1];
+                float mx[2] = {x[0][0], x[0][1]};
+#pragma unroll
+                for (int i = 1; i < 2 * C::SUB; i++) {
+                    mx[0] = fmaxf(mx[0], x[i][0]);
+                    mx[1] = fmaxf(mx[1], x[i][1]);
+                }
+                bool moved = mx[0] > thr[0] || mx[1] > thr[1];
                 __half dm = __float2half_rn(0.f);
                 if (C::Q8) {
                     const __half2* d2 = reinterpret_cast<const __half2*>(&sv[0][0]);
                     __half2 y = d2[0];
 #pragma unroll
-                    for (int j = 1; j < NB; j++) y = __hmax2(y, d2[j]);
+                    for (int j = 1; j < NB * C::SUB; j++) y = __hmax2(y, d2[j]);
                     dm = __hmax(__low2half(y), __high2half(y));
                     moved |= __hgt(dm, top);
                 }
@@ -444,27 +465,26 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                     float al[2];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        float mx = fmaxf(x[0][h], x[1][h]);
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                        const float mn = fmaxf(m[h], mx * sc[h]);
-                        al[h] = m[h] == -INFINITY ? 0.f : pd_ex2(m[h] - mn);
+                        for (int o = 4; o < 32; o <<= 1) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], o));
+                        const float mn = fmaxf(m[h], mx[h] * sc[h]);
+                        al[h] = m[h] == -INFINITY ? 0.f : pd_ex2(m[h] - mn) * up;
                         l[h] *= al[h];
                         m[h] = mn;
                         thr[h] = (mn + PD_TAU) * isc[h];
-                        al[h] *= up;
+                        off[h] = PD_LIFT - mn - (C::Q8 ? (float)E : 0.f);
                     }
 #pragma unroll
                     for (int n = 0; n < NT / 2; n++) {
                         O[n][0] *= al[0]; O[n][1] *= al[1]; O[n][2] *= al[0]; O[n][3] *= al[1];
                     }
                 }
-                float p[2][2];
+                float p[2 * C::SUB][2];
 #pragma unroll
-                for (int i = 0; i < 2; i++)
+                for (int i = 0; i < 2 * C::SUB; i++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        p[i][h] = pd_ex2(fmaf(x[i][h], sc[h], PD_LIFT - m[h]));
+                        p[i][h] = pd_ex2(fmaf(x[i][h], sc[h], off[h]));
                         l[h] += p[i][h];
                     }
                 // ---- O^T += V^T P^T
@@ -481,13 +501,12 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                         uint32_t v[4][4];
 #pragma unroll
                         for (int kk = 0; kk < 4; kk++) {
-                            const int r = pd_row<HD, DT>(2 * t + (kk & 1)) + (kk >> 1) * 8;
                             const uint4 w = *reinterpret_cast<const uint4*>(st + C::KB + j * 2048 + (kk >> 1) * 1024 + v_off[kk & 1]);
                             v[kk][0] = w.x;
                             v[kk][1] = w.y;
                             v[kk][2] = w.z;
                             v[kk][3] = w.w;
-                            if (TAIL && r >= left)   // stale rows may hold anything
+                            if (TAIL && pd_row<HD, DT>(2 * t + (kk & 1)) + (kk >> 1) * 8 >= left)   // stale rows may hold anything
                                 v[kk][0] = v[kk][1] = v[kk][2] = v[kk][3] = 0u;
                         }
 #pragma unroll
@@ -499,36 +518,33 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                         }
                     }
                 } else {
-                    const float down = tc::pow2f(-E);
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
+                    for (int u = 0; u < C::SUB; u++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) p[i][h] *= down;
+                        for (int j = 0; j < NB; j++) {
+                            uint32_t bh[2], bl[2], w[4];
 #pragma unroll
-                    for (int j = 0; j < NB; j++) {
-                        uint32_t bh[2], bl[2], w[4];
+                            for (int i = 0; i < 2; i++) {
+                                const float d = __half2float(sv[2 * u + i][j]);
+                                pd_pair<A>(p[2 * u + i][0] * d, p[2 * u + i][1] * d, bh[i], bl[i]);
+                                bh[i] = pd_transpose(bh[i]);
+                                if (sizeof(A) == 4) bl[i] = pd_transpose(bl[i]);
+                            }
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const float d = __half2float(sv[i][j]);
-                            pd_pair<A>(p[i][0] * d, p[i][1] * d, bh[i], bl[i]);
-                            bh[i] = pd_transpose(bh[i]);
-                            if (sizeof(A) == 4) bl[i] = pd_transpose(bl[i]);
+                            for (int kk = 0; kk < 4; kk++)
+                                w[kk] = *reinterpret_cast<const uint32_t*>(st + C::KB + (16 * u + (kk >> 1) * 8) * HD +
+                                                                           (v_off[kk & 1] ^ (j * 32))) ^
+                                        0x80808080u;
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {   // bytes 2 e, 2 e + 1 of the keys' words
+                                const uint32_t lo = __byte_perm(w[0], w[1], e ? 0x7362 : 0x5140);
+                                const uint32_t hi = __byte_perm(w[2], w[3], e ? 0x7362 : 0x5140);
+                                const uint32_t a0 = pd_codes(lo, 0x4140), a1 = pd_codes(lo, 0x4342);
+                                const uint32_t a2 = pd_codes(hi, 0x4140), a3 = pd_codes(hi, 0x4342);
+                                pd_mma(O[j * 2 + e], a0, a1, a2, a3, bh[0], bh[1]);
+                                if (sizeof(A) == 4) pd_mma(O[j * 2 + e], a0, a1, a2, a3, bl[0], bl[1]);
+                            }
                         }
-#pragma unroll
-                        for (int kk = 0; kk < 4; kk++) {
-                            w[kk] = *reinterpret_cast<const uint32_t*>(st + C::KB + (kk >> 1) * 8 * HD + (v_off[kk & 1] ^ (j * 32))) ^
-                                    0x80808080u;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {   // bytes 2 e, 2 e + 1 of the keys' words
-                            const uint32_t lo = __byte_perm(w[0], w[1], e ? 0x7362 : 0x5140);
-                            const uint32_t hi = __byte_perm(w[2], w[3], e ? 0x7362 : 0x5140);
-                            const uint32_t a0 = pd_codes(lo, 0x4140), a1 = pd_codes(lo, 0x4342);
-                            const uint32_t a2 = pd_codes(hi, 0x4140), a3 = pd_codes(hi, 0x4342);
-                            pd_mma(O[j * 2 + e], a0, a1, a2, a3, bh[0], bh[1]);
-                            if (sizeof(A) == 4) pd_mma(O[j * 2 + e], a0, a1, a2, a3, bl[0], bl[1]);
-                        }
-                    }
                 }
             };
             for (; next < done + seg_n; next += PD_W) {
@@ -540,13 +556,13 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                     slot = 0;
                     parity ^= 1;
                 }
-                const int left = len - ((seg.st + next - done) << 4);   // at least 1
-                if (left >= 16) step(st, ss, std::false_type{}, 16);
+                const int left = len - ((seg.st + next - done) << C::SHIFT);   // at least 1
+                if (left >= C::KEYS) step(st, ss, std::false_type{}, C::KEYS);
                 else step(st, ss, std::true_type{}, left);
             }
         }
         // the next segment and its q, ahead of the meeting
-        PdWalk after = seg;
+        Walk after = seg;
         if (done + seg_n < total) {
             after.go(seg_n, b, H, n_hg, err);
             load_q(after);
@@ -554,12 +570,16 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
         // ---- the warps meet
         {
             const float u = C::Q8 ? tc::pow2f(E) : 1.f;
+            const int prev = slot == 0 ? C::NST - 1 : slot - 1;   // not issued again yet
+            float* meet = reinterpret_cast<float*>(ring_p + prev * 2 * C::KB);
+            if (lane == 0) s_free[warp] = (unsigned)prev;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
-                if (g == 0) meet_ml[warp * PD_HEADS + 2 * t + h] = make_float2(m[h], l[h]);
-                float* row = meet + (warp * PD_HEADS + 2 * t + h) * C::OP + g;
+                if (g == 0)
+                    reinterpret_cast<float2*>(meet + PD_HEADS * C::OP)[2 * t + h] = make_float2(m[h], l[h] * u);
+                float* row = meet + (2 * t + h) * C::OP + g;
                 if (2 * t + h < n_heads)
 #pragma unroll
                     for (int n = 0; n < NT / 2; n++) {
@@ -574,20 +594,24 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
         const int slot_out = gs >= a0 ? 1 : 0;
         float* mp = part + ((size_t)blockIdx.x * 2 + slot_out) * (PD_HEADS * (HD + 2));
         const size_t o0 = (size_t)seg.s * ldo + (size_t)(kvh * group + hg * PD_HEADS) * HD;
+        const float* meets[PD_W];
+#pragma unroll
+        for (int w = 0; w < PD_W; w++)
+            meets[w] = reinterpret_cast<const float*>(sm + (w * C::NST + s_free[w]) * 2 * C::KB);
         for (int i = tid; i < n_heads * HD; i += PD_W * 32) {
             const int h = i / HD, p = i % HD;
             float2 ml[PD_W];
             float M = -INFINITY, L = 0.f, V = 0.f;
 #pragma unroll
             for (int w = 0; w < PD_W; w++) {
-                ml[w] = meet_ml[w * PD_HEADS + h];
+                ml[w] = reinterpret_cast<const float2*>(meets[w] + PD_HEADS * C::OP)[h];
                 M = fmaxf(M, ml[w].x);
             }
 #pragma unroll
             for (int w = 0; w < PD_W; w++) {
                 const float f = ml[w].x == -INFINITY ? 0.f : pd_ex2(ml[w].x - M);
                 L = fmaf(ml[w].y, f, L);
-                V = fmaf(f == 0.f ? 0.f : meet[(w * PD_HEADS + h) * C::OP + p], f, V);
+                V = fmaf(f == 0.f ? 0.f : meets[w][h * C::OP + p], f, V);
             }
             if (whole) {
                 out[o0 + (size_t)h * HD + pd_col<HD, DT>(p)] = (A)(V / L);
@@ -653,7 +677,8 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                 if (tid == 0) tickets[(size_t)seg.s * H + seg.h] = 0u;   // every CTA has arrived
             }
         }
-        __syncthreads();   // the meeting area is free again
+        tc::fence_async_smem();   // the slots go back to the copies
+        __syncthreads();
         done += seg_n;
         seg = after;
     }
