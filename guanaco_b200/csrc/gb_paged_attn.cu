@@ -30,6 +30,9 @@ namespace gb {
 // head, 8 query heads); all
 // steps of the batch, in that order, are cut into one equal run per CTA
 // whatever the sequences' lengths, and the CTA's warps take its steps in turn.
+// Few triples (at most half as many as CTAs): a CTA takes a piece of one, all
+// pieces of one size, so that none crosses into a second triple (another
+// meeting: one sequence of 8193 positions in Q8_0 21 us by runs).
 // Each warp streams its own steps through a ring of TMA copies (16 rows of K and
 // of V, 128- or 64-byte swizzle) and keeps its own (m, l, O); they meet once per
 // segment (the steps of one such triple in this CTA) in shared memory.  A segment cut by CTA borders leaves a
@@ -42,8 +45,8 @@ namespace gb {
 // warp; l and O are in units of 2^E.
 constexpr int PD_W = 4;              // warps
 constexpr int PD_MAX_CTAS = 4;       // CTAs per SM the workspace has room for
-constexpr int PD_MIN_STEPS = 4;      // fewest steps of a CTA
-constexpr int PD_MC = 16;            // partials of a join in flight
+constexpr int PD_MC = 16;            // partials of a join in flight, and of a group
+constexpr int PD_GROUP_TICKETS = GB_MAX_SMS * PD_MAX_CTAS * 2;   // two per CTA, before the segments' tickets
 constexpr int PD_HEADS = 8;          // query heads of a segment
 constexpr float PD_TAU = 8.f, PD_LIFT = 6.f;
 
@@ -178,8 +181,7 @@ __device__ __forceinline__ int pd_col(int p) {
 template <typename A, int HD, int DT>
 __global__ void __launch_bounds__(PD_W * 32, (pd_ctas<HD, DT>()))
 k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedView c, const BatchView b, const A* __restrict__ q, int ldq, int group, int n_hg,
-               A* __restrict__ out, int ldo, unsigned* __restrict__ tickets, float* __restrict__ part, int min_steps,
-               unsigned* err) {
+               A* __restrict__ out, int ldo, unsigned* __restrict__ tickets, float* __restrict__ part, unsigned* err) {
     using C = PdCfg<HD, DT>;
     constexpr int NT = HD / 8;   // output tiles of 8 columns
     constexpr int NB = HD / 32;  // 32-column blocks
@@ -201,32 +203,71 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
     // ---- the batch's steps and this CTA's run of them (steps < 2^31: checked on the host)
     const int per = (b.n_seq + PD_W * 32 - 1) / (PD_W * 32);
     const int s_lo = min(tid * per, b.n_seq), s_hi = min(s_lo + per, b.n_seq);
-    unsigned mine = 0;
-    for (int s = s_lo; s < s_hi; s++) mine += (seq_len(b, s, err) + C::KEYS - 1) >> C::SHIFT;
-    unsigned incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
+    unsigned mine = 0, live = 0;   // steps and sequences with any
+    for (int s = s_lo; s < s_hi; s++) {
+        const unsigned n = (seq_len(b, s, err) + C::KEYS - 1) >> C::SHIFT;
+        mine += n;
+        live += n > 0;
     }
-    if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
-    unsigned T = 0, base = 0;
+    // running sums over the block's threads; total: of all
+    auto scan = [&](unsigned v, unsigned& total) {
+        unsigned incl = v;
 #pragma unroll
-    for (int w = 0; w < PD_W; w++) {
-        if (w < warp) base += s_scan[w];
-        T += s_scan[w];
-    }
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) s_scan[warp] = incl;
+        __syncthreads();
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < PD_W; w++) {
+            if (w < warp) incl += s_scan[w];
+            total += s_scan[w];
+        }
+        return incl;
+    };
+    unsigned T, n_seg;
+    const unsigned incl = scan(mine, T);
     T *= H;
-    const unsigned run = max((T + gridDim.x - 1) / gridDim.x, (unsigned)min_steps);
-    const unsigned a0 = blockIdx.x * run, a1 = min(a0 + run, T);
+    __syncthreads();   // s_scan is free again
+    scan(live, n_seg);
+    n_seg *= H;
     // sequences without keys: zeros
     for (int s = blockIdx.x; s < b.n_seq; s += gridDim.x)
         if (seq_len(b, s, err) == 0)
             for (int i = tid; i < c.n_kv * group * HD; i += PD_W * 32) out[(size_t)s * ldo + i] = (A)0.f;
-    if (a0 >= T) return;
-    {
-        unsigned at = (base + incl - mine) * H;   // first step of sequence s_lo
+    if (T == 0) return;
+    const bool pieces = 2 * n_seg <= gridDim.x;
+    // steps of a CTA: a piece (a multiple of the warps; at most T / run + n_seg of them) or a run
+    const unsigned run = pieces ? ((T + gridDim.x - n_seg - 1) / (gridDim.x - n_seg) + PD_W - 1) / PD_W * PD_W
+                                : (T + gridDim.x - 1) / gridDim.x;
+    unsigned a0 = 0, a1 = 0;   // run: this CTA's steps a0 .. a1 - 1
+    if (pieces) {
+        unsigned count = 0, all;
+        for (int s = s_lo; s < s_hi; s++)
+            count += (((seq_len(b, s, err) + C::KEYS - 1) >> C::SHIFT) + run - 1) / run * H;
+        __syncthreads();
+        unsigned at = scan(count, all) - count;   // first piece of sequence s_lo
+        if (blockIdx.x >= all) return;
+        for (int s = s_lo; s < s_hi; s++) {
+            const unsigned n = (unsigned)(seq_len(b, s, err) + C::KEYS - 1) >> C::SHIFT, per_seg = (n + run - 1) / run;
+            if (blockIdx.x >= at && blockIdx.x < at + per_seg * H) {
+                const unsigned h = (blockIdx.x - at) / per_seg, piece = (blockIdx.x - at) % per_seg;
+                s_start[0] = s;
+                s_start[1] = (int)h;
+                s_start[2] = (int)(piece * run);
+                s_start[3] = (int)n;
+            }
+            at += per_seg * H;
+        }
+        __syncthreads();
+        a1 = min(run, (unsigned)(s_start[3] - s_start[2]));
+    } else {
+        a0 = blockIdx.x * run;
+        a1 = min(a0 + run, T);
+        if (a0 >= T) return;
+        unsigned at = (incl - mine) * H;   // first step of sequence s_lo
         for (int s = s_lo; s < s_hi; s++) {
             const unsigned n = (unsigned)(seq_len(b, s, err) + C::KEYS - 1) >> C::SHIFT, next = at + n * H;
             if (a0 >= at && a0 < next) {
@@ -237,8 +278,8 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
             }
             at = next;
         }
+        __syncthreads();
     }
-    __syncthreads();
     const int total = (int)(a1 - a0);
     using Walk = PdWalk<C::SHIFT>;
     Walk seg = {s_start[0], s_start[1], s_start[2], s_start[3], s_start[1] / n_hg};
@@ -589,10 +630,19 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
             }
         }
         __syncthreads();
-        const unsigned gs = a0 + done - seg.st, ge = gs + seg.nst;   // the whole segment's steps
-        const bool whole = gs >= a0 && ge <= a1;
-        const int slot_out = gs >= a0 ? 1 : 0;
-        float* mp = part + ((size_t)blockIdx.x * 2 + slot_out) * (PD_HEADS * (HD + 2));
+        // the CTAs that hold the segment: c0 .. c1; a CTA's second partial is of the segment that it begins
+        unsigned c0, c1;
+        if (pieces) {
+            c0 = blockIdx.x - (unsigned)seg.st / run;
+            c1 = c0 + ((unsigned)seg.nst + run - 1) / run - 1;
+        } else {
+            const unsigned gs = a0 + done - seg.st;
+            c0 = gs / run;
+            c1 = (gs + seg.nst - 1) / run;
+        }
+        const bool whole = c0 == c1;
+        const unsigned second = PD_HEADS * (HD + 2);
+        float* mp = part + (size_t)blockIdx.x * 2 * second + (c0 == blockIdx.x ? second : 0);
         const size_t o0 = (size_t)seg.s * ldo + (size_t)(kvh * group + hg * PD_HEADS) * HD;
         const float* meets[PD_W];
 #pragma unroll
@@ -624,38 +674,27 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
             }
         }
         if (!whole) {
-            // the CTAs of the segment: those that hold its first and last step
-            const int c0 = (int)(gs / run), c1 = (int)((ge - 1) / run);
-            __syncthreads();
-            if (tid == 0) {
-                unsigned prev;
-                asm volatile("fence.acq_rel.gpu;\n\tatom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
-                             : "=r"(prev)
-                             : "l"(tickets + (size_t)seg.s * H + seg.h)
-                             : "memory");
-                s_last = prev == (unsigned)(c1 - c0);
-            }
-            __syncthreads();
-            if (s_last) {
-                // thread: four neighbouring positions of a head, PD_MC partials in flight
-                constexpr size_t PS = 2 * PD_HEADS * (HD + 2);   // floats of a CTA's two partials
+            constexpr size_t PS = PD_HEADS * (HD + 2);   // floats of a partial: (m, l) [8], O [8][HD]
+            // partials in, in order, thread = four neighbouring positions of a head, PD_MC of them in
+            // flight; out: a partial, or (nullptr) the output
+            auto join = [&](unsigned count, auto at, float* to) {
                 for (int i = 4 * tid; i < n_heads * HD; i += 4 * PD_W * 32) {
                     const int h = i / HD, p = i % HD;
                     float M = -INFINITY, L = 0.f;
                     float4 V = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int cc = c0; cc <= c1; cc += PD_MC) {
+                    for (unsigned k = 0; k < count; k += PD_MC) {
                         float2 ml[PD_MC];
                         float4 v[PD_MC];
                         float mn = M;
 #pragma unroll
-                        for (int u = 0; u < PD_MC; u++) {
-                            const float* pp = part + min(cc + u, c1) * PS + (cc + u == c0 ? PD_HEADS * (HD + 2) : 0);
+                        for (unsigned u = 0; u < PD_MC; u++) {
+                            const float* pp = at(min(k + u, count - 1));
                             ml[u] = __ldcg(reinterpret_cast<const float2*>(pp) + h);
                             v[u] = __ldcg(reinterpret_cast<const float4*>(pp + 2 * PD_HEADS + i));
                         }
 #pragma unroll
-                        for (int u = 0; u < PD_MC; u++) {
-                            if (cc + u > c1) ml[u] = make_float2(-INFINITY, 0.f);
+                        for (unsigned u = 0; u < PD_MC; u++) {
+                            if (k + u >= count) ml[u] = make_float2(-INFINITY, 0.f);
                             mn = fmaxf(mn, ml[u].x);
                         }
                         const float fa = pd_ex2(M - mn);   // 0 before the first partial
@@ -663,18 +702,58 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                         L *= fa;
                         V = make_float4(V.x * fa, V.y * fa, V.z * fa, V.w * fa);
 #pragma unroll
-                        for (int u = 0; u < PD_MC; u++) {
+                        for (unsigned u = 0; u < PD_MC; u++) {
                             const float f = pd_ex2(ml[u].x - M);
                             L = fmaf(ml[u].y, f, L);
                             V = make_float4(fmaf(v[u].x, f, V.x), fmaf(v[u].y, f, V.y), fmaf(v[u].z, f, V.z),
                                             fmaf(v[u].w, f, V.w));
                         }
                     }
-                    const float inv = 1.0f / L, r[4] = {V.x * inv, V.y * inv, V.z * inv, V.w * inv};
+                    if (to) {
+                        *reinterpret_cast<float4*>(to + 2 * PD_HEADS + i) = V;
+                        if (p == 0) {
+                            to[2 * h] = M;
+                            to[2 * h + 1] = L;
+                        }
+                    } else {
+                        const float inv = 1.0f / L, r[4] = {V.x * inv, V.y * inv, V.z * inv, V.w * inv};
 #pragma unroll
-                    for (int u = 0; u < 4; u++) out[o0 + (size_t)h * HD + pd_col<HD, DT>(p + u)] = (A)r[u];
+                        for (int u = 0; u < 4; u++) out[o0 + (size_t)h * HD + pd_col<HD, DT>(p + u)] = (A)r[u];
+                    }
                 }
-                if (tid == 0) tickets[(size_t)seg.s * H + seg.h] = 0u;   // every CTA has arrived
+            };
+            // this CTA's arrival; true in the last of `count`, which re-arms the ticket
+            auto last_of = [&](unsigned* ticket, unsigned count) {
+                __syncthreads();
+                if (tid == 0) {
+                    unsigned prev;
+                    asm volatile("fence.acq_rel.gpu;\n\tatom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
+                                 : "=r"(prev)
+                                 : "l"(ticket)
+                                 : "memory");
+                    s_last = prev == count - 1;
+                    if (s_last) *ticket = 0u;
+                }
+                __syncthreads();
+                return s_last != 0;
+            };
+            const unsigned count = c1 - c0 + 1;
+            unsigned* ticket = tickets + PD_GROUP_TICKETS + (size_t)seg.s * H + seg.h;
+            auto partial = [&](unsigned k) { return part + (size_t)(c0 + k) * 2 * PS + (k == 0 ? PS : 0); };
+            if (count <= 3 * PD_MC) {
+                if (last_of(ticket, count)) join(count, partial, nullptr);
+            } else {   // groups of PD_MC first: one CTA alone would read them all too slowly
+                const unsigned g = (blockIdx.x - c0) / PD_MC, n_groups = (count + PD_MC - 1) / PD_MC;
+                const unsigned in_group = min((unsigned)PD_MC, count - g * PD_MC);
+                // a group's ticket and result stand at its first CTA, where, as with the partials, two
+                // segments may meet: the one that ends there and the one that begins
+                float* groups = part + (size_t)gridDim.x * 2 * PS;
+                auto place = [&](unsigned k) { return (size_t)(c0 + k * PD_MC) * 2 + (k == 0); };
+                auto group = [&](unsigned k) { return groups + place(k) * PS; };
+                if (last_of(tickets + place(g), in_group)) {
+                    join(in_group, [&](unsigned k) { return partial(g * PD_MC + k); }, group(g));
+                    if (last_of(ticket, n_groups)) join(n_groups, group, nullptr);
+                }
             }
         }
         tc::fence_async_smem();   // the slots go back to the copies
@@ -684,7 +763,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
     }
 }
 
-static_assert((size_t)GB_MAX_SMS * PD_MAX_CTAS * 2 * PD_HEADS * (128 + 2) * 4 <= PAGED_PART_BYTES, "workspace");
+static_assert((size_t)GB_MAX_SMS * PD_MAX_CTAS * 4 * PD_HEADS * (128 + 2) * 4 <= PAGED_PART_BYTES, "workspace");
 
 template <typename A, int HD, int DT>
 static cudaError_t launch_decode(const PagedView& c, const BatchView& b, const void* q, int ldq, int group, void* out,
@@ -701,7 +780,7 @@ static cudaError_t launch_decode(const PagedView& c, const BatchView& b, const v
     unsigned* tickets = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(ws) + PAGED_TICKETS_AT);
     return launch_pdl(k_paged_decode<A, HD, DT>, dim3(sm_count() * pd_ctas<HD, DT>()), PD_W * 32, C::SMEM, st, km, vm, c, b,
                       static_cast<const A*>(q), ldq, group, n_hg, static_cast<A*>(out), ldo, tickets,
-                      static_cast<float*>(ws), PD_MIN_STEPS, err);
+                      static_cast<float*>(ws), err);
 }
 
 static int paged_attention(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q, int ldq,
@@ -744,7 +823,7 @@ extern "C" size_t gb_paged_workspace_bytes(int n_heads, int n_kv_heads, int head
     if (n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) || n_seq < 0)
         return 0;
     const int group = n_heads / n_kv_heads, n_hg = (group + PD_HEADS - 1) / PD_HEADS;
-    return PAGED_TICKETS_AT + ((size_t)n_seq * n_kv_heads * n_hg * sizeof(unsigned) + 15) / 16 * 16;
+    return PAGED_TICKETS_AT + (((size_t)PD_GROUP_TICKETS + (size_t)n_seq * n_kv_heads * n_hg) * sizeof(unsigned) + 15) / 16 * 16;
 }
 
 extern "C" int gb_paged_attention_decode(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q,

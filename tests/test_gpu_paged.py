@@ -212,6 +212,16 @@ def test_decode_many_sequences(gb, cuda, cache):
     check_attention(gb, "f32", cache, 8, 2, 64, 16, [1] * 3, [1200, 0, 31], True, ws=ws)
 
 
+@pytest.mark.parametrize("cache", ["f16", "q8_0"])
+def test_decode_long_among_short(gb, cuda, cache):
+    """Long sequences cut over most CTAs between many short ones, and ending
+    where another long one begins."""
+    lens = [3] * 90 + [9000, 9100, 40, 8900] + [5] * 90 + [30000]
+    check_attention(gb, "f32", cache, 4, 2, 64, 32, [1] * len(lens), lens, True)
+    lens = [20000, 20000, 20000]
+    check_attention(gb, "f32", cache, 2, 1, 64, 32, [1] * len(lens), lens, True)
+
+
 PREFILL = [
     # heads, kv, hd, page, q_lens, kv_lens
     (1, 1, 64, 16, [1], [1]),
