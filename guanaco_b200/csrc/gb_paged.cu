@@ -6,6 +6,7 @@
 // the rounded d, so d * code is the nearest value that the stored scale can
 // express.  RoPE rounds as the per-model cache's kernels do (a c - b s,
 // a s + b c, no contraction).
+#include "gb_mt.cuh"
 #include "gb_paged.cuh"
 
 #include <atomic>
@@ -66,8 +67,9 @@ k_kv_append(const PagedView c, const BatchView b, const A* __restrict__ q, int l
             const float* __restrict__ rope, int rope_len, unsigned* err) {
     constexpr int TPH = HD / 8;   // threads per head
     const int per = (n_heads + 2 * c.n_kv) * TPH;
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int t = (int)(e / per), u = (int)(e % per);
+    const unsigned e = blockIdx.x * 256u + threadIdx.x;
+    const int t = (int)(e / (unsigned)per), u = (int)(e % (unsigned)per);
+    griddep_wait();
     const bool live = t < b.n_tokens;
     int s = -1, pos = -1;
     if (live && (s = seq_of(b, t)) >= 0) {
@@ -143,8 +145,9 @@ k_kv_read(const PagedView c, const BatchView b, A* __restrict__ ko, int ldk, A* 
           unsigned* err) {
     constexpr int TPH = HD / 8;
     const int per = 2 * c.n_kv * TPH;
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int t = (int)(e / per), u = (int)(e % per);
+    const unsigned e = blockIdx.x * 256u + threadIdx.x;
+    const int t = (int)(e / (unsigned)per), u = (int)(e % (unsigned)per);
+    griddep_wait();
     if (t >= b.n_tokens) return;
     const int s = seq_of(b, t);
     if (s < 0) return;
@@ -217,13 +220,14 @@ extern "C" int gb_kv_append(const gb_kv_cache* cache, const gb_kv_batch* batch, 
     unsigned* err = paged_err();
     if (!err) return GB_ECUDA;
     const long long threads = (long long)b.n_tokens * (n_heads + 2 * c.n_kv) * (hd / 8);
-    const long long grid = (threads + 255) / 256;
-    if (grid > 0x7fffffffLL) return GB_ELIMIT;
+    if (threads > 0x7fffff00LL) return GB_ELIMIT;
+    const unsigned grid = (unsigned)((threads + 255) / 256);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e;
 #define GB_APPEND(A, HD, DT)                                                                                        \
-    k_kv_append<A, HD, DT><<<(unsigned)grid, 256, 0, st>>>(                                                         \
-        c, b, static_cast<const A*>(q), ldq, n_heads, static_cast<A*>(q_out), ldqo, static_cast<const A*>(k), ldk,  \
-        static_cast<const A*>(v), ldv, rope_cs, rope_len, err)
+    e = launch_pdl(k_kv_append<A, HD, DT>, dim3(grid), 256, 0, st, c, b, static_cast<const A*>(q), ldq, n_heads,    \
+                   static_cast<A*>(q_out), ldqo, static_cast<const A*>(k), ldk, static_cast<const A*>(v), ldv,       \
+                   rope_cs, rope_len, err)
 #define GB_APPEND_DT(A, HD) \
     if (cache->dtype == GB_DT_F16) GB_APPEND(A, HD, GB_DT_F16); else GB_APPEND(A, HD, GB_DT_Q8_0)
     if (dtype == GB_DT_F32) {
@@ -233,7 +237,7 @@ extern "C" int gb_kv_append(const gb_kv_cache* cache, const gb_kv_batch* batch, 
     }
 #undef GB_APPEND_DT
 #undef GB_APPEND
-    return cudaGetLastError() == cudaSuccess ? GB_OK : GB_ECUDA;
+    return e == cudaSuccess ? GB_OK : GB_ECUDA;
 }
 
 extern "C" int gb_kv_read(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, void* k, int ldk, void* v,
@@ -248,11 +252,14 @@ extern "C" int gb_kv_read(const gb_kv_cache* cache, const gb_kv_batch* batch, in
     if (b.n_tokens == 0) return GB_OK;
     unsigned* err = paged_err();
     if (!err) return GB_ECUDA;
-    const long long grid = ((long long)b.n_tokens * 2 * c.n_kv * (hd / 8) + 255) / 256;
-    if (grid > 0x7fffffffLL) return GB_ELIMIT;
+    const long long threads = (long long)b.n_tokens * 2 * c.n_kv * (hd / 8);
+    if (threads > 0x7fffff00LL) return GB_ELIMIT;
+    const unsigned grid = (unsigned)((threads + 255) / 256);
+    cudaError_t e;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define GB_READ(A, HD, DT) \
-    k_kv_read<A, HD, DT><<<(unsigned)grid, 256, 0, st>>>(c, b, static_cast<A*>(k), ldk, static_cast<A*>(v), ldv, err)
+    e = launch_pdl(k_kv_read<A, HD, DT>, dim3(grid), 256, 0, st, c, b, static_cast<A*>(k), ldk, static_cast<A*>(v), \
+                   ldv, err)
 #define GB_READ_DT(A, HD) \
     if (cache->dtype == GB_DT_F16) GB_READ(A, HD, GB_DT_F16); else GB_READ(A, HD, GB_DT_Q8_0)
     if (dtype == GB_DT_F32) {
@@ -262,5 +269,5 @@ extern "C" int gb_kv_read(const gb_kv_cache* cache, const gb_kv_batch* batch, in
     }
 #undef GB_READ_DT
 #undef GB_READ
-    return cudaGetLastError() == cudaSuccess ? GB_OK : GB_ECUDA;
+    return e == cudaSuccess ? GB_OK : GB_ECUDA;
 }

@@ -140,6 +140,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const BatchView& b = a.b;
     const int kvh = blockIdx.x % c.n_kv, y = blockIdx.x / c.n_kv;
 
+    griddep_wait();   // launched ahead of the kernel before it
     // ---- which sequence and query block: the blocks of the sequences in order, the longest of each first
     if (warp == 0) {
         if (lane == 0) s_seq = -1;
@@ -690,8 +691,10 @@ static int launch_prefill(const gb_kv_cache* cache, PpArgs& a, void* ws, cudaStr
     if (split < 1) split = 1;
     a.part = static_cast<float*>(ws);
     a.tickets = reinterpret_cast<unsigned*>(static_cast<uint8_t*>(ws) + PAGED_PART_BYTES);
-    k_paged_prefill<A, HD, DT><<<dim3((unsigned)grid, (unsigned)split), C::THREADS, C::SMEM, st>>>(km, vm, a);
-    return cudaGetLastError() == cudaSuccess ? GB_OK : GB_ECUDA;
+    return launch_pdl(k_paged_prefill<A, HD, DT>, dim3((unsigned)grid, (unsigned)split), C::THREADS, C::SMEM, st, km, vm,
+                      a) == cudaSuccess
+               ? GB_OK
+               : GB_ECUDA;
 }
 
 int paged_prefill(const gb_kv_cache* cache, const PagedView& c, const BatchView& b, int dtype, const void* q, int ldq,

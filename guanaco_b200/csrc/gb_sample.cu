@@ -22,6 +22,8 @@
 //   draw         sums by index, the CTA, the warp, the token of the target
 #include "gb_common.cuh"
 #include "gb_internal.h"
+#include "gb_mt.cuh"
+#include "gb_paged.cuh"
 
 #include <cooperative_groups.h>
 
@@ -115,6 +117,7 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int i0 = min(rank * slice, vocab), n = min(slice, vocab - i0);   // this CTA's indices i0 .. i0 + n - 1
     const float* src = logits + (size_t)row * ldl + i0;
+    griddep_wait();
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");   // every CTA of the cluster runs before remote stores
 
     // ---- the slice and its maximum; -inf up to whole float4s
@@ -585,7 +588,9 @@ extern "C" int gb_sample(const float* logits, int ldl, int rows, int vocab, cons
     constexpr size_t most = (sizeof(gb::SmpShared) + 15) / 16 * 16 + (size_t)GB_SAMPLE_MAX_VOCAB / gb::SMP_CL * sizeof(float);
     static_assert(most <= 227 * 1024, "shared memory");
     if (gb::set_smem_once(reinterpret_cast<const void*>(gb::k_sample), (int)most) != cudaSuccess) return GB_ECUDA;
-    gb::k_sample<<<rows * gb::SMP_CL, gb::SMP_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(
-        logits, ldl, vocab, slice, temperature, top_k, top_p, min_p, u, out);
-    return cudaGetLastError() == cudaSuccess ? GB_OK : GB_ECUDA;
+    return gb::launch_pdl(gb::k_sample, dim3(rows * gb::SMP_CL), gb::SMP_THREADS, (int)smem,
+                          static_cast<cudaStream_t>(stream), logits, ldl, vocab, slice, temperature, top_k, top_p, min_p,
+                          u, out) == cudaSuccess
+               ? GB_OK
+               : GB_ECUDA;
 }
