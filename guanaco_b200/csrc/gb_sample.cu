@@ -18,7 +18,9 @@
 //                in which the running sum reaches the goal; its tokens go to
 //                one CTA, which cuts them by their ranks.  A bin of more than
 //                SMP_CAND tokens (many equal logits) is first cut again by the
-//                whole cluster.
+//                whole cluster.  A top-k whose bin and those before it hold at
+//                most SMP_CAND tokens ends here: CTA 0 filters them and draws,
+//                and no other token's weight is computed.
 //   draw         sums by index, the CTA, the warp, the token of the target
 #include "gb_common.cuh"
 #include "gb_internal.h"
@@ -72,13 +74,13 @@ __device__ __forceinline__ u64 smp_share(u64 total, uint32_t part) {
 
 struct SmpShared {
     uint32_t count[SMP_BINS], wlo[SMP_BINS], whi[SMP_BINS];   // whi:wlo a 64-bit weight
-    u64 cand[SMP_CAND], cand_w[SMP_CAND];                     // ranks and weights of a bin's tokens (CTA 0)
+    u64 cand[SMP_CAND], cand_w[SMP_CAND];                     // ranks of a bin's tokens in this CTA; CTA 0: all, weights
     // written by the cluster's CTAs
     u64 peer_max[SMP_CL], peer_a[SMP_CL], peer_b[SMP_CL], peer_sum[SMP_CL];
-    u64 cut_a, cut_b, cut_rank, cut_sum;                      // results of a search
-    uint32_t cut_bin, n_cand;
+    u64 cut_a, cut_rank;                                      // results of a search
+    uint32_t cut_bin, cut_n, n_cand, peer_n[SMP_CL];
     u64 warp64[SMP_W], warp64b[SMP_W];
-    u64 tot_a, tot_b;
+    u64 tot_a;
     uint32_t n_list;
 };
 
@@ -119,6 +121,13 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
     const float* src = logits + (size_t)row * ldl + i0;
     griddep_wait();
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");   // every CTA of the cluster runs before remote stores
+    const float t = temperature ? __ldg(temperature + row) : 1.f;
+    const int k = top_k ? __ldg(top_k + row) : 0;
+    const float p = top_p ? __ldg(top_p + row) : 1.f;
+    const float mp = min_p && __ldg(min_p + row) > 0.f ? fminf(__ldg(min_p + row), 1.f) : 0.f;
+    const float uf = fminf(fmaxf(__ldg(uu + row), 0.f), 1.f) * 16777216.f;
+    for (int i = tid; i < SMP_BINS; i += SMP_THREADS) sh.count[i] = sh.wlo[i] = sh.whi[i] = 0;
+    if (tid == 0) sh.n_cand = 0;
 
     // ---- the slice and its maximum; -inf up to whole float4s
     const int n4 = (n + 3) >> 2;
@@ -138,26 +147,16 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
         for (int i = tid; i < 4 * n4; i += SMP_THREADS)
             mx = fmaxf(mx, x[i] = i < n ? smp_clean(__ldg(src + i)) : -INFINITY);
     }
-    for (int i = tid; i < SMP_BINS; i += SMP_THREADS) sh.count[i] = sh.wlo[i] = sh.whi[i] = 0;
-    if (tid == 0) sh.n_cand = 0;
     mx = warp_max(mx);
     if (lane == 0) sh.warp64[warp] = smp_key(mx);
     __syncthreads();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    if (tid < SMP_CL) {
-        u64 b = 0;
-#pragma unroll
-        for (int w = 0; w < SMP_W; w++) b = sh.warp64[w] > b ? sh.warp64[w] : b;
-        cl.map_shared_rank(&sh, tid)->peer_max[rank] = b;
+    if (warp == 0) {
+        const uint32_t b = __reduce_max_sync(0xffffffffu, (uint32_t)sh.warp64[lane % SMP_W]);
+        if (lane < SMP_CL) cl.map_shared_rank(&sh, lane)->peer_max[rank] = b;
     }
     cl.sync();
-    {
-        u64 b = 0;
-#pragma unroll
-        for (int c = 0; c < SMP_CL; c++) b = sh.peer_max[c] > b ? sh.peer_max[c] : b;
-        mx = smp_logit((uint32_t)b);
-    }
-    const float t = temperature ? temperature[row] : 1.f;
+    mx = smp_logit(__reduce_max_sync(0xffffffffu, (uint32_t)sh.peer_max[lane % SMP_CL]));
     // The first index of the maximum (all CTAs call it).
     auto first_max = [&] {
         uint32_t at = 0xffffffffu;
@@ -213,9 +212,6 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
         return expf(q);
     };
     auto weight_of = [&](float l) { return smp_weight(exp_of(l)); };
-    const int k = top_k ? top_k[row] : 0;
-    const float p = top_p ? top_p[row] : 1.f;
-    const float mp = min_p && min_p[row] > 0.f ? fminf(min_p[row], 1.f) : 0.f;
     const bool by_k = k > 0 && k < vocab, by_p = p < 1.f;
     u64 cut = 0;   // kept: rank >= cut
 
@@ -231,70 +227,109 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
             for (int i = tid; i < SMP_BINS; i += SMP_THREADS) sh.count[i] = sh.wlo[i] = sh.whi[i] = 0;
             __syncthreads();
         };
-        auto put = [&](int b, u64 w) {   // a 64-bit sum in two words; the high one rarely moves
+        // Weights into bins: a 64-bit sum in two words, the high one moved by a
+        // carry or a weight past 2^32 (the few likely tokens).
+        auto put = [&](int b, u64 w) {
             const uint32_t lo = (uint32_t)w, old = atomicAdd(&sh.wlo[b], lo);
             const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old);
             if (hi) atomicAdd(&sh.whi[b], hi);
         };
         constexpr int PER = SMP_BINS / SMP_CL;
-        // The cluster's sums of this thread's bin (a: tokens, b: weights), their
-        // running sums over the bins up to it, and the sums of all bins.
-        auto merge = [&](u64& own_a, u64& own_b, u64& run_a, u64& run_b, u64& all_a, u64& all_b) {
+        // The cluster's sum of this thread's bin (tokens or weights), the running
+        // sum over the bins up to it, and the sum of all bins.
+        auto merge = [&](bool counts, u64& own, u64& run, u64& all) {
             cl.sync();   // every histogram is done
-            u64 a = 0, b = 0;
+            u64 a = 0, unused = 0;
             if (tid < PER) {
                 const int i = rank * PER + tid;
 #pragma unroll
                 for (int c = 0; c < SMP_CL; c++) {
                     const SmpShared* o = cl.map_shared_rank(&sh, c);
-                    if (by_k) a += o->count[i];
-                    if (by_p) b += (u64)o->whi[i] << 32 | o->wlo[i];
+                    a += counts ? o->count[i] : (u64)o->whi[i] << 32 | o->wlo[i];
                 }
             }
-            own_a = a;
-            own_b = b;
-            smp_scan2(a, b, sh.warp64, sh.warp64b);
-            if (tid == SMP_THREADS - 1) {
-                sh.tot_a = a;
-                sh.tot_b = b;
-            }
+            own = a;
+            smp_scan2(a, unused, sh.warp64, sh.warp64b);
+            if (tid == SMP_THREADS - 1) sh.tot_a = a;
             __syncthreads();
-            if (tid < SMP_CL) {
-                SmpShared* o = cl.map_shared_rank(&sh, tid);
-                o->peer_a[rank] = sh.tot_a;
-                o->peer_b[rank] = sh.tot_b;
-            }
+            if (tid < SMP_CL) cl.map_shared_rank(&sh, tid)->peer_a[rank] = sh.tot_a;
             cl.sync();
-            all_a = all_b = 0;
+            all = 0;
 #pragma unroll
             for (int c = 0; c < SMP_CL; c++) {
-                if (c == rank) {
-                    a += all_a;
-                    b += all_b;
-                }
-                all_a += sh.peer_a[c];
-                all_b += sh.peer_b[c];
+                if (c == rank) a += all;
+                all += sh.peer_a[c];
             }
-            run_a = a;
-            run_b = b;
+            run = a;
         };
-        // The bin at which the running sum reaches goal, and the sums before it: to every CTA.
-        auto cross = [&](u64 goal, bool counts, u64 own_a, u64 own_b, u64 run_a, u64 run_b, u64 off_a, u64 off_b) {
-            const u64 upto = counts ? off_a + run_a : off_b + run_b, own = counts ? own_a : own_b;
+        // The bin at which the running sum (from off) reaches goal, the sums before and with it: to every CTA.
+        auto cross = [&](u64 goal, u64 own, u64 run, u64 off) {
+            const u64 upto = off + run;
             if (tid < PER && upto - own < goal && goal <= upto)   // one thread of the cluster
                 for (int c = 0; c < SMP_CL; c++) {
                     SmpShared* o = cl.map_shared_rank(&sh, c);
                     o->cut_bin = (uint32_t)(rank * PER + tid);
-                    o->cut_a = off_a + run_a - own_a;
-                    o->cut_b = off_b + run_b - own_b;
+                    o->cut_a = upto - own;
+                    o->cut_n = upto < 0xffffffffull ? (uint32_t)upto : 0xffffffffu;
                 }
             cl.sync();
         };
+        // This CTA's tokens of the given bins (level 0: `first`, else of the ranks lo .. hi) into its list; their
+        // number in the cluster, and their first and last rank here.
+        auto gather = [&](auto in_bin, u64& mn, u64& mxr) {
+            mn = ~0ull;
+            mxr = 0;
+            for (int i = tid; i < n4; i += SMP_THREADS) {
+                const float4 v = *reinterpret_cast<const float4*>(x + 4 * i);
+                const float l[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (in_bin(l[j], 4 * i + j)) {
+                        const u64 rk = rank_of(4 * i + j);
+                        mn = rk < mn ? rk : mn;
+                        mxr = rk > mxr ? rk : mxr;
+                        const uint32_t at = atomicAdd(&sh.n_cand, 1u);
+                        if (at < SMP_CAND) sh.cand[at] = rk;
+                    }
+            }
+            __syncthreads();
+            if (tid < SMP_CL) cl.map_shared_rank(&sh, tid)->peer_n[rank] = sh.n_cand;
+            cl.sync();
+            uint32_t m = 0;
+#pragma unroll
+            for (int c = 0; c < SMP_CL; c++) m += sh.peer_n[c];
+            return m;
+        };
+        // In CTA 0: this thread's of the gathered tokens (0: none).
+        auto candidate = [&] {
+            int m = 0, from = -1, at = 0;   // number `at` of CTA `from`
+#pragma unroll
+            for (int c = 0; c < SMP_CL; c++) {
+                const int nc = (int)sh.peer_n[c];
+                if (tid >= m && tid < m + nc) {
+                    from = c;
+                    at = tid - m;
+                }
+                m += nc;
+            }
+            return from >= 0 ? cl.map_shared_rank(&sh, from)->cand[at] : 0ull;
+        };
+        auto block_sum = [&](u64 v) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            __syncthreads();
+            if (lane == 0) sh.warp64[warp] = v;
+            __syncthreads();
+            v = 0;
+#pragma unroll
+            for (int w = 0; w < SMP_W; w++) v += sh.warp64[w];
+            return v;
+        };
         // In CTA 0: the candidate at which the sum, from (ga, gb), reaches goal; to every CTA.
-        auto resolve = [&](u64 goal, bool counts, u64 ga, u64 gb) {
-            const int m = (int)sh.n_cand;
-            bool in = tid < m;
-            const u64 me = in ? sh.cand[tid] : 0, w = in ? sh.cand_w[tid] : 0;
+        auto resolve = [&](u64 goal, bool counts, u64 g, int m) {
+            const u64 me = candidate();
+            bool in = me != 0;
+            const u64 w = !in ? 0 : counts ? 1 : weight_of(smp_logit((uint32_t)(me >> 32)));
             int left = m;
             while (left > 32) {   // cut them by their ranks' leading bits, SMP_THREADS bins
                 u64 lo = in ? me : ~0ull, hi = me;
@@ -324,19 +359,16 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
                     put(bin, w);
                 }
                 __syncthreads();
-                const u64 own_a = sh.count[tid], own_b = (u64)sh.whi[tid] << 32 | sh.wlo[tid];
-                u64 a = own_a, b = own_b;
-                smp_scan2(a, b, sh.warp64, sh.warp64b);
-                const u64 upto = counts ? ga + a : gb + b, own = counts ? own_a : own_b;
-                if (upto - own < goal && goal <= upto) {
-                    sh.n_list = (uint32_t)own_a;
+                const u64 own_n = sh.count[tid], own = (u64)sh.whi[tid] << 32 | sh.wlo[tid];
+                u64 a = own, unused = 0;
+                smp_scan2(a, unused, sh.warp64, sh.warp64b);
+                if (g + a - own < goal && goal <= g + a) {
+                    sh.n_list = (uint32_t)own_n;
                     sh.cut_bin = (uint32_t)tid;
-                    sh.tot_a = ga + a - own_a;
-                    sh.tot_b = gb + b - own_b;
+                    sh.tot_a = g + a - own;
                 }
                 __syncthreads();
-                ga = sh.tot_a;
-                gb = sh.tot_b;
+                g = sh.tot_a;
                 left = (int)sh.n_list;
                 in = in && bin == (int)sh.cut_bin;
             }
@@ -344,86 +376,27 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
             if (tid == 0) sh.n_list = 0;
             __syncthreads();
             if (in) {
-                const uint32_t at = atomicAdd(&sh.n_list, 1u);
-                sh.cand[at] = me;
-                sh.cand_w[at] = w;
+                const uint32_t to = atomicAdd(&sh.n_list, 1u);
+                sh.cand[to] = me;
+                sh.cand_w[to] = w;
             }
             __syncthreads();
             if (warp == 0 && lane < left) {
                 const u64 mine = sh.cand[lane], mine_w = sh.cand_w[lane];
-                u64 above = ga, above_w = gb;
+                u64 before = g;
                 for (int j = 0; j < left; j++)
-                    if (sh.cand[j] > mine) {
-                        above++;
-                        above_w += sh.cand_w[j];
-                    }
-                const u64 before = counts ? above : above_w, own = counts ? 1ull : mine_w;
-                if (before < goal && goal <= before + own)
-                    for (int c = 0; c < SMP_CL; c++) {
-                        SmpShared* o = cl.map_shared_rank(&sh, c);
-                        o->cut_rank = mine;
-                        o->cut_sum = above_w + mine_w;
-                    }
+                    if (sh.cand[j] > mine) before += sh.cand_w[j];
+                if (before < goal && goal <= before + mine_w)
+                    for (int c = 0; c < SMP_CL; c++) cl.map_shared_rank(&sh, c)->cut_rank = mine;
             }
-            __syncthreads();
-            if (tid == 0) sh.n_cand = 0;
         };
 
-        for (int i = tid; i < n4; i += SMP_THREADS) {
-            const float4 v = *reinterpret_cast<const float4*>(x + 4 * i);
-            const float l[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int bin = bin_of(l[j]);
-                if (by_k) atomicAdd(&sh.count[bin], 1u);
-                if (by_p) {
-                    const u64 w = weight_of(l[j]);
-                    if (w) put(bin, w);
-                }
-            }
-        }
-        u64 own_a, own_b, run_a, run_b, all_a, all_b;
-        merge(own_a, own_b, run_a, run_b, all_a, all_b);
-
-        // Cut at which the running sum (of tokens or weights) reaches goal, at
-        // most the sum of all: its rank, and the weights kept.
-        auto search = [&](u64 goal, bool counts, u64& rank_cut, u64& kept) {
-            cross(goal, counts, own_a, own_b, run_a, run_b, 0, 0);
-            uint32_t bin = sh.cut_bin;
-            u64 ga = sh.cut_a, gb = sh.cut_b;
-            if (bin == SMP_BINS - 1) return;   // only tokens without weight are cut
-            u64 lo = 0, hi = ~0ull;
-            int shift = 0;
-            for (bool first = true;; first = false) {
-                SmpShared* o = cl.map_shared_rank(&sh, 0);
-                u64 mn = ~0ull, mxr = 0;
-                auto take = [&](int i, float l) {
-                    const u64 rk = rank_of(i);
-                    mn = rk < mn ? rk : mn;
-                    mxr = rk > mxr ? rk : mxr;
-                    const uint32_t at = atomicAdd(&o->n_cand, 1u);
-                    if (at < SMP_CAND) {
-                        o->cand[at] = rk;
-                        o->cand_w[at] = weight_of(l);
-                    }
-                };
-                for (int i = tid; i < n4; i += SMP_THREADS) {
-                    const float4 v = *reinterpret_cast<const float4*>(x + 4 * i);
-                    const float l[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        bool in = bin_of(l[j]) == (int)bin;
-                        if (!first) {
-                            const u64 rk = rank_of(4 * i + j);
-                            in = rk >= lo && rk <= hi && (hi - rk) >> shift == bin;
-                        }
-                        if (in) take(4 * i + j, l[j]);
-                    }
-                }
-                cl.sync();
-                const uint32_t m = o->n_cand;
-                if (m <= SMP_CAND) break;
-                // too many: bins over the ranks between the first and the last of them
+        // Rank at which the running sum reaches goal, from the crossed bin on.
+        auto search = [&](u64 goal, bool counts, auto weigh) {
+            const uint32_t bin = sh.cut_bin;
+            u64 g = sh.cut_a, lo = 0, hi = ~0ull, mn, mxr;
+            uint32_t m = gather([&](float l, int) { return bin_of(l) == (int)bin; }, mn, mxr);
+            while (m > SMP_CAND) {   // too many: bins over the ranks between the first and the last of them
 #pragma unroll
                 for (int z = 16; z; z >>= 1) {
                     const u64 y = __shfl_xor_sync(0xffffffffu, mn, z), v = __shfl_xor_sync(0xffffffffu, mxr, z);
@@ -447,7 +420,7 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
                     q->peer_b[rank] = mxr;
                 }
                 cl.sync();
-                if (rank == 0 && tid == 0) sh.n_cand = 0;
+                if (tid == 0) sh.n_cand = 0;
                 lo = ~0ull;
                 hi = 0;
 #pragma unroll
@@ -455,123 +428,188 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
                     lo = sh.peer_a[i] < lo ? sh.peer_a[i] : lo;
                     hi = sh.peer_b[i] > hi ? sh.peer_b[i] : hi;
                 }
-                shift = max(0, 64 - __clzll(hi - lo) - 11);   // (hi - lo) >> shift < 2048
+                const int shift = max(0, 64 - __clzll(hi - lo) - 11);   // (hi - lo) >> shift < 2048
                 clear();
                 for (int i = tid; i < n; i += SMP_THREADS) {
                     const u64 rk = rank_of(i);
                     if (rk < lo || rk > hi) continue;
                     const int at = (int)((hi - rk) >> shift);
-                    if (by_k) atomicAdd(&sh.count[at], 1u);
-                    if (by_p) put(at, weight_of(x[i]));
+                    if (counts) atomicAdd(&sh.count[at], 1u);
+                    else put(at, weigh(x[i], i));
                 }
-                u64 oa, ob, ra, rb, ta, tb;
-                merge(oa, ob, ra, rb, ta, tb);
-                cross(goal, counts, oa, ob, ra, rb, ga, gb);
-                bin = sh.cut_bin;
-                ga = sh.cut_a;
-                gb = sh.cut_b;
+                u64 own, run, all;
+                merge(counts, own, run, all);
+                cross(goal, own, run, g);
+                const uint32_t fine = sh.cut_bin;
+                g = sh.cut_a;
+                m = gather([&](float, int i) {
+                    const u64 rk = rank_of(i);
+                    return rk >= lo && rk <= hi && (uint32_t)((hi - rk) >> shift) == fine;
+                }, mn, mxr);
             }
-            if (rank == 0) resolve(goal, counts, ga, gb);
+            if (rank == 0) resolve(goal, counts, g, (int)m);
             cl.sync();
-            rank_cut = sh.cut_rank;
-            kept = sh.cut_sum;
+            if (tid == 0) sh.n_cand = 0;
+            return sh.cut_rank;
         };
-        u64 kept = all_b;
-        if (by_k) search((u64)k, true, cut, kept);
+        u64 own, run, all;
+        if (by_k) {
+            for (int i = tid; i < n4; i += SMP_THREADS) {
+                const float4 v = *reinterpret_cast<const float4*>(x + 4 * i);
+                atomicAdd(&sh.count[bin_of(v.x)], 1u);
+                atomicAdd(&sh.count[bin_of(v.y)], 1u);
+                atomicAdd(&sh.count[bin_of(v.z)], 1u);
+                atomicAdd(&sh.count[bin_of(v.w)], 1u);
+            }
+            merge(true, own, run, all);
+            cross((u64)k, own, run, 0);
+            const int bin = (int)sh.cut_bin;
+            if (bin < SMP_BINS - 1 && sh.cut_n <= SMP_CAND) {   // few: CTA 0 ends it
+                u64 mn, mxr;
+                const int m = (int)gather([&](float l, int) { return bin_of(l) <= bin; }, mn, mxr);
+                const u64 me = rank == 0 ? candidate() : 0;
+                cl.sync();   // after this no CTA touches another's memory
+                if (rank) return;
+                const float e = me ? exp_of(smp_logit((uint32_t)(me >> 32))) : 0.f;
+                const u64 w = me ? smp_weight(e) : 0;
+                if (me) {
+                    sh.cand[tid] = me;
+                    sh.cand_w[tid] = w;
+                }
+                __syncthreads();
+                int pos = 0;
+                u64 before = 0;
+                for (int j = 0; j < m; j++)
+                    if (sh.cand[j] > me) {
+                        pos++;
+                        before += sh.cand_w[j];
+                    }
+                bool in = me && pos < k;
+                if (by_p) {
+                    const u64 goal = smp_share(block_sum(in ? w : 0), (uint32_t)rintf(fmaxf(p, 0.f) * 16777216.f));
+                    in = in && (before < goal || pos == 0);
+                }
+                const u64 mine = in && e >= mp ? w : 0;
+                __syncthreads();
+                if (me) sh.cand_w[tid] = mine;
+                const u64 target = smp_share(block_sum(mine), min((uint32_t)uf, 0xFFFFFFu));
+                u64 upto = 0;   // kept weights of lower indices (larger complements)
+                for (int j = 0; j < m; j++)
+                    if ((uint32_t)sh.cand[j] > (uint32_t)me) upto += sh.cand_w[j];
+                if (target >= upto && target < upto + mine) out[row] = (int)~(uint32_t)me;
+                return;
+            }
+            // (the last bin's tokens have no weight: nothing is cut that could be drawn)
+            if (bin < SMP_BINS - 1) cut = search((u64)k, true, [](float, int) { return 0ull; });
+        }
         if (by_p) {
-            const u64 goal = smp_share(kept, (uint32_t)rintf(fmaxf(p, 0.f) * 16777216.f));
-            u64 c2, unused;
-            if (goal) search(goal, false, c2, unused);
-            else c2 = (u64)smp_key(mx) << 32 | ~first_max();   // the first token alone
+            // tokens that top-k left; all of them: the sum that the share is taken of
+            auto weigh = [&](float l, int i) { return rank_of(i) >= cut ? weight_of(l) : 0ull; };
+            if (by_k) clear();
+            for (int i = tid; i < n4; i += SMP_THREADS) {
+                const float4 v = *reinterpret_cast<const float4*>(x + 4 * i);
+                const float l[4] = {v.x, v.y, v.z, v.w};
+                int bin[4];
+                u64 w[4];
+                uint32_t old[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    bin[j] = bin_of(l[j]);
+                    w[j] = cut ? weigh(l[j], 4 * i + j) : weight_of(l[j]);
+                }
+                // four at once, so that the atomics' round trips overlap
+#pragma unroll
+                for (int j = 0; j < 4; j++) old[j] = bin[j] < SMP_BINS - 1 ? atomicAdd(&sh.wlo[bin[j]], (uint32_t)w[j]) : 0u;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t hi = (uint32_t)(w[j] >> 32) + (old[j] + (uint32_t)w[j] < old[j]);
+                    if (hi) atomicAdd(&sh.whi[bin[j]], hi);
+                }
+            }
+            merge(false, own, run, all);
+            const u64 goal = smp_share(all, (uint32_t)rintf(fmaxf(p, 0.f) * 16777216.f));
+            u64 c2;
+            if (goal) {
+                cross(goal, own, run, 0);
+                c2 = search(goal, false, weigh);
+            } else {
+                c2 = (u64)smp_key(mx) << 32 | ~first_max();   // the first token alone
+            }
             cut = c2 > cut ? c2 : cut;
         }
     }
 
-    // ---- the draw, in index order: warps take consecutive runs of the slice, lanes four neighbours
-    const int run = (slice / 4 + SMP_W - 1) / SMP_W;
-    const int r0 = min(warp * run, n4), r1 = min(r0 + run, n4);
+    // ---- the draw, in index order: threads take consecutive runs of float4s,
+    // each lane from another place of its run on (a warp's reads then fall on
+    // different banks; whole numbers add up the same in any order)
+    const int run = (n4 + SMP_THREADS - 1) / SMP_THREADS;
+    const int r0 = min(tid * run, n4), r1 = min(r0 + run, n4);
     const float cut_l = cut ? smp_logit((uint32_t)(cut >> 32)) : -INFINITY;
     const uint32_t cut_i = cut ? ~(uint32_t)cut : 0xffffffffu;   // the last kept index of logit cut_l
-    // the weights of float4 i after the filters, as parts
-    auto weights = [&](int i, uint32_t (&hi)[4], int (&lo)[4]) {
-        const float4 v = i < r1 ? *reinterpret_cast<const float4*>(x + 4 * i)
-                                : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        const float l[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            hi[j] = 0;
-            lo[j] = 0;
-        }
-        if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) < cut_l) return;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const bool in = l[j] > cut_l || (l[j] == cut_l && (uint32_t)(i0 + 4 * i + j) <= cut_i);
-            const float e = exp_of(l[j]);
-            uint32_t h;
-            int w;
-            smp_parts(e, h, w);
-            hi[j] = in && e >= mp ? h : 0u;
-            lo[j] = in && e >= mp ? w : 0;
-        }
+    auto kept = [&](float l, int i, float& e) {   // token i after the filters
+        e = exp_of(l);
+        return (l > cut_l || (l == cut_l && (uint32_t)(i0 + i) <= cut_i)) && e >= mp;
     };
     u64 sum = 0;
     {
-        uint32_t h4[4], h = 0;   // a lane's part of a slice: at most 2^15 / 512 float4s, 2^17 x 2^8
-        int l4[4], l = 0;
-        for (int i = r0 + lane; i < r1; i += 32) {
-            weights(i, h4, l4);
-            h += h4[0] + h4[1] + h4[2] + h4[3];
-            l += l4[0] + l4[1] + l4[2] + l4[3];
+        uint32_t h = 0;   // at most 2^17 x 2^15 / 512 x 2
+        int lo = 0;
+        int i = r0 + lane % max(run, 1);
+#pragma unroll 2
+        for (int step = 0; step < run; step++) {
+            const float4 v = i < r1 ? *reinterpret_cast<const float4*>(x + 4 * i)
+                                    : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= cut_l) {
+                const float l[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float e;
+                    uint32_t eh;
+                    int el;
+                    const bool in = kept(l[j], 4 * i + j, e);
+                    smp_parts(e, eh, el);
+                    h += in ? eh : 0u;
+                    lo += in ? el : 0;
+                }
+            }
+            i = i + 1 == r0 + run ? r0 : i + 1;
         }
-        sum = smp_join(h, l);
+        sum = smp_join(h, lo);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    u64 incl = sum, unused = 0;
+    smp_scan2(incl, unused, sh.warp64, sh.warp64b);   // running sums over the block
+    if (tid == SMP_THREADS - 1) sh.tot_a = incl;
     __syncthreads();
-    if (lane == 0) sh.warp64[warp] = sum;
-    __syncthreads();
-    if (tid < SMP_CL) {
-        u64 s = 0;
-#pragma unroll
-        for (int w = 0; w < SMP_W; w++) s += sh.warp64[w];
-        cl.map_shared_rank(&sh, tid)->peer_sum[rank] = s;
-    }
+    if (tid < SMP_CL) cl.map_shared_rank(&sh, tid)->peer_sum[rank] = sh.tot_a;
     cl.sync();   // after this no CTA touches another's memory
-    u64 upto = 0, total = 0;
+    u64 upto = incl - sum, total = 0;
 #pragma unroll
     for (int c = 0; c < SMP_CL; c++) {
         if (c < rank) upto += sh.peer_sum[c];
         total += sh.peer_sum[c];
     }
-    for (int w = 0; w < warp; w++) upto += sh.warp64[w];
-    const float uf = fminf(fmaxf(uu[row], 0.f), 1.f) * 16777216.f;
     const u64 target = smp_share(total, min((uint32_t)uf, 0xFFFFFFu));
-    if (target < upto || target >= upto + sum) return;
-    for (int i = r0; i < r1; i += 32) {   // the run that holds the target: find the index
-        uint32_t h4[4];
-        int l4[4];
-        weights(i + lane, h4, l4);
-        const u64 own = smp_join(h4[0] + h4[1] + h4[2] + h4[3], l4[0] + l4[1] + l4[2] + l4[3]);
-        u64 c = own;
+    // the thread whose run holds the target; its warp looks through the run
+    const uint32_t who = __ballot_sync(0xffffffffu, target >= upto && target < upto + sum);
+    if (!who) return;
+    const int src_lane = __ffs(who) - 1;
+    u64 at = __shfl_sync(0xffffffffu, upto, src_lane);
+    const int f0 = 4 * __shfl_sync(0xffffffffu, r0, src_lane), f1 = 4 * __shfl_sync(0xffffffffu, r1, src_lane);
+    for (int i = f0; i < f1; i += 32) {
+        float e;
+        u64 c = 0;
+        if (i + lane < f1 && kept(x[i + lane], i + lane, e)) c = smp_weight(e);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const u64 y = __shfl_up_sync(0xffffffffu, c, o);
             if (lane >= o) c += y;
         }
-        const uint32_t m = __ballot_sync(0xffffffffu, upto + c > target);
+        const uint32_t m = __ballot_sync(0xffffffffu, at + c > target);
         if (m) {
-            if (lane == __ffs(m) - 1) {
-                u64 at = upto + c - own;
-                int j = 0;
-                while (j < 3 && at + smp_join(h4[j], l4[j]) <= target) {
-                    at += smp_join(h4[j], l4[j]);
-                    j++;
-                }
-                out[row] = i0 + 4 * (i + lane) + j;
-            }
+            if (lane == 0) out[row] = i0 + i + __ffs(m) - 1;
             return;
         }
-        upto += __shfl_sync(0xffffffffu, c, 31);
+        at += __shfl_sync(0xffffffffu, c, 31);
     }
 }
 
