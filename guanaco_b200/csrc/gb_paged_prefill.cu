@@ -6,16 +6,19 @@
 // read from the cache serves every head that shares it.  Keys come in tiles of
 // NK.  For each of the two row tiles, alternately:
 //   S = Q K^T    A = Q, B = K, both K-major in shared memory (128-byte swizzle)
-//   softmax      two warpgroups per row tile, a thread takes half the tile's
-//                keys of one row (= tensor-memory lane): scale, causal mask,
-//                running maximum and sum; P = 2^(x - m) back into tensor
-//                memory over S, each half handed over by itself
+//   softmax      a thread takes one row (= tensor-memory lane) or half of its
+//                keys: scale, causal mask, running maximum and sum; P = 2^(x - m)
+//                back into tensor memory over S
 //   O += P V     A = P from tensor memory, B = V as it lies in the cache (rows
 //                = keys, MN-major): V is never transposed
-// While one row tile's softmax runs the tensor cores work for the other.
+// While one row tile's softmax runs the tensor cores work for the other; with
+// tiles of 64 keys fp16 has room for two buffers of S, so the next scores are
+// there when a softmax ends.  fp32 is bound by the tensor cores (three
+// products) and keeps Q's high parts in tensor memory instead, which takes
+// their reads off shared memory.  Two threads per row only exchange a vote per
+// key tile.
 // The maximum moves only when a score exceeds it by more than PP_TAU (log2
-// units), so O in tensor memory is rarely rescaled, and the two threads of a
-// row only exchange a vote per key tile.
+// units), so O in tensor memory is rarely rescaled.
 //
 // Precision.  fp16 activations: Q exact, P rounded to fp16, Q8_0 values rounded
 // to fp16 (each an error of the size of the fp16 output's own rounding).
@@ -39,13 +42,18 @@ namespace gb {
 
 constexpr int PP_POLY = 8;                      // of this many pairs of exponentials one is a polynomial
 constexpr float PP_TAU = 8.f, PP_LIFT = 6.f;   // p <= 2^14; small p stay normal fp16 numbers
-constexpr int PP_SOFT = 512;                    // softmax threads: two warpgroups per row tile
 constexpr int PP_SMEM_MAX = 227 * 1024 - 4096;  // less alignment slack and static shared memory
 
 template <typename A, int HD, int DT>
 struct PpCfg {
     static constexpr bool F32 = sizeof(A) == 4, Q8 = DT == GB_DT_Q8_0;
-    static constexpr int NK = F32 ? 64 : 128;          // keys per tile
+    // fp16, hd 128, F16 cache: tiles of 128 keys (an MMA of N 128 takes 80 cycles,
+    // one of N 64 takes 64), one buffer of S, two threads per row; elsewhere 64
+    // keys, fp16 with two buffers of S and one thread per row.  One prompt of
+    // 8192 tokens that way / the other: F16 hd 128 489 / 597 us, F16 hd 64 580 /
+    // 449 us, Q8_0 hd 128 886 / 713 us.
+    static constexpr bool WIDE = !F32 && !Q8 && HD == 128;
+    static constexpr int NK = WIDE ? 128 : 64;         // keys per tile
     static constexpr int KS = F32 && Q8 ? 2 : 1;       // fp16 parts of K and V (of Q and P: 2 for fp32)
     static constexpr int G = HD / 64;                  // 64-column groups (128 bytes)
     static constexpr int QB = 128 * HD * 2;            // bytes of a row tile's part
@@ -54,12 +62,15 @@ struct PpCfg {
     static constexpr int ST = ST0 > 4 ? 4 : ST0;       // K / V stages
     static constexpr int SMEM = 2 * QB + ST * 2 * KS * KB + 1024;
     static constexpr int PROD = Q8 ? 4 : 1;            // producer warps
-    static constexpr int THREADS = PP_SOFT + 32 + PROD * 32;
-    // tensor memory columns: S (and P over it) of tile i at NK i; fp32: Q's
-    // high parts of tile i at 128 + 64 i; O of tile i at 256 + 128 i
-    static constexpr uint32_t PLO = NK / 4;            // a half's P over its scores: the remainders' columns
-    static constexpr int NH = NK / 2;                  // keys of a thread's half
-    static constexpr bool HOLD = !(Q8 && NH == 64);    // its scores stay in registers (else read twice)
+    static constexpr int TR = F32 || WIDE ? 2 : 1;     // softmax threads per row
+    static constexpr int SOFT = 256 * TR, MMA = SOFT / 32;   // their number; the MMA warp
+    static constexpr int THREADS = SOFT + 32 + PROD * 32;
+    // tensor memory columns: S (and P over it) of row tile i at SW i, in NS
+    // buffers; fp32: Q's high parts at 128 + 64 i; O at 256 + 128 i
+    static constexpr int NS = F32 || WIDE ? 1 : 2;     // buffers of S
+    static constexpr uint32_t SW = NK * NS;
+    static constexpr uint32_t PLO = NK / 4;            // fp32: P's remainders, from a part's first column
+    static constexpr int NH = NK / TR;                 // keys of a softmax thread
     static_assert(ST >= 2, "shared memory");
 };
 
@@ -101,20 +112,18 @@ __device__ __forceinline__ uint32_t pp_pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Among the PP_SOFT / 2 threads of a row tile (barrier id): a vote, a barrier.
+// Among the 256 threads of a row tile with two threads per row (barrier id): a vote, a barrier.
 __device__ __forceinline__ bool pp_vote(int id, bool v) {
     uint32_t any;
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, %2, %3, p;\n\t"
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, %2, 256, p;\n\t"
         "selp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(any)
-        : "r"((uint32_t)v), "r"(id), "n"(PP_SOFT / 2)
+        : "r"((uint32_t)v), "r"(id)
         : "memory");
     return any != 0;
 }
-__device__ __forceinline__ void pp_sync(int id) {
-    asm volatile("barrier.cta.sync.aligned %0, %1;" ::"r"(id), "n"(PP_SOFT / 2) : "memory");
-}
+__device__ __forceinline__ void pp_sync(int id) { asm volatile("barrier.cta.sync.aligned %0, 256;" ::"r"(id) : "memory"); }
 // Byte offset of the 16-byte unit u (8 halves) of row r in a swizzled tile of R rows.
 __device__ __forceinline__ uint32_t pp_off(int r, int u, int R) {
     return (uint32_t)((u >> 3) * R * 128 + r * 128 + (((u ^ r) & 7) << 4));
@@ -130,7 +139,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     uint8_t* qs = sm;                                   // [2 tiles]: Q, for fp32 its remainders
     uint8_t* ks = sm + 2 * C::QB;                       // [ST][KS]
     uint8_t* vs = ks + ST * C::KS * C::KB;              // [ST][KS]
-    __shared__ __align__(8) uint64_t bars[4 * ST + 9];
+    __shared__ __align__(8) uint64_t bars[4 * ST + 13];
     __shared__ float s_row[2][2][128];                  // what the two threads of a row exchange
     __shared__ uint32_t tmem_slot;
     __shared__ int s_seq, s_blk;
@@ -189,21 +198,22 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const int nt0 = min(nt, max((kend0 + NK - 1) / NK - j0, 0));
 
     // ---- rows
-    const int rt = warp >> 3, hf = (warp >> 2) & 1, r = tid & 127;   // softmax threads: row tile, half, row
+    constexpr int TR = C::TR, NH = C::NH, NS = C::NS;
+    const int rt = warp / (4 * TR), hf = (warp >> 2) % TR, r = tid & 127;   // softmax threads: row tile, part, row
     const int qi = q0 + rt * a.bq + r / a.group, h = kvh * a.group + r % a.group;
-    const bool live = warp < 16 && r < a.bq * a.group && qi < n_q;
+    const bool live = warp < C::MMA && r < a.bq * a.group && qi < n_q;
     if (nt_all == 0) {   // nothing to see
         if (live) {
             A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
             const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            for (int d = hf * (HD / 2); d < (hf + 1) * (HD / 2); d += 8) act_store8(dst + d, z);
+            for (int d = hf * (HD / TR); d < (hf + 1) * (HD / TR); d += 8) act_store8(dst + d, z);
         }
         return;
     }
 
     const uint32_t b0 = tc::smem_u32(&bars[0]);
     const uint32_t kfull = b0, kfree = b0 + 8 * ST, vfull = b0 + 16 * ST, vfree = b0 + 24 * ST;   // [ST] each
-    const uint32_t sfull = b0 + 32 * ST, ofull = sfull + 16, tail = sfull + 32, pfull = sfull + 40;   // [2], [2], 1, [2][2]
+    const uint32_t sfull = b0 + 32 * ST, pfull = sfull + 32, odone = sfull + 64, ofull = sfull + 80, tail = sfull + 96;   // [2][2], [2][2], [2], [2], 1
     if (tid == 0) {
         for (int i = 0; i < ST; i++) {
             mbs_init(kfull + 8 * i, C::PROD);
@@ -211,15 +221,18 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             mbs_init(vfull + 8 * i, C::PROD);
             mbs_init(vfree + 8 * i, 1);
         }
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 4; i++) {   // [row tile][buffer]; P with two threads per row: [row tile][half]
             mbs_init(sfull + 8 * i, 1);
-            for (int h2 = 0; h2 < 2; h2++) mbs_init(pfull + 8 * (2 * i + h2), 4);
-            mbs_init(ofull + 8 * i, 1);
+            mbs_init(pfull + 8 * i, 4);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbs_init(odone + 8 * i, 1);   // every P V of a row tile
+            mbs_init(ofull + 8 * i, 1);   // its last
         }
         mbs_init(tail, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 16) tc::tmem_alloc(&tmem_slot, 512);
+    if (warp == C::MMA) tc::tmem_alloc(&tmem_slot, 512);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -228,11 +241,11 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     // ---- Q rows: fp16 into shared memory; fp32 split, the high parts into
     // tensor memory (the A operand of two products of three), the rest into shared memory
     float up_inv = 1.f;   // 2^-e of this thread's row
-    constexpr int UH = HD / 16;   // 8-column units of a thread's half of the row
-    const A* qsrc = static_cast<const A*>(a.q) + (size_t)(t_begin + qi) * a.ldq + (size_t)h * HD + hf * (HD / 2);
+    constexpr int UH = HD / 8 / TR;   // 8-column units of a thread's part of the row
+    const A* qsrc = static_cast<const A*>(a.q) + (size_t)(t_begin + qi) * a.ldq + (size_t)h * HD + hf * (HD / TR);
     uint8_t* qdst = qs + rt * C::QB;
     if (!C::F32) {
-        if (warp < 16) {
+        if (warp < C::MMA) {
 #pragma unroll 4
             for (int u = 0; u < UH; u++) {
                 uint4 w = make_uint4(0u, 0u, 0u, 0u);
@@ -250,9 +263,9 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[u][i]));
         }
-        if (warp < 16) s_row[rt][hf][r] = mx;
+        if (warp < C::MMA) s_row[rt][hf][r] = mx;
         __syncthreads();
-        if (warp < 16) {
+        if (warp < C::MMA) {
             const int e = tc::f16_scale_exp(__float_as_uint(fmaxf(mx, s_row[rt][hf ^ 1][r])));
             const float up = tc::pow2f(e);
             up_inv = tc::pow2f(-e);
@@ -284,7 +297,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     tc::fence_after_sync();
     bool ok = true;
 
-    if (warp == 16) {   // ---- MMA issue: the whole warp, uniform; one lane's instructions
+    if (warp == C::MMA) {   // ---- MMA issue: the whole warp, uniform; one lane's instructions
         {
             // 512 columns are all of tensor memory: its base is 0
             const uint32_t lead = tc::elect();
@@ -296,8 +309,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const uint64_t qd = tc::smem_desc_sw128(tc::smem_u32(qs), 16, 1024);
             const uint64_t kd = tc::smem_desc_sw128(tc::smem_u32(ks), 16, 1024);
             const uint64_t vd = tc::smem_desc_sw128(tc::smem_u32(vs), NK * 128, 1024);
-            auto scores = [&](int i, int st) {   // S_i = Q_i K^T
-                const uint32_t S = (uint32_t)(NK * i);
+            auto scores = [&](int i, int st, int j) {   // S_i = Q_i K^T, the j-th tile's
+                const uint32_t S = C::SW * i + (uint32_t)NK * (j % NS);
                 const uint64_t qa = qd + (uint32_t)(i * (C::QB >> 4)), ka = kd + (uint32_t)(st * (C::KS * C::KB >> 4));
                 if (C::F32) {
                     const uint32_t qh = 128u + 64u * i;
@@ -312,49 +325,52 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 for (int k = 0; k < HD / 16; k++)
                     tc::mma_f16_w(lead, S, qa + (uint32_t)(((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4),
                                 ka + (uint32_t)(((k >> 2) * NK * 128 + (k & 3) * 32) >> 4), idS, C::F32 || k > 0);
-                tc::mma_commit_w(lead, sfull + 8 * i);
+                tc::mma_commit_w(lead, sfull + 8 * (2 * i + j % NS));
             };
-            auto output = [&](int i, int st, int j) {   // O_i (+)= P_i V, as the halves of P arrive
-                const uint32_t O = 256u + 128u * i, P = (uint32_t)(NK * i);
+            auto output = [&](int i, int st, int j) {   // O_i (+)= P_i V
+                const uint32_t O = 256u + 128u * i, P = C::SW * i + (uint32_t)NK * (j % NS);
                 const uint64_t va = vd + (uint32_t)(st * (C::KS * C::KB >> 4));
 #pragma unroll
-                for (int h2 = 0; h2 < 2; h2++) {
-                    wait(pfull + 8 * (2 * i + h2), j & 1);
+                for (int h2 = 0; h2 < TR; h2++) {   // as the parts of P arrive
+                    wait(pfull + 8 * (2 * i + (TR == 2 ? h2 : j % NS)), (j / NS) & 1);
                     tc::fence_after_sync();
 #pragma unroll
                     for (int p = 0; p < (C::F32 ? C::KS + 1 : 1); p++) {   // hi.hi, lo.hi, hi.lo
-                        const uint32_t pa = P + (uint32_t)(C::NH * h2) + (p == 1 ? C::PLO : 0u);
+                        const uint32_t pa = P + (uint32_t)(NH * h2) + (p == 1 ? C::PLO : 0u);
 #pragma unroll
-                        for (int k = 0; k < NK / 32; k++)
+                        for (int k = 0; k < NH / 16; k++)
                             tc::mma_f16_ta_w(lead, O, pa + 8u * k,
-                                           va + (uint32_t)(((p == 2) * C::KB + (h2 * (NK / 32) + k) * 2048) >> 4), idO,
-                                           j > 0 || h2 > 0 || p > 0 || k > 0);
+                                             va + (uint32_t)(((p == 2) * C::KB + (h2 * (NH / 16) + k) * 2048) >> 4), idO,
+                                             j > 0 || h2 > 0 || p > 0 || k > 0);
                     }
                 }
+                tc::mma_commit_w(lead, odone + 8 * i);
             };
             const int tiles[2] = {nt0, two ? nt : 0};   // key tiles of each row tile
-            wait(kfull, 0);
-            tc::fence_after_sync();
-            for (int i = 0; i < 2; i++)
-                if (tiles[i] > 0) scores(i, 0);
-            tc::mma_commit_w(lead, kfree);
+            for (int j = 0; j < min(NS, nt); j++) {
+                wait(kfull + 8 * (j % ST), (j / ST) & 1);
+                tc::fence_after_sync();
+                for (int i = 0; i < 2; i++)
+                    if (j < tiles[i]) scores(i, j % ST, j);
+                tc::mma_commit_w(lead, kfree + 8 * (j % ST));
+            }
             for (int j = 0; j < nt; j++) {
-                const int st = j % ST, sn = (j + 1) % ST;
+                const int jn = j + NS, st = j % ST, sn = jn % ST;   // scores run NS tiles ahead
                 wait(vfull + 8 * st, (j / ST) & 1);
-                if (j + 1 < nt) wait(kfull + 8 * sn, ((j + 1) / ST) & 1);
+                if (jn < nt) wait(kfull + 8 * sn, (jn / ST) & 1);
                 for (int i = 0; i < 2; i++) {
                     if (j >= tiles[i]) continue;
                     output(i, st, j);
-                    if (j + 1 < tiles[i]) scores(i, sn);
-                    else tc::mma_commit_w(lead, ofull + 8 * i);
+                    if (jn < tiles[i]) scores(i, sn, jn);
+                    if (j + 1 == tiles[i]) tc::mma_commit_w(lead, ofull + 8 * i);
                 }
                 tc::mma_commit_w(lead, vfree + 8 * st);
-                if (j + 1 < nt) tc::mma_commit_w(lead, kfree + 8 * sn);
+                if (jn < nt) tc::mma_commit_w(lead, kfree + 8 * sn);
             }
         }
         __syncwarp();
-    } else if (warp > 16) {   // ---- K and V tiles
-        const int pw = warp - 17;
+    } else if (warp > C::MMA) {   // ---- K and V tiles
+        const int pw = warp - C::MMA - 1;
         if (!C::Q8) {
             const int R = min(1 << c.shift, NK);         // rows of a box
             for (int j = 0; j < nt; j++) {
@@ -492,66 +508,62 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
         }
         __syncwarp();
-    } else if (rt == 0 || two) {   // ---- softmax: thread = row, half the keys
-        constexpr int NH = C::NH;
+    } else if (rt == 0 || two) {   // ---- softmax
         const uint32_t lb = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t S = lb + (uint32_t)(NK * rt + NH * hf), O = lb + 256u + 128u * rt + (uint32_t)(hf * (HD / 2));
-        const uint32_t P = S;   // over the scores that this thread has read
+        const uint32_t O = lb + 256u + 128u * rt + (uint32_t)(hf * (HD / TR));
         const float sc = up_inv * (1.4426950408889634f / sqrtf((float)HD));
         const int lim = pos0 + qi;                       // the last key this row sees
         const int lim_min = pos0 + q0 + rt * a.bq;       // and the tile's first query
         const int n_tiles = rt == 0 ? nt0 : nt;          // without any O is not read
-        float m = -INFINITY, l = 0.f;                    // the row's maximum, this half's sum
+        float m = -INFINITY, l = 0.f;                    // the row's maximum, this part's sum
         for (int j = 0; j < n_tiles; j++) {
-            const int key0 = (j0 + j) * NK;
+            const int key0 = (j0 + j) * NK, buf = j % NS;
+            const uint32_t S = lb + C::SW * rt + (uint32_t)(NK * buf + NH * hf);
             const bool masked = key0 + NK - 1 > lim_min;
-            const int left = (live ? lim : -1) - key0 - hf * NH;   // keys 0 .. left of the half are seen
-            if (ok) ok = mbs_wait(sfull + 8 * rt, j & 1, a.err);
+            const int left = (live ? lim : -1) - key0 - hf * NH;   // keys 0 .. left of the part are seen
+            if (ok) ok = mbs_wait(sfull + 8 * (2 * rt + buf), (j / NS) & 1, a.err);
             tc::fence_after_sync();
-            float x[C::HOLD ? NH : 32];
-            float mx = -INFINITY;
-            auto read = [&](int c0, float* y, int n) {   // n scores from key c0, masked; their maximum
-                if (n == 64) tc::tmem_ld32x2(S + c0, S + c0 + 32, *reinterpret_cast<float (*)[32]>(y), *reinterpret_cast<float (*)[32]>(y + 32 * (n / 64)));
-                else tc::tmem_ld32(S + c0, *reinterpret_cast<float (*)[32]>(y));
-                if (masked) {
+            float x[NH], mx = -INFINITY;
+            if (NH == 64)
+                tc::tmem_ld32x2(S, S + 32, *reinterpret_cast<float (*)[32]>(x), *reinterpret_cast<float (*)[32]>(x + NH - 32));
+            else
+                tc::tmem_ld32(S, *reinterpret_cast<float (*)[32]>(x));
+            if (masked) {
 #pragma unroll
-                    for (int i = 0; i < n; i++) y[i] = c0 + i <= left ? y[i] : -INFINITY;
-                }
-#pragma unroll
-                for (int i = 0; i < n; i += 2) mx = fmaxf(mx, fmaxf(y[i], y[i + 1]));
-            };
-            if (C::HOLD) {
-                read(0, x, NH);
-            } else {
-#pragma unroll
-                for (int c0 = 0; c0 < NH; c0 += 32) read(c0, x, 32);
+                for (int i = 0; i < NH; i++) x[i] = i <= left ? x[i] : -INFINITY;
             }
+#pragma unroll
+            for (int i = 0; i < NH; i += 2) mx = fmaxf(mx, fmaxf(x[i], x[i + 1]));
             mx *= sc;
-            // both threads of every row of the tile: does any maximum move?
-            if (pp_vote(1 + rt, mx > m + PP_TAU || (m == -INFINITY && mx > -INFINITY))) {
-                s_row[rt][hf][r] = mx;
-                pp_sync(1 + rt);
-                mx = fmaxf(mx, s_row[rt][hf ^ 1][r]);
-                if (mx > m + PP_TAU || (m == -INFINITY && mx > -INFINITY)) {
-                    const float al = m == -INFINITY ? 0.f : pp_ex2(m - mx);
-                    l *= al;
-                    m = mx;
-                    mx = al;
-                } else {
-                    mx = 1.f;
-                }
-                if (j > 0) {   // P V of the tile before is in O: its commit came before this S
+            auto passes = [&](float v) { return v > m + PP_TAU || (m == -INFINITY && v > -INFINITY); };
+            auto rescale = [&](float v) {   // the maximum moves to v where it passes; O with it
+                const bool move = passes(v);
+                const float al = !move ? 1.f : m == -INFINITY ? 0.f : pp_ex2(m - v);
+                l *= al;
+                m = move ? v : m;
+                if (j > 0) {
+                    // P V of the tile before: with one buffer its commit came before this S; with two the
+                    // commit of the one before that did, so the parity is not ambiguous
+                    if (NS == 2 && ok) ok = mbs_wait(odone + 8 * rt, (j - 1) & 1, a.err);
+                    tc::fence_after_sync();
 #pragma unroll 1
-                    for (int c0 = 0; c0 < HD / 2; c0 += 16) {
+                    for (int c0 = 0; c0 < HD / TR; c0 += 16) {
                         float o[16];
                         tc::tmem_ld16(O + c0, o);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] *= mx;
+                        for (int i = 0; i < 16; i++) o[i] *= al;
                         tc::tmem_st16(O + c0, o);
                     }
                     tc::fence_before_sync();
                 }
-                pp_sync(1 + rt);   // O is rescaled before either half of P is handed over; s_row is free again
+            };
+            if (TR == 1) {
+                if (__any_sync(0xffffffffu, passes(mx))) rescale(mx);
+            } else if (pp_vote(1 + rt, passes(mx))) {   // of all rows of the tile
+                s_row[rt][hf][r] = mx;
+                pp_sync(1 + rt);
+                rescale(fmaxf(mx, s_row[rt][hf ^ 1][r]));
+                pp_sync(1 + rt);   // O is rescaled before either part of P is handed over; s_row is free again
                 tc::fence_after_sync();
             }
             const float off = PP_LIFT - (m == -INFINITY ? 0.f : m);
@@ -559,8 +571,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
             for (int c0 = 0; c0 < NH; c0 += 32) {
-                if (!C::HOLD) read(c0, x, 32);
-                const float* y = C::HOLD ? x + c0 : x;
+                const float* y = x + c0;
                 uint32_t ph[16], pl[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
@@ -574,27 +585,29 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         pl[i] = pp_pack(v.x - f.x, v.y - f.y);
                     }
                 }
-                tc::tmem_st16_nowait(P + c0 / 2, ph);
-                if (C::F32) tc::tmem_st16_nowait(P + C::PLO + c0 / 2, pl);
+                tc::tmem_st16_nowait(S + c0 / 2, ph);   // over the scores that this thread has read
+                if (C::F32) tc::tmem_st16_nowait(S + C::PLO + c0 / 2, pl);
             }
             l += sum.x + sum.y;
             tc::tmem_wait_st();
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbs_arrive(pfull + 8 * (2 * rt + hf));
+            if (lane == 0) mbs_arrive(pfull + 8 * (2 * rt + (TR == 2 ? hf : buf)));
         }
         if (n_tiles > 0) {
             if (ok) ok = mbs_wait(ofull + 8 * rt, 0, a.err);
             tc::fence_after_sync();
         }
-        s_row[rt][hf][r] = l;
-        pp_sync(1 + rt);
-        l += s_row[rt][hf ^ 1][r];
+        if (TR == 2) {
+            s_row[rt][hf][r] = l;
+            pp_sync(1 + rt);
+            l += s_row[rt][hf ^ 1][r];
+        }
         if (n_split == 1) {
             const float inv = l > 0.f ? 1.0f / l : 0.f;   // no keys: zeros
-            A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD + hf * (HD / 2);
+            A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD + hf * (HD / TR);
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD / 2; c0 += 32) {
+            for (int c0 = 0; c0 < HD / TR; c0 += 32) {
                 float o[32];
                 tc::tmem_ld32(O + c0, o);
                 if (live) {
@@ -614,17 +627,17 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 pp[128] = l;
             }
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD / 2; c0 += 32) {
+            for (int c0 = 0; c0 < HD / TR; c0 += 32) {
                 float o[32];
                 tc::tmem_ld32(O + c0, o);
 #pragma unroll
-                for (int i = 0; i < 32; i++) pp[(2 + hf * (HD / 2) + c0 + i) * 128] = l > 0.f ? o[i] : 0.f;
+                for (int i = 0; i < 32; i++) pp[(2 + hf * (HD / TR) + c0 + i) * 128] = l > 0.f ? o[i] : 0.f;
             }
         }
     }
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == 16) {
+    if (warp == C::MMA) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, 512);
     }
@@ -653,7 +666,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const float inv = L > 0.f ? 1.0f / L : 0.f;
         A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
 #pragma unroll 1
-        for (int c0 = hf * (HD / 2); c0 < (hf + 1) * (HD / 2); c0 += 8) {
+        for (int c0 = hf * (HD / TR); c0 < (hf + 1) * (HD / TR); c0 += 8) {
             float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             for (int z = 0; z < n_split; z++) {
                 const float mz = __ldcg(pp + z * step);
