@@ -8,6 +8,7 @@
 // a s + b c, no contraction).
 #include "gb_mt.cuh"
 #include "gb_paged.cuh"
+#include "gb_tc.cuh"
 
 #include <atomic>
 
@@ -56,125 +57,198 @@ int paged_views(const gb_kv_cache* c, const gb_kv_batch* b, PagedView* pv, Batch
     return GB_OK;
 }
 
+// ---------------------------------------------------------------- where a token goes
+// Token t's place: false for padding; pos < 0 or page < 0: nowhere (recorded).
+struct Place {
+    int pos, page, row;
+};
+__device__ __forceinline__ bool place_of(const PagedView& c, const BatchView& b, int t, unsigned* err, Place& o) {
+    const int s = t < b.n_tokens ? seq_of(b, t) : -1;
+    if (s < 0) return false;
+    const int end = b.cu ? __ldg(b.cu + s + 1) : t + 1;
+    o.pos = seq_len(b, s, err) - (end - t);
+    o.page = -1;
+    if (o.pos < 0) {
+        atomicExch(err, (unsigned)(-GB_EPOS));
+        return true;
+    }
+    o.page = page_of(c, b, s, o.pos, err);
+    o.row = o.pos & ((1 << c.shift) - 1);
+    return true;
+}
+
+// Both kernels stream: a thread takes 8 columns (4 RoPE pairs, a quarter of a
+// Q8_0 block: its maximum by two shuffles) of U heads of one token, looks the
+// token's place and rotation up once and has the U heads' loads in flight
+// together; neighbouring threads take neighbouring columns.  U = 2 where that
+// leaves every SM KV_CTAS CTAs, 1 for a decode batch, whose threads would be
+// few.  15,179 prompt tokens (fp32, Q8_0) written and read back: 140 us, 5.8
+// TB/s; U = 1 153 us; at most 42 registers a thread (without the bound 156 us);
+// CTAs that look a few tokens up for all their threads 155 us (the lookup then
+// stands before every load).
+constexpr int KV_THREADS = 128, KV_CTAS = 16;
+
 // ---------------------------------------------------------------- append
-// A thread takes 8 columns of one head of one token: 4 RoPE pairs, and a
-// quarter of a Q8_0 block (its maximum by two shuffles).  Heads of a token in
-// the order q, k, v; the threads of a warp take neighbouring columns.
-template <typename A, int HD, int DT>
-__global__ void __launch_bounds__(256)
+// 8 values of a Q8_0 block whose largest magnitude is mx: their codes to *to,
+// the block's scale returned.  x / d correctly rounded is the product with the
+// rounded reciprocal and one step on its remainder (Markstein, IBM J. Res. Dev.
+// 34, 1990; d has 11 bits, never a fraction of all ones).  Clamped before
+// instead of after; adding 1.5 2^23 rounds to an integer, whose two's
+// complement is the low byte (the conversions run at a quarter of the rate).
+__device__ __forceinline__ __half quantise8(const float (&x)[8], float mx, uint2* to) {
+    const __half d = __float2half_rn(fminf(__fdiv_rn(mx, 127.f), 65504.f));
+    const float df = __half2float(d), rd = __frcp_rn(df), lim = 127.f * df;
+    uint32_t y[8], w[2];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float v = x[j] == x[j] ? fminf(fmaxf(x[j], -lim), lim) : 0.f;
+        const float y0 = v * rd;
+        y[j] = __float_as_uint(fmaf(fmaf(-df, y0, v), rd, y0) + 12582912.f);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+        w[j] = __byte_perm(__byte_perm(y[4 * j], y[4 * j + 1], 0x0040),
+                           __byte_perm(y[4 * j + 2], y[4 * j + 3], 0x0040), 0x5410);
+    *to = df > 0.f ? make_uint2(w[0], w[1]) : make_uint2(0u, 0u);
+    return d;
+}
+
+// Heads of a token in the order q, k, v.
+template <typename A, int HD, int DT, int U>
+__global__ void __launch_bounds__(KV_THREADS, 1536 / KV_THREADS)
 k_kv_append(const PagedView c, const BatchView b, const A* __restrict__ q, int ldq, int n_heads, A* __restrict__ q_out,
             int ldqo, const A* __restrict__ k, int ldk, const A* __restrict__ v, int ldv,
             const float* __restrict__ rope, int rope_len, unsigned* err) {
     constexpr int TPH = HD / 8;   // threads per head
-    const int per = (n_heads + 2 * c.n_kv) * TPH;
-    const unsigned e = blockIdx.x * 256u + threadIdx.x;
-    const int t = (int)(e / (unsigned)per), u = (int)(e % (unsigned)per);
+    const int heads = n_heads + 2 * c.n_kv, slots = (heads + U - 1) / U;   // head i of a thread: slot + i slots
+    const unsigned e = blockIdx.x * KV_THREADS + threadIdx.x, per = (unsigned)(slots * TPH);
+    const int t = (int)(e / per), slot = (int)(e % per) / TPH, col = (int)(e % TPH) * 8;
     griddep_wait();
-    const bool live = t < b.n_tokens;
-    int s = -1, pos = -1;
-    if (live && (s = seq_of(b, t)) >= 0) {
-        const int end = b.cu ? __ldg(b.cu + s + 1) : t + 1;
-        const int len = seq_len(b, s, err);
-        pos = len - (end - t);
-        if (pos < 0) atomicExch(err, (unsigned)(-GB_EPOS));
-    }
-    int head = u / TPH;
-    const int col = (u % TPH) * 8;
-    const bool rotate = rope && head < n_heads + c.n_kv;
-    if (rotate && pos >= rope_len) {
+    Place at = {-1, -1, 0};
+    if (place_of(c, b, t, err, at) && rope && at.pos >= rope_len) {
         atomicExch(err, (unsigned)(-GB_EPOS));
-        pos = -1;
+        at.pos = -1;
     }
-    const bool ok = pos >= 0;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (ok) {
-        const A* src = head < n_heads ? q + (size_t)t * ldq + (size_t)head * HD
-                     : head < n_heads + c.n_kv ? k + (size_t)t * ldk + (size_t)(head - n_heads) * HD
-                                               : v + (size_t)t * ldv + (size_t)(head - n_heads - c.n_kv) * HD;
-        act_load8(src + col, x);
-        if (rotate) {
-            float cs[8];
-            act_load8(rope + (size_t)pos * HD + col, cs);
+    const bool ok = at.pos >= 0;
+    float x[U][8], cs[8];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float a = x[2 * i], bb = x[2 * i + 1], co = cs[2 * i], si = cs[2 * i + 1];
-                x[2 * i] = __fsub_rn(__fmul_rn(a, co), __fmul_rn(bb, si));
-                x[2 * i + 1] = __fadd_rn(__fmul_rn(a, si), __fmul_rn(bb, co));
+    for (int i = 0; i < U; i++) {
+        const int head = slot + i * slots;
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[i][j] = 0.f;
+        if (ok && head < heads) {
+            const A* src = head < n_heads ? q + (size_t)t * ldq + (size_t)head * HD
+                         : head < n_heads + c.n_kv ? k + (size_t)t * ldk + (size_t)(head - n_heads) * HD
+                                                   : v + (size_t)t * ldv + (size_t)(head - n_heads - c.n_kv) * HD;
+            act_load8(src + col, x[i]);
+        }
+    }
+    if (ok && rope) act_load8(rope + (size_t)at.pos * HD + col, cs);
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+        const int head = slot + i * slots;
+        if (ok && rope && head < n_heads + c.n_kv) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float a = x[i][2 * j], bb = x[i][2 * j + 1], co = cs[2 * j], si = cs[2 * j + 1];
+                x[i][2 * j] = __fsub_rn(__fmul_rn(a, co), __fmul_rn(bb, si));
+                x[i][2 * j + 1] = __fadd_rn(__fmul_rn(a, si), __fmul_rn(bb, co));
             }
         }
-    }
-    if (ok && head < n_heads) act_store8(q_out + (size_t)t * ldqo + (size_t)head * HD + col, x);
-    // K and V; every lane takes part in the shuffles
-    float mx = 0.f;
-    if (DT == GB_DT_Q8_0) {
+        float mx = 0.f;
+        if (DT == GB_DT_Q8_0) {   // every lane takes part
 #pragma unroll
-        for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]));   // NaN passed over
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    }
-    if (!ok || head < n_heads) return;
-    head -= n_heads;
-    uint8_t* pool = head < c.n_kv ? c.k : c.v;
-    if (head >= c.n_kv) head -= c.n_kv;
-    const int page = page_of(c, b, s, pos, err);
-    if (page < 0) return;
-    const int row = pos & ((1 << c.shift) - 1);
-    uint8_t* slab = pool + (size_t)page * c.page_bytes + (size_t)head * c.slab;
-    if (DT == GB_DT_F16) {
-        *reinterpret_cast<uint4*>(slab + ((size_t)row * HD + col) * 2) = pack_half8(x);
-    } else {
-        const __half d = __float2half_rn(fminf(__fdiv_rn(mx, 127.f), 65504.f));
-        const float df = __half2float(d);
-        uint32_t w[2] = {0u, 0u};
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float y = df > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[i], df)), -127.f), 127.f) : 0.f;
-            const int code = x[i] == x[i] ? (int)y : 0;
-            w[i >> 2] |= (uint32_t)(code & 0xff) << (8 * (i & 3));
+            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[i][j]));   // NaN passed over
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         }
-        *reinterpret_cast<uint2*>(slab + (size_t)row * HD + col) = make_uint2(w[0], w[1]);
-        if ((col & 31) == 0)
-            reinterpret_cast<__half*>(slab + ((size_t)HD << c.shift))[row * (HD / 32) + col / 32] = d;
+        if (!ok || head >= heads) continue;
+        if (head < n_heads) {
+            act_store8(q_out + (size_t)t * ldqo + (size_t)head * HD + col, x[i]);
+            continue;
+        }
+        if (at.page < 0) continue;
+        const bool is_v = head >= n_heads + c.n_kv;
+        uint8_t* slab = (is_v ? c.v : c.k) + (size_t)at.page * c.page_bytes +
+                        (size_t)(head - n_heads - (is_v ? c.n_kv : 0)) * c.slab;
+        if (DT == GB_DT_F16) {
+            *reinterpret_cast<uint4*>(slab + ((size_t)at.row * HD + col) * 2) = pack_half8(x[i]);
+        } else {
+            const __half d = quantise8(x[i], mx, reinterpret_cast<uint2*>(slab + (size_t)at.row * HD + col));
+            if ((col & 31) == 0)
+                reinterpret_cast<__half*>(slab + ((size_t)HD << c.shift))[at.row * (HD / 32) + col / 32] = d;
+        }
     }
 }
 
 // ---------------------------------------------------------------- read
-template <typename A, int HD, int DT>
-__global__ void __launch_bounds__(256)
+// Heads of a token in the order k, v.
+template <typename A, int HD, int DT, int U>
+__global__ void __launch_bounds__(KV_THREADS, 1536 / KV_THREADS)
 k_kv_read(const PagedView c, const BatchView b, A* __restrict__ ko, int ldk, A* __restrict__ vo, int ldv,
           unsigned* err) {
     constexpr int TPH = HD / 8;
-    const int per = 2 * c.n_kv * TPH;
-    const unsigned e = blockIdx.x * 256u + threadIdx.x;
-    const int t = (int)(e / (unsigned)per), u = (int)(e % (unsigned)per);
+    const int heads = 2 * c.n_kv, slots = (heads + U - 1) / U;
+    const unsigned e = blockIdx.x * KV_THREADS + threadIdx.x, per = (unsigned)(slots * TPH);
+    const int t = (int)(e / per), slot = (int)(e % per) / TPH, col = (int)(e % TPH) * 8;
     griddep_wait();
-    if (t >= b.n_tokens) return;
-    const int s = seq_of(b, t);
-    if (s < 0) return;
-    const int end = b.cu ? __ldg(b.cu + s + 1) : t + 1;
-    const int pos = seq_len(b, s, err) - (end - t);
-    int head = u / TPH;
-    const int col = (u % TPH) * 8;
-    const bool is_v = head >= c.n_kv;
-    if (is_v) head -= c.n_kv;
-    if (pos < 0) atomicExch(err, (unsigned)(-GB_EPOS));
-    const int page = pos < 0 ? -1 : page_of(c, b, s, pos, err);
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};   // a row without a place reads as zeros
-    if (page >= 0) {
-        const int row = pos & ((1 << c.shift) - 1);
-        const uint8_t* slab = (is_v ? c.v : c.k) + (size_t)page * c.page_bytes + (size_t)head * c.slab;
-        if (DT == GB_DT_F16) {
-            act_load8(reinterpret_cast<const __half*>(slab) + (size_t)row * HD + col, x);
-        } else {
-            const uint2 w = __ldg(reinterpret_cast<const uint2*>(slab + (size_t)row * HD + col));
-            const float d = __half2float(
-                reinterpret_cast<const __half*>(slab + ((size_t)HD << c.shift))[row * (HD / 32) + col / 32]);
+    Place at;
+    if (!place_of(c, b, t, err, at)) return;
+    uint4 w[U];
+    __half d[U];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = d * (float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+    for (int i = 0; i < U; i++) {
+        const int head = slot + i * slots;
+        const bool is_v = head >= c.n_kv;
+        w[i] = make_uint4(0u, 0u, 0u, 0u);   // a row without a place reads as zeros
+        d[i] = __float2half_rn(0.f);
+        if (at.page < 0 || head >= heads) continue;
+        const uint8_t* slab = (is_v ? c.v : c.k) + (size_t)at.page * c.page_bytes +
+                              (size_t)(head - (is_v ? c.n_kv : 0)) * c.slab;
+        if (DT == GB_DT_F16) {
+            w[i] = ldg4(slab + ((size_t)at.row * HD + col) * 2);
+        } else {
+            const uint2 y = __ldg(reinterpret_cast<const uint2*>(slab + (size_t)at.row * HD + col));
+            w[i].x = y.x;
+            w[i].y = y.y;
+            d[i] = __ldg(reinterpret_cast<const __half*>(slab + ((size_t)HD << c.shift)) + at.row * (HD / 32) + col / 32);
         }
     }
-    A* dst = is_v ? vo : ko;
-    if (dst) act_store8(dst + (size_t)t * (is_v ? ldv : ldk) + (size_t)head * HD + col, x);
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+        const int head = slot + i * slots;
+        if (head >= heads) continue;
+        const bool is_v = head >= c.n_kv;
+        A* dst = is_v ? vo : ko;
+        if (!dst) continue;
+        float x[8];
+        if (DT == GB_DT_F16) {
+            const uint32_t y[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y[j]));
+                x[2 * j] = f.x;
+                x[2 * j + 1] = f.y;
+            }
+        } else {
+            const float df = __half2float(d[i]);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const uint32_t y = (j ? w[i].y : w[i].x) ^ 0x80808080u;   // 128 more than the codes
+                x[4 * j] = df * tc::byte_as_float<0>(y, 128.f);
+                x[4 * j + 1] = df * tc::byte_as_float<1>(y, 128.f);
+                x[4 * j + 2] = df * tc::byte_as_float<2>(y, 128.f);
+                x[4 * j + 3] = df * tc::byte_as_float<3>(y, 128.f);
+            }
+        }
+        act_store8(dst + (size_t)t * (is_v ? ldv : ldk) + (size_t)(head - (is_v ? c.n_kv : 0)) * HD + col, x);
+    }
+}
+
+// CTAs of a call over `heads` heads of every token, u of them a thread; 0: too many.
+static unsigned kv_grid(int n_tokens, int heads, int hd, int u) {
+    const long long threads = (long long)n_tokens * ((heads + u - 1) / u) * (hd / 8);
+    return threads > 0x7fffff00LL ? 0u : (unsigned)((threads + KV_THREADS - 1) / KV_THREADS);
 }
 
 }  // namespace gb
@@ -219,15 +293,16 @@ extern "C" int gb_kv_append(const gb_kv_cache* cache, const gb_kv_batch* batch, 
     if (b.n_tokens == 0) return GB_OK;
     unsigned* err = paged_err();
     if (!err) return GB_ECUDA;
-    const long long threads = (long long)b.n_tokens * (n_heads + 2 * c.n_kv) * (hd / 8);
-    if (threads > 0x7fffff00LL) return GB_ELIMIT;
-    const unsigned grid = (unsigned)((threads + 255) / 256);
+    const int heads = n_heads + 2 * c.n_kv;
+    const bool many = kv_grid(b.n_tokens, heads, hd, 2) >= (unsigned)(KV_CTAS * sm_count());
+    const unsigned grid = kv_grid(b.n_tokens, heads, hd, many ? 2 : 1);
+    if (!grid) return GB_ELIMIT;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
 #define GB_APPEND(A, HD, DT)                                                                                        \
-    e = launch_pdl(k_kv_append<A, HD, DT>, dim3(grid), 256, 0, st, c, b, static_cast<const A*>(q), ldq, n_heads,    \
-                   static_cast<A*>(q_out), ldqo, static_cast<const A*>(k), ldk, static_cast<const A*>(v), ldv,       \
-                   rope_cs, rope_len, err)
+    e = launch_pdl(many ? k_kv_append<A, HD, DT, 2> : k_kv_append<A, HD, DT, 1>, dim3(grid), KV_THREADS, 0, st, c, b,       \
+                   static_cast<const A*>(q), ldq, n_heads, static_cast<A*>(q_out), ldqo, static_cast<const A*>(k),   \
+                   ldk, static_cast<const A*>(v), ldv, rope_cs, rope_len, err)
 #define GB_APPEND_DT(A, HD) \
     if (cache->dtype == GB_DT_F16) GB_APPEND(A, HD, GB_DT_F16); else GB_APPEND(A, HD, GB_DT_Q8_0)
     if (dtype == GB_DT_F32) {
@@ -252,14 +327,14 @@ extern "C" int gb_kv_read(const gb_kv_cache* cache, const gb_kv_batch* batch, in
     if (b.n_tokens == 0) return GB_OK;
     unsigned* err = paged_err();
     if (!err) return GB_ECUDA;
-    const long long threads = (long long)b.n_tokens * 2 * c.n_kv * (hd / 8);
-    if (threads > 0x7fffff00LL) return GB_ELIMIT;
-    const unsigned grid = (unsigned)((threads + 255) / 256);
+    const bool many = kv_grid(b.n_tokens, 2 * c.n_kv, hd, 2) >= (unsigned)(KV_CTAS * sm_count());
+    const unsigned grid = kv_grid(b.n_tokens, 2 * c.n_kv, hd, many ? 2 : 1);
+    if (!grid) return GB_ELIMIT;
     cudaError_t e;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define GB_READ(A, HD, DT) \
-    e = launch_pdl(k_kv_read<A, HD, DT>, dim3(grid), 256, 0, st, c, b, static_cast<A*>(k), ldk, static_cast<A*>(v), \
-                   ldv, err)
+    e = launch_pdl(many ? k_kv_read<A, HD, DT, 2> : k_kv_read<A, HD, DT, 1>, dim3(grid), KV_THREADS, 0, st, c, b, \
+                   static_cast<A*>(k), ldk, static_cast<A*>(v), ldv, err)
 #define GB_READ_DT(A, HD) \
     if (cache->dtype == GB_DT_F16) GB_READ(A, HD, GB_DT_F16); else GB_READ(A, HD, GB_DT_Q8_0)
     if (dtype == GB_DT_F32) {
