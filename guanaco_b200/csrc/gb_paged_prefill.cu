@@ -26,6 +26,13 @@
 // an fp16 value and an fp16 remainder, and so are Q8_0 values (code x scale
 // has 18 bits): hi.hi + lo.hi (+ hi.lo), fp32 sums.
 //
+// The tensor cores' additions into O truncate, always towards zero, so over a
+// long axis O comes out low (Q8_0, 8192 tokens: 1.1e-5, against 1.1e-6 of plain
+// fp32 in another order).  fp32 therefore starts O anew every PP_FLUSH tiles and
+// adds what was there, rounded to nearest, to a running sum in the workspace
+// (L2-resident, 128 KB per SM): 4.2e-6 at any length for 16 tiles and 7 % of
+// the time; every 4 tiles 2.6e-6 and 26 %, every 2 tiles 2.4e-6 and 50 %.
+//
 // An F16 cache's tiles are TMA copies, one box per page and 64 columns; Q8_0
 // tiles are dequantised by four warps, a row per thread.  Rows past the last
 // key are zeroed in V (stale cache rows may hold anything).
@@ -41,6 +48,7 @@
 namespace gb {
 
 constexpr int PP_POLY = 8;                      // of this many pairs of exponentials one is a polynomial
+constexpr int PP_FLUSH = 16;                    // fp32: key tiles whose P V stay in tensor memory
 constexpr float PP_TAU = 8.f, PP_LIFT = 6.f;   // p <= 2^14; small p stay normal fp16 numbers
 constexpr int PP_SMEM_MAX = 227 * 1024 - 4096;  // less alignment slack and static shared memory
 
@@ -341,7 +349,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         for (int k = 0; k < NH / 16; k++)
                             tc::mma_f16_ta_w(lead, O, pa + 8u * k,
                                              va + (uint32_t)(((p == 2) * C::KB + (h2 * (NH / 16) + k) * 2048) >> 4), idO,
-                                             j > 0 || h2 > 0 || p > 0 || k > 0);
+                                             (C::F32 ? j % PP_FLUSH : j) > 0 || h2 > 0 || p > 0 || k > 0);
                     }
                 }
                 tc::mma_commit_w(lead, odone + 8 * i);
@@ -516,6 +524,23 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const int lim_min = pos0 + q0 + rt * a.bq;       // and the tile's first query
         const int n_tiles = rt == 0 ? nt0 : nt;          // without any O is not read
         float m = -INFINITY, l = 0.f;                    // the row's maximum, this part's sum
+        // fp32: the running sum of O's columns in the workspace, [HD][128 rows]: this CTA's partial when the keys are
+        // split, else the SM's (a CTA fills an SM); to be scaled by `rs`
+        float* run = a.part;
+        float rs = 1.f;
+        if (C::F32) {
+            unsigned sm_id;
+            asm volatile("mov.u32 %0, %%smid;" : "=r"(sm_id));
+            const size_t slot = n_split > 1 ? (size_t)blockIdx.y * gridDim.x + blockIdx.x : (size_t)min(sm_id, GB_MAX_SMS - 1u);
+            run += (slot * 2 + rt) * (HD + 2) * 128 + (size_t)(2 + hf * (HD / TR)) * 128 + r;
+        }
+        // O's columns c0 .. + 15 with what the running sum holds of them
+        auto read_o = [&](int c0, float (&o)[16], bool more) {
+            tc::tmem_ld16(O + c0, o);
+            if (C::F32 && more)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[i] = fmaf(__ldcg(run + (size_t)(c0 + i) * 128), rs, o[i]);
+        };
         for (int j = 0; j < n_tiles; j++) {
             const int key0 = (j0 + j) * NK, buf = j % NS;
             const uint32_t S = lb + C::SW * rt + (uint32_t)(NK * buf + NH * hf);
@@ -536,12 +561,14 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             for (int i = 0; i < NH; i += 2) mx = fmaxf(mx, fmaxf(x[i], x[i + 1]));
             mx *= sc;
             auto passes = [&](float v) { return v > m + PP_TAU || (m == -INFINITY && v > -INFINITY); };
+            const bool flush = C::F32 && j > 0 && j % PP_FLUSH == 0;
             auto rescale = [&](float v) {   // the maximum moves to v where it passes; O with it
                 const bool move = passes(v);
                 const float al = !move ? 1.f : m == -INFINITY ? 0.f : pp_ex2(m - v);
                 l *= al;
+                rs *= al;
                 m = move ? v : m;
-                if (j > 0) {
+                if (j > 0 && !flush) {
                     // P V of the tile before: with one buffer its commit came before this S; with two the
                     // commit of the one before that did, so the parity is not ambiguous
                     if (NS == 2 && ok) ok = mbs_wait(odone + 8 * rt, (j - 1) & 1, a.err);
@@ -557,14 +584,34 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     tc::fence_before_sync();
                 }
             };
+            auto add_up = [&] {   // what O holds (all P V before this tile) into the running sum
+#pragma unroll 1
+                for (int c0 = 0; c0 < HD / TR; c0 += 16) {
+                    float o[16];
+                    read_o(c0, o, j > PP_FLUSH && rs != 1.f);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        float* to = run + (size_t)(c0 + i) * 128;
+                        if (j == PP_FLUSH || rs != 1.f) __stcg(to, o[i]);   // the maximum has moved since: rescaled
+                        else asm volatile("red.global.add.f32 [%0], %1;" ::"l"(to), "f"(o[i]) : "memory");   // its one writer
+                    }
+                }
+                rs = 1.f;
+                tc::fence_before_sync();
+            };
             if (TR == 1) {
                 if (__any_sync(0xffffffffu, passes(mx))) rescale(mx);
             } else if (pp_vote(1 + rt, passes(mx))) {   // of all rows of the tile
+                if (flush) add_up();
                 s_row[rt][hf][r] = mx;
                 pp_sync(1 + rt);
                 rescale(fmaxf(mx, s_row[rt][hf ^ 1][r]));
                 pp_sync(1 + rt);   // O is rescaled before either part of P is handed over; s_row is free again
                 tc::fence_after_sync();
+            }
+            else if (flush) {
+                add_up();
+                pp_sync(1 + rt);   // O is read before P is handed over
             }
             const float off = PP_LIFT - (m == -INFINITY ? 0.f : m);
             const float2 sc2 = make_float2(sc, sc), off2 = make_float2(off, off);
@@ -603,16 +650,17 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             pp_sync(1 + rt);
             l += s_row[rt][hf ^ 1][r];
         }
+        const bool more = n_tiles > PP_FLUSH;
         if (n_split == 1) {
             const float inv = l > 0.f ? 1.0f / l : 0.f;   // no keys: zeros
             A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD + hf * (HD / TR);
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD / TR; c0 += 32) {
-                float o[32];
-                tc::tmem_ld32(O + c0, o);
+            for (int c0 = 0; c0 < HD / TR; c0 += 16) {
+                float o[16];
+                read_o(c0, o, more);
                 if (live) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
+                    for (int i = 0; i < 16; i += 8) {
                         float v[8];
 #pragma unroll
                         for (int x = 0; x < 8; x++) v[x] = l > 0.f ? o[i + x] * inv : 0.f;
@@ -627,11 +675,11 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 pp[128] = l;
             }
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD / TR; c0 += 32) {
-                float o[32];
-                tc::tmem_ld32(O + c0, o);
+            for (int c0 = 0; c0 < HD / TR; c0 += 16) {
+                float o[16];
+                read_o(c0, o, more);
 #pragma unroll
-                for (int i = 0; i < 32; i++) pp[(2 + hf * (HD / TR) + c0 + i) * 128] = l > 0.f ? o[i] : 0.f;
+                for (int i = 0; i < 16; i++) pp[(2 + hf * (HD / TR) + c0 + i) * 128] = l > 0.f ? o[i] : 0.f;
             }
         }
     }

@@ -248,6 +248,13 @@ def test_prefill(gb, cuda, act, cache, heads, kv, hd, page, q_lens, kv_lens):
     check_attention(gb, act, cache, heads, kv, hd, page, q_lens, kv_lens, False, pad=16 if kv == 2 else 0)
 
 
+@pytest.mark.parametrize("cache", ["f16", "q8_0"])
+def test_prefill_fp32_holds_its_precision_over_a_long_axis(gb, cuda, cache):
+    """Enough query blocks that the keys are not split over CTAs: one CTA adds
+    up all of a row's 6000 keys."""
+    check_attention(gb, "f32", cache, 32, 32, 64, 64, [700], [6000], False)
+
+
 @pytest.mark.parametrize("act", ["f32", "f16"])
 @pytest.mark.parametrize("cache", ["f16", "q8_0"])
 @pytest.mark.parametrize("scale", [1e-4, 30.0])
