@@ -26,12 +26,14 @@
 // an fp16 value and an fp16 remainder, and so are Q8_0 values (code x scale
 // has 18 bits): hi.hi + lo.hi (+ hi.lo), fp32 sums.
 //
-// The tensor cores' additions into O truncate, always towards zero, so over a
-// long axis O comes out low (Q8_0, 8192 tokens: 1.1e-5, against 1.1e-6 of plain
-// fp32 in another order).  fp32 therefore starts O anew every PP_FLUSH tiles and
-// adds what was there, rounded to nearest, to a running sum in the workspace
-// (L2-resident, 128 KB per SM): 4.2e-6 at any length for 16 tiles and 7 % of
-// the time; every 4 tiles 2.6e-6 and 26 %, every 2 tiles 2.4e-6 and 50 %.
+// The tensor cores' additions truncate, always towards zero: their sums come
+// out low.  fp32 adds the products with remainders into S first, so that the
+// truncations are of their size, and starts O anew every PP_FLUSH tiles, adding
+// what was there, rounded to nearest, to a running sum in the workspace
+// (L2-resident, 128 KB per SM).  Error against 64 bits of five prompts of up to
+// 2700 tokens (Q8_0; plain fp32 in another order 8.6e-7) and time: every 16
+// tiles 2.3e-6, 175 us; 8 1.7e-6; 4 1.2e-6, 194 us; 2 8.9e-7, 211 us; never, and
+// the remainders last, 1.1e-5 on 8192 tokens.
 //
 // An F16 cache's tiles are TMA copies, one box per page and 64 columns; Q8_0
 // tiles are dequantised by four warps, a row per thread.  Rows past the last
@@ -48,7 +50,7 @@
 namespace gb {
 
 constexpr int PP_POLY = 8;                      // of this many pairs of exponentials one is a polynomial
-constexpr int PP_FLUSH = 16;                    // fp32: key tiles whose P V stay in tensor memory
+constexpr int PP_FLUSH = 4;                    // fp32: key tiles whose P V stay in tensor memory
 constexpr float PP_TAU = 8.f, PP_LIFT = 6.f;   // p <= 2^14; small p stay normal fp16 numbers
 constexpr int PP_SMEM_MAX = 227 * 1024 - 4096;  // less alignment slack and static shared memory
 
@@ -320,19 +322,20 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             auto scores = [&](int i, int st, int j) {   // S_i = Q_i K^T, the j-th tile's
                 const uint32_t S = C::SW * i + (uint32_t)NK * (j % NS);
                 const uint64_t qa = qd + (uint32_t)(i * (C::QB >> 4)), ka = kd + (uint32_t)(st * (C::KS * C::KB >> 4));
-                if (C::F32) {
-                    const uint32_t qh = 128u + 64u * i;
-#pragma unroll
-                    for (int p = 0; p < C::KS; p++)
-#pragma unroll
-                        for (int k = 0; k < HD / 16; k++)
-                            tc::mma_f16_ta_w(lead, S, qh + 8u * k, ka + (uint32_t)((p * C::KB + (k >> 2) * NK * 128 + (k & 3) * 32) >> 4),
-                                           idS, p > 0 || k > 0);
-                }
+                // fp32: the small products first, so that the sums truncate at their size
 #pragma unroll
                 for (int k = 0; k < HD / 16; k++)
                     tc::mma_f16_w(lead, S, qa + (uint32_t)(((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4),
-                                ka + (uint32_t)(((k >> 2) * NK * 128 + (k & 3) * 32) >> 4), idS, C::F32 || k > 0);
+                                ka + (uint32_t)(((k >> 2) * NK * 128 + (k & 3) * 32) >> 4), idS, k > 0);
+                if (C::F32) {
+                    const uint32_t qh = 128u + 64u * i;
+#pragma unroll
+                    for (int p = C::KS - 1; p >= 0; p--)
+#pragma unroll
+                        for (int k = 0; k < HD / 16; k++)
+                            tc::mma_f16_ta_w(lead, S, qh + 8u * k, ka + (uint32_t)((p * C::KB + (k >> 2) * NK * 128 + (k & 3) * 32) >> 4),
+                                           idS, true);
+                }
                 tc::mma_commit_w(lead, sfull + 8 * (2 * i + j % NS));
             };
             auto output = [&](int i, int st, int j) {   // O_i (+)= P_i V
@@ -524,22 +527,27 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const int lim_min = pos0 + q0 + rt * a.bq;       // and the tile's first query
         const int n_tiles = rt == 0 ? nt0 : nt;          // without any O is not read
         float m = -INFINITY, l = 0.f;                    // the row's maximum, this part's sum
-        // fp32: the running sum of O's columns in the workspace, [HD][128 rows]: this CTA's partial when the keys are
-        // split, else the SM's (a CTA fills an SM); to be scaled by `rs`
+        // fp32: the running sum of O's columns in the workspace, [HD / 4][128 rows][4]: this CTA's partial when the keys are
+        // split, else the SM's (a CTA fills an SM)
         float* run = a.part;
-        float rs = 1.f;
         if (C::F32) {
             unsigned sm_id;
             asm volatile("mov.u32 %0, %%smid;" : "=r"(sm_id));
             const size_t slot = n_split > 1 ? (size_t)blockIdx.y * gridDim.x + blockIdx.x : (size_t)min(sm_id, GB_MAX_SMS - 1u);
-            run += (slot * 2 + rt) * (HD + 2) * 128 + (size_t)(2 + hf * (HD / TR)) * 128 + r;
+            run += (slot * 2 + rt) * (HD + 2) * 128 + (size_t)(2 + hf * (HD / TR)) * 128 + 4 * r;
         }
         // O's columns c0 .. + 15 with what the running sum holds of them
         auto read_o = [&](int c0, float (&o)[16], bool more) {
             tc::tmem_ld16(O + c0, o);
             if (C::F32 && more)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[i] = fmaf(__ldcg(run + (size_t)(c0 + i) * 128), rs, o[i]);
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 w = __ldcg(reinterpret_cast<const float4*>(run + (c0 + i) * 128));
+                    o[i] += w.x;
+                    o[i + 1] += w.y;
+                    o[i + 2] += w.z;
+                    o[i + 3] += w.w;
+                }
         };
         for (int j = 0; j < n_tiles; j++) {
             const int key0 = (j0 + j) * NK, buf = j % NS;
@@ -566,7 +574,6 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const bool move = passes(v);
                 const float al = !move ? 1.f : m == -INFINITY ? 0.f : pp_ex2(m - v);
                 l *= al;
-                rs *= al;
                 m = move ? v : m;
                 if (j > 0 && !flush) {
                     // P V of the tile before: with one buffer its commit came before this S; with two the
@@ -583,20 +590,30 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     }
                     tc::fence_before_sync();
                 }
+                if (C::F32 && j >= PP_FLUSH && al != 1.f) {   // the running sum too
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HD / TR; c0 += 4) {
+                        float4* w = reinterpret_cast<float4*>(run + c0 * 128);
+                        const float4 v = __ldcg(w);
+                        __stcg(w, make_float4(v.x * al, v.y * al, v.z * al, v.w * al));
+                    }
+                }
             };
             auto add_up = [&] {   // what O holds (all P V before this tile) into the running sum
 #pragma unroll 1
                 for (int c0 = 0; c0 < HD / TR; c0 += 16) {
                     float o[16];
-                    read_o(c0, o, j > PP_FLUSH && rs != 1.f);
+                    tc::tmem_ld16(O + c0, o);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        float* to = run + (size_t)(c0 + i) * 128;
-                        if (j == PP_FLUSH || rs != 1.f) __stcg(to, o[i]);   // the maximum has moved since: rescaled
-                        else asm volatile("red.global.add.f32 [%0], %1;" ::"l"(to), "f"(o[i]) : "memory");   // its one writer
+                    for (int i = 0; i < 16; i += 4) {
+                        float* to = run + (c0 + i) * 128;
+                        if (j == PP_FLUSH)
+                            __stcg(reinterpret_cast<float4*>(to), make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+                        else   // its one writer
+                            asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(o[i]), "f"(o[i + 1]),
+                                         "f"(o[i + 2]), "f"(o[i + 3]) : "memory");
                     }
                 }
-                rs = 1.f;
                 tc::fence_before_sync();
             };
             if (TR == 1) {
@@ -668,18 +685,21 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     }
                 }
             }
-        } else {   // [HD + 2][128 rows] of this CTA's tile
-            float* pp = a.part + (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + rt) * (HD + 2) * 128 + r;
+        } else {   // m [128 rows], l [128], O [HD / 4][128][4] of this CTA's tile
+            float* pp = a.part + (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + rt) * (HD + 2) * 128;
             if (hf == 0) {
-                pp[0] = m;
-                pp[128] = l;
+                pp[r] = m;
+                pp[128 + r] = l;
             }
+            pp += (2 + hf * (HD / TR)) * 128 + 4 * r;
 #pragma unroll 1
             for (int c0 = 0; c0 < HD / TR; c0 += 16) {
                 float o[16];
                 read_o(c0, o, more);
 #pragma unroll
-                for (int i = 0; i < 16; i++) pp[(2 + hf * (HD / TR) + c0 + i) * 128] = l > 0.f ? o[i] : 0.f;
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<float4*>(pp + (c0 + i) * 128) =
+                        l > 0.f ? make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         }
     }
@@ -720,7 +740,13 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 const float mz = __ldcg(pp + z * step);
                 const float f = mz > -INFINITY ? pp_ex2(mz - M) * inv : 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = fmaf(f, __ldcg(pp + z * step + (2 + c0 + i) * 128), v[i]);
+                for (int i = 0; i < 8; i += 4) {
+                    const float4 w = __ldcg(reinterpret_cast<const float4*>(pp + 3 * r + z * step + (2 + c0 + i) * 128));
+                    v[i] = fmaf(f, w.x, v[i]);
+                    v[i + 1] = fmaf(f, w.y, v[i + 1]);
+                    v[i + 2] = fmaf(f, w.z, v[i + 2]);
+                    v[i + 3] = fmaf(f, w.w, v[i + 3]);
+                }
             }
             act_store8(dst + c0, v);
         }
