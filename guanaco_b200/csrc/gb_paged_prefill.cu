@@ -28,12 +28,13 @@
 //
 // The tensor cores' additions truncate, always towards zero: their sums come
 // out low.  fp32 adds the products with remainders into S first, so that the
-// truncations are of their size, and starts O anew every PP_FLUSH tiles, adding
-// what was there, rounded to nearest, to a running sum in the workspace
-// (L2-resident, 128 KB per SM).  Error against 64 bits of five prompts of up to
-// 2700 tokens (Q8_0; plain fp32 in another order 8.6e-7) and time: every 16
-// tiles 2.3e-6, 175 us; 8 1.7e-6; 4 1.2e-6, 194 us; 2 8.9e-7, 211 us; never, and
-// the remainders last, 1.1e-5 on 8192 tokens.
+// truncations are of their size, keeps those of P V apart where there is room
+// (hd 64), and starts O anew every FLUSH tiles, adding what was there, rounded
+// to nearest, to a running sum in the workspace (L2-resident, 128 KB per SM).
+// Error against 64 bits of five prompts of up to 2700 tokens in Q8_0 (plain fp32
+// in another order 8.6e-7) and time, hd 128: every 16 tiles 2.3e-6, 175 us; 8
+// 1.7e-6; 4 1.2e-6, 194 us; 2 8.9e-7, 211 us; hd 64 (6.7e-7): 16 8.9e-7; 8 7.2e-7;
+// 4 5.6e-7.  Never, with the remainders last: 1.1e-5 on 8192 tokens.
 //
 // An F16 cache's tiles are TMA copies, one box per page and 64 columns; Q8_0
 // tiles are dequantised by four warps, a row per thread.  Rows past the last
@@ -50,7 +51,6 @@
 namespace gb {
 
 constexpr int PP_POLY = 8;                      // of this many pairs of exponentials one is a polynomial
-constexpr int PP_FLUSH = 4;                    // fp32: key tiles whose P V stay in tensor memory
 constexpr float PP_TAU = 8.f, PP_LIFT = 6.f;   // p <= 2^14; small p stay normal fp16 numbers
 constexpr int PP_SMEM_MAX = 227 * 1024 - 4096;  // less alignment slack and static shared memory
 
@@ -71,7 +71,9 @@ struct PpCfg {
     static constexpr int ST0 = (PP_SMEM_MAX - 2 * QB) / (2 * KS * KB);
     static constexpr int ST = ST0 > 4 ? 4 : ST0;       // K / V stages
     static constexpr int SMEM = 2 * QB + ST * 2 * KS * KB + 1024;
-    static constexpr int PROD = Q8 ? 4 : 1;            // producer warps
+    // producer warps; fp32 at hd 64: two leave every thread 96 registers instead of
+    // 80 (five prompts of up to 2700 tokens 107 / 113 us; hd 128, twice the rows' bytes, 224 / 193 us)
+    static constexpr int PROD = !Q8 ? 1 : F32 && HD == 64 ? 2 : 4;
     static constexpr int TR = F32 || WIDE ? 2 : 1;     // softmax threads per row
     static constexpr int SOFT = 256 * TR, MMA = SOFT / 32;   // their number; the MMA warp
     static constexpr int THREADS = SOFT + 32 + PROD * 32;
@@ -81,6 +83,8 @@ struct PpCfg {
     static constexpr uint32_t SW = NK * NS;
     static constexpr uint32_t PLO = NK / 4;            // fp32: P's remainders, from a part's first column
     static constexpr int NH = NK / TR;                 // keys of a softmax thread
+    static constexpr uint32_t OS = F32 && HD == 64 ? 64 : 0;   // there is room for O's small products, from O's first column
+    static constexpr int FLUSH = OS ? 8 : 4;           // fp32: key tiles whose P V stay in tensor memory
     static_assert(ST >= 2, "shared memory");
 };
 
@@ -248,53 +252,71 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     tc::fence_after_sync();
     const uint32_t tmem = tmem_slot;
 
-    // ---- Q rows: fp16 into shared memory; fp32 split, the high parts into
-    // tensor memory (the A operand of two products of three), the rest into shared memory
+    // ---- Q rows, 16 bytes a lane (a thread per row would touch 32 lines at a
+    // time: 22,000 cycles for fp32 at hd 128): fp16 into shared memory; fp32
+    // scaled and split, the remainders into shared memory, the high parts
+    // through the K / V stages into tensor memory (the A operand of two products of three)
     float up_inv = 1.f;   // 2^-e of this thread's row
-    constexpr int UH = HD / 8 / TR;   // 8-column units of a thread's part of the row
-    const A* qsrc = static_cast<const A*>(a.q) + (size_t)(t_begin + qi) * a.ldq + (size_t)h * HD + hf * (HD / TR);
-    uint8_t* qdst = qs + rt * C::QB;
-    if (!C::F32) {
-        if (warp < C::MMA) {
-#pragma unroll 4
-            for (int u = 0; u < UH; u++) {
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (live) w = ldg4(qsrc + 8 * u);
-                *reinterpret_cast<uint4*>(qdst + pp_off(r, hf * UH + u, 128)) = w;
+    {
+        constexpr int LPR = HD * (int)sizeof(A) / 16, RPW = 32 / LPR, STEP = C::THREADS / 32 * RPW;   // lanes of a row, rows of a warp, of the block
+        constexpr int U = 4;                             // loads in flight
+        const int rows = two ? 256 : 128, la = lane % LPR;
+        for (int i0 = warp * RPW + lane / LPR; i0 - lane / LPR < rows; i0 += U * STEP) {
+            uint4 w[U];
+#pragma unroll
+            for (int v = 0; v < U; v++) {
+                const int i = i0 + v * STEP, rr = i & 127, qq = q0 + (i >> 7) * a.bq + rr / a.group;
+                w[v] = make_uint4(0u, 0u, 0u, 0u);
+                if (i < rows && rr < a.bq * a.group && qq < n_q)
+                    w[v] = ldg4(static_cast<const A*>(a.q) + (size_t)(t_begin + qq) * a.ldq +
+                                (size_t)(kvh * a.group + rr % a.group) * HD + la * (16 / (int)sizeof(A)));
+            }
+#pragma unroll
+            for (int v = 0; v < U; v++) {
+                const int i = i0 + v * STEP, rr = i & 127, tile = i >> 7;
+                if constexpr (!C::F32) {
+                    if (i < rows) *reinterpret_cast<uint4*>(qs + tile * C::QB + pp_off(rr, la, 128)) = w[v];
+                } else {
+                    const float x[4] = {__uint_as_float(w[v].x), __uint_as_float(w[v].y), __uint_as_float(w[v].z), __uint_as_float(w[v].w)};
+                    float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+                    for (int o = LPR / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    const int e = tc::f16_scale_exp(__float_as_uint(mx));
+                    const float up = tc::pow2f(e);
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int c2 = 0; c2 < 2; c2++) {
+                        const float y = x[2 * c2] * up, z = x[2 * c2 + 1] * up;
+                        hi[c2] = pp_pack(y, z);
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[c2]));
+                        lo[c2] = pp_pack(y - f.x, z - f.y);
+                    }
+                    if (i < rows) {
+                        const uint32_t at = (uint32_t)(tile * C::QB) + pp_off(rr, la >> 1, 128) + 8u * (la & 1);
+                        *reinterpret_cast<uint2*>(ks + at) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2*>(qs + at) = make_uint2(lo[0], lo[1]);
+                        if (la == 0) s_row[tile][0][rr] = tc::pow2f(-e);
+                    }
+                }
             }
         }
-    } else {
-        float x[UH][8], mx = 0.f;
-#pragma unroll
-        for (int u = 0; u < UH; u++) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[u][i] = 0.f;
-            if (live) act_load8(qsrc + 8 * u, x[u]);
-#pragma unroll
-            for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[u][i]));
-        }
-        if (warp < C::MMA) s_row[rt][hf][r] = mx;
+    }
+    if constexpr (C::F32) {
+        static_assert(2 * C::QB <= ST * 2 * C::KS * C::KB, "the high parts fit the stages");
         __syncthreads();
-        if (warp < C::MMA) {
-            const int e = tc::f16_scale_exp(__float_as_uint(fmaxf(mx, s_row[rt][hf ^ 1][r])));
-            const float up = tc::pow2f(e);
-            up_inv = tc::pow2f(-e);
+        if (warp < C::MMA && (rt == 0 || two)) {
+            up_inv = s_row[rt][0][r];
             const uint32_t qh = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 64u * rt + (uint32_t)(hf * (HD / 4));
 #pragma unroll
-            for (int u = 0; u < UH; u += 4) {
+            for (int u = 0; u < HD / 8 / TR; u += 4) {
                 uint32_t hi[16];
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
-                    float lo[8];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float y = x[u + v][2 * i] * up, z = x[u + v][2 * i + 1] * up;
-                        hi[4 * v + i] = pp_pack(y, z);
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[4 * v + i]));
-                        lo[2 * i] = y - f.x;
-                        lo[2 * i + 1] = z - f.y;
-                    }
-                    *reinterpret_cast<uint4*>(qdst + pp_off(r, hf * UH + u + v, 128)) = pack_half8(lo);
+                    const uint4 w = *reinterpret_cast<const uint4*>(ks + rt * C::QB + pp_off(r, hf * (HD / 8 / TR) + u + v, 128));
+                    hi[4 * v] = w.x;
+                    hi[4 * v + 1] = w.y;
+                    hi[4 * v + 2] = w.z;
+                    hi[4 * v + 3] = w.w;
                 }
                 tc::tmem_st16_nowait(qh + 4 * u, hi);
             }
@@ -350,9 +372,9 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         const uint32_t pa = P + (uint32_t)(NH * h2) + (p == 1 ? C::PLO : 0u);
 #pragma unroll
                         for (int k = 0; k < NH / 16; k++)
-                            tc::mma_f16_ta_w(lead, O, pa + 8u * k,
+                            tc::mma_f16_ta_w(lead, O + (p > 0 ? C::OS : 0u), pa + 8u * k,
                                              va + (uint32_t)(((p == 2) * C::KB + (h2 * (NH / 16) + k) * 2048) >> 4), idO,
-                                             (C::F32 ? j % PP_FLUSH : j) > 0 || h2 > 0 || p > 0 || k > 0);
+                                             (C::F32 ? j % C::FLUSH : j) > 0 || h2 > 0 || p > (C::OS ? 1 : 0) || k > 0);
                     }
                 }
                 tc::mma_commit_w(lead, odone + 8 * i);
@@ -437,7 +459,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         } else {
             // a thread: row (key) rr of the tile and 16-column runs u0 .., four at
             // a time; the next four are loaded before these are converted
-            constexpr int TPR = 128 / NK;                // threads per row
+            constexpr int TPR = C::Q8 ? C::PROD * 32 / NK : 1;   // threads per row
             constexpr int SUB = HD / 64 / TPR > 0 ? HD / 64 / TPR : 1;   // groups of four runs per thread and tile
             constexpr int NU = HD / 16 / TPR / SUB;      // runs of a group (two at hd 64 with two threads per row)
             const int pt = pw * 32 + lane, rr = pt % NK, u0 = (pt / NK) * SUB * NU;
@@ -536,9 +558,22 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const size_t slot = n_split > 1 ? (size_t)blockIdx.y * gridDim.x + blockIdx.x : (size_t)min(sm_id, GB_MAX_SMS - 1u);
             run += (slot * 2 + rt) * (HD + 2) * 128 + (size_t)(2 + hf * (HD / TR)) * 128 + 4 * r;
         }
-        // O's columns c0 .. + 15 with what the running sum holds of them
+        auto ld_o = [&](int c0, float (&o)[16]) {        // O's columns c0 .. + 15
+            if constexpr (C::OS == 0) {
+                tc::tmem_ld16(O + c0, o);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i += 8) {
+                    float big[8], small[8];
+                    tc::tmem_ld8x2(O + c0 + i, O + C::OS + c0 + i, big, small);
+#pragma unroll
+                    for (int x = 0; x < 8; x++) o[i + x] = big[x] + small[x];
+                }
+            }
+        };
+        // with what the running sum holds of them
         auto read_o = [&](int c0, float (&o)[16], bool more) {
-            tc::tmem_ld16(O + c0, o);
+            ld_o(c0, o);
             if (C::F32 && more)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
@@ -569,7 +604,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             for (int i = 0; i < NH; i += 2) mx = fmaxf(mx, fmaxf(x[i], x[i + 1]));
             mx *= sc;
             auto passes = [&](float v) { return v > m + PP_TAU || (m == -INFINITY && v > -INFINITY); };
-            const bool flush = C::F32 && j > 0 && j % PP_FLUSH == 0;
+            const bool flush = C::F32 && j > 0 && j % C::FLUSH == 0;
             auto rescale = [&](float v) {   // the maximum moves to v where it passes; O with it
                 const bool move = passes(v);
                 const float al = !move ? 1.f : m == -INFINITY ? 0.f : pp_ex2(m - v);
@@ -581,16 +616,17 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     if (NS == 2 && ok) ok = mbs_wait(odone + 8 * rt, (j - 1) & 1, a.err);
                     tc::fence_after_sync();
 #pragma unroll 1
-                    for (int c0 = 0; c0 < HD / TR; c0 += 16) {
+                    for (int n = 0; n < (C::OS ? 2 : 1) * (HD / TR / 16); n++) {
+                        const uint32_t at = O + (n < HD / TR / 16 ? 16u * n : C::OS + 16u * (n - HD / TR / 16));
                         float o[16];
-                        tc::tmem_ld16(O + c0, o);
+                        tc::tmem_ld16(at, o);
 #pragma unroll
                         for (int i = 0; i < 16; i++) o[i] *= al;
-                        tc::tmem_st16(O + c0, o);
+                        tc::tmem_st16(at, o);
                     }
                     tc::fence_before_sync();
                 }
-                if (C::F32 && j >= PP_FLUSH && al != 1.f) {   // the running sum too
+                if (C::F32 && j >= C::FLUSH && al != 1.f) {   // the running sum too
 #pragma unroll 1
                     for (int c0 = 0; c0 < HD / TR; c0 += 4) {
                         float4* w = reinterpret_cast<float4*>(run + c0 * 128);
@@ -603,11 +639,11 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll 1
                 for (int c0 = 0; c0 < HD / TR; c0 += 16) {
                     float o[16];
-                    tc::tmem_ld16(O + c0, o);
+                    ld_o(c0, o);
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         float* to = run + (c0 + i) * 128;
-                        if (j == PP_FLUSH)
+                        if (j == C::FLUSH)
                             __stcg(reinterpret_cast<float4*>(to), make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
                         else   // its one writer
                             asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(o[i]), "f"(o[i + 1]),
@@ -667,23 +703,43 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             pp_sync(1 + rt);
             l += s_row[rt][hf ^ 1][r];
         }
-        const bool more = n_tiles > PP_FLUSH;
+        const bool more = n_tiles > C::FLUSH;
         if (n_split == 1) {
+            // Through the row tile's part of Q, which no MMA reads any more, so
+            // that a warp writes whole runs of rows: 32 rows of RB bytes at a time.
+            constexpr int WB = C::QB / (4 * TR), RB = WB / 32 < 128 ? WB / 32 : 128, UN = RB / 16;
+            constexpr int CP = RB / (int)sizeof(A);      // columns at a time
+            static_assert(CP % 16 == 0 && HD / TR % CP == 0 && (UN == 8 || UN == 4), "rows of the staging area");
+            uint8_t* wb = qs + rt * C::QB + warp % (4 * TR) * WB;
+            auto at = [&](int row, int u) { return wb + row * RB + ((u ^ (UN == 8 ? row & 7 : (row >> 1) & 3)) << 4); };
             const float inv = l > 0.f ? 1.0f / l : 0.f;   // no keys: zeros
-            A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD + hf * (HD / TR);
+            const unsigned long long dst = live ? reinterpret_cast<unsigned long long>(
+                static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD + hf * (HD / TR)) : 0ull;
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD / TR; c0 += 16) {
-                float o[16];
-                read_o(c0, o, more);
-                if (live) {
+            for (int c1 = 0; c1 < HD / TR; c1 += CP) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < CP; c0 += 16) {
+                    float o[16];
+                    read_o(c1 + c0, o, more);
 #pragma unroll
-                    for (int i = 0; i < 16; i += 8) {
-                        float v[8];
+                    for (int i = 0; i < 16; i++) o[i] = l > 0.f ? o[i] * inv : 0.f;
 #pragma unroll
-                        for (int x = 0; x < 8; x++) v[x] = l > 0.f ? o[i + x] * inv : 0.f;
-                        act_store8(dst + c0 + i, v);
+                    for (int i = 0; i < (int)sizeof(A); i++) {   // 16 columns: 2 or 4 units
+                        const int n = 16 / (int)sizeof(A);
+                        uint4 w;
+                        if constexpr (C::F32) w = make_uint4(__float_as_uint(o[n * i]), __float_as_uint(o[n * i + 1]), __float_as_uint(o[n * i + 2]), __float_as_uint(o[n * i + 3]));
+                        else w = make_uint4(pp_pack(o[n * i], o[n * i + 1]), pp_pack(o[n * i + 2], o[n * i + 3]), pp_pack(o[n * i + 4], o[n * i + 5]), pp_pack(o[n * i + 6], o[n * i + 7]));
+                        *reinterpret_cast<uint4*>(at(lane, c0 / n + i)) = w;
                     }
                 }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < UN; i++) {
+                    const int row = (i * 32 + lane) / UN, u = lane % UN;
+                    const unsigned long long to = __shfl_sync(0xffffffffu, dst, row);
+                    if (to) *reinterpret_cast<uint4*>(to + c1 * sizeof(A) + 16 * u) = *reinterpret_cast<const uint4*>(at(row, u));
+                }
+                __syncwarp();
             }
         } else {   // m [128 rows], l [128], O [HD / 4][128][4] of this CTA's tile
             float* pp = a.part + (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + rt) * (HD + 2) * 128;
