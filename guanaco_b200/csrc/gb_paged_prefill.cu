@@ -164,31 +164,61 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const int kvh = blockIdx.x % c.n_kv, y = blockIdx.x / c.n_kv;
 
     griddep_wait();   // launched ahead of the kernel before it
-    // ---- which sequence and query block: the blocks of the sequences in order, the longest of each first
+    // ---- which sequence and query block.  Up to 32 sequences: the y-th of all
+    // blocks by their key tiles, the longest first; more: the sequences in order
     if (warp == 0) {
         if (lane == 0) s_seq = -1;
         __syncwarp();
-        int base = 0;
-        for (int s0 = 0; s0 < b.n_seq; s0 += 32) {
-            const int s = s0 + lane;
-            int n = 0;
-            if (s < b.n_seq) n = b.cu ? max(__ldg(b.cu + s + 1) - __ldg(b.cu + s), 0) : 1;
-            const int nb = (n + 2 * a.bq - 1) / (2 * a.bq);
-            int incl = nb;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += v;
-            }
-            const unsigned hit = __ballot_sync(0xffffffffu, y < base + incl);
-            if (hit) {
-                if (lane == __ffs(hit) - 1) {
-                    s_seq = s;
-                    s_blk = nb - 1 - (y - (base + incl - nb));
+        const int bb = 2 * a.bq;
+        auto queries = [&](int s) { return s >= b.n_seq ? 0 : b.cu ? max(__ldg(b.cu + s + 1) - __ldg(b.cu + s), 0) : 1; };
+        if (b.n_seq <= 32) {
+            const int n = queries(lane), nb = (n + bb - 1) / bb, pos = n ? seq_len(b, lane, a.err) - n : 0;
+            // blocks of this lane's sequence with at least t key tiles: their keys end past (t - 1) NK
+            auto count = [&](int t) {
+                if (t <= 0) return nb;
+                const int past = (t - 1) * NK + 1 - pos;   // queries of the sequence before the first such block's end
+                return past > n ? 0 : nb - max((past + bb - 1) / bb - 1, 0);
+            };
+            int lo = 0, hi = __reduce_max_sync(0xffffffffu, n ? max(pos + n + NK - 1, 0) / NK : 0) + 1;
+            if (y < __reduce_add_sync(0xffffffffu, nb)) {
+                while (hi - lo > 1) {   // more than y blocks have lo tiles, at most y have hi
+                    const int mid = (lo + hi) >> 1;
+                    if (__reduce_add_sync(0xffffffffu, count(mid)) > y) lo = mid;
+                    else hi = mid;
                 }
-                break;
+                const int longer = count(hi), same = count(lo) - longer;
+                int incl = same;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += v;
+                }
+                const int at = y - __reduce_add_sync(0xffffffffu, longer) - (incl - same);
+                if (at >= 0 && at < same) {
+                    s_seq = lane;
+                    s_blk = nb - 1 - longer - at;
+                }
             }
-            base += __shfl_sync(0xffffffffu, incl, 31);
+        } else {
+            int base = 0;
+            for (int s0 = 0; s0 < b.n_seq; s0 += 32) {
+                const int nb = (queries(s0 + lane) + bb - 1) / bb;
+                int incl = nb;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += v;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, y < base + incl);
+                if (hit) {
+                    if (lane == __ffs(hit) - 1) {
+                        s_seq = s0 + lane;
+                        s_blk = nb - 1 - (y - (base + incl - nb));
+                    }
+                    break;
+                }
+                base += __shfl_sync(0xffffffffu, incl, 31);
+            }
         }
     }
     __syncthreads();
@@ -247,55 +277,73 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == C::MMA) tc::tmem_alloc(&tmem_slot, 512);
-    tc::fence_before_sync();
-    __syncthreads();
-    tc::fence_after_sync();
-    const uint32_t tmem = tmem_slot;
 
-    // ---- Q rows, 16 bytes a lane (a thread per row would touch 32 lines at a
-    // time: 22,000 cycles for fp32 at hd 128): fp16 into shared memory; fp32
+    // ---- Q rows, eight lanes a row (a thread per row would touch 32 lines at
+    // a time: 22,000 cycles for fp32 at hd 128): fp16 into shared memory; fp32
     // scaled and split, the remainders into shared memory, the high parts
     // through the K / V stages into tensor memory (the A operand of two products of three)
     float up_inv = 1.f;   // 2^-e of this thread's row
     {
-        constexpr int LPR = HD * (int)sizeof(A) / 16, RPW = 32 / LPR, STEP = C::THREADS / 32 * RPW;   // lanes of a row, rows of a warp, of the block
-        constexpr int U = 4;                             // loads in flight
-        const int rows = two ? 256 : 128, la = lane % LPR;
-        for (int i0 = warp * RPW + lane / LPR; i0 - lane / LPR < rows; i0 += U * STEP) {
-            uint4 w[U];
+        constexpr int NV = HD / 64, LD = C::F32 ? 2 : 1;           // a lane's runs of 8 columns, loads of each
+        constexpr int U = NV * LD == 4 ? 2 : 4;                    // rows in flight
+        constexpr int STEP = C::THREADS / 8;                       // rows of the block
+        const int rows = two ? 256 : 128, la = lane & 7;
+        for (int i0 = tid >> 3; i0 - (lane >> 3) < rows; i0 += U * STEP) {
+            uint4 w[U][NV][LD];
 #pragma unroll
             for (int v = 0; v < U; v++) {
                 const int i = i0 + v * STEP, rr = i & 127, qq = q0 + (i >> 7) * a.bq + rr / a.group;
-                w[v] = make_uint4(0u, 0u, 0u, 0u);
-                if (i < rows && rr < a.bq * a.group && qq < n_q)
-                    w[v] = ldg4(static_cast<const A*>(a.q) + (size_t)(t_begin + qq) * a.ldq +
-                                (size_t)(kvh * a.group + rr % a.group) * HD + la * (16 / (int)sizeof(A)));
+                const bool in = i < rows && rr < a.bq * a.group && qq < n_q;
+                const A* src = static_cast<const A*>(a.q) + (size_t)(t_begin + qq) * a.ldq +
+                               (size_t)(kvh * a.group + rr % a.group) * HD + 8 * la;
+#pragma unroll
+                for (int x = 0; x < NV; x++)
+#pragma unroll
+                    for (int z = 0; z < LD; z++)
+                        w[v][x][z] = in ? ldg4(src + 64 * x + 4 * z) : make_uint4(0u, 0u, 0u, 0u);
             }
 #pragma unroll
             for (int v = 0; v < U; v++) {
                 const int i = i0 + v * STEP, rr = i & 127, tile = i >> 7;
                 if constexpr (!C::F32) {
-                    if (i < rows) *reinterpret_cast<uint4*>(qs + tile * C::QB + pp_off(rr, la, 128)) = w[v];
-                } else {
-                    const float x[4] = {__uint_as_float(w[v].x), __uint_as_float(w[v].y), __uint_as_float(w[v].z), __uint_as_float(w[v].w)};
-                    float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+                    if (i < rows)
 #pragma unroll
-                    for (int o = LPR / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        for (int x = 0; x < NV; x++)
+                            *reinterpret_cast<uint4*>(qs + tile * C::QB + pp_off(rr, 8 * x + la, 128)) = w[v][x][0];
+                } else {
+                    float f[NV][8], mx = 0.f;
+#pragma unroll
+                    for (int x = 0; x < NV; x++)
+#pragma unroll
+                        for (int z = 0; z < 2; z++) {
+                            const uint4 g = w[v][x][z];
+                            f[x][4 * z] = __uint_as_float(g.x);
+                            f[x][4 * z + 1] = __uint_as_float(g.y);
+                            f[x][4 * z + 2] = __uint_as_float(g.z);
+                            f[x][4 * z + 3] = __uint_as_float(g.w);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) mx = fmaxf(mx, fabsf(f[x][4 * z + k]));
+                        }
+#pragma unroll
+                    for (int o = 4; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                     const int e = tc::f16_scale_exp(__float_as_uint(mx));
                     const float up = tc::pow2f(e);
-                    uint32_t hi[2], lo[2];
-#pragma unroll
-                    for (int c2 = 0; c2 < 2; c2++) {
-                        const float y = x[2 * c2] * up, z = x[2 * c2 + 1] * up;
-                        hi[c2] = pp_pack(y, z);
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[c2]));
-                        lo[c2] = pp_pack(y - f.x, z - f.y);
-                    }
                     if (i < rows) {
-                        const uint32_t at = (uint32_t)(tile * C::QB) + pp_off(rr, la >> 1, 128) + 8u * (la & 1);
-                        *reinterpret_cast<uint2*>(ks + at) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2*>(qs + at) = make_uint2(lo[0], lo[1]);
                         if (la == 0) s_row[tile][0][rr] = tc::pow2f(-e);
+#pragma unroll
+                        for (int x = 0; x < NV; x++) {
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const float y0 = f[x][2 * k] * up, y1 = f[x][2 * k + 1] * up;
+                                hi[k] = pp_pack(y0, y1);
+                                const float2 h2 = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+                                lo[k] = pp_pack(y0 - h2.x, y1 - h2.y);
+                            }
+                            const uint32_t at = (uint32_t)(tile * C::QB) + pp_off(rr, 8 * x + la, 128);
+                            *reinterpret_cast<uint4*>(ks + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4*>(qs + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        }
                     }
                 }
             }
@@ -303,10 +351,12 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     }
     if constexpr (C::F32) {
         static_assert(2 * C::QB <= ST * 2 * C::KS * C::KB, "the high parts fit the stages");
+        tc::fence_before_sync();
         __syncthreads();
+        tc::fence_after_sync();
         if (warp < C::MMA && (rt == 0 || two)) {
             up_inv = s_row[rt][0][r];
-            const uint32_t qh = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 64u * rt + (uint32_t)(hf * (HD / 4));
+            const uint32_t qh = tmem_slot + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 64u * rt + (uint32_t)(hf * (HD / 4));
 #pragma unroll
             for (int u = 0; u < HD / 8 / TR; u += 4) {
                 uint32_t hi[16];
@@ -327,6 +377,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
     bool ok = true;
 
     if (warp == C::MMA) {   // ---- MMA issue: the whole warp, uniform; one lane's instructions
@@ -717,10 +768,23 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD + hf * (HD / TR)) : 0ull;
 #pragma unroll 1
             for (int c1 = 0; c1 < HD / TR; c1 += CP) {
-#pragma unroll 1
+                float4 sum[C::F32 ? CP / 4 : 1];             // all of a run's loads in flight
+                if (C::F32 && more)
+#pragma unroll
+                    for (int i = 0; i < CP / 4; i++) sum[i] = __ldcg(reinterpret_cast<const float4*>(run + (c1 + 4 * i) * 128));
+#pragma unroll
                 for (int c0 = 0; c0 < CP; c0 += 16) {
                     float o[16];
-                    read_o(c1 + c0, o, more);
+                    ld_o(c1 + c0, o);
+                    if (C::F32 && more)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const float4 w = sum[C::F32 ? (c0 + i) / 4 : 0];
+                            o[i] += w.x;
+                            o[i + 1] += w.y;
+                            o[i + 2] += w.z;
+                            o[i + 3] += w.w;
+                        }
 #pragma unroll
                     for (int i = 0; i < 16; i++) o[i] = l > 0.f ? o[i] * inv : 0.f;
 #pragma unroll
