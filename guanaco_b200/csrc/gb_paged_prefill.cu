@@ -11,27 +11,29 @@
 //                back into tensor memory over S
 //   O += P V     A = P from tensor memory, B = V as it lies in the cache (rows
 //                = keys, MN-major): V is never transposed
-// While one row tile's softmax runs the tensor cores work for the other; with
-// tiles of 64 keys fp16 has room for two buffers of S, so the next scores are
-// there when a softmax ends.  fp32 is bound by the tensor cores (three
-// products) and keeps Q's high parts in tensor memory instead, which takes
-// their reads off shared memory.  Two threads per row only exchange a vote per
-// key tile.
+// While one row tile's softmax runs the tensor cores work for the other.  With
+// one product per operand and tiles of 64 keys there is room for two buffers of
+// S, so the next scores are there when a softmax ends.  With several products
+// (fp32 activations, a Q8_0 cache) the tensor cores are the bound, and Q (its
+// high parts) is kept in tensor memory, which takes its reads off shared
+// memory.  Two threads per row only exchange a vote per key tile.
 // The maximum moves only when a score exceeds it by more than PP_TAU (log2
 // units), so O in tensor memory is rarely rescaled.
 //
-// Precision.  fp16 activations: Q exact, P rounded to fp16, Q8_0 values rounded
-// to fp16 (each an error of the size of the fp16 output's own rounding).
-// fp32 activations: Q (scaled by a power of two per row) and P are split into
-// an fp16 value and an fp16 remainder, and so are Q8_0 values (code x scale
-// has 18 bits): hi.hi + lo.hi (+ hi.lo), fp32 sums.
+// Precision.  P is rounded to fp16 for fp16 activations (an error of the size of
+// the fp16 output's own rounding); for fp32 ones Q (scaled by a power of two per
+// row) and P are split into an fp16 value and an fp16 remainder.  Q8_0 values
+// (code x scale has 18 bits) are always split so, a product for each part:
+// hi.hi + lo.hi + hi.lo for fp32, hi.hi + hi.lo for fp16.  (K and V rounded to
+// fp16 instead: error against 64 bits 4.0e-4, that of the output's rounding alone 2.1e-4,
+// and 91 us; split 2.8e-4 and 106 us; five prompts of up to 968 tokens.)
 //
 // The tensor cores' additions truncate, always towards zero: their sums come
 // out low.  fp32 adds the products with remainders into S first, so that the
 // truncations are of their size, keeps those of P V apart where there is room
 // (hd 64), and starts O anew every FLUSH tiles, adding what was there, rounded
 // to nearest, to a running sum in the workspace (L2-resident, 128 KB per SM).
-// Error against 64 bits of five prompts of up to 2700 tokens in Q8_0 (plain fp32
+// Error against 64 bits of five prompts of up to 968 tokens in Q8_0 (plain fp32
 // in another order 8.6e-7) and time, hd 128: every 16 tiles 2.3e-6, 175 us; 8
 // 1.7e-6; 4 1.2e-6, 194 us; 2 8.9e-7, 211 us; hd 64 (6.7e-7): 16 8.9e-7; 8 7.2e-7;
 // 4 5.6e-7.  Never, with the remainders last: 1.1e-5 on 8192 tokens.
@@ -57,14 +59,15 @@ constexpr int PP_SMEM_MAX = 227 * 1024 - 4096;  // less alignment slack and stat
 template <typename A, int HD, int DT>
 struct PpCfg {
     static constexpr bool F32 = sizeof(A) == 4, Q8 = DT == GB_DT_Q8_0;
-    // fp16, hd 128, F16 cache: tiles of 128 keys (an MMA of N 128 takes 80 cycles,
-    // one of N 64 takes 64), one buffer of S, two threads per row; elsewhere 64
-    // keys, fp16 with two buffers of S and one thread per row.  One prompt of
-    // 8192 tokens that way / the other: F16 hd 128 489 / 597 us, F16 hd 64 580 /
-    // 449 us, Q8_0 hd 128 886 / 713 us.
+    // fp16, F16 cache, hd 128: tiles of 128 keys (an MMA of N 128 takes 80 cycles,
+    // one of N 64 takes 64), one buffer of S, two threads per row; hd 64: 64 keys,
+    // two buffers and one thread per row.  One prompt of 8192 tokens that way /
+    // the other: hd 128 489 / 597 us, hd 64 580 / 449 us.  Several products per
+    // operand: one buffer, two threads per row (Q8_0 hd 128 896 us, with two
+    // buffers and Q in shared memory 1543 us).
     static constexpr bool WIDE = !F32 && !Q8 && HD == 128;
     static constexpr int NK = WIDE ? 128 : 64;         // keys per tile
-    static constexpr int KS = F32 && Q8 ? 2 : 1;       // fp16 parts of K and V (of Q and P: 2 for fp32)
+    static constexpr int KS = Q8 ? 2 : 1;              // fp16 parts of K and V (of Q and P: 2 for fp32)
     static constexpr int G = HD / 64;                  // 64-column groups (128 bytes)
     static constexpr int QB = 128 * HD * 2;            // bytes of a row tile's part
     static constexpr int KB = NK * HD * 2;             // bytes of a K (or V) tile's part
@@ -72,14 +75,15 @@ struct PpCfg {
     static constexpr int ST = ST0 > 4 ? 4 : ST0;       // K / V stages
     static constexpr int SMEM = 2 * QB + ST * 2 * KS * KB + 1024;
     // producer warps; fp32 at hd 64: two leave every thread 96 registers instead of
-    // 80 (five prompts of up to 2700 tokens 107 / 113 us; hd 128, twice the rows' bytes, 224 / 193 us)
+    // 80 (five prompts of up to 968 tokens 107 / 113 us; hd 128, twice the rows' bytes, 224 / 193 us)
     static constexpr int PROD = !Q8 ? 1 : F32 && HD == 64 ? 2 : 4;
-    static constexpr int TR = F32 || WIDE ? 2 : 1;     // softmax threads per row
+    static constexpr bool QT = F32 || Q8;              // Q, or its high parts, in tensor memory
+    static constexpr int TR = QT || WIDE ? 2 : 1;      // softmax threads per row
     static constexpr int SOFT = 256 * TR, MMA = SOFT / 32;   // their number; the MMA warp
     static constexpr int THREADS = SOFT + 32 + PROD * 32;
     // tensor memory columns: S (and P over it) of row tile i at SW i, in NS
     // buffers; fp32: Q's high parts at 128 + 64 i; O at 256 + 128 i
-    static constexpr int NS = F32 || WIDE ? 1 : 2;     // buffers of S
+    static constexpr int NS = QT || WIDE ? 1 : 2;      // buffers of S
     static constexpr uint32_t SW = NK * NS;
     static constexpr uint32_t PLO = NK / 4;            // fp32: P's remainders, from a part's first column
     static constexpr int NH = NK / TR;                 // keys of a softmax thread
@@ -309,7 +313,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     if (i < rows)
 #pragma unroll
                         for (int x = 0; x < NV; x++)
-                            *reinterpret_cast<uint4*>(qs + tile * C::QB + pp_off(rr, 8 * x + la, 128)) = w[v][x][0];
+                            *reinterpret_cast<uint4*>((C::QT ? ks : qs) + tile * C::QB + pp_off(rr, 8 * x + la, 128)) = w[v][x][0];
                 } else {
                     float f[NV][8], mx = 0.f;
 #pragma unroll
@@ -349,13 +353,13 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
         }
     }
-    if constexpr (C::F32) {
+    if constexpr (C::QT) {
         static_assert(2 * C::QB <= ST * 2 * C::KS * C::KB, "the high parts fit the stages");
         tc::fence_before_sync();
         __syncthreads();
         tc::fence_after_sync();
         if (warp < C::MMA && (rt == 0 || two)) {
-            up_inv = s_row[rt][0][r];
+            if (C::F32) up_inv = s_row[rt][0][r];
             const uint32_t qh = tmem_slot + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 64u * rt + (uint32_t)(hf * (HD / 4));
 #pragma unroll
             for (int u = 0; u < HD / 8 / TR; u += 4) {
@@ -395,19 +399,20 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             auto scores = [&](int i, int st, int j) {   // S_i = Q_i K^T, the j-th tile's
                 const uint32_t S = C::SW * i + (uint32_t)NK * (j % NS);
                 const uint64_t qa = qd + (uint32_t)(i * (C::QB >> 4)), ka = kd + (uint32_t)(st * (C::KS * C::KB >> 4));
-                // fp32: the small products first, so that the sums truncate at their size
+                // the small products first, so that the sums truncate at their size
+                if (C::F32 || !C::QT)
 #pragma unroll
-                for (int k = 0; k < HD / 16; k++)
-                    tc::mma_f16_w(lead, S, qa + (uint32_t)(((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4),
-                                ka + (uint32_t)(((k >> 2) * NK * 128 + (k & 3) * 32) >> 4), idS, k > 0);
-                if (C::F32) {
+                    for (int k = 0; k < HD / 16; k++)
+                        tc::mma_f16_w(lead, S, qa + (uint32_t)(((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4),
+                                      ka + (uint32_t)(((k >> 2) * NK * 128 + (k & 3) * 32) >> 4), idS, k > 0);
+                if (C::QT) {
                     const uint32_t qh = 128u + 64u * i;
 #pragma unroll
                     for (int p = C::KS - 1; p >= 0; p--)
 #pragma unroll
                         for (int k = 0; k < HD / 16; k++)
                             tc::mma_f16_ta_w(lead, S, qh + 8u * k, ka + (uint32_t)((p * C::KB + (k >> 2) * NK * 128 + (k & 3) * 32) >> 4),
-                                           idS, true);
+                                           idS, C::F32 || p < C::KS - 1 || k > 0);
                 }
                 tc::mma_commit_w(lead, sfull + 8 * (2 * i + j % NS));
             };
@@ -419,7 +424,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     wait(pfull + 8 * (2 * i + (TR == 2 ? h2 : j % NS)), (j / NS) & 1);
                     tc::fence_after_sync();
 #pragma unroll
-                    for (int p = 0; p < (C::F32 ? C::KS + 1 : 1); p++) {   // hi.hi, lo.hi, hi.lo
+                    for (int p = 0; p < C::KS + 1; p++) {   // hi.hi, lo.hi (fp32), hi.lo
+                        if (!C::F32 && p == 1) continue;
                         const uint32_t pa = P + (uint32_t)(NH * h2) + (p == 1 ? C::PLO : 0u);
 #pragma unroll
                         for (int k = 0; k < NH / 16; k++)
