@@ -26,6 +26,12 @@ namespace gb {
 // heads) pairs and enter the second as (2 keys, head) pairs: an 8 x 8
 // transposition in registers (movmatrix).
 //
+// The tensor cores' additions truncate, so for fp32 the products with remainders
+// come first or apart and each step's P V starts from zero and is added to O
+// rounded to nearest (96 sequences of up to 8066 keys, F16 cache: error against 64 bits
+// 2.4e-6 -> 6.5e-7, where plain fp32 has 1.3e-6, and 271 -> 273 us; Q8_0 1.7e-6 -> 3.3e-7 (1.2e-6),
+// 221 -> 235 us).
+//
 // Work: a step is 16 keys (Q8_0: 32, the same bytes) of one (sequence, KV
 // head, 8 query heads); all
 // steps of the batch, in that order, are cut into one equal run per CTA
@@ -123,6 +129,21 @@ __device__ __forceinline__ void pd_split(float x, float y, uint32_t& hi, uint32_
 // rounded to fp16 without a remainder (q is fp16 already; for a probability
 // the error is of the size of the output's own rounding, 2.9e-4 against
 // 2.1e-4 of the 64-bit result together).
+// o += A b.  fp32: with b's remainders first, from zero and then added rounded
+// to nearest, as the tensor cores' additions truncate.
+template <typename A>
+__device__ __forceinline__ void pd_add(float (&o)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&bh)[2],
+                                       const uint32_t (&bl)[2]) {
+    if (sizeof(A) == 2) {
+        pd_mma(o, a0, a1, a2, a3, bh[0], bh[1]);
+        return;
+    }
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    pd_mma(s, a0, a1, a2, a3, bl[0], bl[1]);
+    pd_mma(s, a0, a1, a2, a3, bh[0], bh[1]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] += s[i];
+}
 template <typename A>
 __device__ __forceinline__ void pd_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
     if (sizeof(A) == 4) {
@@ -405,7 +426,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                 // ---- raw scores x[i][h] of keys rg + 8 i, heads 2 t + h
                 float x[2 * C::SUB][2];
                 if (!C::Q8) {
-                    float sa[4] = {0.f, 0.f, 0.f, 0.f};
+                    float sa[4] = {0.f, 0.f, 0.f, 0.f}, sl[4] = {0.f, 0.f, 0.f, 0.f};   // sl: with q's remainders
 #pragma unroll
                     for (int j = 0; j < NB; j++) {
                         const uint8_t* kp = st + (j >> 1) * 2048 + (k_off ^ ((j & 1) * 64));
@@ -414,10 +435,13 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                         pd_mma(sa, k0.x, k1.x, k0.y, k1.y, qh[2 * j][0], qh[2 * j][1]);
                         pd_mma(sa, k0.z, k1.z, k0.w, k1.w, qh[2 * j + 1][0], qh[2 * j + 1][1]);
                         if (sizeof(A) == 4) {
-                            pd_mma(sa, k0.x, k1.x, k0.y, k1.y, ql[2 * j][0], ql[2 * j][1]);
-                            pd_mma(sa, k0.z, k1.z, k0.w, k1.w, ql[2 * j + 1][0], ql[2 * j + 1][1]);
+                            pd_mma(sl, k0.x, k1.x, k0.y, k1.y, ql[2 * j][0], ql[2 * j][1]);
+                            pd_mma(sl, k0.z, k1.z, k0.w, k1.w, ql[2 * j + 1][0], ql[2 * j + 1][1]);
                         }
                     }
+                    if (sizeof(A) == 4)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sa[i] += sl[i];
                     x[0][0] = sa[0]; x[0][1] = sa[1]; x[1][0] = sa[2]; x[1][1] = sa[3];
                 } else {
 #pragma unroll
@@ -440,12 +464,12 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                             const uint32_t c0 = pd_codes(w0.y, 0x4140), c1 = pd_codes(w1.y, 0x4140);
                             const uint32_t c2 = pd_codes(w0.y, 0x4342), c3 = pd_codes(w1.y, 0x4342);
                             float sa[4] = {0.f, 0.f, 0.f, 0.f};
-                            pd_mma(sa, a0, a1, a2, a3, qh[2 * j][0], qh[2 * j][1]);
-                            pd_mma(sa, c0, c1, c2, c3, qh[2 * j + 1][0], qh[2 * j + 1][1]);
-                            if (sizeof(A) == 4) {
+                            if (sizeof(A) == 4) {   // the small products first
                                 pd_mma(sa, a0, a1, a2, a3, ql[2 * j][0], ql[2 * j][1]);
                                 pd_mma(sa, c0, c1, c2, c3, ql[2 * j + 1][0], ql[2 * j + 1][1]);
                             }
+                            pd_mma(sa, a0, a1, a2, a3, qh[2 * j][0], qh[2 * j][1]);
+                            pd_mma(sa, c0, c1, c2, c3, qh[2 * j + 1][0], qh[2 * j + 1][1]);
                             const float d0 = __half2float(sk[0][j]), d1 = __half2float(sk[1][j]);
                             x[2 * u][0] = fmaf(sa[0], d0, x[2 * u][0]);
                             x[2 * u][1] = fmaf(sa[1], d0, x[2 * u][1]);
@@ -554,8 +578,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                         for (int e = 0; e < 4; e++) {
                             const uint32_t a0 = __byte_perm(v[0][e], v[1][e], 0x5410), a1 = __byte_perm(v[0][e], v[1][e], 0x7632);
                             const uint32_t a2 = __byte_perm(v[2][e], v[3][e], 0x5410), a3 = __byte_perm(v[2][e], v[3][e], 0x7632);
-                            pd_mma(O[j * 4 + e], a0, a1, a2, a3, bh[0], bh[1]);
-                            if (sizeof(A) == 4) pd_mma(O[j * 4 + e], a0, a1, a2, a3, bl[0], bl[1]);
+                            pd_add<A>(O[j * 4 + e], a0, a1, a2, a3, bh, bl);
                         }
                     }
                 } else {
@@ -582,8 +605,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                                 const uint32_t hi = __byte_perm(w[2], w[3], e ? 0x7362 : 0x5140);
                                 const uint32_t a0 = pd_codes(lo, 0x4140), a1 = pd_codes(lo, 0x4342);
                                 const uint32_t a2 = pd_codes(hi, 0x4140), a3 = pd_codes(hi, 0x4342);
-                                pd_mma(O[j * 2 + e], a0, a1, a2, a3, bh[0], bh[1]);
-                                if (sizeof(A) == 4) pd_mma(O[j * 2 + e], a0, a1, a2, a3, bl[0], bl[1]);
+                                pd_add<A>(O[j * 2 + e], a0, a1, a2, a3, bh, bl);
                             }
                         }
                 }
