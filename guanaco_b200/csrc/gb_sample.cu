@@ -21,7 +21,15 @@
 //                whole cluster.  A top-k whose bin and those before it hold at
 //                most SMP_CAND tokens ends here: CTA 0 filters them and draws,
 //                and no other token's weight is computed.
-//   draw         sums by index, the CTA, the warp, the token of the target
+//   draw         sums by index, the CTA, the warp, the token of the target.
+//                After a top-p cut each CTA knows its kept weights from its
+//                histogram, and only the one with the target goes on.
+// A row is a chain of these phases, which the clusters of other rows fill: 1 row
+// of 32,000 takes 8.7 us, 256 rows of 128,256 (top-p) 225 us = 585 GB/s, 46,000
+// cycles a row and cluster: 14,500 until the maximum is known (HBM), 14,000 for
+// the weights (40 instructions each), the rest four exchanges over the
+// cluster, the bin's tokens and their ranks.  Other splits of 256 rows measured
+// slower: 16 CTAs a row, three CTAs of 384 threads an SM.
 #include "gb_common.cuh"
 #include "gb_internal.h"
 #include "gb_mt.cuh"
@@ -74,6 +82,7 @@ __device__ __forceinline__ u64 smp_share(u64 total, uint32_t part) {
 
 struct SmpShared {
     uint32_t count[SMP_BINS], wlo[SMP_BINS], whi[SMP_BINS];   // whi:wlo a 64-bit weight
+    u64 last[32];                                             // the candidates that a search ends with
     u64 cand[SMP_CAND], cand_w[SMP_CAND];                     // ranks of a bin's tokens in this CTA; CTA 0: all, weights
     // written by the cluster's CTAs
     u64 peer_max[SMP_CL], peer_a[SMP_CL], peer_b[SMP_CL], peer_sum[SMP_CL];
@@ -84,27 +93,20 @@ struct SmpShared {
     uint32_t n_list;
 };
 
-// Inclusive sums over the block's threads of two values.
-__device__ __forceinline__ void smp_scan2(u64& a, u64& b, u64* sa, u64* sb) {
+// Inclusive sums over the block's threads.
+__device__ __forceinline__ u64 smp_scan(u64 a, u64* sums) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const u64 x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
-        if (lane >= o) {
-            a += x;
-            b += y;
-        }
+        const u64 x = __shfl_up_sync(0xffffffffu, a, o);
+        if (lane >= o) a += x;
     }
     __syncthreads();
-    if (lane == 31) {
-        sa[warp] = a;
-        sb[warp] = b;
-    }
+    if (lane == 31) sums[warp] = a;
     __syncthreads();
-    for (int w = 0; w < warp; w++) {
-        a += sa[w];
-        b += sb[w];
-    }
+#pragma unroll
+    for (int w = 0; w < SMP_W; w++) a += w < warp ? sums[w] : 0ull;
+    return a;
 }
 
 __global__ void __cluster_dims__(SMP_CL, 1, 1) __launch_bounds__(SMP_THREADS, 2)
@@ -196,9 +198,9 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
     // (l - max) / t correctly rounded: quotient from the rounded reciprocal and
     // one step on its remainder (Markstein, IBM J. Res. Dev. 34, 1990, theorem
     // on division: exact unless t's fraction is all ones), away from over- and
-    // underflow; any other t takes the division.  Distances past 30 t weigh
-    // nothing: 2^40 e^-30 rounds to 0.
-    const float far = -30.f * t, rt = __frcp_rn(t);
+    // underflow; any other t takes the division.  Distances past 28.5 t weigh
+    // nothing: 2^40 e^-28.5 rounds to 0.
+    const float far = -28.5f * t, rt = __frcp_rn(t);
     const bool quick = t > 8.6736174e-19f && t < 1.1529215e18f && (__float_as_uint(t) & 0x7fffffu) != 0x7fffffu;
     auto exp_of = [&](float l) {
         const float d = fmaxf(l - mx, far);
@@ -207,20 +209,33 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
             q = d * rt;
             q = fmaf(fmaf(-t, q, d), rt, q);
         } else {
-            q = __fdiv_rn(d, t);
+            q = __fdiv_rn(d, fminf(t, 3.4028235e38f));   // (-inf / inf is no number)
         }
         return expf(q);
     };
     auto weight_of = [&](float l) { return smp_weight(exp_of(l)); };
     const bool by_k = k > 0 && k < vocab, by_p = p < 1.f;
     u64 cut = 0;   // kept: rank >= cut
+    u64 own_kept = 0;   // this thread's part of this CTA's kept weights, if they are known without a pass
+    bool known = false;
+    auto block_sum = [&](u64 v) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        __syncthreads();
+        if (lane == 0) sh.warp64[warp] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int w = 0; w < SMP_W; w++) v += sh.warp64[w];
+        return v;
+    };
 
     if (by_k || by_p) {
-        // e < 2^-41 rounds to 0 and ln 2^41 = 28.42: the last bin (from 28.47) holds no weight
-        const float inv_bin = SMP_BINS / (28.5f * t);
-        auto bin_of = [&](float l) {   // monotone in l; 0 where NaN (inf - inf, 0 inf)
-            const float d = fminf(fmaxf((mx - l) * inv_bin, 0.f), (float)(SMP_BINS - 1));
-            return (int)(__float_as_uint(d + 8388608.f) - 0x4B000000u);   // rounded
+        // Monotone in l.  The last bin, from 28.493 t on, holds no weight: ln 2^41 = 28.42.
+        const float inv_bin = fminf((SMP_BINS - 1) / (28.5f * t), 3.4028235e38f);
+        auto bin_of = [&](float l) {   // rounded; no number (t infinite, l masked): the last
+            const float d = fmaxf(l - mx, far);
+            return (int)min(__float_as_uint(fmaf(d, -inv_bin, 8388608.f)) - 0x4B000000u, (uint32_t)SMP_BINS - 1);
         };
         auto rank_of = [&](int i) { return (u64)smp_key(x[i]) << 32 | ~(uint32_t)(i0 + i); };
         auto clear = [&] {
@@ -239,7 +254,7 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
         // sum over the bins up to it, and the sum of all bins.
         auto merge = [&](bool counts, u64& own, u64& run, u64& all) {
             cl.sync();   // every histogram is done
-            u64 a = 0, unused = 0;
+            u64 a = 0;
             if (tid < PER) {
                 const int i = rank * PER + tid;
 #pragma unroll
@@ -249,7 +264,7 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
                 }
             }
             own = a;
-            smp_scan2(a, unused, sh.warp64, sh.warp64b);
+            a = smp_scan(a, sh.warp64);
             if (tid == SMP_THREADS - 1) sh.tot_a = a;
             __syncthreads();
             if (tid < SMP_CL) cl.map_shared_rank(&sh, tid)->peer_a[rank] = sh.tot_a;
@@ -279,18 +294,30 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
         auto gather = [&](auto in_bin, u64& mn, u64& mxr) {
             mn = ~0ull;
             mxr = 0;
-            for (int i = tid; i < n4; i += SMP_THREADS) {
-                const float4 v = *reinterpret_cast<const float4*>(x + 4 * i);
-                const float l[4] = {v.x, v.y, v.z, v.w};
+            for (int i = tid; i < n4; i += 4 * SMP_THREADS) {   // four reads in flight
+                float4 v[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (in_bin(l[j], 4 * i + j)) {
-                        const u64 rk = rank_of(4 * i + j);
-                        mn = rk < mn ? rk : mn;
-                        mxr = rk > mxr ? rk : mxr;
-                        const uint32_t at = atomicAdd(&sh.n_cand, 1u);
-                        if (at < SMP_CAND) sh.cand[at] = rk;
-                    }
+                for (int z = 0; z < 4; z++) {
+                    const int at = i + z * SMP_THREADS;
+                    v[z] = at < n4 ? *reinterpret_cast<const float4*>(x + 4 * at) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                uint32_t hit = 0;
+#pragma unroll
+                for (int z = 0; z < 4; z++) {
+                    const float l[4] = {v[z].x, v[z].y, v[z].z, v[z].w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (i + z * SMP_THREADS < n4 && in_bin(l[j], 4 * (i + z * SMP_THREADS) + j)) hit |= 1u << (4 * z + j);
+                }
+                while (hit) {
+                    const int z = __ffs(hit) - 1;
+                    hit &= hit - 1;
+                    const u64 rk = rank_of(4 * (i + (z >> 2) * SMP_THREADS) + (z & 3));
+                    mn = rk < mn ? rk : mn;
+                    mxr = rk > mxr ? rk : mxr;
+                    const uint32_t at = atomicAdd(&sh.n_cand, 1u);
+                    if (at < SMP_CAND) sh.cand[at] = rk;
+                }
             }
             __syncthreads();
             if (tid < SMP_CL) cl.map_shared_rank(&sh, tid)->peer_n[rank] = sh.n_cand;
@@ -314,18 +341,7 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
             }
             return from >= 0 ? cl.map_shared_rank(&sh, from)->cand[at] : 0ull;
         };
-        auto block_sum = [&](u64 v) {
-#pragma unroll
-            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            __syncthreads();
-            if (lane == 0) sh.warp64[warp] = v;
-            __syncthreads();
-            v = 0;
-#pragma unroll
-            for (int w = 0; w < SMP_W; w++) v += sh.warp64[w];
-            return v;
-        };
-        // In CTA 0: the candidate at which the sum, from (ga, gb), reaches goal; to every CTA.
+        // In CTA 0: the candidate at which the sum, from g, reaches goal; to every CTA.
         auto resolve = [&](u64 goal, bool counts, u64 g, int m) {
             const u64 me = candidate();
             bool in = me != 0;
@@ -360,8 +376,7 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
                 }
                 __syncthreads();
                 const u64 own_n = sh.count[tid], own = (u64)sh.whi[tid] << 32 | sh.wlo[tid];
-                u64 a = own, unused = 0;
-                smp_scan2(a, unused, sh.warp64, sh.warp64b);
+                const u64 a = smp_scan(own, sh.warp64);
                 if (g + a - own < goal && goal <= g + a) {
                     sh.n_list = (uint32_t)own_n;
                     sh.cut_bin = (uint32_t)tid;
@@ -377,15 +392,15 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
             __syncthreads();
             if (in) {
                 const uint32_t to = atomicAdd(&sh.n_list, 1u);
-                sh.cand[to] = me;
+                sh.last[to] = me;
                 sh.cand_w[to] = w;
             }
             __syncthreads();
             if (warp == 0 && lane < left) {
-                const u64 mine = sh.cand[lane], mine_w = sh.cand_w[lane];
+                const u64 mine = sh.last[lane], mine_w = sh.cand_w[lane];
                 u64 before = g;
                 for (int j = 0; j < left; j++)
-                    if (sh.cand[j] > mine) before += sh.cand_w[j];
+                    if (sh.last[j] > mine) before += sh.cand_w[j];
                 if (before < goal && goal <= before + mine_w)
                     for (int c = 0; c < SMP_CL; c++) cl.map_shared_rank(&sh, c)->cut_rank = mine;
             }
@@ -396,6 +411,10 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
             const uint32_t bin = sh.cut_bin;
             u64 g = sh.cut_a, lo = 0, hi = ~0ull, mn, mxr;
             uint32_t m = gather([&](float l, int) { return bin_of(l) == (int)bin; }, mn, mxr);
+            if (!counts && m <= SMP_CAND) {   // this CTA's kept weights: the bins before, and of this one the ranks from the cut on
+                known = !(mp > 0.f);
+                for (int i = tid; i < (int)bin; i += SMP_THREADS) own_kept += (u64)sh.whi[i] << 32 | sh.wlo[i];
+            }
             while (m > SMP_CAND) {   // too many: bins over the ranks between the first and the last of them
 #pragma unroll
                 for (int z = 16; z; z >>= 1) {
@@ -449,8 +468,11 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
             }
             if (rank == 0) resolve(goal, counts, g, (int)m);
             cl.sync();
+            const u64 at = sh.cut_rank;
+            if (known && tid < (int)sh.peer_n[rank] && sh.cand[tid] >= at)
+                own_kept += weight_of(smp_logit((uint32_t)(sh.cand[tid] >> 32)));
             if (tid == 0) sh.n_cand = 0;
-            return sh.cut_rank;
+            return at;
         };
         u64 own, run, all;
         if (by_k) {
@@ -506,8 +528,11 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
             // tokens that top-k left; all of them: the sum that the share is taken of
             auto weigh = [&](float l, int i) { return rank_of(i) >= cut ? weight_of(l) : 0ull; };
             if (by_k) clear();
+            float4 v, next = make_float4(0.f, 0.f, 0.f, 0.f);   // read ahead of the atomics
+            if (tid < n4) next = *reinterpret_cast<const float4*>(x + 4 * tid);
             for (int i = tid; i < n4; i += SMP_THREADS) {
-                const float4 v = *reinterpret_cast<const float4*>(x + 4 * i);
+                v = next;
+                if (i + SMP_THREADS < n4) next = *reinterpret_cast<const float4*>(x + 4 * (i + SMP_THREADS));
                 const float l[4] = {v.x, v.y, v.z, v.w};
                 int bin[4];
                 u64 w[4];
@@ -550,7 +575,23 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
         e = exp_of(l);
         return (l > cut_l || (l == cut_l && (uint32_t)(i0 + i) <= cut_i)) && e >= mp;
     };
-    u64 sum = 0;
+    u64 upto = 0, total = 0, sum = 0;   // kept weights before this CTA (then this thread), all, this thread's
+    auto exchange = [&](u64 own) {
+        if (tid < SMP_CL) cl.map_shared_rank(&sh, tid)->peer_sum[rank] = own;
+        cl.sync();   // after this no CTA touches another's memory
+#pragma unroll
+        for (int c = 0; c < SMP_CL; c++) {
+            if (c < rank) upto += sh.peer_sum[c];
+            total += sh.peer_sum[c];
+        }
+        return smp_share(total, min((uint32_t)uf, 0xFFFFFFu));
+    };
+    u64 target = 0;
+    if (known) {   // only the CTA that the target falls into looks for it
+        const u64 own = block_sum(own_kept);
+        target = exchange(own);
+        if (target < upto || target >= upto + own) return;
+    }
     {
         uint32_t h = 0;   // at most 2^17 x 2^15 / 512 x 2
         int lo = 0;
@@ -576,19 +617,13 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
         }
         sum = smp_join(h, lo);
     }
-    u64 incl = sum, unused = 0;
-    smp_scan2(incl, unused, sh.warp64, sh.warp64b);   // running sums over the block
-    if (tid == SMP_THREADS - 1) sh.tot_a = incl;
-    __syncthreads();
-    if (tid < SMP_CL) cl.map_shared_rank(&sh, tid)->peer_sum[rank] = sh.tot_a;
-    cl.sync();   // after this no CTA touches another's memory
-    u64 upto = incl - sum, total = 0;
-#pragma unroll
-    for (int c = 0; c < SMP_CL; c++) {
-        if (c < rank) upto += sh.peer_sum[c];
-        total += sh.peer_sum[c];
+    const u64 incl = smp_scan(sum, sh.warp64);   // running sums over the block
+    if (!known) {
+        if (tid == SMP_THREADS - 1) sh.tot_a = incl;
+        __syncthreads();
+        target = exchange(sh.tot_a);
     }
-    const u64 target = smp_share(total, min((uint32_t)uf, 0xFFFFFFu));
+    upto += incl - sum;
     // the thread whose run holds the target; its warp looks through the run
     const uint32_t who = __ballot_sync(0xffffffffu, target >= upto && target < upto + sum);
     if (!who) return;

@@ -119,3 +119,21 @@ def test_frequencies(gb, cuda):
     got = torch.bincount(torch.tensor(draw(gb, x, u)), minlength=5) / n
     # a boundary of the running sum moves at most one grid point
     assert (got - p.cpu()).abs().max() <= 2.0 / n
+
+
+@pytest.mark.parametrize("vocab", [5, 3001])
+def test_infinite_temperature(gb, cuda, vocab):
+    """Every token that is not masked weighs the same; a masked one nothing."""
+    logits = rows(6, vocab, 9)
+    logits[:, ::3] = float("-inf")
+    left = [i for i in range(vocab) if i % 3]
+    u = [0.0, 0.2, 0.5, 0.7, 0.9, 0.99]
+    want = [left[int(len(left) * torch.tensor(v).mul(2**24).floor().item() / 2**24)] for v in u]
+    assert draw(gb, logits, u, [float("inf")] * 6) == want
+    assert draw(gb, logits, u, [float("inf")] * 6, k=[vocab - 1] * 6, p=[1.0] * 6) == want
+    # nucleus of equal weights: the largest logits, ties by index
+    half = draw(gb, logits, u, [float("inf")] * 6, p=[0.5] * 6)
+    for r, tok in enumerate(half):
+        order = sorted(left, key=lambda i: (-logits[r, i].item(), i))
+        kept = sorted(order[: -(-len(left) // 2)])
+        assert tok == kept[int(len(kept) * torch.tensor(u[r]).mul(2**24).floor().item() / 2**24)]
