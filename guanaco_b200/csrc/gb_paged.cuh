@@ -39,9 +39,11 @@ inline bool paged_rows_ok(int dtype, const void* p, int ld, int width) {
 }
 // Workspace of the attention entry points: partials (of the prompts' CTAs that
 // share a row block, only launched when all of them fit the SMs; or of the
-// single tokens' CTAs), then a ticket per row block, then two per CTA of the
-// single tokens and one per (sequence, KV head, 8 query heads).  Tickets are zero between calls, and never where a
-// call of another shape leaves partials.
+// single tokens' CTAs) or the prompts' running sums; then a ticket per row
+// block, which marks a running sum's place as taken where blocks are not
+// shared; then two per CTA of the single tokens and one per (sequence, KV head,
+// 8 query heads).  Tickets are zero between calls, and never where a call of
+// another shape leaves partials.
 constexpr size_t PAGED_PART_BYTES = (size_t)GB_MAX_SMS * 2 * (128 + 2) * 128 * sizeof(float);
 constexpr size_t PAGED_TICKETS_AT = PAGED_PART_BYTES + GB_MAX_SMS * sizeof(unsigned);
 // Packed prompts (gb_paged_prefill.cu).

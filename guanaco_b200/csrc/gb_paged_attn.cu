@@ -817,12 +817,14 @@ static int paged_attention(const gb_kv_cache* cache, const gb_kv_batch* batch, i
         !paged_rows_ok(dtype, out, ldo, n_heads * hd))
         return GB_EINVAL;
     if (b.n_tokens == 0) return GB_OK;
+    const int group = n_heads / c.n_kv;
+    const long long heads8 = (long long)c.n_kv * ((group + PD_HEADS - 1) / PD_HEADS);
+    if (decode ? (double)b.n_seq * (b.cap / 16 + 1) * heads8 > 0x7fffffff   // steps
+               : group > 128)                                               // rows of a query
+        return GB_ELIMIT;
     unsigned* err = paged_err();
     if (!err) return GB_ECUDA;
-    const int group = n_heads / c.n_kv;
     if (decode) {
-        const long long heads8 = (long long)c.n_kv * ((group + PD_HEADS - 1) / PD_HEADS);
-        if ((long long)b.n_seq * (b.cap / 16 + 1) * heads8 > 0x7fffffffLL) return GB_ELIMIT;   // steps
         cudaError_t e = cudaErrorInvalidValue;
 #define GB_DECODE(T, A, HD, DT)                                \
     if (dtype == T && hd == HD && cache->dtype == DT)          \

@@ -160,7 +160,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __shared__ __align__(8) uint64_t bars[4 * ST + 13];
     __shared__ float s_row[2][2][128];                  // what the two threads of a row exchange
     __shared__ uint32_t tmem_slot;
-    __shared__ int s_seq, s_blk;
+    __shared__ int s_seq, s_blk, s_slot;
     __shared__ unsigned s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedView& c = a.c;
@@ -281,6 +281,26 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == C::MMA) tc::tmem_alloc(&tmem_slot, 512);
+    // Where fp32 keeps a running sum: as many CTAs as slots have one each; of
+    // more, no more than SMs run at a time (a CTA takes all of an SM's tensor
+    // memory), so that a free slot is found from the SM's number on.
+    const bool claim = C::F32 && (size_t)gridDim.x * gridDim.y > GB_MAX_SMS && nt > C::FLUSH;
+    if (C::F32 && tid == 0) {
+        s_slot = blockIdx.y * gridDim.x + blockIdx.x;
+        if (claim) {
+            unsigned at;
+            asm volatile("mov.u32 %0, %%smid;" : "=r"(at));
+            int tries = 64 * GB_MAX_SMS;
+            for (at %= GB_MAX_SMS; atomicCAS(a.tickets + at, 0u, 1u) != 0u; at = (at + 1) % GB_MAX_SMS)
+                if (--tries == 0) {   // a workspace that was never zeroed, or is shared
+                    atomicExch(a.err, (unsigned)(-GB_ETIMEOUT));
+                    break;
+                }
+            __threadfence();
+            s_slot = (int)at;
+        }
+        else if (s_slot >= GB_MAX_SMS) s_slot = 0;   // no running sum
+    }
 
     // ---- Q rows, eight lanes a row (a thread per row would touch 32 lines at
     // a time: 22,000 cycles for fp32 at hd 128): fp16 into shared memory; fp32
@@ -607,13 +627,10 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         const int n_tiles = rt == 0 ? nt0 : nt;          // without any O is not read
         float m = -INFINITY, l = 0.f;                    // the row's maximum, this part's sum
         // fp32: the running sum of O's columns in the workspace, [HD / 4][128 rows][4]: this CTA's partial when the keys are
-        // split, else the SM's (a CTA fills an SM)
+        // split, else a slot of its own for as long as it runs
         float* run = a.part;
         if (C::F32) {
-            unsigned sm_id;
-            asm volatile("mov.u32 %0, %%smid;" : "=r"(sm_id));
-            const size_t slot = n_split > 1 ? (size_t)blockIdx.y * gridDim.x + blockIdx.x : (size_t)min(sm_id, GB_MAX_SMS - 1u);
-            run += (slot * 2 + rt) * (HD + 2) * 128 + (size_t)(2 + hf * (HD / TR)) * 128 + 4 * r;
+            run += ((size_t)s_slot * 2 + rt) * (HD + 2) * 128 + (size_t)(2 + hf * (HD / TR)) * 128 + 4 * r;
         }
         auto ld_o = [&](int c0, float (&o)[16]) {        // O's columns c0 .. + 15
             if constexpr (C::OS == 0) {
@@ -835,6 +852,10 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, 512);
     }
+    if (claim && tid == 0) {
+        __threadfence();
+        atomicExch(a.tickets + s_slot, 0u);
+    }
     if (n_split == 1) return;
     // ---- the last split of this row block joins them
     if (tid == 0) {
@@ -920,7 +941,6 @@ int paged_prefill(const gb_kv_cache* cache, const PagedView& c, const BatchView&
     a.ldq = ldq;
     a.ldo = ldo;
     a.group = n_heads / c.n_kv;
-    if (a.group > 128) return GB_ELIMIT;
     a.bq = 128 / a.group;
     a.err = err;
     const int hd = cache->head_dim;

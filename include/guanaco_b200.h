@@ -286,7 +286,8 @@ typedef struct {
  * rotated at its position first, and when q is not NULL the rotated q
  * (n_heads heads) goes to q_out (which may be q).  Q8_0: per 32 columns
  * d = half(max |x| / 127) (at most 65504), code = x / d rounded to nearest
- * even; NaN and d = 0 give code 0.  Rows 16-byte aligned.  Asynchronous. */
+ * even; NaN and d = 0 give code 0.  Rows 16-byte aligned.  GB_ELIMIT: more
+ * threads than a grid holds (2^31 tokens x heads, about).  Asynchronous. */
 int gb_kv_append(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q, int ldq, int n_heads,
                  void* q_out, int ldqo, const void* k, int ldk, const void* v, int ldv, const float* rope_cs,
                  int rope_len, void* stream);
@@ -301,9 +302,14 @@ int gb_kv_read(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, vo
  * zeros.  n_heads a multiple of n_kv_heads.  fp32 softmax and sums.
  * _decode: one token per sequence (cu_seqlens NULL), split over the cache's
  * length and joined.  _prefill: packed prompts of any lengths, on the tensor
- * cores.  ws: gb_paged_workspace_bytes(...) bytes for the largest n_seq it
- * will serve, 16-byte aligned, zeroed once; calls that share it must not
- * overlap in time.  Asynchronous. */
+ * cores.  ws: gb_paged_workspace_bytes(...) bytes (about 26 MB) for the
+ * largest n_seq it will serve, 16-byte aligned, zeroed once; calls that share
+ * it must not overlap in time.  GB_ELIMIT: _prefill with more than 128 query
+ * heads per KV head; _decode where n_seq x the table's positions / 16 x heads
+ * passes 2^31.  Precision: fp32 rows as two fp16 parts (22 bits) in every
+ * product; fp16 rows with the probabilities rounded to fp16.  _prefill reads
+ * Q8_0 values as two fp16 parts: those beyond 65504 become infinite, as in an
+ * F16 cache.  Asynchronous. */
 size_t gb_paged_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int n_seq);
 int gb_paged_attention_decode(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q, int ldq,
                               int n_heads, void* out, int ldo, void* ws, void* stream);

@@ -255,6 +255,14 @@ def test_prefill_fp32_holds_its_precision_over_a_long_axis(gb, cuda, cache):
     check_attention(gb, "f32", cache, 32, 32, 64, 64, [700], [6000], False)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prefill_of_many_blocks(gb, cuda, hd):
+    """More CTAs than places for a running sum, each over enough keys to need
+    one; up to 32 sequences (longest blocks first, empty ones among them) and more."""
+    check_attention(gb, "f32", "f16", 8, 8, hd, 32, [300, 0, 1, 700, 129], [900, 40, 777, 700, 1200], False)
+    check_attention(gb, "f32", "q8_0", 8, 8, hd, 16, [40 + s % 3 for s in range(36)], [600 + 7 * s for s in range(36)], False)
+
+
 @pytest.mark.parametrize("act", ["f32", "f16"])
 @pytest.mark.parametrize("cache", ["f16", "q8_0"])
 @pytest.mark.parametrize("scale", [1e-4, 30.0])

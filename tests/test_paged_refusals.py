@@ -74,6 +74,15 @@ def test_rows(gb):
     assert L.gb_paged_attention_decode(c, C.addressof(packed), 0, P, 256, 4, P, 256, P, None) == E
 
 
+def test_limits(gb):
+    """Sizes that the kernels' indices do not hold."""
+    L, c0, b0 = gb.lib(), cache(gb, n_kv_heads=1), batch(gb)
+    c, b = C.addressof(c0), C.addressof(b0)
+    assert L.gb_paged_attention_prefill(c, b, 0, P, 129 * 64, 129, P, 129 * 64, P, None) == gb.GB_ELIMIT
+    many = batch(gb, n_seq=100, n_tokens=100, table_stride=1 << 26)   # 100 x 2^26 steps of 16 positions
+    assert L.gb_paged_attention_decode(c, C.addressof(many), 0, P, 256, 4, P, 256, P, None) == gb.GB_ELIMIT
+
+
 def test_empty_batches_do_nothing(gb):
     L, c0, b0 = gb.lib(), cache(gb), batch(gb, n_seq=0, n_tokens=0)
     c, b = C.addressof(c0), C.addressof(b0)
