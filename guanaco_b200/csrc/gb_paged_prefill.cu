@@ -157,7 +157,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     uint8_t* qs = sm;                                   // [2 tiles]: Q, for fp32 its remainders
     uint8_t* ks = sm + 2 * C::QB;                       // [ST][KS]
     uint8_t* vs = ks + ST * C::KS * C::KB;              // [ST][KS]
-    __shared__ __align__(8) uint64_t bars[4 * ST + 13];
+    __shared__ __align__(8) uint64_t bars[4 * ST + 14];
     __shared__ float s_row[2][2][128];                  // what the two threads of a row exchange
     __shared__ uint32_t tmem_slot;
     __shared__ int s_seq, s_blk, s_slot;
@@ -167,6 +167,28 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const BatchView& b = a.b;
     const int kvh = blockIdx.x % c.n_kv, y = blockIdx.x / c.n_kv;
 
+    const uint32_t b0 = tc::smem_u32(&bars[0]);
+    const uint32_t kfull = b0, kfree = b0 + 8 * ST, vfull = b0 + 16 * ST, vfree = b0 + 24 * ST;   // [ST] each
+    const uint32_t sfull = b0 + 32 * ST, pfull = sfull + 32, odone = sfull + 64, ofull = sfull + 80, tail = sfull + 96, qread = sfull + 104;   // [2][2], [2][2], [2], [2], 1, 1
+    if (tid == 32) {
+        for (int i = 0; i < ST; i++) {
+            mbs_init(kfull + 8 * i, C::PROD);
+            mbs_init(kfree + 8 * i, 1);
+            mbs_init(vfull + 8 * i, C::PROD);
+            mbs_init(vfree + 8 * i, 1);
+        }
+        for (int i = 0; i < 4; i++) {   // [row tile][buffer]; P with two threads per row: [row tile][half]
+            mbs_init(sfull + 8 * i, 1);
+            mbs_init(pfull + 8 * i, 4);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbs_init(odone + 8 * i, 1);   // every P V of a row tile
+            mbs_init(ofull + 8 * i, 1);   // its last
+        }
+        mbs_init(tail, 1);
+        mbs_init(qread, C::MMA);          // Q's high parts have left the V stages
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     griddep_wait();   // launched ahead of the kernel before it
     // ---- which sequence and query block.  Up to 32 sequences: the y-th of all
     // blocks by their key tiles, the longest first; more: the sequences in order
@@ -259,58 +281,46 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         return;
     }
 
-    const uint32_t b0 = tc::smem_u32(&bars[0]);
-    const uint32_t kfull = b0, kfree = b0 + 8 * ST, vfull = b0 + 16 * ST, vfree = b0 + 24 * ST;   // [ST] each
-    const uint32_t sfull = b0 + 32 * ST, pfull = sfull + 32, odone = sfull + 64, ofull = sfull + 80, tail = sfull + 96;   // [2][2], [2][2], [2], [2], 1
-    if (tid == 0) {
-        for (int i = 0; i < ST; i++) {
-            mbs_init(kfull + 8 * i, C::PROD);
-            mbs_init(kfree + 8 * i, 1);
-            mbs_init(vfull + 8 * i, C::PROD);
-            mbs_init(vfree + 8 * i, 1);
-        }
-        for (int i = 0; i < 4; i++) {   // [row tile][buffer]; P with two threads per row: [row tile][half]
-            mbs_init(sfull + 8 * i, 1);
-            mbs_init(pfull + 8 * i, 4);
-        }
-        for (int i = 0; i < 2; i++) {
-            mbs_init(odone + 8 * i, 1);   // every P V of a row tile
-            mbs_init(ofull + 8 * i, 1);   // its last
-        }
-        mbs_init(tail, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == C::MMA) tc::tmem_alloc(&tmem_slot, 512);
-    // Where fp32 keeps a running sum: as many CTAs as slots have one each; of
+    // Where fp32 keeps a running sum: as many CTAs as places have one each; of
     // more, no more than SMs run at a time (a CTA takes all of an SM's tensor
-    // memory), so that a free slot is found from the SM's number on.
+    // memory), so that a free place is found from the SM's number on.
     const bool claim = C::F32 && (size_t)gridDim.x * gridDim.y > GB_MAX_SMS && nt > C::FLUSH;
-    if (C::F32 && tid == 0) {
-        s_slot = blockIdx.y * gridDim.x + blockIdx.x;
-        if (claim) {
-            unsigned at;
-            asm volatile("mov.u32 %0, %%smid;" : "=r"(at));
-            int tries = 64 * GB_MAX_SMS;
-            for (at %= GB_MAX_SMS; atomicCAS(a.tickets + at, 0u, 1u) != 0u; at = (at + 1) % GB_MAX_SMS)
-                if (--tries == 0) {   // a workspace that was never zeroed, or is shared
-                    atomicExch(a.err, (unsigned)(-GB_ETIMEOUT));
-                    break;
-                }
-            __threadfence();
-            s_slot = (int)at;
+    auto start_sync = [&] {   // of all but the producers, which start on K at once
+        tc::fence_before_sync();
+        asm volatile("barrier.cta.sync.aligned 3, %0;" ::"n"(C::SOFT + 32) : "memory");
+        tc::fence_after_sync();
+    };
+    if (warp == C::MMA) {
+        tc::tmem_alloc(&tmem_slot, 512);
+        if (C::F32 && lane == 0) {
+            s_slot = blockIdx.y * gridDim.x + blockIdx.x;
+            if (claim) {
+                unsigned at;
+                asm volatile("mov.u32 %0, %%smid;" : "=r"(at));
+                int tries = 64 * GB_MAX_SMS;
+                for (at %= GB_MAX_SMS; atomicCAS(a.tickets + at, 0u, 1u) != 0u; at = (at + 1) % GB_MAX_SMS)
+                    if (--tries == 0) {   // a workspace that was never zeroed, or is shared
+                        atomicExch(a.err, (unsigned)(-GB_ETIMEOUT));
+                        break;
+                    }
+                __threadfence();
+                s_slot = (int)at;
+            } else if (s_slot >= GB_MAX_SMS) {
+                s_slot = 0;   // no running sum
+            }
         }
-        else if (s_slot >= GB_MAX_SMS) s_slot = 0;   // no running sum
+        __syncwarp();
     }
 
     // ---- Q rows, eight lanes a row (a thread per row would touch 32 lines at
     // a time: 22,000 cycles for fp32 at hd 128): fp16 into shared memory; fp32
     // scaled and split, the remainders into shared memory, the high parts
-    // through the K / V stages into tensor memory (the A operand of two products of three)
+    // through the V stages into tensor memory (the A operand of two products of three)
     float up_inv = 1.f;   // 2^-e of this thread's row
-    {
+    if (warp < C::MMA) {
         constexpr int NV = HD / 64, LD = C::F32 ? 2 : 1;           // a lane's runs of 8 columns, loads of each
         constexpr int U = NV * LD == 4 ? 2 : 4;                    // rows in flight
-        constexpr int STEP = C::THREADS / 8;                       // rows of the block
+        constexpr int STEP = C::SOFT / 8;                          // rows of the block
         const int rows = two ? 256 : 128, la = lane & 7;
         for (int i0 = tid >> 3; i0 - (lane >> 3) < rows; i0 += U * STEP) {
             uint4 w[U][NV][LD];
@@ -333,7 +343,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     if (i < rows)
 #pragma unroll
                         for (int x = 0; x < NV; x++)
-                            *reinterpret_cast<uint4*>((C::QT ? ks : qs) + tile * C::QB + pp_off(rr, 8 * x + la, 128)) = w[v][x][0];
+                            *reinterpret_cast<uint4*>((C::QT ? vs : qs) + tile * C::QB + pp_off(rr, 8 * x + la, 128)) = w[v][x][0];
                 } else {
                     float f[NV][8], mx = 0.f;
 #pragma unroll
@@ -365,7 +375,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                                 lo[k] = pp_pack(y0 - h2.x, y1 - h2.y);
                             }
                             const uint32_t at = (uint32_t)(tile * C::QB) + pp_off(rr, 8 * x + la, 128);
-                            *reinterpret_cast<uint4*>(ks + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4*>(vs + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                             *reinterpret_cast<uint4*>(qs + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                         }
                     }
@@ -373,35 +383,38 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
         }
     }
-    if constexpr (C::QT) {
-        static_assert(2 * C::QB <= ST * 2 * C::KS * C::KB, "the high parts fit the stages");
-        tc::fence_before_sync();
-        __syncthreads();
-        tc::fence_after_sync();
-        if (warp < C::MMA && (rt == 0 || two)) {
-            if (C::F32) up_inv = s_row[rt][0][r];
-            const uint32_t qh = tmem_slot + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 64u * rt + (uint32_t)(hf * (HD / 4));
+    if (warp <= C::MMA) {
+        if constexpr (C::QT) {
+            static_assert(2 * C::QB <= ST * C::KS * C::KB, "the high parts fit the stages of V");
+            start_sync();
+            if (warp < C::MMA) {
+                if (rt == 0 || two) {
+                    if (C::F32) up_inv = s_row[rt][0][r];
+                    const uint32_t qh = tmem_slot + ((uint32_t)((warp & 3) * 32) << 16) + 128u + 64u * rt + (uint32_t)(hf * (HD / 4));
 #pragma unroll
-            for (int u = 0; u < HD / 8 / TR; u += 4) {
-                uint32_t hi[16];
+                    for (int u = 0; u < HD / 8 / TR; u += 4) {
+                        uint32_t hi[16];
 #pragma unroll
-                for (int v = 0; v < 4; v++) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(ks + rt * C::QB + pp_off(r, hf * (HD / 8 / TR) + u + v, 128));
-                    hi[4 * v] = w.x;
-                    hi[4 * v + 1] = w.y;
-                    hi[4 * v + 2] = w.z;
-                    hi[4 * v + 3] = w.w;
+                        for (int v = 0; v < 4; v++) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(vs + rt * C::QB + pp_off(r, hf * (HD / 8 / TR) + u + v, 128));
+                            hi[4 * v] = w.x;
+                            hi[4 * v + 1] = w.y;
+                            hi[4 * v + 2] = w.z;
+                            hi[4 * v + 3] = w.w;
+                        }
+                        tc::tmem_st16_nowait(qh + 4 * u, hi);
+                    }
+                    tc::tmem_wait_st();
                 }
-                tc::tmem_st16_nowait(qh + 4 * u, hi);
+                tc::fence_async_smem();   // V's copies come after these reads
+                __syncwarp();
+                if (lane == 0) mbs_arrive(qread);
             }
-            tc::tmem_wait_st();
         }
+        tc::fence_async_smem();
+        start_sync();
     }
-    tc::fence_async_smem();
-    tc::fence_before_sync();
-    __syncthreads();
-    tc::fence_after_sync();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = warp <= C::MMA ? tmem_slot : 0u;
     bool ok = true;
 
     if (warp == C::MMA) {   // ---- MMA issue: the whole warp, uniform; one lane's instructions
@@ -507,6 +520,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
                 if (j >= ST) {
                     if (ok) ok = mbs_wait(vfree + 8 * st, ((j / ST) - 1) & 1, a.err);
+                } else if (C::QT && j == 0) {
+                    if (ok) ok = mbs_wait(qread, 0, a.err);
                 }
                 const uint32_t vbar = part ? tail : vfull + 8 * st;
                 if (lane == 0) mbs_expect(vbar, bytes);
@@ -577,6 +592,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     else load(at_next, j + 1, 0, 0, nxt);
                     if (j >= ST && sub == 0) {
                         if (ok) ok = mbs_wait((kv ? vfree : kfree) + 8 * st, ((j / ST) - 1) & 1, a.err);
+                    } else if (j == 0 && kv && sub == 0) {
+                        if (ok) ok = mbs_wait(qread, 0, a.err);
                     }
                     uint8_t* dst = (kv ? vs : ks) + st * C::KS * C::KB;
 #pragma unroll
