@@ -308,17 +308,17 @@ _ACT: dict = {}   # torch dtype -> dtype code of activation rows
 
 
 def _rows(fn, n_tokens, a, b):
-    """(dtype code, width) of two tensors of activation rows [n_tokens][width]
-    (F32 or F16, unit inner stride)."""
+    """(dtype code, width, row strides) of two tensors of activation rows
+    [n_tokens][width] (F32 or F16, unit inner stride)."""
     if not _ACT:
         import torch
         _ACT.update({torch.float32: DT_F32, torch.float16: DT_F16})
     t = a.dtype
-    sa, sb = a.shape, b.shape
+    sa, sb, la, lb = a.shape, b.shape, a.stride(), b.stride()
     if (t not in _ACT or b.dtype is not t or len(sa) != 2 or len(sb) != 2 or sa[1] != sb[1] or sa[0] < n_tokens
-            or sb[0] < n_tokens or a.stride(1) != 1 or b.stride(1) != 1):
+            or sb[0] < n_tokens or la[1] != 1 or lb[1] != 1):
         raise GBError(fn, GB_EINVAL)
-    return _ACT[t], sa[1]
+    return _ACT[t], sa[1], la[0], lb[0]
 
 
 def kv_page_bytes(dtype, n_kv_heads, head_dim, page_size) -> int:
@@ -329,7 +329,7 @@ def kv_append(cache, batch, k, v, q=None, q_out=None, rope_cs=None, stream=None)
     """Write the batch's k / v rows into the cache, rotated and quantised; with
     q, also its rotated rows into q_out."""
     n, hd = batch.n_tokens, cache.head_dim
-    dt, width = _rows("gb_kv_append", n, k, v)
+    dt, width, ldk, ldv = _rows("gb_kv_append", n, k, v)
     if width != cache.n_kv_heads * hd:
         raise GBError("gb_kv_append", GB_EINVAL)
     pq = pqo = None
@@ -337,24 +337,23 @@ def kv_append(cache, batch, k, v, q=None, q_out=None, rope_cs=None, stream=None)
     if q is not None:
         if q_out is None:
             raise GBError("gb_kv_append", GB_EINVAL)
-        dq, wq = _rows("gb_kv_append", n, q, q_out)
+        dq, wq, ldq, ldqo = _rows("gb_kv_append", n, q, q_out)
         if dq != dt or wq % hd:
             raise GBError("gb_kv_append", GB_EINVAL)
-        pq, pqo, ldq, ldqo, nh = q.data_ptr(), q_out.data_ptr(), q.stride(0), q_out.stride(0), wq // hd
+        pq, pqo, nh = q.data_ptr(), q_out.data_ptr(), wq // hd
     pcs, rope_len = (None, 0) if rope_cs is None else (rope_cs.data_ptr(), rope_cs.numel() // hd)
-    rc = lib().gb_kv_append(cache.ref, batch.ref, dt, pq, ldq, nh, pqo, ldqo, k.data_ptr(), k.stride(0), v.data_ptr(),
-                            v.stride(0), pcs, rope_len, _stream(stream))
+    rc = lib().gb_kv_append(cache.ref, batch.ref, dt, pq, ldq, nh, pqo, ldqo, k.data_ptr(), ldk, v.data_ptr(), ldv,
+                            pcs, rope_len, _stream(stream))
     if rc:
         raise GBError("gb_kv_append", rc)
 
 
 def kv_read(cache, batch, k, v, stream=None) -> None:
     """The cache's values at the batch's tokens, into k and v rows."""
-    dt, width = _rows("gb_kv_read", batch.n_tokens, k, v)
+    dt, width, ldk, ldv = _rows("gb_kv_read", batch.n_tokens, k, v)
     if width != cache.n_kv_heads * cache.head_dim:
         raise GBError("gb_kv_read", GB_EINVAL)
-    rc = lib().gb_kv_read(cache.ref, batch.ref, dt, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-                          _stream(stream))
+    rc = lib().gb_kv_read(cache.ref, batch.ref, dt, k.data_ptr(), ldk, v.data_ptr(), ldv, _stream(stream))
     if rc:
         raise GBError("gb_kv_read", rc)
 
@@ -365,7 +364,7 @@ def paged_workspace_bytes(n_heads, n_kv_heads, head_dim, n_seq) -> int:
 
 def _paged_attention(name, fn, cache, batch, q, out, ws, stream):
     hd = cache.head_dim
-    dt, width = _rows(name, batch.n_tokens, q, out)
+    dt, width, ldq, ldo = _rows(name, batch.n_tokens, q, out)
     nh = width // hd
     key = (nh, cache.n_kv_heads, hd)
     need = batch._ws_need.get(key)
@@ -375,8 +374,7 @@ def _paged_attention(name, fn, cache, batch, q, out, ws, stream):
         raise GBError(name, GB_EINVAL)
     if ws.nbytes < need:
         raise GBError(name, GB_ESIZE)
-    rc = fn(cache.ref, batch.ref, dt, q.data_ptr(), q.stride(0), nh, out.data_ptr(), out.stride(0), ws.data_ptr(),
-            _stream(stream))
+    rc = fn(cache.ref, batch.ref, dt, q.data_ptr(), ldq, nh, out.data_ptr(), ldo, ws.data_ptr(), _stream(stream))
     if rc:
         raise GBError(name, rc)
 
