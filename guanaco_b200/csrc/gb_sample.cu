@@ -112,17 +112,50 @@ __device__ __forceinline__ u64 smp_scan(u64 a, u64* sums) {
 __global__ void __cluster_dims__(SMP_CL, 1, 1) __launch_bounds__(SMP_THREADS, 2)
 k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const float* __restrict__ temperature,
          const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p,
-         const float* __restrict__ uu, int* __restrict__ out) {
+         const float* __restrict__ uu, int* __restrict__ out, bool longest_first) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     SmpShared& sh = *reinterpret_cast<SmpShared*>(smem_raw);
     float* x = reinterpret_cast<float*>(smem_raw + (sizeof(SmpShared) + 15) / 16 * 16);   // [slice]
     cg::cluster_group cl = cg::this_cluster();
-    const int rank = cl.block_rank(), row = blockIdx.x / SMP_CL;
+    const int rank = cl.block_rank();
+    int row = blockIdx.x / SMP_CL;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int i0 = min(rank * slice, vocab), n = min(slice, vocab - i0);   // this CTA's indices i0 .. i0 + n - 1
-    const float* src = logits + (size_t)row * ldl + i0;
     griddep_wait();
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");   // every CTA of the cluster runs before remote stores
+    if (longest_first) {   // this cluster's row (of at most SMP_THREADS) in the order of their kinds
+        const int r = tid;
+        const bool in = r < (int)(gridDim.x / SMP_CL);
+        int kind = 0;   // a search by weight, the draw alone, a top-k that one CTA ends, greedy
+        if (in) {
+            const float rt = temperature ? __ldg(temperature + r) : 1.f;
+            const int rk = top_k ? __ldg(top_k + r) : 0;
+            const bool cut_k = rk > 0 && rk < vocab, cut_p = top_p && __ldg(top_p + r) < 1.f;
+            kind = !(rt > 0.f) ? 3 : cut_k && rk <= SMP_CAND ? 2 : !cut_k && !cut_p ? 1 : 0;
+        }
+        u64 counts = 0, before = 0, all = 0;   // 16 bits a kind
+        int at = 0;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t m = __ballot_sync(0xffffffffu, in && kind == q);
+            counts |= (u64)__popc(m) << (16 * q);
+            if (kind == q) at = __popc(m & ((1u << lane) - 1u));
+        }
+        if (lane == 0) sh.warp64[warp] = counts;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < SMP_W; w++) {
+            before += w < warp ? sh.warp64[w] : 0ull;
+            all += sh.warp64[w];
+        }
+        at += (int)(before >> (16 * kind) & 0xffffu);
+#pragma unroll
+        for (int q = 0; q < 3; q++) at += q < kind ? (int)(all >> (16 * q) & 0xffffu) : 0;
+        if (in && at == row) sh.cut_bin = (uint32_t)r;
+        __syncthreads();
+        row = (int)sh.cut_bin;
+    }
+    const float* src = logits + (size_t)row * ldl + i0;
     const float t = temperature ? __ldg(temperature + row) : 1.f;
     const int k = top_k ? __ldg(top_k + row) : 0;
     const float p = top_p ? __ldg(top_p + row) : 1.f;
@@ -661,9 +694,16 @@ extern "C" int gb_sample(const float* logits, int ldl, int rows, int vocab, cons
     constexpr size_t most = (sizeof(gb::SmpShared) + 15) / 16 * 16 + (size_t)GB_SAMPLE_MAX_VOCAB / gb::SMP_CL * sizeof(float);
     static_assert(most <= 227 * 1024, "shared memory");
     if (gb::set_smem_once(reinterpret_cast<const void*>(gb::k_sample), (int)most) != cudaSuccess) return GB_ECUDA;
+    // More rows than two CTAs an SM take at once: those that need a search first.
+    // 128,256 tokens, five kinds of settings by turns / all rows alike: 61 rows 43 -> 33 /
+    // 60 -> 62 us, 100 rows 68 -> 59 / 99 -> 102 us, 256 rows 144 -> 140 / 223 -> 233 us:
+    // up to four times as many.
+    const int at_once = 2 * gb::sm_count() / gb::SMP_CL;
+    const bool longest_first = (temperature || top_k || top_p) && rows > at_once && rows <= 4 * at_once &&
+                               rows <= gb::SMP_THREADS;
     return gb::launch_pdl(gb::k_sample, dim3(rows * gb::SMP_CL), gb::SMP_THREADS, (int)smem,
                           static_cast<cudaStream_t>(stream), logits, ldl, vocab, slice, temperature, top_k, top_p, min_p,
-                          u, out) == cudaSuccess
+                          u, out, longest_first) == cudaSuccess
                ? GB_OK
                : GB_ECUDA;
 }

@@ -137,3 +137,16 @@ def test_infinite_temperature(gb, cuda, vocab):
         order = sorted(left, key=lambda i: (-logits[r, i].item(), i))
         kept = sorted(order[: -(-len(left) // 2)])
         assert tok == kept[int(len(kept) * torch.tensor(u[r]).mul(2**24).floor().item() / 2**24)]
+
+
+@pytest.mark.parametrize("n", [38, 61, 148, 149])
+def test_batches_of_different_rows(gb, cuda, n):
+    """More rows than run at once are taken in another order; each row's token
+    is the one that it gives alone."""
+    logits = rows(n, 5003, n)
+    u = [(i * 0.37 + 0.05) % 1.0 for i in range(n)]
+    t, k = [0.0 if i % 5 == 0 else 0.9 for i in range(n)], [40 if i % 5 in (2, 4) else 700 if i % 7 == 3 else 0 for i in range(n)]
+    p, m = [0.9 if i % 5 >= 3 else 1.0 for i in range(n)], [0.05 if i % 5 == 4 else 0.0 for i in range(n)]
+    got = draw(gb, logits, u, t, k, p, m)
+    assert got == expect(logits, u, t, k, p, m)
+    assert got == [draw(gb, logits[i:i + 1], u[i:i + 1], t[i:i + 1], k[i:i + 1], p[i:i + 1], m[i:i + 1])[0] for i in range(n)]
