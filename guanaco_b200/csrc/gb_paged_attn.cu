@@ -49,6 +49,11 @@ namespace gb {
 // + PD_LIFT) keeps the fp16 parts of small probabilities normal.  Q8_0: p
 // times a scale is brought below 2^14 by a power of two, 2^-E, shared by the
 // warp; l and O are in units of 2^E.
+//
+// 96 sequences of up to 8066 keys, 32 / 8 heads of 128, fp16: F16 cache 273 us, 6150
+// GB/s, bound by HBM; Q8_0 179 us, 4980 GB/s, bound by instructions (59 % issued
+// at the 12 warps an SM that O's and q's registers leave; most turn codes into
+// fragments).  One sequence of 8193, fp32, F16 cache: 13.5 us, latency.
 constexpr int PD_W = 4;              // warps
 constexpr int PD_MAX_CTAS = 4;       // CTAs per SM the workspace has room for
 constexpr int PD_MC = 16;            // partials of a join in flight, and of a group
