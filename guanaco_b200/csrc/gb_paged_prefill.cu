@@ -45,10 +45,10 @@
 // Few rows over a long axis: the host cuts the keys over gridDim.y CTAs, which
 // leave (m, l, O) partials; the last to arrive joins them in order.
 //
-// 32 / 8 heads of 128: one prompt of 8192, fp16, F16 cache 480 us, 1140 TFLOP/s, where
+// 32 / 8 heads of 128: one prompt of 8192, fp16, F16 cache 475 us, 1157 TFLOP/s, where
 // the exponentials and the tensor cores take turns; five prompts of up to 968, fp32,
-// Q8_0 154 us, 223 TFLOP/s of three products: the tensor cores, 2300 cycles for
-// 128 rows and 64 keys, and 35,000 cycles a CTA before and after them.
+// Q8_0 149 us, 232 TFLOP/s of three products: the tensor cores, 2300 cycles for
+// 128 rows and 64 keys, and 30,000 cycles a CTA before and after them.
 #include "gb_mt.cuh"
 #include "gb_paged.cuh"
 #include "gb_tc.cuh"
@@ -324,17 +324,21 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     float up_inv = 1.f;   // 2^-e of this thread's row
     if (warp < C::MMA) {
         constexpr int NV = HD / 64, LD = C::F32 ? 2 : 1;           // a lane's runs of 8 columns, loads of each
-        constexpr int U = NV * LD == 4 ? 2 : 4;                    // rows in flight
-        constexpr int STEP = C::SOFT / 8;                          // rows of the block
-        const int rows = two ? 256 : 128, la = lane & 7;
-        for (int i0 = tid >> 3; i0 - (lane >> 3) < rows; i0 += U * STEP) {
+        constexpr int STEP = C::SOFT / 8, U = 128 / STEP;          // rows of the block at a time, of a thread in flight
+        const int la = lane & 7;
+        int qo[U], ho[U];                                          // their queries (past the tile's: none) and columns
+#pragma unroll
+        for (int v = 0; v < U; v++) {
+            const int rr = (tid >> 3) + v * STEP;
+            qo[v] = rr < a.bq * a.group ? rr / a.group : 1 << 30;
+            ho[v] = (kvh * a.group + rr % a.group) * HD + 8 * la;
+        }
+        for (int tile = 0; tile < (two ? 2 : 1); tile++) {
             uint4 w[U][NV][LD];
 #pragma unroll
             for (int v = 0; v < U; v++) {
-                const int i = i0 + v * STEP, rr = i & 127, qq = q0 + (i >> 7) * a.bq + rr / a.group;
-                const bool in = i < rows && rr < a.bq * a.group && qq < n_q;
-                const A* src = static_cast<const A*>(a.q) + (size_t)(t_begin + qq) * a.ldq +
-                               (size_t)(kvh * a.group + rr % a.group) * HD + 8 * la;
+                const bool in = qo[v] < n_q - q0 - tile * a.bq;
+                const A* src = static_cast<const A*>(a.q) + (size_t)(t_begin + q0 + tile * a.bq + qo[v]) * a.ldq + ho[v];
 #pragma unroll
                 for (int x = 0; x < NV; x++)
 #pragma unroll
@@ -343,9 +347,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
 #pragma unroll
             for (int v = 0; v < U; v++) {
-                const int i = i0 + v * STEP, rr = i & 127, tile = i >> 7;
+                const int rr = (tid >> 3) + v * STEP;
                 if constexpr (!C::F32) {
-                    if (i < rows)
 #pragma unroll
                         for (int x = 0; x < NV; x++)
                             *reinterpret_cast<uint4*>((C::QT ? vs : qs) + tile * C::QB + pp_off(rr, 8 * x + la, 128)) = w[v][x][0];
@@ -367,22 +370,20 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     for (int o = 4; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                     const int e = tc::f16_scale_exp(__float_as_uint(mx));
                     const float up = tc::pow2f(e);
-                    if (i < rows) {
-                        if (la == 0) s_row[tile][0][rr] = tc::pow2f(-e);
+                    if (la == 0) s_row[tile][0][rr] = tc::pow2f(-e);
 #pragma unroll
-                        for (int x = 0; x < NV; x++) {
-                            uint32_t hi[4], lo[4];
+                    for (int x = 0; x < NV; x++) {
+                        uint32_t hi[4], lo[4];
 #pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                const float y0 = f[x][2 * k] * up, y1 = f[x][2 * k + 1] * up;
-                                hi[k] = pp_pack(y0, y1);
-                                const float2 h2 = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-                                lo[k] = pp_pack(y0 - h2.x, y1 - h2.y);
-                            }
-                            const uint32_t at = (uint32_t)(tile * C::QB) + pp_off(rr, 8 * x + la, 128);
-                            *reinterpret_cast<uint4*>(vs + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                            *reinterpret_cast<uint4*>(qs + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        for (int k = 0; k < 4; k++) {
+                            const float y0 = f[x][2 * k] * up, y1 = f[x][2 * k + 1] * up;
+                            hi[k] = pp_pack(y0, y1);
+                            const float2 h2 = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+                            lo[k] = pp_pack(y0 - h2.x, y1 - h2.y);
                         }
+                        const uint32_t at = (uint32_t)(tile * C::QB) + pp_off(rr, 8 * x + la, 128);
+                        *reinterpret_cast<uint4*>(vs + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(qs + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
             }
@@ -790,6 +791,17 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             __syncwarp();
             if (lane == 0) mbs_arrive(pfull + 8 * (2 * rt + (TR == 2 ? hf : buf)));
         }
+        // through which the output goes: 32 rows of RB bytes, CP columns, a warp
+        constexpr int WB = C::QB / (4 * TR), RB = WB / 32 < 128 ? WB / 32 : 128, UN = RB / 16;
+        constexpr int CP = RB / (int)sizeof(A);
+        const bool more = n_tiles > C::FLUSH;
+        float4 held[C::F32 ? CP / 4 : 1];                // the running sum's, read ahead
+        auto read_ahead = [&](int c1) {
+            if (C::F32 && more && n_split == 1)
+#pragma unroll
+                for (int i = 0; i < CP / 4; i++) held[i] = __ldcg(reinterpret_cast<const float4*>(run + (c1 + 4 * i) * 128));
+        };
+        read_ahead(0);
         if (n_tiles > 0) {
             if (ok) ok = mbs_wait(ofull + 8 * rt, 0, a.err);
             tc::fence_after_sync();
@@ -799,12 +811,9 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             pp_sync(1 + rt);
             l += s_row[rt][hf ^ 1][r];
         }
-        const bool more = n_tiles > C::FLUSH;
         if (n_split == 1) {
             // Through the row tile's part of Q, which no MMA reads any more, so
-            // that a warp writes whole runs of rows: 32 rows of RB bytes at a time.
-            constexpr int WB = C::QB / (4 * TR), RB = WB / 32 < 128 ? WB / 32 : 128, UN = RB / 16;
-            constexpr int CP = RB / (int)sizeof(A);      // columns at a time
+            // that a warp writes whole runs of rows.
             static_assert(CP % 16 == 0 && HD / TR % CP == 0 && (UN == 8 || UN == 4), "rows of the staging area");
             uint8_t* wb = qs + rt * C::QB + warp % (4 * TR) * WB;
             auto at = [&](int row, int u) { return wb + row * RB + ((u ^ (UN == 8 ? row & 7 : (row >> 1) & 3)) << 4); };
@@ -813,10 +822,6 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD + hf * (HD / TR)) : 0ull;
 #pragma unroll 1
             for (int c1 = 0; c1 < HD / TR; c1 += CP) {
-                float4 sum[C::F32 ? CP / 4 : 1];             // all of a run's loads in flight
-                if (C::F32 && more)
-#pragma unroll
-                    for (int i = 0; i < CP / 4; i++) sum[i] = __ldcg(reinterpret_cast<const float4*>(run + (c1 + 4 * i) * 128));
 #pragma unroll
                 for (int c0 = 0; c0 < CP; c0 += 16) {
                     float o[16];
@@ -824,7 +829,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     if (C::F32 && more)
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) {
-                            const float4 w = sum[C::F32 ? (c0 + i) / 4 : 0];
+                            const float4 w = held[C::F32 ? (c0 + i) / 4 : 0];
                             o[i] += w.x;
                             o[i + 1] += w.y;
                             o[i + 2] += w.z;
@@ -841,6 +846,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         *reinterpret_cast<uint4*>(at(lane, c0 / n + i)) = w;
                     }
                 }
+                if (c1 + CP < HD / TR) read_ahead(c1 + CP);
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < UN; i++) {
