@@ -341,7 +341,11 @@ def kv_append(cache, batch, k, v, q=None, q_out=None, rope_cs=None, stream=None)
         if dq != dt or wq % hd:
             raise GBError("gb_kv_append", GB_EINVAL)
         pq, pqo, nh = q.data_ptr(), q_out.data_ptr(), wq // hd
-    pcs, rope_len = (None, 0) if rope_cs is None else (rope_cs.data_ptr(), rope_cs.numel() // hd)
+    pcs, rope_len = None, 0
+    if rope_cs is not None:   # rows of hd floats, one after another
+        if _ACT.get(rope_cs.dtype) != DT_F32 or rope_cs.numel() % hd or not rope_cs.is_contiguous():
+            raise GBError("gb_kv_append", GB_EINVAL)
+        pcs, rope_len = rope_cs.data_ptr(), rope_cs.numel() // hd
     rc = lib().gb_kv_append(cache.ref, batch.ref, dt, pq, ldq, nh, pqo, ldqo, k.data_ptr(), ldk, v.data_ptr(), ldv,
                             pcs, rope_len, _stream(stream))
     if rc:

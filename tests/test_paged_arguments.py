@@ -1,0 +1,60 @@
+"""CPU: what the Python layer of the batched-serving entry points refuses
+before the library is called, and what it takes."""
+import pytest
+import torch
+
+i32 = torch.int32
+
+
+def zeros(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+class Calls:
+    """Stands in for the library: records each call's arguments, returns 0."""
+
+    def __init__(self, gb):
+        self._gb, self._lib, self.made = gb, gb.lib(), []
+
+    def __getattr__(self, name):
+        if name in ("gb_kv_page_bytes", "gb_paged_workspace_bytes"):
+            return getattr(self._lib, name)
+
+        def call(*a):
+            self.made.append((name, a))
+            return 0
+        return call
+
+
+@pytest.fixture
+def calls(gb, monkeypatch):
+    c = Calls(gb)
+    monkeypatch.setattr(gb, "lib", lambda: c)
+    return c
+
+
+def cache(gb, hd=64, kv=2, pages=4, page=16):
+    n = pages * gb.kv_page_bytes(gb.DT_Q8_0, kv, hd, page)
+    return gb.KVCache(gb.DT_Q8_0, kv, hd, page, pages, zeros(n, dtype=torch.uint8), zeros(n, dtype=torch.uint8))
+
+
+def batch(gb, n=3, width=8):
+    return gb.KVBatch(n, n, zeros(n, dtype=i32), zeros(n, width, dtype=i32))
+
+
+def test_rotation_tables_that_are_not_rows_of_floats(gb, calls):
+    """The kernel reads fp32 rows of head_dim, one after another, rope_len of them."""
+    c, b = cache(gb), batch(gb)
+
+    def append(cs):
+        gb.kv_append(c, b, zeros(3, 128), zeros(3, 128), rope_cs=cs, stream=0)
+
+    append(zeros(10 * 64))
+    append(zeros(10, 32, 2))
+    assert [a[13] for _, a in calls.made] == [10, 10]
+    for cs in (zeros(10 * 64, dtype=torch.float16), zeros(10, 64, dtype=torch.bfloat16),
+               zeros(10, 64, dtype=torch.float64), zeros(10, 128)[:, :64], zeros(64, 10).T, zeros(10 * 64 + 1)):
+        with pytest.raises(gb.GBError) as e:
+            append(cs)
+        assert e.value.rc == gb.GB_EINVAL
+    assert len(calls.made) == 2
