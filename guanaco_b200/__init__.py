@@ -300,6 +300,9 @@ class KVBatch(C.Structure):
             raise GBError("KVBatch", GB_EINVAL)
         super().__init__(n_seq, n_tokens, _ptr(cu_seqlens), _ptr(kv_len), _ptr(page_table), page_table.stride(0))
         self._keep = (kv_len, page_table, cu_seqlens)
+        self._max_seq = min(kv_len.numel(), page_table.shape[0])   # n_seq may be set anew, up to what the tensors hold
+        if cu_seqlens is not None:
+            self._max_seq = min(self._max_seq, cu_seqlens.numel() - 1)
         self._ws_need = {}
         self.ref = C.addressof(self)
 
@@ -307,9 +310,13 @@ class KVBatch(C.Structure):
 _ACT: dict = {}   # torch dtype -> dtype code of activation rows
 
 
-def _rows(fn, n_tokens, a, b):
+def _rows(fn, batch, a, b):
     """(dtype code, width, row strides) of two tensors of activation rows
-    [n_tokens][width] (F32 or F16, unit inner stride)."""
+    [n_tokens][width] (F32 or F16, unit inner stride) for a batch that its
+    arrays hold."""
+    n_tokens = batch.n_tokens
+    if batch.n_seq > batch._max_seq:
+        raise GBError(fn, GB_ESIZE)
     if not _ACT:
         import torch
         _ACT.update({torch.float32: DT_F32, torch.float16: DT_F16})
@@ -328,8 +335,8 @@ def kv_page_bytes(dtype, n_kv_heads, head_dim, page_size) -> int:
 def kv_append(cache, batch, k, v, q=None, q_out=None, rope_cs=None, stream=None) -> None:
     """Write the batch's k / v rows into the cache, rotated and quantised; with
     q, also its rotated rows into q_out."""
-    n, hd = batch.n_tokens, cache.head_dim
-    dt, width, ldk, ldv = _rows("gb_kv_append", n, k, v)
+    hd = cache.head_dim
+    dt, width, ldk, ldv = _rows("gb_kv_append", batch, k, v)
     if width != cache.n_kv_heads * hd:
         raise GBError("gb_kv_append", GB_EINVAL)
     pq = pqo = None
@@ -337,7 +344,7 @@ def kv_append(cache, batch, k, v, q=None, q_out=None, rope_cs=None, stream=None)
     if q is not None:
         if q_out is None:
             raise GBError("gb_kv_append", GB_EINVAL)
-        dq, wq, ldq, ldqo = _rows("gb_kv_append", n, q, q_out)
+        dq, wq, ldq, ldqo = _rows("gb_kv_append", batch, q, q_out)
         if dq != dt or wq % hd:
             raise GBError("gb_kv_append", GB_EINVAL)
         pq, pqo, nh = q.data_ptr(), q_out.data_ptr(), wq // hd
@@ -354,7 +361,7 @@ def kv_append(cache, batch, k, v, q=None, q_out=None, rope_cs=None, stream=None)
 
 def kv_read(cache, batch, k, v, stream=None) -> None:
     """The cache's values at the batch's tokens, into k and v rows."""
-    dt, width, ldk, ldv = _rows("gb_kv_read", batch.n_tokens, k, v)
+    dt, width, ldk, ldv = _rows("gb_kv_read", batch, k, v)
     if width != cache.n_kv_heads * cache.head_dim:
         raise GBError("gb_kv_read", GB_EINVAL)
     rc = lib().gb_kv_read(cache.ref, batch.ref, dt, k.data_ptr(), ldk, v.data_ptr(), ldv, _stream(stream))
@@ -368,9 +375,9 @@ def paged_workspace_bytes(n_heads, n_kv_heads, head_dim, n_seq) -> int:
 
 def _paged_attention(name, fn, cache, batch, q, out, ws, stream):
     hd = cache.head_dim
-    dt, width, ldq, ldo = _rows(name, batch.n_tokens, q, out)
+    dt, width, ldq, ldo = _rows(name, batch, q, out)
     nh = width // hd
-    key = (nh, cache.n_kv_heads, hd)
+    key = (nh, cache.n_kv_heads, hd, batch.n_seq)
     need = batch._ws_need.get(key)
     if need is None:   # (0 for a head layout that the call itself refuses)
         need = batch._ws_need[key] = paged_workspace_bytes(nh, cache.n_kv_heads, hd, batch.n_seq)

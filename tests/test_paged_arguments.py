@@ -58,3 +58,33 @@ def test_rotation_tables_that_are_not_rows_of_floats(gb, calls):
             append(cs)
         assert e.value.rc == gb.GB_EINVAL
     assert len(calls.made) == 2
+
+
+def test_a_batch_whose_size_is_set_anew(gb, calls):
+    """n_seq and n_tokens are fields of the structure: the workspace that a call
+    asks for follows them, and no more sequences are taken than the arrays hold."""
+    c = cache(gb)
+    b = gb.KVBatch(2, 2, zeros(4096, dtype=i32), zeros(4096, 8, dtype=i32))
+    small = zeros(gb.paged_workspace_bytes(4, 2, 64, 2), dtype=torch.uint8)
+    large = zeros(gb.paged_workspace_bytes(4, 2, 64, 4096), dtype=torch.uint8)
+    assert large.numel() > small.numel()
+    x = zeros(5000, 256)
+    gb.paged_attention_decode(c, b, x, x, small, stream=0)
+    b.n_seq = b.n_tokens = 4096
+    for attend in (gb.paged_attention_decode, gb.paged_attention_prefill):
+        with pytest.raises(gb.GBError) as e:
+            attend(c, b, x, x, small, stream=0)
+        assert e.value.rc == gb.GB_ESIZE
+        attend(c, b, x, x, large, stream=0)
+    n = len(calls.made)
+    b.n_seq = b.n_tokens = 4097
+    kv = zeros(5000, 128)
+    for f in (lambda: gb.paged_attention_decode(c, b, x, x, large, stream=0),
+              lambda: gb.kv_append(c, b, kv, kv, stream=0), lambda: gb.kv_read(c, b, kv, kv, stream=0)):
+        with pytest.raises(gb.GBError):
+            f()
+    packed = gb.KVBatch(2, 5, zeros(9, dtype=i32), zeros(9, 8, dtype=i32), zeros(4, dtype=i32))
+    packed.n_seq = 4   # cu_seqlens holds three
+    with pytest.raises(gb.GBError):
+        gb.kv_append(c, packed, kv, kv, stream=0)
+    assert len(calls.made) == n
