@@ -286,9 +286,10 @@ class KVCache(C.Structure):
 
 class KVBatch(C.Structure):
     """gb_kv_batch: int32 device tensors cu_seqlens [n_seq + 1] (None: one
-    token per sequence), kv_len [n_seq] and page_table [n_seq][stride]."""
+    token per sequence), kv_len [n_seq] and page_table [n_seq][pages] (rows may
+    be further apart than they are long)."""
     _fields_ = [("n_seq", C.c_int), ("n_tokens", C.c_int), ("cu_seqlens", C.c_void_p), ("kv_len", C.c_void_p),
-                ("page_table", C.c_void_p), ("table_stride", C.c_int)]
+                ("page_table", C.c_void_p), ("table_stride", C.c_int), ("table_width", C.c_int)]
 
     def __init__(self, n_seq, n_tokens, kv_len, page_table, cu_seqlens=None):
         import torch
@@ -296,9 +297,10 @@ class KVBatch(C.Structure):
             if t is not None and (t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous()):
                 raise GBError("KVBatch", GB_EINVAL)
         if (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] < n_seq
-                or page_table.stride(1) != 1):
+                or page_table.shape[1] == 0 or page_table.stride(1) != 1):
             raise GBError("KVBatch", GB_EINVAL)
-        super().__init__(n_seq, n_tokens, _ptr(cu_seqlens), _ptr(kv_len), _ptr(page_table), page_table.stride(0))
+        super().__init__(n_seq, n_tokens, _ptr(cu_seqlens), _ptr(kv_len), _ptr(page_table), page_table.stride(0),
+                         page_table.shape[1])
         self._keep = (kv_len, page_table, cu_seqlens)
         self._max_seq = min(kv_len.numel(), page_table.shape[0])   # n_seq may be set anew, up to what the tensors hold
         if cu_seqlens is not None:

@@ -38,8 +38,10 @@ int paged_views(const gb_kv_cache* c, const gb_kv_batch* b, PagedView* pv, Batch
     if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) return GB_ESHAPE;
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) return GB_EINVAL;
     if (b->n_seq < 0 || b->n_tokens < 0 || b->table_stride <= 0) return GB_EINVAL;
+    if (b->table_width < 0 || b->table_width > b->table_stride) return GB_EINVAL;
     if (!b->cu_seqlens && b->n_tokens != b->n_seq) return GB_EINVAL;
-    if ((long long)b->table_stride * c->page_size > 0x7fffffffLL) return GB_ELIMIT;
+    const int width = b->table_width ? b->table_width : b->table_stride;
+    if ((long long)width * c->page_size > 0x7fffffffLL) return GB_ELIMIT;
     pv->k = static_cast<uint8_t*>(c->k);
     pv->v = static_cast<uint8_t*>(c->v);
     pv->n_kv = c->n_kv_heads;
@@ -53,7 +55,7 @@ int paged_views(const gb_kv_cache* c, const gb_kv_batch* b, PagedView* pv, Batch
     bv->n_seq = b->n_seq;
     bv->n_tokens = b->n_tokens;
     bv->stride = b->table_stride;
-    bv->cap = b->table_stride * c->page_size;
+    bv->cap = width * c->page_size;
     return GB_OK;
 }
 

@@ -23,7 +23,7 @@ struct PagedView {
 struct BatchView {
     const int *cu, *len, *table;
     int n_seq, n_tokens, stride;
-    int cap;            // table stride * page_size: no sequence may be longer
+    int cap;            // table width * page_size: no sequence may be longer
 };
 
 inline uint32_t paged_slab(int dtype, int hd, int page) {

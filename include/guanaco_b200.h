@@ -268,7 +268,7 @@ size_t gb_kv_page_bytes(int dtype, int n_kv_heads, int head_dim, int page_size);
  * kv_len[s] - (cu_seqlens[s + 1] - t), row position % page_size of page
  * page_table[s * table_stride + position / page_size].  cu_seqlens NULL: one
  * token per sequence (n_tokens == n_seq).  Tokens past cu_seqlens[n_seq] are
- * padding and left alone.  A length or page outside the table or the pool, or
+ * padding and left alone.  A length past table_width pages, a page outside the pool, or
  * a negative position when writing or reading, records GB_EPOS
  * (gb_paged_error); memory outside the pools is never touched.  Such a token
  * is not written and reads as zeros; a sequence with such a length counts as
@@ -278,6 +278,7 @@ typedef struct {
     int n_seq, n_tokens;
     const int *cu_seqlens, *kv_len, *page_table;
     int table_stride;
+    int table_width;   /* entries of a table row, where rows are further apart than that; 0: table_stride */
 } gb_kv_batch;
 
 /* Writes the batch's k and v rows (n_tokens rows of n_kv_heads * head_dim,

@@ -1,0 +1,50 @@
+"""GPU: lengths, pages, tables and workspaces at their limits: what is out of
+range is recorded and skipped, and calls next to it are as they were."""
+import pytest
+import torch
+
+import paged_ref as R
+from helpers import rel_l2
+
+pytestmark = pytest.mark.gpu
+
+
+def cu_of(q_lens):
+    return torch.tensor([sum(q_lens[:i]) for i in range(len(q_lens) + 1)], dtype=torch.int32, device="cuda")
+
+
+def rows_of(n, width, seed, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(n, width, generator=g, device="cuda").to(dtype)
+
+
+def workspace(gb, heads, c, n_seq):
+    return torch.zeros(gb.paged_workspace_bytes(heads, c.n_kv, c.hd, n_seq), dtype=torch.uint8, device="cuda")
+
+
+def test_a_length_past_the_part_of_a_table(gb, cuda):
+    """A view of some of a wide table's columns: a length past them is recorded,
+    although the entries beside the view are pages of the pool."""
+    c = R.Cache(gb, R.F16, 2, 64, 16, [64, 40], 5, spare=20)
+    wide = torch.zeros(2, 9, dtype=torch.int32, device="cuda")
+    wide[:, 2:6] = c.table[:, :4].clamp(min=0)
+    part = wide[:, 2:6]
+    q, out, ws = rows_of(2, 4 * 64, 1), rows_of(2, 4 * 64, 2), workspace(gb, 4, c, 2)
+    k = rows_of(2, 2 * 64, 3)
+    for lens, bad in (([64, 40], False), ([65, 40], True)):
+        n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        step = gb.KVBatch(2, 2, n, part)
+        packed = gb.KVBatch(2, 2, n, part, cu_of([1, 1]))
+        c.kv_lens = [0 if x > 64 else x for x in lens]   # counts as empty
+        ref = R.attention(q, c, [1, 1]).cpu()
+        for attend, b in ((gb.paged_attention_decode, step), (gb.paged_attention_prefill, packed)):
+            out.fill_(3)
+            attend(c.h, b, q, out, ws)
+            assert gb.paged_error(clear=True) == (gb.GB_EPOS if bad else 0)
+            assert rel_l2(out.cpu(), ref) <= 1e-5
+            assert out[0].any().item() != bad
+        before = [p.clone() for p in c.pools]
+        if bad:
+            gb.kv_append(c.h, gb.KVBatch(1, 1, n, part), k, k)
+            assert gb.paged_error(clear=True) == gb.GB_EPOS
+            assert all(torch.equal(a, b) for a, b in zip(before, c.pools))

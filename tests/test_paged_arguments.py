@@ -88,3 +88,33 @@ def test_a_batch_whose_size_is_set_anew(gb, calls):
     with pytest.raises(gb.GBError):
         gb.kv_append(c, packed, kv, kv, stream=0)
     assert len(calls.made) == n
+
+
+def test_a_table_that_is_part_of_a_wider_one(gb, calls):
+    """Sequences are bounded by the entries of a row, not by the distance of the
+    rows: the last row's entries past them may lie past the end of memory."""
+    wide = zeros(3, 16, dtype=i32)
+    b = gb.KVBatch(3, 3, zeros(3, dtype=i32), wide[:, 12:])
+    assert (b.table_stride, b.table_width) == (16, 4)
+    b = gb.KVBatch(3, 3, zeros(3, dtype=i32), wide)
+    assert (b.table_stride, b.table_width) == (16, 16)
+    with pytest.raises(gb.GBError):
+        gb.KVBatch(3, 3, zeros(3, dtype=i32), wide[:, :0])
+
+
+def test_table_widths(gb):
+    import ctypes as C
+    P, L = 1 << 20, gb.lib()
+    c = gb.KVCache.__new__(gb.KVCache)
+    for n, v in dict(dtype=2, n_kv_heads=2, head_dim=64, page_size=16, n_pages=4, k=P, v=P).items():
+        setattr(c, n, v)
+
+    def read(stride, width, n=3):
+        b = gb.KVBatch.__new__(gb.KVBatch)
+        for f, v in dict(n_seq=n, n_tokens=n, kv_len=P, page_table=P, table_stride=stride, table_width=width).items():
+            setattr(b, f, v)
+        return L.gb_kv_read(C.addressof(c), C.addressof(b), 0, P, 128, P, 128, None)
+
+    assert read(8, -1) == gb.GB_EINVAL and read(8, 9) == gb.GB_EINVAL
+    assert read(1 << 28, 1 << 28) == gb.GB_ELIMIT and read(1 << 28, 0) == gb.GB_ELIMIT
+    assert read(1 << 28, 8, n=0) == 0 and read(8, 0, n=0) == 0
