@@ -282,11 +282,12 @@ extern "C" int gb_kv_append(const gb_kv_cache* cache, const gb_kv_batch* batch, 
     int rc = paged_views(cache, batch, &c, &b);
     if (rc) return rc;
     if (dtype != GB_DT_F32 && dtype != GB_DT_F16) return GB_EINVAL;
-    const int hd = cache->head_dim, kvd = c.n_kv * hd;
+    const int hd = cache->head_dim;
+    const long long kvd = (long long)c.n_kv * hd;
     if (!paged_rows_ok(dtype, k, ldk, kvd) || !paged_rows_ok(dtype, v, ldv, kvd)) return GB_EINVAL;
     if (q) {
-        if (n_heads <= 0 || !rope_cs || !paged_rows_ok(dtype, q, ldq, n_heads * hd) ||
-            !paged_rows_ok(dtype, q_out, ldqo, n_heads * hd))
+        if (n_heads <= 0 || !rope_cs || !paged_rows_ok(dtype, q, ldq, (long long)n_heads * hd) ||
+            !paged_rows_ok(dtype, q_out, ldqo, (long long)n_heads * hd))
             return GB_EINVAL;
     } else {
         n_heads = 0;
@@ -324,7 +325,8 @@ extern "C" int gb_kv_read(const gb_kv_cache* cache, const gb_kv_batch* batch, in
     int rc = paged_views(cache, batch, &c, &b);
     if (rc) return rc;
     if (dtype != GB_DT_F32 && dtype != GB_DT_F16) return GB_EINVAL;
-    const int hd = cache->head_dim, kvd = c.n_kv * hd;
+    const int hd = cache->head_dim;
+    const long long kvd = (long long)c.n_kv * hd;
     if ((!k && !v) || (k && !paged_rows_ok(dtype, k, ldk, kvd)) || (v && !paged_rows_ok(dtype, v, ldv, kvd))) return GB_EINVAL;
     if (b.n_tokens == 0) return GB_OK;
     unsigned* err = paged_err();

@@ -34,7 +34,7 @@ inline uint32_t paged_slab(int dtype, int hd, int page) {
 int paged_views(const gb_kv_cache* c, const gb_kv_batch* b, PagedView* pv, BatchView* bv);
 // Activation rows: 16-byte aligned, at least `width` apart and apart by whole
 // 16-byte runs.
-inline bool paged_rows_ok(int dtype, const void* p, int ld, int width) {
+inline bool paged_rows_ok(int dtype, const void* p, int ld, long long width) {
     return p && !(reinterpret_cast<uintptr_t>(p) & 15) && ld >= width && ld % (dtype == GB_DT_F16 ? 8 : 4) == 0;
 }
 // Workspace of the attention entry points: partials (of the prompts' CTAs that

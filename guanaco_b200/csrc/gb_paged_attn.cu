@@ -818,8 +818,9 @@ static int paged_attention(const gb_kv_cache* cache, const gb_kv_batch* batch, i
     if (rc) return rc;
     if (dtype != GB_DT_F32 && dtype != GB_DT_F16) return GB_EINVAL;
     const int hd = cache->head_dim;
-    if (n_heads <= 0 || n_heads % c.n_kv || !ws || (reinterpret_cast<uintptr_t>(ws) & 15) || !paged_rows_ok(dtype, q, ldq, n_heads * hd) ||
-        !paged_rows_ok(dtype, out, ldo, n_heads * hd))
+    const long long width = (long long)n_heads * hd;
+    if (n_heads <= 0 || n_heads % c.n_kv || !ws || (reinterpret_cast<uintptr_t>(ws) & 15) ||
+        !paged_rows_ok(dtype, q, ldq, width) || !paged_rows_ok(dtype, out, ldo, width))
         return GB_EINVAL;
     if (b.n_tokens == 0) return GB_OK;
     const int group = n_heads / c.n_kv;

@@ -118,3 +118,26 @@ def test_table_widths(gb):
     assert read(8, -1) == gb.GB_EINVAL and read(8, 9) == gb.GB_EINVAL
     assert read(1 << 28, 1 << 28) == gb.GB_ELIMIT and read(1 << 28, 0) == gb.GB_ELIMIT
     assert read(1 << 28, 8, n=0) == 0 and read(8, 0, n=0) == 0
+
+
+def test_head_counts_whose_width_passes_32_bits(gb):
+    """2^25 heads of 128 are 2^32 columns: no row is that wide."""
+    import ctypes as C
+    P, L, E = 1 << 20, gb.lib(), gb.GB_EINVAL
+
+    def structs(kv):
+        c, b = gb.KVCache.__new__(gb.KVCache), gb.KVBatch.__new__(gb.KVBatch)
+        for n, v in dict(dtype=2, n_kv_heads=kv, head_dim=128, page_size=16, n_pages=4, k=P, v=P).items():
+            setattr(c, n, v)
+        for n, v in dict(n_seq=1, n_tokens=1, kv_len=P, page_table=P, table_stride=8).items():
+            setattr(b, n, v)
+        return (c, b), C.addressof(c), C.addressof(b)
+
+    keep, c, b = structs(2)
+    many = 1 << 25
+    assert L.gb_kv_append(c, b, 0, P, 256, many, P, 256, P, 256, P, 256, P, 9, None) == E
+    for f in (L.gb_paged_attention_decode, L.gb_paged_attention_prefill):
+        assert f(c, b, 0, P, 256, many, P, 256, P, None) == E
+    keep, c, b = structs(many)
+    assert L.gb_kv_append(c, b, 0, None, 0, 0, None, 0, P, 256, P, 256, None, 0, None) == E
+    assert L.gb_kv_read(c, b, 0, P, 256, P, 256, None) == E
