@@ -279,6 +279,8 @@ class KVCache(C.Structure):
         for t in (k_pool, v_pool):
             if need <= 0 or (not isinstance(t, int) and t.numel() * t.element_size() < need):
                 raise GBError("KVCache", GB_ESIZE)
+            if not isinstance(t, int) and not t.is_contiguous():
+                raise GBError("KVCache", GB_EINVAL)
         super().__init__(dtype, n_kv_heads, head_dim, page_size, n_pages, _ptr(k_pool), _ptr(v_pool))
         self._keep = (k_pool, v_pool)
         self.ref = C.addressof(self)
@@ -299,6 +301,8 @@ class KVBatch(C.Structure):
         if (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] < n_seq
                 or page_table.shape[1] == 0 or page_table.stride(1) != 1):
             raise GBError("KVBatch", GB_EINVAL)
+        if page_table.stride(0) > _INT_MAX:
+            raise GBError("KVBatch", GB_ELIMIT)
         super().__init__(n_seq, n_tokens, _ptr(cu_seqlens), _ptr(kv_len), _ptr(page_table), page_table.stride(0),
                          page_table.shape[1])
         self._keep = (kv_len, page_table, cu_seqlens)
@@ -310,6 +314,7 @@ class KVBatch(C.Structure):
 
 
 _ACT: dict = {}   # torch dtype -> dtype code of activation rows
+_INT_MAX = 0x7fffffff
 
 
 def _rows(fn, batch, a, b):
@@ -327,6 +332,8 @@ def _rows(fn, batch, a, b):
     if (t not in _ACT or b.dtype is not t or len(sa) != 2 or len(sb) != 2 or sa[1] != sb[1] or sa[0] < n_tokens
             or sb[0] < n_tokens or la[1] != 1 or lb[1] != 1):
         raise GBError(fn, GB_EINVAL)
+    if la[0] > _INT_MAX or lb[0] > _INT_MAX:   # the library's strides are ints
+        raise GBError(fn, GB_ELIMIT)
     return _ACT[t], sa[1], la[0], lb[0]
 
 
@@ -383,7 +390,7 @@ def _paged_attention(name, fn, cache, batch, q, out, ws, stream):
     need = batch._ws_need.get(key)
     if need is None:   # (0 for a head layout that the call itself refuses)
         need = batch._ws_need[key] = paged_workspace_bytes(nh, cache.n_kv_heads, hd, batch.n_seq)
-    if width % hd:
+    if width % hd or not ws.is_contiguous():
         raise GBError(name, GB_EINVAL)
     if ws.nbytes < need:
         raise GBError(name, GB_ESIZE)
@@ -414,6 +421,8 @@ def sample(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=None,
     shape = logits.shape
     if len(shape) != 2 or logits.dtype is not f32 or logits.stride(1) != 1:
         raise GBError("gb_sample", GB_EINVAL)
+    if logits.stride(0) > _INT_MAX:
+        raise GBError("gb_sample", GB_ELIMIT)
     n, ptr = shape[0], []
     for t, dt in ((temperature, f32), (top_k, i32), (top_p, f32), (min_p, f32), (u, f32), (out, i32)):
         if t is None and len(ptr) < 4:   # u and out are needed

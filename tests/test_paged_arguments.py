@@ -141,3 +141,32 @@ def test_head_counts_whose_width_passes_32_bits(gb):
     keep, c, b = structs(many)
     assert L.gb_kv_append(c, b, 0, None, 0, 0, None, 0, P, 256, P, 256, None, 0, None) == E
     assert L.gb_kv_read(c, b, 0, P, 256, P, 256, None) == E
+
+
+def test_strides_past_32_bits_and_gaps(gb, calls):
+    """The library's strides are 32-bit, and pools and the workspace are whole
+    runs of memory: others are refused, not cut or run over."""
+    c, b = cache(gb), batch(gb)
+    meta = dict(device="meta")
+
+    def far(rows, width, dtype=torch.float32):   # rows 2^32 + width apart
+        return torch.empty(rows, (1 << 32) + width, dtype=dtype, **meta)[:, :width]
+
+    x, kv, ws = zeros(3, 256), zeros(3, 128), zeros(1 << 25, dtype=torch.uint8)
+    for f in (lambda: gb.kv_append(c, b, far(3, 128), kv, stream=0), lambda: gb.kv_append(c, b, kv, far(3, 128), stream=0),
+              lambda: gb.kv_read(c, b, kv, far(3, 128), stream=0),
+              lambda: gb.paged_attention_decode(c, b, far(3, 256), x, ws, stream=0),
+              lambda: gb.paged_attention_prefill(c, b, x, far(3, 256), ws, stream=0),
+              lambda: gb.sample(far(3, 100), zeros(3, dtype=i32), zeros(3), stream=0),
+              lambda: gb.KVBatch(3, 3, zeros(3, dtype=i32), far(3, 8, i32))):
+        with pytest.raises(gb.GBError) as e:
+            f()
+        assert e.value.rc == gb.GB_ELIMIT
+    n = 4 * gb.kv_page_bytes(gb.DT_Q8_0, 2, 64, 16)
+    whole, gaps = zeros(n, dtype=torch.uint8), zeros(n, 2, dtype=torch.uint8)[:, 0]
+    for k, v in ((whole, gaps), (gaps, whole)):
+        with pytest.raises(gb.GBError):
+            gb.KVCache(gb.DT_Q8_0, 2, 64, 16, 4, k, v)
+    with pytest.raises(gb.GBError):
+        gb.paged_attention_decode(c, b, x, x, zeros(1 << 25, 2, dtype=torch.uint8)[:, 0], stream=0)
+    assert not calls.made
