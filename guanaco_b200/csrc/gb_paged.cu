@@ -31,7 +31,7 @@ unsigned* paged_err() {
 }
 
 int paged_views(const gb_kv_cache* c, const gb_kv_batch* b, PagedView* pv, BatchView* bv) {
-    if (!c || !b || !c->k || !c->v || !b->kv_len || !b->page_table) return GB_EINVAL;
+    if (!c || !b || !c->k || !c->v || (b->n_seq > 0 && (!b->kv_len || !b->page_table))) return GB_EINVAL;
     if (c->dtype != GB_DT_F16 && c->dtype != GB_DT_Q8_0) return GB_EINVAL;
     if (c->n_kv_heads <= 0 || c->n_pages <= 0) return GB_EINVAL;
     if (c->head_dim != 64 && c->head_dim != 128) return GB_ESHAPE;
@@ -282,6 +282,7 @@ extern "C" int gb_kv_append(const gb_kv_cache* cache, const gb_kv_batch* batch, 
     int rc = paged_views(cache, batch, &c, &b);
     if (rc) return rc;
     if (dtype != GB_DT_F32 && dtype != GB_DT_F16) return GB_EINVAL;
+    if (b.n_seq == 0 || b.n_tokens == 0) return GB_OK;   // (rows of none may be anywhere)
     const int hd = cache->head_dim;
     const long long kvd = (long long)c.n_kv * hd;
     if (!paged_rows_ok(dtype, k, ldk, kvd) || !paged_rows_ok(dtype, v, ldv, kvd)) return GB_EINVAL;
@@ -293,7 +294,6 @@ extern "C" int gb_kv_append(const gb_kv_cache* cache, const gb_kv_batch* batch, 
         n_heads = 0;
     }
     if (rope_cs && (rope_len <= 0 || (reinterpret_cast<uintptr_t>(rope_cs) & 15))) return GB_EINVAL;
-    if (b.n_tokens == 0) return GB_OK;
     unsigned* err = paged_err();
     if (!err) return GB_ECUDA;
     const int heads = n_heads + 2 * c.n_kv;
@@ -325,10 +325,10 @@ extern "C" int gb_kv_read(const gb_kv_cache* cache, const gb_kv_batch* batch, in
     int rc = paged_views(cache, batch, &c, &b);
     if (rc) return rc;
     if (dtype != GB_DT_F32 && dtype != GB_DT_F16) return GB_EINVAL;
+    if (b.n_seq == 0 || b.n_tokens == 0) return GB_OK;   // (rows of none may be anywhere)
     const int hd = cache->head_dim;
     const long long kvd = (long long)c.n_kv * hd;
     if ((!k && !v) || (k && !paged_rows_ok(dtype, k, ldk, kvd)) || (v && !paged_rows_ok(dtype, v, ldv, kvd))) return GB_EINVAL;
-    if (b.n_tokens == 0) return GB_OK;
     unsigned* err = paged_err();
     if (!err) return GB_ECUDA;
     const bool many = kv_grid(b.n_tokens, 2 * c.n_kv, hd, 2) >= (unsigned)(KV_CTAS * sm_count());

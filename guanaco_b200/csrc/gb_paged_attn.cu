@@ -817,12 +817,12 @@ static int paged_attention(const gb_kv_cache* cache, const gb_kv_batch* batch, i
     int rc = paged_views(cache, batch, &c, &b);
     if (rc) return rc;
     if (dtype != GB_DT_F32 && dtype != GB_DT_F16) return GB_EINVAL;
+    if (b.n_seq == 0 || b.n_tokens == 0) return GB_OK;   // (rows of none may be anywhere)
     const int hd = cache->head_dim;
     const long long width = (long long)n_heads * hd;
     if (n_heads <= 0 || n_heads % c.n_kv || !ws || (reinterpret_cast<uintptr_t>(ws) & 15) ||
         !paged_rows_ok(dtype, q, ldq, width) || !paged_rows_ok(dtype, out, ldo, width))
         return GB_EINVAL;
-    if (b.n_tokens == 0) return GB_OK;
     const int group = n_heads / c.n_kv;
     const long long heads8 = (long long)c.n_kv * ((group + PD_HEADS - 1) / PD_HEADS);
     if (decode ? (double)b.n_seq * (b.cap / 16 + 1) * heads8 > 0x7fffffff   // steps

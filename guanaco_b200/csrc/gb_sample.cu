@@ -685,9 +685,10 @@ k_sample(const float* __restrict__ logits, int ldl, int vocab, int slice, const 
 
 extern "C" int gb_sample(const float* logits, int ldl, int rows, int vocab, const float* temperature, const int* top_k,
                          const float* top_p, const float* min_p, const float* u, int* out, void* stream) {
-    if (!logits || !u || !out || rows < 0 || vocab <= 0 || ldl < vocab) return GB_EINVAL;
+    if (rows < 0 || vocab <= 0 || ldl < vocab) return GB_EINVAL;
     if (vocab > GB_SAMPLE_MAX_VOCAB) return GB_ELIMIT;
     if (rows == 0) return GB_OK;
+    if (!logits || !u || !out) return GB_EINVAL;
     if (rows > 0x7fffffff / gb::SMP_CL) return GB_ELIMIT;
     const int slice = ((vocab + gb::SMP_CL - 1) / gb::SMP_CL + 3) / 4 * 4;
     const size_t smem = (sizeof(gb::SmpShared) + 15) / 16 * 16 + (size_t)slice * sizeof(float);

@@ -273,7 +273,8 @@ size_t gb_kv_page_bytes(int dtype, int n_kv_heads, int head_dim, int page_size);
  * (gb_paged_error); memory outside the pools is never touched.  Such a token
  * is not written and reads as zeros; a sequence with such a length counts as
  * empty; attention over such a page gives its sequence unspecified values.
- * page_table entries past a sequence's length are not read. */
+ * page_table entries past a sequence's length are not read.  A batch without
+ * sequences or tokens does nothing, and needs no arrays or rows. */
 typedef struct {
     int n_seq, n_tokens;
     const int *cu_seqlens, *kv_len, *page_table;

@@ -170,3 +170,24 @@ def test_strides_past_32_bits_and_gaps(gb, calls):
     with pytest.raises(gb.GBError):
         gb.paged_attention_decode(c, b, x, x, zeros(1 << 25, 2, dtype=torch.uint8)[:, 0], stream=0)
     assert not calls.made
+
+
+def test_no_tokens_and_no_sequences(gb):
+    """Empty tensors have no address: they are taken, and nothing is launched.
+    A batch of padding alone (packed tokens, no sequences) too."""
+    c = cache(gb)
+    z = dict(dtype=i32)
+    ws = zeros(gb.paged_workspace_bytes(4, 2, 64, 2), dtype=torch.uint8)
+    for n in (0, 3):   # rows
+        x, kv = zeros(n, 256), zeros(n, 128)
+        batches = [gb.KVBatch(0, n, zeros(0, **z), zeros(0, 8, **z), zeros(1, **z))]
+        if n == 0:
+            batches += [gb.KVBatch(0, 0, zeros(0, **z), zeros(0, 8, **z)),
+                        gb.KVBatch(2, 0, zeros(2, **z), zeros(2, 8, **z), zeros(3, **z))]
+        for b in batches:
+            gb.kv_append(c, b, kv, kv, q=x, q_out=x, rope_cs=zeros(64), stream=0)
+            gb.kv_read(c, b, kv, kv, stream=0)
+            gb.paged_attention_prefill(c, b, x, x, ws, stream=0)
+            if not b.cu_seqlens:
+                gb.paged_attention_decode(c, b, x, x, ws, stream=0)
+    gb.sample(zeros(0, 9), zeros(0, **z), zeros(0), stream=0)
