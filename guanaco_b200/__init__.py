@@ -301,9 +301,10 @@ class KVBatch(C.Structure):
         if (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] < n_seq
                 or page_table.shape[1] == 0 or page_table.stride(1) != 1):
             raise GBError("KVBatch", GB_EINVAL)
-        if page_table.stride(0) > _INT_MAX:
+        stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
+        if stride > _INT_MAX:
             raise GBError("KVBatch", GB_ELIMIT)
-        super().__init__(n_seq, n_tokens, _ptr(cu_seqlens), _ptr(kv_len), _ptr(page_table), page_table.stride(0),
+        super().__init__(n_seq, n_tokens, _ptr(cu_seqlens), _ptr(kv_len), _ptr(page_table), stride,
                          page_table.shape[1])
         self._keep = (kv_len, page_table, cu_seqlens)
         self._max_seq = min(kv_len.numel(), page_table.shape[0])   # n_seq may be set anew, up to what the tensors hold
@@ -332,9 +333,10 @@ def _rows(fn, batch, a, b):
     if (t not in _ACT or b.dtype is not t or len(sa) != 2 or len(sb) != 2 or sa[1] != sb[1] or sa[0] < n_tokens
             or sb[0] < n_tokens or la[1] != 1 or lb[1] != 1):
         raise GBError(fn, GB_EINVAL)
-    if la[0] > _INT_MAX or lb[0] > _INT_MAX:   # the library's strides are ints
+    lda, ldb = la[0] if sa[0] > 1 else sa[1], lb[0] if sb[0] > 1 else sa[1]   # one row: the next is nowhere
+    if lda > _INT_MAX or ldb > _INT_MAX:   # the library's strides are ints
         raise GBError(fn, GB_ELIMIT)
-    return _ACT[t], sa[1], la[0], lb[0]
+    return _ACT[t], sa[1], lda, ldb
 
 
 def kv_page_bytes(dtype, n_kv_heads, head_dim, page_size) -> int:
@@ -421,9 +423,10 @@ def sample(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=None,
     shape = logits.shape
     if len(shape) != 2 or logits.dtype is not f32 or logits.stride(1) != 1:
         raise GBError("gb_sample", GB_EINVAL)
-    if logits.stride(0) > _INT_MAX:
-        raise GBError("gb_sample", GB_ELIMIT)
     n, ptr = shape[0], []
+    ldl = logits.stride(0) if n > 1 else shape[1]   # one row: the next is nowhere
+    if ldl > _INT_MAX:
+        raise GBError("gb_sample", GB_ELIMIT)
     for t, dt in ((temperature, f32), (top_k, i32), (top_p, f32), (min_p, f32), (u, f32), (out, i32)):
         if t is None and len(ptr) < 4:   # u and out are needed
             ptr.append(None)
@@ -431,7 +434,7 @@ def sample(logits, out, u, temperature=None, top_k=None, top_p=None, min_p=None,
         if t is None or t.dtype is not dt or t.numel() < n or not t.is_contiguous():
             raise GBError("gb_sample", GB_EINVAL)
         ptr.append(t.data_ptr())
-    rc = lib().gb_sample(logits.data_ptr(), logits.stride(0), n, shape[1], *ptr, _stream(stream))
+    rc = lib().gb_sample(logits.data_ptr(), ldl, n, shape[1], *ptr, _stream(stream))
     if rc:
         raise GBError("gb_sample", rc)
 

@@ -191,3 +191,23 @@ def test_no_tokens_and_no_sequences(gb):
             if not b.cu_seqlens:
                 gb.paged_attention_decode(c, b, x, x, ws, stream=0)
     gb.sample(zeros(0, 9), zeros(0, **z), zeros(0), stream=0)
+
+
+def test_one_row_of_any_stride(gb, calls):
+    """The distance to the next row of a single one means nothing."""
+    def column(width, dtype=torch.float32):
+        t = zeros(width, 1, dtype=dtype).t()
+        assert t.shape == (1, width) and t.stride() == (1, 1)
+        return t
+
+    c = cache(gb)
+    b = gb.KVBatch(1, 1, zeros(1, dtype=i32), column(8, i32))
+    assert (b.table_stride, b.table_width) == (8, 8)
+    gb.kv_append(c, b, column(128), column(128), q=column(256), q_out=column(256), rope_cs=zeros(64), stream=0)
+    gb.kv_read(c, b, column(128), column(128), stream=0)
+    ws = zeros(gb.paged_workspace_bytes(4, 2, 64, 2), dtype=torch.uint8)
+    gb.paged_attention_decode(c, b, column(256), column(256), ws, stream=0)
+    gb.sample(column(9), zeros(1, dtype=i32), zeros(1), stream=0)
+    ld = {n: [a[i] for i in at] for (n, a), at in zip(calls.made, ((4, 7, 9, 11), (4, 6), (4, 7), (1,)))}
+    assert ld == {"gb_kv_append": [256, 256, 128, 128], "gb_kv_read": [128, 128],
+                  "gb_paged_attention_decode": [256, 256], "gb_sample": [9]}
