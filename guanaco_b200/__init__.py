@@ -371,11 +371,14 @@ def kv_append(cache, batch, k, v, q=None, q_out=None, rope_cs=None, stream=None)
 
 
 def kv_read(cache, batch, k, v, stream=None) -> None:
-    """The cache's values at the batch's tokens, into k and v rows."""
-    dt, width, ldk, ldv = _rows("gb_kv_read", batch, k, v)
+    """The cache's values at the batch's tokens, into k and v rows (or one of
+    them, the other None)."""
+    if k is None and v is None:
+        raise GBError("gb_kv_read", GB_EINVAL)
+    dt, width, ldk, ldv = _rows("gb_kv_read", batch, v if k is None else k, k if v is None else v)
     if width != cache.n_kv_heads * cache.head_dim:
         raise GBError("gb_kv_read", GB_EINVAL)
-    rc = lib().gb_kv_read(cache.ref, batch.ref, dt, k.data_ptr(), ldk, v.data_ptr(), ldv, _stream(stream))
+    rc = lib().gb_kv_read(cache.ref, batch.ref, dt, _ptr(k), ldk, _ptr(v), ldv, _stream(stream))
     if rc:
         raise GBError("gb_kv_read", rc)
 

@@ -48,3 +48,31 @@ def test_a_length_past_the_part_of_a_table(gb, cuda):
             gb.kv_append(c.h, gb.KVBatch(1, 1, n, part), k, k)
             assert gb.paged_error(clear=True) == gb.GB_EPOS
             assert all(torch.equal(a, b) for a, b in zip(before, c.pools))
+
+
+@pytest.mark.parametrize("cache", [R.F16, R.Q8_0])
+def test_reading_k_or_v_alone(gb, cuda, cache):
+    c = R.Cache(gb, cache, 2, 64, 16, [30, 7], 5)
+    b = gb.KVBatch(2, 37, c.len, c.table, cu_of([30, 7]))
+    for which in (0, 1):
+        x = torch.full((37, 128), 3.0, device="cuda")
+        gb.kv_read(c.h, b, *((x, None) if which == 0 else (None, x)))
+        assert torch.equal(x, torch.cat([c.get(c.pools[which], s, n) for s, n in ((0, 30), (1, 7))]).float().flatten(1))
+    assert gb.paged_error() == 0
+
+
+def test_a_position_past_the_rotation_table(gb, cuda):
+    """Recorded; the token is not written and its q_out row is left as it was."""
+    c = R.Cache(gb, R.F16, 2, 64, 16, [20, 33], 5)
+    before = [p.clone() for p in c.pools]
+    cs = torch.empty(32 * 64, device="cuda")
+    gb.rope_table(cs, 32, 64)
+    q, k, q_out = rows_of(2, 4 * 64, 1), rows_of(2, 2 * 64, 2), torch.full((2, 4 * 64), 3.0, device="cuda")
+    gb.kv_append(c.h, gb.KVBatch(2, 2, c.len, c.table), k, k, q=q, q_out=q_out, rope_cs=cs)
+    assert gb.paged_error(clear=True) == gb.GB_EPOS
+    turn = cs.view(-1, 64)
+    assert torch.equal(q_out[:1], R.rope(q[:1].unflatten(1, (4, 64)), turn[19:20]).flatten(1))
+    assert (q_out[1] == 3).all()
+    for pool, old, x in zip(c.pools, before, (R.rope(k[:1].unflatten(1, (2, 64)), turn[19:20]), k[:1].unflatten(1, (2, 64)))):
+        c.parts(old)[0][c.table[0, 1].long(), :, 3] = x[0].half()
+        assert torch.equal(pool, old)

@@ -211,3 +211,14 @@ def test_one_row_of_any_stride(gb, calls):
     ld = {n: [a[i] for i in at] for (n, a), at in zip(calls.made, ((4, 7, 9, 11), (4, 6), (4, 7), (1,)))}
     assert ld == {"gb_kv_append": [256, 256, 128, 128], "gb_kv_read": [128, 128],
                   "gb_paged_attention_decode": [256, 256], "gb_sample": [9]}
+
+
+def test_reading_k_or_v_alone(gb, calls):
+    c, b = cache(gb), batch(gb)
+    x = zeros(3, 160)[:, :128]
+    gb.kv_read(c, b, x, None, stream=0)
+    gb.kv_read(c, b, None, x, stream=0)
+    assert [a[3:7] for _, a in calls.made] == [(x.data_ptr(), 160, None, 160), (None, 160, x.data_ptr(), 160)]
+    for k, v in ((None, None), (None, zeros(3, 64)), (zeros(2, 128), None)):
+        with pytest.raises(gb.GBError):
+            gb.kv_read(c, b, k, v, stream=0)
