@@ -109,6 +109,8 @@ class Server:
         self.waiting, self.running = [], []
 
     def submit(self, request):
+        if not request.prompt or request.n_new < 1:
+            raise ValueError("a request has a prompt and asks for tokens")
         if -(-(len(request.prompt) + request.n_new) // self.page) > len(self.free) + sum(
                 len(r.pages) for r in self.running) or len(request.prompt) + request.n_new > self.m.max_seq:
             raise ValueError("request longer than the cache")
