@@ -444,9 +444,10 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                             pd_mma(sl, k0.z, k1.z, k0.w, k1.w, ql[2 * j + 1][0], ql[2 * j + 1][1]);
                         }
                     }
+                    // an infinite score stands: the remainder of q may have the other sign than q
                     if (sizeof(A) == 4)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) sa[i] += sl[i];
+                        for (int i = 0; i < 4; i++) sa[i] = fabsf(sa[i]) == INFINITY ? sa[i] : sa[i] + sl[i];
                     x[0][0] = sa[0]; x[0][1] = sa[1]; x[1][0] = sa[2]; x[1][1] = sa[3];
                 } else {
 #pragma unroll

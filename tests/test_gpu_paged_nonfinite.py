@@ -1,0 +1,161 @@
+"""GPU: attention over the paged cache where q, K or V hold NaN, infinities or
+values past fp16's range: the rows and columns that are no number or infinite
+are those of the definition, and every other one is as exact as ever.
+
+The definition: a token's softmax and sum run over the positions that it sees
+and no others, so what stands at a later position never reaches it.  An output
+element is finite in the kernel where it is in 64 bits (rounded to the output's
+type).
+
+Tolerances (L2 of a row against its own size), derived as for finite values:
+F32 activations 22 significant bits of q and of the probabilities, 3e-5; F16
+activations the output's rounding and the probabilities' (2^-11 / sqrt 3 =
+2.8e-4 each, 4e-4 together) and a factor of 3 for a single row, 1.2e-3."""
+import pytest
+import torch
+
+import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+F32, F16 = torch.float32, torch.float16
+TOL = {F32: 3e-5, F16: 1.2e-3}
+ACT = {"f32": F32, "f16": F16}
+CACHE = {"f16": R.F16, "q8_0": R.Q8_0}
+
+
+def cu_of(q_lens):
+    return torch.tensor([sum(q_lens[:i]) for i in range(len(q_lens) + 1)], dtype=torch.int32, device="cuda")
+
+
+def definition(q, c, q_lens):
+    """fp64 [tokens][heads * hd], over the seen positions alone."""
+    out, t0, hd, kv = [], 0, c.hd, c.n_kv
+    for s, n in enumerate(q_lens):
+        m = c.kv_lens[s]
+        x = q[t0: t0 + n].double().reshape(n, kv, -1, 1, hd)
+        t0 += n
+        k, v = (c.get(p, s, m).transpose(0, 1) for p in c.pools)       # [kv][m][hd]
+        o = torch.zeros(n, kv, x.shape[2], hd, dtype=torch.float64, device="cuda")
+        for i in range(n):
+            see = m - n + i + 1
+            if see > 0:
+                sc = (x[i] * k[:, None, :see]).sum(-1) / hd ** 0.5       # [kv][group][see]
+                p = torch.softmax(sc, -1)
+                o[i] = (p[..., None] * v[:, None, :see]).sum(-2)
+        out.append(o.reshape(n, -1))
+    return torch.cat(out)
+
+
+def check(gb, c, q, q_lens, decode, what=""):
+    hd = c.hd
+    heads = q.shape[1] // hd
+    out = torch.full_like(q, 3.0)
+    ws = torch.zeros(gb.paged_workspace_bytes(heads, c.n_kv, hd, len(q_lens)), dtype=torch.uint8, device="cuda")
+    batch = gb.KVBatch(len(q_lens), sum(q_lens), c.len, c.table, None if decode else cu_of(q_lens))
+    (gb.paged_attention_decode if decode else gb.paged_attention_prefill)(c.h, batch, q, out, ws)
+    ref = definition(q, c, q_lens)
+    there = torch.isfinite(ref.to(q.dtype))
+    wrong = (torch.isfinite(out) != there).nonzero()
+    assert not len(wrong), (what, len(wrong), wrong[:4].tolist())
+    # a head's row by itself, against its own size (in 64 bits: a column may pass the output's type)
+    err = torch.where(there, out.double() - ref, 0.0).unflatten(1, (heads, hd)).norm(dim=-1)
+    size = torch.where(torch.isfinite(ref), ref, 0.0).unflatten(1, (heads, hd)).norm(dim=-1)
+    assert (err <= TOL[q.dtype] * size).all(), (what, (err / size.clamp(min=1e-300)).max().item())
+    # the workspace is ready for the next call, and fit for finite rows
+    again = torch.empty_like(out)
+    (gb.paged_attention_decode if decode else gb.paged_attention_prefill)(c.h, batch, q, again, ws)
+    assert torch.equal(torch.nan_to_num(again, nan=5.0), torch.nan_to_num(out, nan=5.0)), what
+    assert gb.paged_error() == 0
+
+
+def rows(n, width, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (1.5 * torch.randn(n, width, generator=g, device="cuda")).to(dtype)
+
+
+def put_value(c, pool, s, pos, head, col, value):
+    """A value (for Q8_0 its block's scale) in the cache."""
+    pg, r = c.table[s, pos // c.page].item(), pos % c.page
+    halves, scales = c.parts(pool)
+    if scales is not None:
+        scales[pg, head, r, col // 32] = value
+    else:
+        halves[pg, head, r, col] = value
+
+
+FORMS = [(a, c, hd) for a in ("f32", "f16") for c in ("f16", "q8_0") for hd in (64, 128)]
+
+
+# ------------------------------------------------------------------ single tokens
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("act,hd", [(a, hd) for a in ("f32", "f16") for hd in (64, 128)])
+def test_decode_in_an_f16_cache_at_every_place(gb, cuda, act, hd, value, which):
+    """K (0) or V (1) at every position modulo 16."""
+    every_place(gb, act, "f16", hd, value, which, True)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("act,hd", [(a, hd) for a in ("f32", "f16") for hd in (64, 128)])
+def test_decode_in_a_q8_0_cache_at_every_place(gb, cuda, act, hd, which):
+    """A block's scale (an append writes finite ones)."""
+    every_place(gb, act, "q8_0", hd, NAN, which, True)
+
+
+def every_place(gb, act, cache, hd, value, which, decode):
+    n = 1 if decode else 64
+    q = rows(64, 4 * hd, ACT[act], 4)[:n]
+    for pos in list(range(64, 80)) + [0, 98]:
+        c = R.Cache(gb, CACHE[cache], 2, hd, 32, [99], pos)
+        put_value(c, c.pools[which], 0, pos, pos % 2, (7 * pos) % hd, value)
+        check(gb, c, q, [n], decode, pos)
+
+
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("act,cache,hd", FORMS)
+def test_decode_in_q(gb, cuda, act, cache, hd, value):
+    """One query head's row, and no other."""
+    in_q(gb, act, cache, hd, value, True, [1, 1])
+
+
+def in_q(gb, act, cache, hd, value, decode, q_lens):
+    c = R.Cache(gb, CACHE[cache], 2, hd, 16, [100, 37], 1)
+    q = rows(sum(q_lens), 4 * hd, ACT[act], 2)
+    q[sum(q_lens) - 1, hd + 5] = value
+    q[0, 3 * hd - 1] = value
+    check(gb, c, q, q_lens, decode)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decode_q8_0_beyond_the_largest_half(gb, cuda, act, hd, which):
+    """An append's scale reaches 65504, its values 127 times that: they are finite."""
+    beyond(gb, act, hd, which, True)
+
+
+def beyond(gb, act, hd, which, decode):
+    n = 1 if decode else 64
+    for pos, size in ((5, 7e4), (60, 3e5), (70, 5e6), (98, 1e5)):
+        c = R.Cache(gb, R.Q8_0, 2, hd, 32, [99], pos)
+        x = torch.randn(99, 2, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(pos))
+        x[pos, 1, 3::5] = size
+        c.put(c.pools[which], 0, x)
+        check(gb, c, rows(n, 4 * hd, ACT[act], 4), [n], decode, pos)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("cache,value", [("f16", NAN), ("f16", INF), ("q8_0", NAN)])
+@pytest.mark.parametrize("act", ["f32", "f16"])
+def test_decode_over_a_long_axis(gb, cuda, act, cache, value, which):
+    """Keys split over CTAs and joined."""
+    long_axis(gb, act, cache, value, which, True, 1)
+
+
+def long_axis(gb, act, cache, value, which, decode, n):
+    for pos in (3, 2990):
+        c = R.Cache(gb, CACHE[cache], 1, 128, 64, [3000], 6)
+        put_value(c, c.pools[which], 0, pos, 0, 77, value)
+        check(gb, c, rows(n, 4 * 128, ACT[act], 5), [n], decode, pos)
