@@ -543,7 +543,8 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                         l[h] *= al[h];
                         m[h] = mn;
                         thr[h] = (mn + PD_TAU) * isc[h];
-                        off[h] = PD_LIFT - mn - (C::Q8 ? (float)E : 0.f);
+                        // (a head with scores of -inf alone so far, moved by another's: they weigh nothing)
+                        off[h] = PD_LIFT - (mn == -INFINITY ? 0.f : mn) - (C::Q8 ? (float)E : 0.f);
                     }
 #pragma unroll
                     for (int n = 0; n < NT / 2; n++) {

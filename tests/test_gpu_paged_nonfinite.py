@@ -89,6 +89,37 @@ FORMS = [(a, c, hd) for a in ("f32", "f16") for c in ("f16", "q8_0") for hd in (
 
 
 # ------------------------------------------------------------------ single tokens
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("kv_len,some", [(40, 20), (300, 299)])
+def test_decode_scores_of_minus_infinity(gb, cuda, act, kv_len, some):
+    """Keys whose score is -inf weigh nothing, for heads that see finite ones
+    beside them and next to heads that do not."""
+    minus_infinity(gb, act, kv_len, some, True, 1)
+
+
+def minus_infinity(gb, act, kv_len, some, decode, n):
+    hd = 64
+    c = R.Cache(gb, R.F16, 1, hd, 64, [kv_len], 7)
+    pos = torch.arange(kv_len, device="cuda")
+    pages, at = c.table[0, pos // 64].long(), pos % 64
+    halves, _ = c.parts(c.pools[0])
+    halves[pages[:some], 0, at[:some], 9] = INF
+    q = rows(n, 8 * hd, ACT[act], 8)
+    q[:, 9::hd] = -q[:, 9::hd].abs() - 0.1
+    check(gb, c, q, [n], decode, "the first keys")
+    q[:, 9 + 3 * hd] *= -1                     # +inf for head 3 alone: no number
+    check(gb, c, q, [n], decode, "head 3")
+    q[:, 9 + 3 * hd] = 0.0                     # 0 x inf: no number either
+    check(gb, c, q, [n], decode, "head 3, zero")
+    halves[pages, 0, at, 11] = INF             # -inf at every position, but for head 5
+    q[:, 11::hd] = -q[:, 11::hd].abs() - 0.1
+    q[:, 9 + 3 * hd] = -0.25
+    check(gb, c, q, [n], decode, "nothing left")
+    halves[pages, 0, at, 9] = 0.25             # head 5: +inf at every position
+    q[:, 11 + 5 * hd] *= -1
+    check(gb, c, q, [n], decode, "nothing left, head 5")
+
+
 @pytest.mark.parametrize("which", [0, 1])
 @pytest.mark.parametrize("value", [NAN, INF, -INF])
 @pytest.mark.parametrize("act,hd", [(a, hd) for a in ("f32", "f16") for hd in (64, 128)])
