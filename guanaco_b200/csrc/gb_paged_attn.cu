@@ -726,13 +726,14 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                             if (k + u >= count) ml[u] = make_float2(-INFINITY, 0.f);
                             mn = fmaxf(mn, ml[u].x);
                         }
-                        const float fa = pd_ex2(M - mn);   // 0 before the first partial
+                        const float ref = mn == -INFINITY ? 0.f : mn;   // (partials of scores of -inf alone)
+                        const float fa = pd_ex2(M - ref);   // 0 before the first partial
                         M = mn;
                         L *= fa;
                         V = make_float4(V.x * fa, V.y * fa, V.z * fa, V.w * fa);
 #pragma unroll
                         for (unsigned u = 0; u < PD_MC; u++) {
-                            const float f = pd_ex2(ml[u].x - M);
+                            const float f = pd_ex2(ml[u].x - ref);
                             L = fmaf(ml[u].y, f, L);
                             V = make_float4(fmaf(v[u].x, f, V.x), fmaf(v[u].y, f, V.y), fmaf(v[u].z, f, V.z),
                                             fmaf(v[u].w, f, V.w));

@@ -97,6 +97,12 @@ def test_decode_scores_of_minus_infinity(gb, cuda, act, kv_len, some):
     minus_infinity(gb, act, kv_len, some, True, 1)
 
 
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("kv_len,some", [(3000, 2500), (20011, 17000)])
+def test_decode_ctas_with_scores_of_minus_infinity_alone(gb, cuda, act, kv_len, some):
+    minus_infinity(gb, act, kv_len, some, True, 1)
+
+
 def minus_infinity(gb, act, kv_len, some, decode, n):
     hd = 64
     c = R.Cache(gb, R.F16, 1, hd, 64, [kv_len], 7)
