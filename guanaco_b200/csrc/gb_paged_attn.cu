@@ -690,7 +690,7 @@ k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
             for (int w = 0; w < PD_W; w++) {
                 const float f = ml[w].x == -INFINITY ? 0.f : pd_ex2(ml[w].x - M);
                 L = fmaf(ml[w].y, f, L);
-                V = fmaf(f == 0.f ? 0.f : meets[w][h * C::OP + p], f, V);
+                V = fmaf(meets[w][h * C::OP + p], f, V);   // (an infinity that weighs nothing is no number)
             }
             if (whole) {
                 out[o0 + (size_t)h * HD + pd_col<HD, DT>(p)] = (A)(V / L);

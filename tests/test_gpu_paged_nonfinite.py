@@ -150,6 +150,22 @@ def every_place(gb, act, cache, hd, value, which, decode):
         check(gb, c, q, [n], decode, pos)
 
 
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("kv_lens", [[99], [2000], [99] * 400])
+def test_decode_an_infinite_value_that_weighs_next_to_nothing(gb, cuda, act, kv_lens):
+    """A key hundreds of units below the maximum, in a warp that sees the
+    maximum or another: in 64 bits its infinite value still is one."""
+    c = R.Cache(gb, R.F16, 1, 64, 32, kv_lens, 4)
+    n, m = len(kv_lens), kv_lens[0]
+    q = rows(n, 64, ACT[act], 4)
+    for s in range(n):
+        x = torch.zeros(m, 1, 64, device="cuda")
+        x[m - 1, 0] = 400 * q[s].float() / q[s].float().norm()
+        c.put(c.pools[0], s, x)
+        put_value(c, c.pools[1], s, (37 * s) % (m - 1), 0, 40, INF)
+    check(gb, c, q, [1] * n, True)
+
+
 @pytest.mark.parametrize("value", [NAN, INF, -INF])
 @pytest.mark.parametrize("act,cache,hd", FORMS)
 def test_decode_in_q(gb, cuda, act, cache, hd, value):
