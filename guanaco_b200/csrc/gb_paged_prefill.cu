@@ -116,10 +116,17 @@ __device__ __forceinline__ float pp_ex2(float x) {
 // 2^x of a pair without the special function unit, whose 16 results a cycle
 // bound the kernel: x = j + r, j the nearest integer, 2^r by the degree-4
 // polynomial of least relative error on [-1/2, 1/2] (2.6e-6, a hundredth of
-// P's rounding), j added to the exponent.  x is kept above -126.
+// P's rounding), j added to the exponent.  x is kept above -126; one that is no
+// number (0x7fffffff through all of it) comes out as the largest float, an
+// infinity as a half, so its row's output is not finite.
+__device__ __forceinline__ float pp_max_nan(float a, float b) {   // no number if either is none
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 __device__ __forceinline__ float2 pp_ex2_poly(float2 x) {
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
+    x.x = pp_max_nan(x.x, -126.f);
+    x.y = pp_max_nan(x.y, -126.f);
     const float2 big = make_float2(12582912.f, 12582912.f);   // 1.5 2^23: adding it rounds to an integer
     const float2 t = __fadd2_rn(x, big);
     const float2 j = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
@@ -817,7 +824,9 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             static_assert(CP % 16 == 0 && HD / TR % CP == 0 && (UN == 8 || UN == 4), "rows of the staging area");
             uint8_t* wb = qs + rt * C::QB + warp % (4 * TR) * WB;
             auto at = [&](int row, int u) { return wb + row * RB + ((u ^ (UN == 8 ? row & 7 : (row >> 1) & 3)) << 4); };
-            const float inv = l > 0.f ? 1.0f / l : 0.f;   // no keys: zeros
+            // a row that sees no key: zeros; keys with scores of -inf alone: no number
+            const bool sees = lim >= 0;
+            const float inv = m == -INFINITY ? NAN : 1.0f / l;
             const unsigned long long dst = live ? reinterpret_cast<unsigned long long>(
                 static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD + hf * (HD / TR)) : 0ull;
 #pragma unroll 1
@@ -836,7 +845,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                             o[i + 3] += w.w;
                         }
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] = l > 0.f ? o[i] * inv : 0.f;
+                    for (int i = 0; i < 16; i++) o[i] = sees ? o[i] * inv : 0.f;
 #pragma unroll
                     for (int i = 0; i < (int)sizeof(A); i++) {   // 16 columns: 2 or 4 units
                         const int n = 16 / (int)sizeof(A);
@@ -870,7 +879,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
                     *reinterpret_cast<float4*>(pp + (c0 + i) * 128) =
-                        l > 0.f ? make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        n_tiles > 0 ? make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         }
     }
@@ -906,7 +915,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const float mz = __ldcg(pp + z * step);
             if (mz > -INFINITY) L = fmaf(__ldcg(pp + z * step + 128), pp_ex2(mz - M), L);
         }
-        const float inv = L > 0.f ? 1.0f / L : 0.f;
+        const bool sees = pos0 + qi >= 0;   // else zeros
+        const float inv = 1.0f / L;
         A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
 #pragma unroll 1
         for (int c0 = hf * (HD / TR); c0 < (hf + 1) * (HD / TR); c0 += 8) {
@@ -923,6 +933,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     v[i + 3] = fmaf(f, w.w, v[i + 3]);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = !sees ? 0.f : M == -INFINITY ? NAN : v[i];
             act_store8(dst + c0, v);
         }
     }

@@ -212,3 +212,21 @@ def long_axis(gb, act, cache, value, which, decode, n):
         c = R.Cache(gb, CACHE[cache], 1, 128, 64, [3000], 6)
         put_value(c, c.pools[which], 0, pos, 0, 77, value)
         check(gb, c, rows(n, 4 * 128, ACT[act], 5), [n], decode, pos)
+
+
+# ------------------------------------------------------------------ packed prompts
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("act,cache,hd", FORMS)
+def test_prefill_in_q(gb, cuda, act, cache, hd, value):
+    in_q(gb, act, cache, hd, value, False, [100, 9])
+
+
+@pytest.mark.parametrize("act,cache,hd", FORMS)
+def test_prefill_no_number_in_k_at_every_place(gb, cuda, act, cache, hd):
+    every_place(gb, act, cache, hd, NAN, 0, False)
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("cache", ["f16", "q8_0"])
+def test_prefill_no_number_in_k_over_a_long_axis(gb, cuda, act, cache):
+    long_axis(gb, act, cache, NAN, 0, False, 16)
