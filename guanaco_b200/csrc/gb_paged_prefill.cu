@@ -42,6 +42,13 @@
 // tiles are dequantised by four warps, a row per thread.  Rows past the last
 // key are zeroed in V (stale cache rows may hold anything).
 //
+// Rows whose result is not finite are computed once more by a warp each, from
+// the definition in fp32 (pp_row): P V also runs over the keys that a row does
+// not see, where an infinity or no number times the weight 0 is no number, and
+// an infinite K times q's two parts, or a Q8_0 value beyond 65504 as two halves,
+// may be none although the score or the value is a number.  Finite inputs of ordinary size
+// never come here; a prompt all of whose rows do is some 50 times slower.
+//
 // Few rows over a long axis: the host cuts the keys over gridDim.y CTAs, which
 // leave (m, l, O) partials; the last to arrive joins them in order.
 //
@@ -159,9 +166,83 @@ __device__ __forceinline__ uint32_t pp_off(int r, int u, int R) {
     return (uint32_t)((u >> 3) * R * 128 + r * 128 + (((u ^ r) & 7) << 4));
 }
 
+// CO columns from col on of row r of a slab.
+template <int HD, int DT, int CO>
+__device__ __forceinline__ void pp_cached(const uint8_t* slab, int shift, int r, int col, float (&x)[CO]) {
+    if (DT == GB_DT_F16) {
+        const __half2* p = reinterpret_cast<const __half2*>(slab + ((size_t)r * HD + col) * 2);
+#pragma unroll
+        for (int i = 0; i < CO; i += 2) {
+            const float2 f = __half22float2(p[i / 2]);
+            x[i] = f.x;
+            x[i + 1] = f.y;
+        }
+    } else {
+        const int8_t* p = reinterpret_cast<const int8_t*>(slab + (size_t)r * HD + col);
+        const float d = __half2float(reinterpret_cast<const __half*>(slab + ((size_t)HD << shift))[r * (HD / 32) + col / 32]);
+#pragma unroll
+        for (int i = 0; i < CO; i++) x[i] = d * (float)p[i];
+    }
+}
+// Head h of token t, which sees the first n keys (n > 0) of sequence seq: one
+// warp, from the definition.
+template <typename A, int HD, int DT>
+__device__ __noinline__ void pp_row(const PpArgs& a, int seq, int kvh, int t, int h, int n) {
+    constexpr int CO = HD / 32, KEYS = 4;   // columns of a lane; keys at a time (one page)
+    const int col = (threadIdx.x & 31) * CO;
+    const PagedView& c = a.c;
+    const float sc = 1.4426950408889634f / sqrtf((float)HD);
+    float q[CO], o[CO], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < CO; i++) {
+        q[i] = (float)static_cast<const A*>(a.q)[(size_t)t * a.ldq + (size_t)h * HD + col + i];
+        o[i] = 0.f;
+    }
+#pragma unroll 1
+    for (int key0 = 0; key0 < n; key0 += KEYS) {
+        const int page = max(page_of(c, a.b, seq, key0, a.err), 0), row = key0 & ((1 << c.shift) - 1);
+        const size_t slab = (size_t)page * c.page_bytes + (size_t)kvh * c.slab;
+        float x[KEYS], v[KEYS][CO], mn = m;
+#pragma unroll
+        for (int u = 0; u < KEYS; u++) {
+            float k[CO];
+#pragma unroll
+            for (int i = 0; i < CO; i++) v[u][i] = k[i] = 0.f;
+            if (key0 + u < n) {
+                pp_cached<HD, DT, CO>(c.k + slab, c.shift, row + u, col, k);
+                pp_cached<HD, DT, CO>(c.v + slab, c.shift, row + u, col, v[u]);
+            }
+            x[u] = 0.f;
+#pragma unroll
+            for (int i = 0; i < CO; i++) x[u] = fmaf(q[i], k[i], x[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < KEYS; u++) {
+            x[u] = key0 + u < n ? warp_sum(x[u]) * sc : -INFINITY;
+            mn = fmaxf(mn, x[u]);
+        }
+        const float ref = mn == -INFINITY ? 0.f : mn, al = pp_ex2(m - ref);   // 0 before the first finite score
+        m = mn;
+        l *= al;
+#pragma unroll
+        for (int i = 0; i < CO; i++) o[i] *= al;
+#pragma unroll
+        for (int u = 0; u < KEYS; u++) {
+            const float p = pp_ex2(x[u] - ref);
+            l += p;
+#pragma unroll
+            for (int i = 0; i < CO; i++) o[i] = fmaf(p, v[u][i], o[i]);
+        }
+    }
+    A* dst = static_cast<A*>(a.out) + (size_t)t * a.ldo + (size_t)h * HD + col;
+#pragma unroll
+    for (int i = 0; i < CO; i++) dst[i] = (A)(m == -INFINITY ? NAN : o[i] / l);
+}
+
 template <typename A, int HD, int DT>
 __global__ void __launch_bounds__((PpCfg<A, HD, DT>::THREADS), 1)
-k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PpArgs a) {
+k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                const __grid_constant__ PpArgs a) {
     using C = PpCfg<A, HD, DT>;
     constexpr int NK = C::NK, ST = C::ST;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -173,7 +254,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __shared__ float s_row[2][2][128];                  // what the two threads of a row exchange
     __shared__ uint32_t tmem_slot;
     __shared__ int s_seq, s_blk, s_slot;
-    __shared__ unsigned s_last;
+    __shared__ unsigned s_last, s_again[8];             // s_again: rows whose result is not finite
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedView& c = a.c;
     const BatchView& b = a.b;
@@ -201,6 +282,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         mbs_init(qread, C::MMA);          // Q's high parts have left the V stages
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (tid < 8) s_again[tid] = 0u;
     griddep_wait();   // launched ahead of the kernel before it
     // ---- which sequence and query block.  Up to 32 sequences: the y-th of all
     // blocks by their key tiles, the longest first; more: the sequences in order
@@ -428,7 +510,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         start_sync();
     }
     const uint32_t tmem = warp <= C::MMA ? tmem_slot : 0u;
-    bool ok = true;
+    bool ok = true, again = false;
 
     if (warp == C::MMA) {   // ---- MMA issue: the whole warp, uniform; one lane's instructions
         {
@@ -827,6 +909,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             // a row that sees no key: zeros; keys with scores of -inf alone: no number
             const bool sees = lim >= 0;
             const float inv = m == -INFINITY ? NAN : 1.0f / l;
+            float odd = 0.f;                                  // no number once a result is not finite
             const unsigned long long dst = live ? reinterpret_cast<unsigned long long>(
                 static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD + hf * (HD / TR)) : 0ull;
 #pragma unroll 1
@@ -845,7 +928,10 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                             o[i + 3] += w.w;
                         }
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] = sees ? o[i] * inv : 0.f;
+                    for (int i = 0; i < 16; i++) {
+                        o[i] = sees ? o[i] * inv : 0.f;
+                        odd = fmaf(o[i], 0.f, odd);
+                    }
 #pragma unroll
                     for (int i = 0; i < (int)sizeof(A); i++) {   // 16 columns: 2 or 4 units
                         const int n = 16 / (int)sizeof(A);
@@ -865,6 +951,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
                 __syncwarp();
             }
+            again = live && odd != 0.f;
+            if (again) atomicOr(&s_again[4 * rt + (r >> 5)], 1u << (r & 31));
         } else {   // m [128 rows], l [128], O [HD / 4][128][4] of this CTA's tile
             float* pp = a.part + (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + rt) * (HD + 2) * 128;
             if (hf == 0) {
@@ -884,7 +972,15 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         }
     }
     tc::fence_before_sync();
-    __syncthreads();
+    again = __syncthreads_or(again);
+    auto once_more = [&] {   // the noted rows, a warp each
+#pragma unroll 1
+        for (int i = warp; i < 256; i += C::THREADS / 32)
+            if (s_again[i >> 5] >> (i & 31) & 1u) {
+                const int x = i & 127, at = q0 + (i >> 7) * a.bq + x / a.group;
+                pp_row<A, HD, DT>(a, seq, kvh, t_begin + at, kvh * a.group + x % a.group, pos0 + at + 1);
+            }
+    };
     if (warp == C::MMA) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, 512);
@@ -893,7 +989,10 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         __threadfence();
         atomicExch(a.tickets + s_slot, 0u);
     }
-    if (n_split == 1) return;
+    if (n_split == 1) {
+        if (again) once_more();
+        return;
+    }
     // ---- the last split of this row block joins them
     if (tid == 0) {
         unsigned prev;
@@ -916,6 +1015,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             if (mz > -INFINITY) L = fmaf(__ldcg(pp + z * step + 128), pp_ex2(mz - M), L);
         }
         const bool sees = pos0 + qi >= 0;   // else zeros
+        float odd = 0.f;
         const float inv = 1.0f / L;
         A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
 #pragma unroll 1
@@ -934,10 +1034,16 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = !sees ? 0.f : M == -INFINITY ? NAN : v[i];
+            for (int i = 0; i < 8; i++) {
+                v[i] = !sees ? 0.f : M == -INFINITY ? NAN : v[i];
+                odd = fmaf(v[i], 0.f, odd);
+            }
             act_store8(dst + c0, v);
         }
+        again = odd != 0.f;
+        if (again) atomicOr(&s_again[4 * rt + (r >> 5)], 1u << (r & 31));
     }
+    if (__syncthreads_or(again)) once_more();
 }
 
 template <typename A, int HD, int DT>

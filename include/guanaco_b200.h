@@ -309,9 +309,11 @@ int gb_kv_read(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, vo
  * it must not overlap in time.  GB_ELIMIT: _prefill with more than 128 query
  * heads per KV head; _decode where n_seq x the table's positions / 16 x heads
  * passes 2^31.  Precision: fp32 rows as two fp16 parts (22 bits) in every
- * product; fp16 rows with the probabilities rounded to fp16.  _prefill reads
- * Q8_0 values as two fp16 parts: what sees one beyond 65504 (the largest of
- * an F16 cache too) is infinite or no number.  Asynchronous. */
+ * product; fp16 rows with the probabilities rounded to fp16.  Rows are
+ * infinite or no number where the sums above are; what stands past a token's
+ * position does not reach it.  _prefill computes rows that come out so, or
+ * come near Q8_0 values beyond 65504, once more, much slower.  (Q8_0 scales
+ * are finite, as appended.)  Asynchronous. */
 size_t gb_paged_workspace_bytes(int n_heads, int n_kv_heads, int head_dim, int n_seq);
 int gb_paged_attention_decode(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q, int ldq,
                               int n_heads, void* out, int ldo, void* ws, void* stream);

@@ -230,3 +230,61 @@ def test_prefill_no_number_in_k_at_every_place(gb, cuda, act, cache, hd):
 @pytest.mark.parametrize("cache", ["f16", "q8_0"])
 def test_prefill_no_number_in_k_over_a_long_axis(gb, cuda, act, cache):
     long_axis(gb, act, cache, NAN, 0, False, 16)
+
+
+@pytest.mark.parametrize("value", [INF, -INF])
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prefill_infinite_k_at_every_place(gb, cuda, act, hd, value):
+    every_place(gb, act, "f16", hd, value, 0, False)
+
+
+@pytest.mark.parametrize("cache,value", [("f16", NAN), ("f16", INF), ("f16", -INF), ("q8_0", NAN)])
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prefill_in_v_at_every_place(gb, cuda, act, cache, hd, value):
+    """Rows that do not see the position are as if it were not there."""
+    every_place(gb, act, cache, hd, value, 1, False)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prefill_q8_0_beyond_the_largest_half(gb, cuda, act, hd, which):
+    """Finite values, and those of later tokens leave earlier rows alone."""
+    beyond(gb, act, hd, which, False)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("cache,value", [("f16", NAN), ("f16", INF), ("q8_0", NAN)])
+@pytest.mark.parametrize("act", ["f32", "f16"])
+def test_prefill_few_rows_over_a_long_axis(gb, cuda, act, cache, value, which):
+    """Keys split over CTAs and joined: a value early, and one that only the last rows see."""
+    long_axis(gb, act, cache, value, which, False, 16)
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("kv_len,some", [(40, 20), (300, 280), (3000, 2500)])
+def test_prefill_scores_of_minus_infinity(gb, cuda, act, kv_len, some):
+    minus_infinity(gb, act, kv_len, some, False, 16)
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("cache,value", [("f16", NAN), ("f16", INF), ("q8_0", NAN)])
+def test_prefill_tokens_that_see_nothing_stay_zero(gb, cuda, act, cache, value):
+    """More tokens than cached rows: the first see nothing, whatever stands in
+    the rows that the others see."""
+    for which in (0, 1):
+        c = R.Cache(gb, CACHE[cache], 2, 64, 16, [12], 3)
+        put_value(c, c.pools[which], 0, 1, 1, 20, value)
+        check(gb, c, rows(40, 4 * 64, ACT[act], 2), [40], False)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prefill_sums_kept_in_the_workspace(gb, cuda, hd):
+    """fp32 over enough keys for a running sum, which a row that is computed
+    once more leaves to the next one as it should be."""
+    c = R.Cache(gb, R.F16, 4, hd, 64, [1100, 300], 3)
+    for pos in (1090, 700, 30):
+        put_value(c, c.pools[1], 0, pos, 2, 20, INF)
+    check(gb, c, rows(400, 4 * hd, F32, 2), [100, 300], False)
