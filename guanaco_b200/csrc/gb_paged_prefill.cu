@@ -254,6 +254,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __shared__ float s_row[2][2][128];                  // what the two threads of a row exchange
     __shared__ uint32_t tmem_slot;
     __shared__ int s_seq, s_blk, s_slot;
+    __shared__ bool s_claimed;
     __shared__ unsigned s_last, s_again[8];             // s_again: rows whose result is not finite
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedView& c = a.c;
@@ -392,8 +393,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 unsigned at;
                 asm volatile("mov.u32 %0, %%smid;" : "=r"(at));
                 int tries = 64 * GB_MAX_SMS;
-                for (at %= GB_MAX_SMS; atomicCAS(a.tickets + at, 0u, 1u) != 0u; at = (at + 1) % GB_MAX_SMS)
-                    if (--tries == 0) {   // a workspace that was never zeroed, or is shared
+                for (at %= GB_MAX_SMS; !(s_claimed = atomicCAS(a.tickets + at, 0u, 1u) == 0u); at = (at + 1) % GB_MAX_SMS)
+                    if (--tries == 0) {   // a workspace that was never zeroed, or is shared: the place stays another's
                         atomicExch(a.err, (unsigned)(-GB_ETIMEOUT));
                         break;
                     }
@@ -985,7 +986,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, 512);
     }
-    if (claim && tid == 0) {
+    if (claim && tid == 0 && s_claimed) {
         __threadfence();
         atomicExch(a.tickets + s_slot, 0u);
     }

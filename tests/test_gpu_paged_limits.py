@@ -76,3 +76,26 @@ def test_a_position_past_the_rotation_table(gb, cuda):
     for pool, old, x in zip(c.pools, before, (R.rope(k[:1].unflatten(1, (2, 64)), turn[19:20]), k[:1].unflatten(1, (2, 64)))):
         c.parts(old)[0][c.table[0, 1].long(), :, 3] = x[0].half()
         assert torch.equal(pool, old)
+
+
+PLACES_AT, PLACES = 192 * 2 * (128 + 2) * 128 * 4, 192   # of running sums in the workspace: behind the sums
+
+
+def test_a_workspace_without_free_places(gb, cuda):
+    """Never zeroed, say: the search for a place ends, is recorded, and places
+    that a CTA did not take stay taken."""
+    c = R.Cache(gb, R.F16, 32, 64, 32, [700, 900], 5)
+    q_lens = [700, 900]
+    q = rows_of(sum(q_lens), 32 * 64, 1)
+    out = torch.empty_like(q)
+    ws = workspace(gb, 32, c, 2)
+    places = ws[PLACES_AT: PLACES_AT + 4 * PLACES].view(torch.int32)
+    batch = gb.KVBatch(2, sum(q_lens), c.len, c.table, cu_of(q_lens))
+    places.fill_(1)
+    gb.paged_attention_prefill(c.h, batch, q, out, ws)
+    assert gb.paged_error(clear=True) == gb.GB_ETIMEOUT
+    assert (places == 1).all()
+    places.zero_()
+    gb.paged_attention_prefill(c.h, batch, q, out, ws)
+    assert gb.paged_error() == 0 and not places.any()
+    assert rel_l2(out.cpu(), R.attention(q, c, q_lens).cpu()) <= 1e-5
