@@ -99,3 +99,25 @@ def test_a_workspace_without_free_places(gb, cuda):
     gb.paged_attention_prefill(c.h, batch, q, out, ws)
     assert gb.paged_error() == 0 and not places.any()
     assert rel_l2(out.cpu(), R.attention(q, c, q_lens).cpu()) <= 1e-5
+
+
+@pytest.mark.parametrize("cache", [R.F16, R.Q8_0])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_places_with_the_longest_blocks_first(gb, cuda, cache, hd):
+    """Up to 32 sequences, and more CTAs than places for a running sum, each
+    over enough keys to need one: 32 heads of one each, two tiles of 128 queries a CTA."""
+    q_lens, kv_lens = [300, 0, 1, 700, 129], [900, 40, 777, 700, 1200]
+    assert sum(-(-n // 256) for n in q_lens) * 32 > PLACES
+    c = R.Cache(gb, cache, 32, hd, 32, kv_lens, 5)
+    q = rows_of(sum(q_lens), 32 * hd, 1)
+    ref = R.attention(q, c, q_lens).cpu()
+    out, ws = torch.empty_like(q), workspace(gb, 32, c, 5)
+    batch = gb.KVBatch(5, sum(q_lens), c.len, c.table, cu_of(q_lens))
+    got = []
+    for _ in range(2):
+        gb.paged_attention_prefill(c.h, batch, q, out, ws)
+        assert rel_l2(out.cpu(), ref) <= 1e-5
+        got.append(out.clone())
+    assert torch.equal(*got) and gb.paged_error() == 0
+    assert not ws[PLACES_AT: PLACES_AT + 4 * PLACES].any()
+    assert ws[:PLACES_AT].any()
