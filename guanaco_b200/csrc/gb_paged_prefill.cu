@@ -66,6 +66,7 @@ namespace gb {
 
 constexpr int PP_POLY = 8;                      // of this many pairs of exponentials one is a polynomial
 constexpr float PP_TAU = 8.f, PP_LIFT = 6.f;   // p <= 2^14; small p stay normal fp16 numbers
+constexpr int PP_SPLIT = 4;                     // key tiles at least of a CTA where keys are split
 constexpr int PP_SMEM_MAX = 227 * 1024 - 4096;  // less alignment slack and static shared memory
 
 template <typename A, int HD, int DT>
@@ -354,7 +355,8 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const bool two = q0 + a.bq < n_q;                    // the second row tile has queries
     const int kend = len == 0 ? 0 : pos0 + min(q0 + 2 * a.bq, n_q);   // keys 0 .. kend - 1
     const int nt_all = kend > 0 ? (kend + NK - 1) / NK : 0;
-    const int per = (nt_all + gridDim.y - 1) / gridDim.y;
+    // keys split over gridDim.y CTAs, but at least PP_SPLIT tiles a CTA: the host knows the table's width alone
+    const int per = gridDim.y == 1 ? nt_all : max(PP_SPLIT, (int)((nt_all + gridDim.y - 1) / gridDim.y));
     const int n_split = nt_all > 0 ? (nt_all + per - 1) / per : 1;
     if ((int)blockIdx.y >= n_split) return;
     const int j0 = blockIdx.y * per, nt = min(per, nt_all - j0);   // this CTA's key tiles j0 ..
@@ -1064,10 +1066,10 @@ static int launch_prefill(const gb_kv_cache* cache, PpArgs& a, void* ws, cudaStr
     if (blocks > a.b.n_tokens) blocks = a.b.n_tokens;
     const long long grid = blocks * a.c.n_kv;
     if (grid > 0x7fffffffLL) return GB_ELIMIT;
-    // fewer CTAs than half the SMs: cut the keys too, at least 4 tiles a CTA
+    // fewer CTAs than half the SMs: cut the keys too
     const int sms = sm_count();
     long long split = sms / grid;
-    const long long most = ((long long)a.b.cap + 4 * C::NK - 1) / (4 * C::NK);
+    const long long most = ((long long)a.b.cap + PP_SPLIT * C::NK - 1) / (PP_SPLIT * C::NK);
     if (split > most) split = most;
     if (split < 1) split = 1;
     a.part = static_cast<float*>(ws);

@@ -121,3 +121,21 @@ def test_places_with_the_longest_blocks_first(gb, cuda, cache, hd):
     assert torch.equal(*got) and gb.paged_error() == 0
     assert not ws[PLACES_AT: PLACES_AT + 4 * PLACES].any()
     assert ws[:PLACES_AT].any()
+
+
+@pytest.mark.parametrize("cache", [R.F16, R.Q8_0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_a_table_much_wider_than_the_sequences(gb, cuda, cache, dtype):
+    """Few rows and a server's table of 8192 positions: a short prompt's keys
+    are not cut into pieces of a tile, which would leave partials; a longer
+    prompt's are."""
+    for n, pieces in ((200, False), (2000, True)):
+        c = R.Cache(gb, cache, 2, 128, 32, [n], 5)
+        table = torch.full((1, 256), -7, dtype=torch.int32, device="cuda")
+        table[:, : c.table.shape[1]] = c.table
+        q = rows_of(40, 8 * 128, 1, dtype)
+        out, ws = torch.empty_like(q), workspace(gb, 8, c, 1)
+        gb.paged_attention_prefill(c.h, gb.KVBatch(1, 40, c.len, table, cu_of([40])), q, out, ws)
+        assert rel_l2(out.float().cpu(), R.attention(q, c, [40]).cpu()) <= (1e-5 if dtype == torch.float32 else 1.5e-3)
+        assert gb.paged_error() == 0
+        assert ws.any().item() == pieces
