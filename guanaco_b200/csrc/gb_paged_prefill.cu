@@ -46,8 +46,11 @@
 // the definition in fp32 (pp_row): P V also runs over the keys that a row does
 // not see, where an infinity or no number times the weight 0 is no number, and
 // an infinite K times q's two parts, or a Q8_0 value beyond 65504 as two halves,
-// may be none although the score or the value is a number.  Finite inputs of ordinary size
-// never come here; a prompt all of whose rows do is some 50 times slower.
+// may be none although the score or the value is a number.  Finite inputs of
+// ordinary size never come here.  One prompt of 8192, fp16, F16 cache, with an
+// infinity in V at the first position (each row rightly shows it: found at
+// once) 1.06 ms instead of 0.48, at the last (the 256 rows of 8 CTAs that it
+// spoils: 8192 keys each) 20.9 ms.
 //
 // Few rows over a long axis: the host cuts the keys over gridDim.y CTAs, which
 // leave (m, l, O) partials; the last to arrive joins them in order.
@@ -167,75 +170,117 @@ __device__ __forceinline__ uint32_t pp_off(int r, int u, int R) {
     return (uint32_t)((u >> 3) * R * 128 + r * 128 + (((u ^ r) & 7) << 4));
 }
 
-// CO columns from col on of row r of a slab.
-template <int HD, int DT, int CO>
-__device__ __forceinline__ void pp_cached(const uint8_t* slab, int shift, int r, int col, float (&x)[CO]) {
-    if (DT == GB_DT_F16) {
-        const __half2* p = reinterpret_cast<const __half2*>(slab + ((size_t)r * HD + col) * 2);
+// N (2, 4, 8) columns from col on, a multiple of N, of row r of a slab.
+template <int HD, int DT, int N>
+__device__ __forceinline__ void pp_cached(const uint8_t* slab, int shift, int r, int col, float (&x)[N]) {
+    constexpr int B = DT == GB_DT_F16 ? 2 * N : N;   // bytes
+    const uint8_t* p = slab + ((size_t)r * HD + col) * (B / N);
+    uint32_t w[B < 4 ? 1 : B / 4];
+    if constexpr (B == 16) {
+        const uint4 y = ldg4(p);
+        w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
+    } else if constexpr (B == 8) {
+        const uint2 y = __ldg(reinterpret_cast<const uint2*>(p));
+        w[0] = y.x; w[1] = y.y;
+    } else if constexpr (B == 4) {
+        w[0] = ldg1(p);
+    } else {
+        w[0] = ldg_u16(p);
+    }
+    if constexpr (DT == GB_DT_F16) {
 #pragma unroll
-        for (int i = 0; i < CO; i += 2) {
-            const float2 f = __half22float2(p[i / 2]);
+        for (int i = 0; i < N; i += 2) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i / 2]));
             x[i] = f.x;
             x[i + 1] = f.y;
         }
     } else {
-        const int8_t* p = reinterpret_cast<const int8_t*>(slab + (size_t)r * HD + col);
-        const float d = __half2float(reinterpret_cast<const __half*>(slab + ((size_t)HD << shift))[r * (HD / 32) + col / 32]);
+        const float d = __half2float(__ldg(reinterpret_cast<const __half*>(slab + ((size_t)HD << shift)) + r * (HD / 32) + col / 32));
 #pragma unroll
-        for (int i = 0; i < CO; i++) x[i] = d * (float)p[i];
+        for (int i = 0; i < N; i++) x[i] = d * (float)(int8_t)(w[i / 4] >> (8 * (i % 4)) & 0xffu);
     }
 }
-// Head h of token t, which sees the first n keys (n > 0) of sequence seq: one
-// warp, from the definition.
+// Head h of token t, which sees the first n keys (n > 0) of sequence seq, whose
+// output is not finite: one warp, 32 keys at a time, HD / 32 columns a lane.  Once the columns that are not finite are so
+// here too, the output is left as it is: its other columns are right.
 template <typename A, int HD, int DT>
 __device__ __noinline__ void pp_row(const PpArgs& a, int seq, int kvh, int t, int h, int n) {
-    constexpr int CO = HD / 32, KEYS = 4;   // columns of a lane; keys at a time (one page)
-    const int col = (threadIdx.x & 31) * CO;
+    constexpr int CO = HD / 32, V = 8;   // columns of a lane, rows in flight (of one page)
+    const int lane = threadIdx.x & 31, col = lane * CO, rows = 1 << a.c.shift;
     const PagedView& c = a.c;
+    const A* q = static_cast<const A*>(a.q) + (size_t)t * a.ldq + (size_t)h * HD + col;
+    A* dst = static_cast<A*>(a.out) + (size_t)t * a.ldo + (size_t)h * HD + col;
     const float sc = 1.4426950408889634f / sqrtf((float)HD);
-    float q[CO], o[CO], m = -INFINITY, l = 0.f;
+    float qx[CO], o[CO], m = -INFINITY, l = 0.f;   // l: of this lane's keys
+    bool odd[CO];
 #pragma unroll
     for (int i = 0; i < CO; i++) {
-        q[i] = (float)static_cast<const A*>(a.q)[(size_t)t * a.ldq + (size_t)h * HD + col + i];
+        qx[i] = (float)q[i];
         o[i] = 0.f;
+        odd[i] = !isfinite((float)dst[i]);
     }
 #pragma unroll 1
-    for (int key0 = 0; key0 < n; key0 += KEYS) {
-        const int page = max(page_of(c, a.b, seq, key0, a.err), 0), row = key0 & ((1 << c.shift) - 1);
-        const size_t slab = (size_t)page * c.page_bytes + (size_t)kvh * c.slab;
-        float x[KEYS], v[KEYS][CO], mn = m;
+    for (int key0 = 0; key0 < n; key0 += 32) {
+        const int key = min(key0 + lane, n - 1);
+        const size_t slab = (size_t)max(page_of(c, a.b, seq, key, a.err), 0) * c.page_bytes + (size_t)kvh * c.slab;
+        float x = 0.f;
+        // a row's columns over the lanes, V rows in flight; lane j gets the sum of key j
+#pragma unroll 1
+        for (int j0 = 0; j0 < min(32, n - key0); j0 += V) {
+            const uint8_t* at = c.k + __shfl_sync(0xffffffffu, slab, j0);
+            float k[V][CO], s[V];
 #pragma unroll
-        for (int u = 0; u < KEYS; u++) {
-            float k[CO];
+            for (int j = 0; j < V; j++)
+                pp_cached<HD, DT, CO>(at, c.shift, min(key0 + j0 + j, n - 1) & (rows - 1), col, k[j]);
 #pragma unroll
-            for (int i = 0; i < CO; i++) v[u][i] = k[i] = 0.f;
-            if (key0 + u < n) {
-                pp_cached<HD, DT, CO>(c.k + slab, c.shift, row + u, col, k);
-                pp_cached<HD, DT, CO>(c.v + slab, c.shift, row + u, col, v[u]);
+            for (int j = 0; j < V; j++) {
+                s[j] = 0.f;
+#pragma unroll
+                for (int i = 0; i < CO; i++) s[j] = fmaf(qx[i], k[j][i], s[j]);
             }
-            x[u] = 0.f;
+            // halves of the lanes exchange halves of the keys, three times
 #pragma unroll
-            for (int i = 0; i < CO; i++) x[u] = fmaf(q[i], k[i], x[u]);
-        }
+            for (int w = V / 2; w; w >>= 1) {
+                const bool up = lane & (w * (32 / V));
 #pragma unroll
-        for (int u = 0; u < KEYS; u++) {
-            x[u] = key0 + u < n ? warp_sum(x[u]) * sc : -INFINITY;
-            mn = fmaxf(mn, x[u]);
+                for (int j = 0; j < w; j++) {
+                    const float give = up ? s[j] : s[j + w], keep = up ? s[j + w] : s[j];
+                    s[j] = keep + __shfl_xor_sync(0xffffffffu, give, w * (32 / V));
+                }
+            }
+            s[0] += __shfl_xor_sync(0xffffffffu, s[0], 1);
+            s[0] += __shfl_xor_sync(0xffffffffu, s[0], 2);
+            const float y = __shfl_sync(0xffffffffu, s[0], (lane % V) * (32 / V));
+            if (lane / V == j0 / V) x = y;
         }
-        const float ref = mn == -INFINITY ? 0.f : mn, al = pp_ex2(m - ref);   // 0 before the first finite score
+        x = key0 + lane < n ? x * sc : -INFINITY;
+        const float mn = fmaxf(m, warp_max(x)), ref = mn == -INFINITY ? 0.f : mn, al = pp_ex2(m - ref);   // 0 before the first finite score
+        const float p = pp_ex2(x - ref);
         m = mn;
-        l *= al;
+        l = fmaf(l, al, p);
 #pragma unroll
         for (int i = 0; i < CO; i++) o[i] *= al;
+#pragma unroll 1
+        for (int j0 = 0; j0 < min(32, n - key0); j0 += V) {
+            const uint8_t* at = c.v + __shfl_sync(0xffffffffu, slab, j0);
+            float v[V][CO];
 #pragma unroll
-        for (int u = 0; u < KEYS; u++) {
-            const float p = pp_ex2(x[u] - ref);
-            l += p;
+            for (int j = 0; j < V; j++)
+                pp_cached<HD, DT, CO>(at, c.shift, min(key0 + j0 + j, n - 1) & (rows - 1), col, v[j]);
 #pragma unroll
-            for (int i = 0; i < CO; i++) o[i] = fmaf(p, v[u][i], o[i]);
+            for (int j = 0; j < V; j++) {
+                const float w = __shfl_sync(0xffffffffu, p, j0 + j);
+#pragma unroll
+                for (int i = 0; i < CO; i++)
+                    if (key0 + j0 + j < n) o[i] = fmaf(w, v[j][i], o[i]);
+            }
         }
+        bool same = true;
+#pragma unroll
+        for (int i = 0; i < CO; i++) same = same && (!odd[i] || !isfinite(o[i]));
+        if (__all_sync(0xffffffffu, same)) return;
     }
-    A* dst = static_cast<A*>(a.out) + (size_t)t * a.ldo + (size_t)h * HD + col;
+    l = warp_sum(l);
 #pragma unroll
     for (int i = 0; i < CO; i++) dst[i] = (A)(m == -INFINITY ? NAN : o[i] / l);
 }
