@@ -696,12 +696,16 @@ extern "C" int gb_sample(const float* logits, int ldl, int rows, int vocab, cons
     static_assert(most <= 227 * 1024, "shared memory");
     if (gb::set_smem_once(reinterpret_cast<const void*>(gb::k_sample), (int)most) != cudaSuccess) return GB_ECUDA;
     // More rows than two CTAs an SM take at once: those that need a search first.
-    // 128,256 tokens, five kinds of settings by turns / all rows alike: 61 rows 43 -> 33 /
-    // 60 -> 62 us, 100 rows 68 -> 59 / 99 -> 102 us, 256 rows 144 -> 140 / 223 -> 233 us:
-    // up to four times as many.
+    // Five kinds of settings by turns, without / with; all rows top-p (us):
+    //   vocabulary 32,000    38 rows 17 / 15, 26 / 28     100 rows 32 / 32, 48 / 52
+    //              64,000    61      28 / 24, 40 / 42     100      41 / 37, 65 / 69
+    //              96,000   100      58 / 51, 85 / 89     148      77 / 72, 117 / 123
+    //             128,256   100      68 / 59, 99 / 103    148      90 / 83, 136 / 142
+    // It gains where rows are long and few: a row per 800 tokens, at most four
+    // times as many as run at once.
     const int at_once = 2 * gb::sm_count() / gb::SMP_CL;
     const bool longest_first = (temperature || top_k || top_p) && rows > at_once && rows <= 4 * at_once &&
-                               rows <= gb::SMP_THREADS;
+                               rows <= vocab / 800 && rows <= gb::SMP_THREADS;
     return gb::launch_pdl(gb::k_sample, dim3(rows * gb::SMP_CL), gb::SMP_THREADS, (int)smem,
                           static_cast<cudaStream_t>(stream), logits, ldl, vocab, slice, temperature, top_k, top_p, min_p,
                           u, out, longest_first) == cudaSuccess
