@@ -50,10 +50,13 @@ namespace gb {
 // times a scale is brought below 2^14 by a power of two, 2^-E, shared by the
 // warp; l and O are in units of 2^E.
 //
-// 96 sequences of up to 8066 keys, 32 / 8 heads of 128, fp16: F16 cache 273 us, 6150
-// GB/s, bound by HBM; Q8_0 179 us, 4980 GB/s, bound by instructions (59 % issued
-// at the 12 warps an SM that O's and q's registers leave; most turn codes into
-// fragments).  One sequence of 8193, fp32, F16 cache: 13.5 us, latency.
+// 96 sequences of up to 8066 keys, 32 / 8 heads of 128, in a CUDA graph: F16 cache, fp16
+// 264 us, 6360 GB/s, fp32 271 us, 6200 GB/s, bound by HBM; Q8_0, fp16 180 us, 4970
+// GB/s (190 us a call among others), fp32 235 us, 3800 GB/s: some 480
+// instructions per 16 keys and 8 heads, most of them turning codes into
+// fragments, at the 12 warps an SM that O's and q's registers leave, issue
+// 59 % of the cycles and leave HBM at 58 % (fp32 also spills 192 bytes).  One
+// sequence of 8193, fp32, F16 cache: 13.7 us, latency.
 constexpr int PD_W = 4;              // warps
 constexpr int PD_MAX_CTAS = 4;       // CTAs per SM the workspace has room for
 constexpr int PD_MC = 16;            // partials of a join in flight, and of a group
@@ -130,10 +133,6 @@ __device__ __forceinline__ void pd_split(float x, float y, uint32_t& hi, uint32_
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&r);
 }
-// A pair of values as operands: split for fp32 activations; for fp16 ones
-// rounded to fp16 without a remainder (q is fp16 already; for a probability
-// the error is of the size of the output's own rounding, 2.9e-4 against
-// 2.1e-4 of the 64-bit result together).
 // o += A b.  fp32: with b's remainders first, from zero and then added rounded
 // to nearest, as the tensor cores' additions truncate.
 template <typename A>
@@ -149,6 +148,10 @@ __device__ __forceinline__ void pd_add(float (&o)[4], uint32_t a0, uint32_t a1, 
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] += s[i];
 }
+// A pair of values as operands: split for fp32 activations; for fp16 ones
+// rounded to fp16 without a remainder (q is fp16 already; for a probability
+// the error is of the size of the output's own rounding, 2.7e-4 against
+// 2.1e-4 of the 64-bit result together).
 template <typename A>
 __device__ __forceinline__ void pd_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
     if (sizeof(A) == 4) {

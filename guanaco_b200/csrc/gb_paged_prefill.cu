@@ -200,8 +200,8 @@ __device__ __forceinline__ void pp_cached(const uint8_t* slab, int shift, int r,
         for (int i = 0; i < N; i++) x[i] = d * (float)(int8_t)(w[i / 4] >> (8 * (i % 4)) & 0xffu);
     }
 }
-// Head h of token t, which sees the first n keys (n > 0) of sequence seq, whose
-// output is not finite: one warp, 32 keys at a time, HD / 32 columns a lane.  Once the columns that are not finite are so
+// Head h of token t, which sees the first n keys of sequence seq (none: zeros),
+// whose output is not finite: one warp, 32 keys at a time, HD / 32 columns a lane.  Once the columns that are not finite are so
 // here too, the output is left as it is: its other columns are right.
 template <typename A, int HD, int DT>
 __device__ __noinline__ void pp_row(const PpArgs& a, int seq, int kvh, int t, int h, int n) {
@@ -282,7 +282,7 @@ __device__ __noinline__ void pp_row(const PpArgs& a, int seq, int kvh, int t, in
     }
     l = warp_sum(l);
 #pragma unroll
-    for (int i = 0; i < CO; i++) dst[i] = (A)(m == -INFINITY ? NAN : o[i] / l);
+    for (int i = 0; i < CO; i++) dst[i] = (A)(n <= 0 ? 0.f : m == -INFINITY ? NAN : o[i] / l);
 }
 
 template <typename A, int HD, int DT>
@@ -954,8 +954,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             static_assert(CP % 16 == 0 && HD / TR % CP == 0 && (UN == 8 || UN == 4), "rows of the staging area");
             uint8_t* wb = qs + rt * C::QB + warp % (4 * TR) * WB;
             auto at = [&](int row, int u) { return wb + row * RB + ((u ^ (UN == 8 ? row & 7 : (row >> 1) & 3)) << 4); };
-            // a row that sees no key: zeros; keys with scores of -inf alone: no number
-            const bool sees = lim >= 0;
+            // keys with scores of -inf alone: no number; no keys: the same, and zeros by pp_row
             const float inv = m == -INFINITY ? NAN : 1.0f / l;
             float odd = 0.f;                                  // no number once a result is not finite
             const unsigned long long dst = live ? reinterpret_cast<unsigned long long>(
@@ -977,7 +976,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         }
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        o[i] = sees ? o[i] * inv : 0.f;
+                        o[i] *= inv;
                         odd = fmaf(o[i], 0.f, odd);
                     }
 #pragma unroll
@@ -1062,7 +1061,6 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             const float mz = __ldcg(pp + z * step);
             if (mz > -INFINITY) L = fmaf(__ldcg(pp + z * step + 128), pp_ex2(mz - M), L);
         }
-        const bool sees = pos0 + qi >= 0;   // else zeros
         float odd = 0.f;
         const float inv = 1.0f / L;
         A* dst = static_cast<A*>(a.out) + (size_t)(t_begin + qi) * a.ldo + (size_t)h * HD;
@@ -1083,7 +1081,7 @@ k_paged_prefill(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                v[i] = !sees ? 0.f : M == -INFINITY ? NAN : v[i];
+                v[i] = M == -INFINITY ? NAN : v[i];
                 odd = fmaf(v[i], 0.f, odd);
             }
             act_store8(dst + c0, v);
