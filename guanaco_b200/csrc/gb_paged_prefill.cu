@@ -49,15 +49,16 @@
 // may be none although the score or the value is a number.  Finite inputs of
 // ordinary size never come here.  One prompt of 8192, fp16, F16 cache, with an
 // infinity in V at the first position (each row rightly shows it: found at
-// once) 1.06 ms instead of 0.48, at the last (the 256 rows of 8 CTAs that it
-// spoils: 8192 keys each) 20.9 ms.
+// once) 1.05 ms instead of 0.48, at the last (the 256 rows of 8 CTAs that it
+// spoils: 8192 keys each) 20.8 ms.
 //
 // Few rows over a long axis: the host cuts the keys over gridDim.y CTAs, which
 // leave (m, l, O) partials; the last to arrive joins them in order.
 //
-// 32 / 8 heads of 128: one prompt of 8192, fp16, F16 cache 475 us, 1157 TFLOP/s, where
+// 32 / 8 heads of 128, in a CUDA graph: one prompt of 8192, fp16, F16 cache 474-487
+// us, 1130-1160 TFLOP/s (a call among others 552-562 us, under the power cap), where
 // the exponentials and the tensor cores take turns; five prompts of up to 968, fp32,
-// Q8_0 149 us, 232 TFLOP/s of three products: the tensor cores, 2300 cycles for
+// Q8_0 147-151 us, 231 TFLOP/s of three products: the tensor cores, 2300 cycles for
 // 128 rows and 64 keys, and 30,000 cycles a CTA before and after them.
 #include "gb_mt.cuh"
 #include "gb_paged.cuh"
@@ -78,7 +79,7 @@ struct PpCfg {
     // fp16, F16 cache, hd 128: tiles of 128 keys (an MMA of N 128 takes 80 cycles,
     // one of N 64 takes 64), one buffer of S, two threads per row; hd 64: 64 keys,
     // two buffers and one thread per row.  One prompt of 8192 tokens that way /
-    // the other: hd 128 489 / 597 us, hd 64 580 / 449 us.  Several products per
+    // the other, when this was chosen: hd 128 489 / 597 us, hd 64 580 / 449 us.  Several products per
     // operand: one buffer, two threads per row (Q8_0 hd 128 896 us, with two
     // buffers and Q in shared memory 1543 us).
     static constexpr bool WIDE = !F32 && !Q8 && HD == 128;

@@ -25,10 +25,12 @@
 //                After a top-p cut each CTA knows its kept weights from its
 //                histogram, and only the one with the target goes on.
 // A row is a chain of these phases, which the clusters of other rows fill: 1 row
-// of 32,000 takes 8.7 us, 256 rows of 128,256 (top-p) 225 us = 585 GB/s, 46,000
-// cycles a row and cluster: 14,500 until the maximum is known (HBM), 14,000 for
-// the weights (40 instructions each), the rest four exchanges over the
-// cluster, the bin's tokens and their ranks.  Other splits of 256 rows measured
+// of 32,000 takes 8.8 us, 256 rows of 128,256 with top-p 225 us = 585 GB/s, 46,000
+// cycles a row and cluster: 14,500 until the maximum is known (an HBM round trip
+// that each wave of clusters pays), 14,000 for the weights (40 instructions each),
+// 17,500 four exchanges over the cluster, the bin's tokens and their ranks.  The
+// same rows greedy 71 us, unfiltered or with min-p 120, with top-k 40 129, with
+// top-k 2000 194.  Other splits of 256 rows measured
 // slower: 16 CTAs a row, three CTAs of 384 threads an SM.
 #include "gb_common.cuh"
 #include "gb_internal.h"

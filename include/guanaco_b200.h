@@ -288,7 +288,8 @@ typedef struct {
  * rotated at its position first, and when q is not NULL the rotated q
  * (n_heads heads) goes to q_out (which may be q).  Q8_0: per 32 columns
  * d = half(max |x| / 127) (at most 65504), code = x / d rounded to nearest
- * even; NaN and d = 0 give code 0.  Rows 16-byte aligned.  GB_ELIMIT: more
+ * even; NaN and d = 0 give code 0.  F16: beyond 65504 an infinity.  Rows
+ * 16-byte aligned.  GB_ELIMIT: more
  * threads than a grid holds (2^31 tokens x heads, about).  Asynchronous. */
 int gb_kv_append(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, const void* q, int ldq, int n_heads,
                  void* q_out, int ldqo, const void* k, int ldk, const void* v, int ldv, const float* rope_cs,
@@ -301,7 +302,8 @@ int gb_kv_read(const gb_kv_cache* cache, const gb_kv_batch* batch, int dtype, vo
 /* Attention of the batch's query rows q [n_tokens][n_heads * head_dim] over
  * the cache: a token at position p sees rows 0 .. p of its sequence (append
  * first); scores scaled by 1 / sqrt(head_dim); a token that sees nothing gets
- * zeros.  n_heads a multiple of n_kv_heads.  fp32 softmax and sums.
+ * zeros.  n_heads a multiple of n_kv_heads.  out: apart from q.  fp32 softmax
+ * and sums.
  * _decode: one token per sequence (cu_seqlens NULL), split over the cache's
  * length and joined.  _prefill: packed prompts of any lengths, on the tensor
  * cores.  ws: gb_paged_workspace_bytes(...) bytes (about 26 MB) for the
