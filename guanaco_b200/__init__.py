@@ -333,10 +333,11 @@ def _rows(fn, batch, a, b):
     if (t not in _ACT or b.dtype is not t or len(sa) != 2 or len(sb) != 2 or sa[1] != sb[1] or sa[0] < n_tokens
             or sb[0] < n_tokens or la[1] != 1 or lb[1] != 1):
         raise GBError(fn, GB_EINVAL)
-    lda, ldb = la[0] if sa[0] > 1 else sa[1], lb[0] if sb[0] > 1 else sa[1]   # one row: the next is nowhere
+    width = sa[1]
+    lda, ldb = la[0] if sa[0] > 1 else width, lb[0] if sb[0] > 1 else width   # one row: the next is nowhere
     if lda > _INT_MAX or ldb > _INT_MAX:   # the library's strides are ints
         raise GBError(fn, GB_ELIMIT)
-    return _ACT[t], sa[1], lda, ldb
+    return _ACT[t], width, lda, ldb
 
 
 def kv_page_bytes(dtype, n_kv_heads, head_dim, page_size) -> int:
@@ -361,9 +362,10 @@ def kv_append(cache, batch, k, v, q=None, q_out=None, rope_cs=None, stream=None)
         pq, pqo, nh = q.data_ptr(), q_out.data_ptr(), wq // hd
     pcs, rope_len = None, 0
     if rope_cs is not None:   # rows of hd floats, one after another
-        if _ACT.get(rope_cs.dtype) != DT_F32 or rope_cs.numel() % hd or not rope_cs.is_contiguous():
+        rope_len, rest = divmod(rope_cs.numel(), hd)
+        if rest or _ACT.get(rope_cs.dtype) != DT_F32 or not rope_cs.is_contiguous():
             raise GBError("gb_kv_append", GB_EINVAL)
-        pcs, rope_len = rope_cs.data_ptr(), rope_cs.numel() // hd
+        pcs = rope_cs.data_ptr()
     rc = lib().gb_kv_append(cache.ref, batch.ref, dt, pq, ldq, nh, pqo, ldqo, k.data_ptr(), ldk, v.data_ptr(), ldv,
                             pcs, rope_len, _stream(stream))
     if rc:
@@ -378,7 +380,8 @@ def kv_read(cache, batch, k, v, stream=None) -> None:
     dt, width, ldk, ldv = _rows("gb_kv_read", batch, v if k is None else k, k if v is None else v)
     if width != cache.n_kv_heads * cache.head_dim:
         raise GBError("gb_kv_read", GB_EINVAL)
-    rc = lib().gb_kv_read(cache.ref, batch.ref, dt, _ptr(k), ldk, _ptr(v), ldv, _stream(stream))
+    rc = lib().gb_kv_read(cache.ref, batch.ref, dt, None if k is None else k.data_ptr(), ldk,
+                          None if v is None else v.data_ptr(), ldv, _stream(stream))
     if rc:
         raise GBError("gb_kv_read", rc)
 
